@@ -31,7 +31,7 @@ _TYPES = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
 _SIZE = {"bf16": 2, "fp16": 2, "fp32": 4}
 _EPS = 1e-5
 _LOG2E = 1.4426950408889634
-_ONE = 2 ** 32            # the weight of a row's likeliest token
+_ONE = 2 ** 31            # the weight of a row's likeliest token
 
 
 def _package():
@@ -288,13 +288,13 @@ def _plain_sample(s):
     top = l.amax(1, keepdim=True)
     warm = t >= 1e-6
     scale = torch.full_like(t, _LOG2E) / torch.where(warm, t, 1.0)
-    # weights are whole 2^-32ths of the likeliest token's, so that no sum depends on its order
-    w = torch.exp2(torch.where(l == top, 0.0, (l - top) * scale[:, None])) * _ONE
-    w = torch.where(l > -math.inf, w.round(), 0.0).long()
-    order = l.sort(dim=1, descending=True, stable=True).indices
+    # weights are whole 2^-31ths of the likeliest token's, so that no sum depends on its order
+    x = torch.where(l > -math.inf, torch.where(l == top, 0.0, (l - top) * scale[:, None]), -math.inf)
+    w = (torch.exp2(x) * _ONE).round().long()
+    order = x.sort(dim=1, descending=True, stable=True).indices
     sorted_w, rank = w.gather(1, order), torch.arange(l.shape[1], device="cuda")
     k = torch.where(warm[:, None], k, 1)
-    kept = ((k <= 0) | (rank < k)) & (sorted_w >= (least.double() * _ONE).ceil().long().clamp(min=1)[:, None])
+    kept = ((k <= 0) | (rank < k)) & (sorted_w >= (least.double() * _ONE).ceil().long().clamp(1, _ONE)[:, None])
     sorted_w = sorted_w * kept
     total, upto = sorted_w.sum(1), sorted_w.cumsum(1)
     need = torch.where(p < 1, (p.double() * total.double()).ceil().long().clamp(min=1), total)
