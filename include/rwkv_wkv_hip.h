@@ -347,6 +347,76 @@ int wkv_timemix_head(void *stream, int B, int C, int H, const void *r, const voi
 int wkv_l2wrap_backward(void *stream, int rows, int V, int dtype, float factor, const void *y, const float *mask,
                         void *gy);
 
+/* ---- The operators of a state space block and of the end of a serving loop (no counterpart in the reference).
+ *
+ * An operand with strides: a (B, T, width) array, or (B, T, G, N) for b and c, whose last dimension is contiguous; `batch`, `token`
+ * and `group` are the strides of the others, in elements.  p has to be aligned to an element only.  lengths, where it is
+ * taken: B device ints, or NULL (every sequence has T tokens); tokens from a sequence's length on are not read, their outputs and
+ * gradients are zero, and a state stands after the sequence's last token.  Every gradient is complete and repeats to the bit. */
+typedef struct {
+    const void *p;
+    long long batch, token, group;
+} wkv_rows;
+
+/* The causal convolution of W taps (2 to 4) per channel in front of the scan, with xx = x continued to the left by the W-1 inputs of state_in:
+ *   pre[t] = bias + sum_k weight[:, k] xx[t - (W-1) + k],   y = silu ? pre sigmoid(pre) : pre
+ * x, y (B,T,D), state_in, state_out (B, W-1, D) in `dtype`; weight (D, W), bias (D) or NULL in `param_dtype`, fp32 or `dtype`; state_in NULL: zeros.
+ * state_out may be state_in for a single token (T = 1). */
+int wkv_causal_conv_forward(void *stream, int B, int T, int D, int W, int dtype, int param_dtype, int silu, const wkv_rows *x, const void *weight,
+                            const void *bias, const void *state_in, const int *lengths, void *y, void *state_out);
+
+/* Its backward: gstate_out (of state_out), gbias and gstate_in may be NULL; gweight, gbias in `param_dtype`. */
+size_t wkv_causal_conv_backward_workspace(int B, int T, int D, int W, int dtype);
+int wkv_causal_conv_backward(void *stream, int B, int T, int D, int W, int dtype, int param_dtype, int silu, const wkv_rows *x, const void *weight,
+                             const void *bias, const void *state_in, const int *lengths, const void *gy, const void *gstate_out, void *gx,
+                             void *gweight, void *gbias, void *gstate_in, void *workspace, size_t workspace_bytes);
+
+/* The selective state space scan, N states (1 to 64) per channel, G groups of D / G channels:
+ *   step = softplus(dt + dt_bias),  h[t] = exp(step A) h[t-1] + step x b[t],  y[t] = (c[t] . h[t] + skip x[t]) silu(z[t])
+ * x, dt, z (or NULL: no gate), y (B,T,D), b, c (B,T,G,N) in `dtype`; A (D,N), skip, dt_bias (D; or NULL) fp32; state (B,D,N) fp32,
+ * state_in NULL: zeros.  checkpoints: NULL, or wkv_selective_scan_checkpoint_bytes for a backward call.  workspace:
+ * wkv_selective_scan_forward_workspace bytes (none are needed for a single token without checkpoints, where state_out may be state_in). */
+size_t wkv_selective_scan_checkpoint_bytes(int B, int T, int D, int N, int G, int dtype);
+size_t wkv_selective_scan_forward_workspace(int B, int T, int D, int N, int G, int dtype);
+int wkv_selective_scan_forward(void *stream, int B, int T, int D, int N, int G, int dtype, const wkv_rows *x, const wkv_rows *dt, const float *A,
+                               const wkv_rows *b, const wkv_rows *c, const float *skip, const wkv_rows *z, const float *dt_bias, const float *state_in,
+                               const int *lengths, void *y, float *state_out, float *checkpoints, void *workspace, size_t workspace_bytes);
+
+/* Its backward, from the forward call's checkpoints: gx, gdt, gz (B,T,D), gb, gc (B,T,G,N) contiguous in `dtype`, gA, gskip, gdt_bias and gstate_in fp32;
+ * gstate_out, gskip, gdt_bias and gstate_in may be NULL. */
+size_t wkv_selective_scan_backward_workspace(int B, int T, int D, int N, int G, int dtype);
+int wkv_selective_scan_backward(void *stream, int B, int T, int D, int N, int G, int dtype, const wkv_rows *x, const wkv_rows *dt, const float *A,
+                                const wkv_rows *b, const wkv_rows *c, const float *skip, const wkv_rows *z, const float *dt_bias, const int *lengths,
+                                const float *checkpoints, const void *gy, const float *gstate_out, void *gx, void *gdt, float *gA, void *gb, void *gc,
+                                float *gskip, void *gz, float *gdt_bias, float *gstate_in, void *workspace, size_t workspace_bytes);
+
+/* The residual's addition and the root-mean-square norm over rows of C elements:
+ *   r = x + residual (NULL: x),   y = r / sqrt(mean(r^2) + eps) * weight
+ * x, y in `dtype`; residual, residual_out (r; or NULL) in `residual_dtype`, weight in `weight_dtype`, each fp32 or `dtype`.  Row strides in
+ * elements; outputs are contiguous.  q, scale non-NULL instead of y: y in 8 bits (e4m3), y = q scale[row], scale = max|y| / 448 (1 for a row of
+ * zeros).  rstd: (rows), for a backward call, or NULL. */
+int wkv_rms_norm_forward(void *stream, int rows, int C, int dtype, int residual_dtype, int weight_dtype, float eps, const void *x, long long x_stride,
+                         const void *residual, long long residual_stride, const void *weight, void *y, void *q, float *scale, void *residual_out,
+                         float *rstd);
+
+/* Its backward: x and residual as the forward call had them, or x NULL and the forward call's residual_out as the residual where that is
+ * fp32; gresidual_out its gradient, or NULL; gx in `dtype`, gresidual (NULL where it would be gx again) in `residual_dtype`, gweight in
+ * `weight_dtype`. */
+size_t wkv_rms_norm_backward_workspace(int rows, int C);
+int wkv_rms_norm_backward(void *stream, int rows, int C, int dtype, int residual_dtype, int weight_dtype, const void *x, long long x_stride,
+                          const void *residual, long long residual_stride, const void *weight, const float *rstd, const void *gy,
+                          const void *gresidual_out, void *gx, void *gresidual, void *gweight, void *workspace, size_t workspace_bytes);
+
+/* One token per row of logits (rows, V), V up to 2^20, from one random number u in [0, 1) per row.  Settings come per row or, with a NULL pointer, as
+ * one value: temperature (below 1e-6: the likeliest token), top_k (0 or less: off), top_p (1: off), min_p (0: off).  Tokens are weighted by
+ * exp((logit - max) / temperature), in whole 2^-31ths, and ordered by that exponent, ties by index; kept are the first top_k, of those the
+ * ones whose weight is at least min_p, of those the shortest beginning with a share top_p of their weight; the token drawn is the first, by index, at
+ * which the kept weights' sum passes u times their total.  logprob: the log of the probability it was drawn with.  NaN counts as
+ * -infinity; a row of nothing else: token -1, logprob -infinity. */
+int wkv_sample(void *stream, int rows, int V, int dtype, const void *logits, long long stride, const float *u, const float *temperature,
+               float temperature_value, const int *top_k, int top_k_value, const float *top_p, float top_p_value, const float *min_p, float min_p_value,
+               long long *token, float *logprob);
+
 #ifdef __cplusplus
 }
 #endif

@@ -33,7 +33,10 @@ namespace {
     X(wkv_widen_rows) X(wkv_shift_mix_forward) X(wkv_shift_mix_backward) X(wkv_shift_mix_backward_workspace)                  \
     X(wkv_lora_mix_forward) X(wkv_lora_mix_backward) X(wkv_lora_mix_backward_workspace) X(wkv_ln_gate_forward)                \
     X(wkv_ln_gate_backward) X(wkv_ln_gate_backward_workspace) X(wkv_relu_square_forward) X(wkv_relu_square_backward)          \
-    X(wkv_sigmoid_mul_forward) X(wkv_sigmoid_mul_backward)
+    X(wkv_sigmoid_mul_forward) X(wkv_sigmoid_mul_backward) X(wkv_causal_conv_forward) X(wkv_causal_conv_backward)             \
+    X(wkv_causal_conv_backward_workspace) X(wkv_selective_scan_checkpoint_bytes) X(wkv_selective_scan_forward_workspace)      \
+    X(wkv_selective_scan_forward) X(wkv_selective_scan_backward_workspace) X(wkv_selective_scan_backward)                     \
+    X(wkv_rms_norm_forward) X(wkv_rms_norm_backward_workspace) X(wkv_rms_norm_backward) X(wkv_sample)
 struct {
 #define X(name) decltype(&::name) name = nullptr;
     WKV_ABI(X)
@@ -416,6 +419,7 @@ PyObject *py_wkv4(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 #include "host_layers.h"
+#include "host_ssm.h"
 
 // bind(path of the kernel library, WKVError, torch.nn.Linear, torch.nn.GroupNorm, (the dictionaries of hooks on all modules))
 PyObject *py_bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -439,7 +443,7 @@ PyObject *py_bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(wkv56), METHOD(forward56), METHOD(backward56), METHOD(decay_operand), METHOD(wkv4), METHOD(timemix),
-                         METHOD(channelmix),
+                         METHOD(channelmix), METHOD(causal_conv), METHOD(selective_scan), METHOD(rms_norm), METHOD(rms_norm_fp8), METHOD(sample),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native host side of rwkv_wkv_hip", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

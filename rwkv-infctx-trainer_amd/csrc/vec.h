@@ -1,0 +1,40 @@
+// V consecutive elements as floats: one, or as many as make whole 16-byte pieces (p aligned to 16 bytes then).
+#pragma once
+#include "common.h"
+
+namespace wkv {
+
+template <class T, int V> __device__ __forceinline__ void load_vec(const T *p, float (&o)[V]) {
+    if constexpr (V == 1) {
+        o[0] = to_float(*p);
+    } else {
+        constexpr int EACH = 16 / sizeof(T);
+        static_assert(V % EACH == 0, "whole 16-byte pieces");
+#pragma unroll
+        for (int q = 0; q < V; q += EACH) {
+            const uint4 raw = *reinterpret_cast<const uint4 *>(p + q);
+            T e[EACH];
+            __builtin_memcpy(e, &raw, 16);
+#pragma unroll
+            for (int i = 0; i < EACH; i++) o[q + i] = to_float(e[i]);
+        }
+    }
+}
+template <class T, int V> __device__ __forceinline__ void store_vec(T *p, const float (&o)[V]) {
+    if constexpr (V == 1) {
+        *p = from_float<T>(o[0]);
+    } else {
+        constexpr int EACH = 16 / sizeof(T);
+#pragma unroll
+        for (int q = 0; q < V; q += EACH) {
+            T e[EACH];
+#pragma unroll
+            for (int i = 0; i < EACH; i++) e[i] = from_float<T>(o[q + i]);
+            uint4 raw;
+            __builtin_memcpy(&raw, e, 16);
+            *reinterpret_cast<uint4 *>(p + q) = raw;
+        }
+    }
+}
+
+}  // namespace wkv

@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_float, c_int, c_size_t, c_uint, c_void_p
+from ctypes import c_char_p, c_float, c_int, c_longlong, c_size_t, c_uint, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("RWKV_WKV_LIB", os.path.join(_HERE, "librwkv_wkv_hip.so"))
@@ -68,6 +68,18 @@ SIGNATURES = {
     "wkv_lora_mix_rows": (_I, [_P, _I, _I] + [_P] * 6),
     "wkv_timemix_head": (_I, [_P, _I, _I, _I] + [_P] * 10 + [c_float, c_float] + [_P] * 3),
     "wkv_l2wrap_backward": (_I, [_P, _I, _I, _I, c_float, _P, _P, _P]),
+    "wkv_causal_conv_forward": (_I, [_P] + [_I] * 7 + [_P] * 7),
+    "wkv_causal_conv_backward_workspace": (c_size_t, [_I] * 5),
+    "wkv_causal_conv_backward": (_I, [_P] + [_I] * 7 + [_P] * 11 + [_P, c_size_t]),
+    "wkv_selective_scan_checkpoint_bytes": (c_size_t, [_I] * 6),
+    "wkv_selective_scan_forward_workspace": (c_size_t, [_I] * 6),
+    "wkv_selective_scan_forward": (_I, [_P] + [_I] * 6 + [_P] * 13 + [_P, c_size_t]),
+    "wkv_selective_scan_backward_workspace": (c_size_t, [_I] * 6),
+    "wkv_selective_scan_backward": (_I, [_P] + [_I] * 6 + [_P] * 21 + [_P, c_size_t]),
+    "wkv_rms_norm_forward": (_I, [_P] + [_I] * 5 + [c_float, _P, c_longlong, _P, c_longlong] + [_P] * 6),
+    "wkv_rms_norm_backward_workspace": (c_size_t, [_I] * 2),
+    "wkv_rms_norm_backward": (_I, [_P] + [_I] * 5 + [_P, c_longlong, _P, c_longlong] + [_P] * 7 + [_P, c_size_t]),
+    "wkv_sample": (_I, [_P, _I, _I, _I, _P, c_longlong, _P, _P, c_float, _P, _I, _P, c_float, _P, c_float, _P, _P]),
 }
 
 _lib = None
