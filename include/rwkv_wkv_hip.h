@@ -350,7 +350,7 @@ int wkv_l2wrap_backward(void *stream, int rows, int V, int dtype, float factor, 
 /* ---- The operators of a state space block and of the end of a serving loop (no counterpart in the reference).
  *
  * An operand with strides: a (B, T, width) array, or (B, T, G, N) for b and c, whose last dimension is contiguous; `batch`, `token`
- * and `group` are the strides of the others, in elements.  p has to be aligned to an element only.  lengths, where it is
+ * and `group` are the strides of the others, in elements (the scan: token below 2^24).  p has to be aligned to an element only.  lengths, where it is
  * taken: B device ints, or NULL (every sequence has T tokens); tokens from a sequence's length on are not read, their outputs and
  * gradients are zero, and a state stands after the sequence's last token.  Every gradient is complete and repeats to the bit. */
 typedef struct {

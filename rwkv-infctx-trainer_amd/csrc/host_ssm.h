@@ -20,10 +20,15 @@ Tensor plain_float(const Tensor &t) { return t.defined() ? plain(as_float(t)) : 
 Tensor plain_parameter(const Tensor &t, at::ScalarType streams) {
     return !t.defined() || t.scalar_type() == streams ? plain(t) : plain_float(t);
 }
-// a stream or vector operand: any strides over a contiguous last dimension
-Tensor strided(const Tensor &t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
+// a stream or vector operand: any strides over a contiguous last dimension (a tile's tokens have to lie within 32-bit offsets)
+Tensor strided(const Tensor &t) {
+    if (!t.defined() || ((t.stride(-1) == 1 || t.size(-1) == 1) && (t.size(1) == 1 || t.stride(1) < (1 << 24)))) return t;
+    return t.contiguous();
+}
 wkv_rows rows_of(const Tensor &t) {
-    return t.defined() ? wkv_rows{t.data_ptr(), t.stride(0), t.stride(1), t.dim() == 4 ? t.stride(2) : 0} : wkv_rows{};
+    if (!t.defined()) return wkv_rows{};
+    auto step = [&](int64_t d) { return t.size(d) > 1 ? (long long)t.stride(d) : 0; };          // (that of a single element means nothing)
+    return wkv_rows{t.data_ptr(), step(0), step(1), t.dim() == 4 ? step(2) : 0};
 }
 Tensor lengths_of(const Tensor &t, int64_t B) {
     if (!t.defined()) return t;

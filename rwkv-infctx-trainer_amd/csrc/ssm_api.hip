@@ -52,7 +52,7 @@ bool conv_wide(const wkv_rows *x, int D, int dtype) {
 
 // ---- scan
 int check_scan(int B, int T, int D, int N, int G, int dtype) {
-    if (N <= 0 || N > scan::MAX_STATES || G <= 0 || D % G != 0 || (long long)D * N >= (1ll << 30)) return WKV_ERR_DIMS;
+    if (N <= 0 || N > scan::MAX_STATES || G <= 0 || D % G != 0 || D >= scan::MAX_TOKEN_STRIDE || (long long)D * N >= (1ll << 30)) return WKV_ERR_DIMS;
     if (int st = check_streams(B, T, D, dtype)) return st;
     // (grids: at most 64 segments of workgroups of 16 channels)
     return (long long)B * G * ((D / G + 15) / 16) * 64 >= (1ll << 31) || (long long)B * T * G * N >= (1ll << 31) ? WKV_ERR_DIMS : WKV_OK;
@@ -63,6 +63,7 @@ int check_scan_operands(int dtype, const wkv_rows *x, const wkv_rows *dt, const 
     for (const wkv_rows *r : {x, dt, z, b, c}) {
         if (r && !r->p) return WKV_ERR_NULL;
         if (r && !aligned_to(r->p, element(dtype))) return WKV_ERR_ALIGN;
+        if (r && (r->token < 0 || r->token >= scan::MAX_TOKEN_STRIDE)) return WKV_ERR_DIMS;
     }
     return WKV_OK;
 }

@@ -25,7 +25,7 @@ namespace scan {
 
 constexpr int TILE = 16;                    // tokens per tile = states per lane row
 constexpr int PITCH = TILE + 4;             // floats between two states' tokens in LDS: whole 16-byte pieces, every bank once
-constexpr int MAX_STATES = 64;
+constexpr int MAX_STATES = 64, MAX_TOKEN_STRIDE = 1 << 24;       // (a tile's tokens are addressed with 32-bit byte offsets)
 
 struct Rows {                               // (B, T, .) with a contiguous last dimension; strides in elements
     const void *p;
@@ -64,28 +64,46 @@ template <int I> __device__ __forceinline__ float row_lane(float x) {
 template <int CTRL> __device__ __forceinline__ float dpp(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
 }
-constexpr int ROR8 = 0x128, ROR4 = 0x124, ROR12 = 0x12c, SWAP2 = 0x4e, SWAP1 = 0xb1;      // row_ror:n, quad_perm [2,3,0,1], [1,0,3,2]
+// (a value the compiler does not connect with `v`: a broadcast of it is made where it is used and held in no register)
+__device__ __forceinline__ float again(float v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+constexpr int ROR8 = 0x128, ROR4 = 0x124, SWAP2 = 0x4e, SWAP1 = 0xb1;      // row_ror:n, quad_perm [2,3,0,1], [1,0,3,2]
 
-// v[i] of 16 lanes summed over the row, the sum of v[n] in lane n: each step adds two registers' halves into one
-__device__ __forceinline__ float reduce_row(float (&v)[TILE], int n) {
-    float a[8], b[4], c[2];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float lo = v[i] + dpp<ROR8>(v[i]), hi = v[i + 8] + dpp<ROR8>(v[i + 8]);
-        a[i] = n & 8 ? hi : lo;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const float lo = a[i] + dpp<ROR12>(a[i]), hi = a[i + 4] + dpp<ROR4>(a[i + 4]);      // (lanes of the other half of eight are not read)
-        b[i] = n & 4 ? hi : lo;
-    }
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const float lo = b[i] + dpp<SWAP2>(b[i]), hi = b[i + 2] + dpp<SWAP2>(b[i + 2]);
-        c[i] = n & 2 ? hi : lo;
-    }
-    const float lo = c[0] + dpp<SWAP1>(c[0]), hi = c[1] + dpp<SWAP1>(c[1]);
-    return n & 1 ? hi : lo;
+// v[i] of 16 lanes summed over the row, the sum of v[n] in lane n: each step adds two registers' halves into one.  A DPP's bank mask
+// writes a register's groups of four lanes one by one, so the steps of eight and four lanes need no selection: 33 instructions
+// instead of 45.  (Written out because the compiler selects; a register is not to be read by a DPP within two instructions of its
+// write, which the s_nop and the order see to.)
+__device__ __forceinline__ float reduce_row(float (&v)[TILE]) {
+#define WKV_HALVES(a, b, c, d, e, f, g, h)                                                                               \
+    asm("s_nop 1\n"                                                                                                      \
+        "v_add_f32_dpp %0, %0, %0 row_ror:8 row_mask:0xf bank_mask:0x3\nv_add_f32_dpp %0, %4, %4 row_ror:8 row_mask:0xf bank_mask:0xc\n" \
+        "v_add_f32_dpp %1, %1, %1 row_ror:8 row_mask:0xf bank_mask:0x3\nv_add_f32_dpp %1, %5, %5 row_ror:8 row_mask:0xf bank_mask:0xc\n" \
+        "v_add_f32_dpp %2, %2, %2 row_ror:8 row_mask:0xf bank_mask:0x3\nv_add_f32_dpp %2, %6, %6 row_ror:8 row_mask:0xf bank_mask:0xc\n" \
+        "v_add_f32_dpp %3, %3, %3 row_ror:8 row_mask:0xf bank_mask:0x3\nv_add_f32_dpp %3, %7, %7 row_ror:8 row_mask:0xf bank_mask:0xc"   \
+        : "+v"(a), "+v"(b), "+v"(c), "+v"(d) : "v"(e), "v"(f), "v"(g), "v"(h))
+    WKV_HALVES(v[0], v[1], v[2], v[3], v[8], v[9], v[10], v[11]);
+    WKV_HALVES(v[4], v[5], v[6], v[7], v[12], v[13], v[14], v[15]);
+#undef WKV_HALVES
+    const uint64_t m2 = 0xccccccccccccccccull, m1 = 0xaaaaaaaaaaaaaaaaull;      // the lanes whose token has the bit
+    asm("s_nop 1\n"
+        "v_add_f32_dpp %0, %0, %0 row_ror:12 row_mask:0xf bank_mask:0x5\nv_add_f32_dpp %0, %4, %4 row_ror:4 row_mask:0xf bank_mask:0xa\n"
+        "v_add_f32_dpp %1, %1, %1 row_ror:12 row_mask:0xf bank_mask:0x5\nv_add_f32_dpp %1, %5, %5 row_ror:4 row_mask:0xf bank_mask:0xa\n"
+        "v_add_f32_dpp %2, %2, %2 row_ror:12 row_mask:0xf bank_mask:0x5\nv_add_f32_dpp %2, %6, %6 row_ror:4 row_mask:0xf bank_mask:0xa\n"
+        "v_add_f32_dpp %3, %3, %3 row_ror:12 row_mask:0xf bank_mask:0x5\nv_add_f32_dpp %3, %7, %7 row_ror:4 row_mask:0xf bank_mask:0xa\n"
+        "v_add_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
+        "v_add_f32_dpp %2, %2, %2 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
+        "v_add_f32_dpp %1, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
+        "v_add_f32_dpp %3, %3, %3 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
+        "v_cndmask_b32_e64 %0, %0, %2, %8\n"
+        "v_cndmask_b32_e64 %1, %1, %3, %8\n"
+        "s_nop 1\n"
+        "v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
+        "v_add_f32_dpp %1, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
+        "v_cndmask_b32_e64 %0, %0, %1, %9"
+        : "+v"(v[0]), "+v"(v[1]), "+v"(v[2]), "+v"(v[3]) : "v"(v[4]), "v"(v[5]), "v"(v[6]), "v"(v[7]), "s"(m2), "s"(m1));
+    return v[0];
 }
 
 // v[i] summed over the wavefront's four rows: out[i] holds token i + 4 row, state n
@@ -103,11 +121,13 @@ __device__ __forceinline__ void reduce_rows(const float (&v)[TILE], float (&out)
     }
 }
 
-// log(1 + e^v), with the part of e that 1 + e rounds away
+// log(1 + e^v): e^v with what v log2(e) rounds away, the logarithm with what 1 + e^v does
 __device__ __forceinline__ float softplus(float v) {
-    const float e = expf(fminf(v, 20.f)), u = 1.f + e;
-    const float s = fmaf(__builtin_amdgcn_logf(u), LN2, (e - (u - 1.f)) * __builtin_amdgcn_rcpf(u));
-    return v > 20.f ? v : v != v ? v : s;
+    const float c = fminf(fmaxf(v, -100.f), 20.f), t = c * LOG2E, low = fmaf(c, 1.925963033e-8f, fmaf(c, LOG2E, -t));
+    float e = exp2_fast(t);
+    e = fmaf(e, low * LN2, e);
+    const float u = 1.f + e, s = fmaf(__builtin_amdgcn_logf(u), LN2, (e - (u - 1.f)) * __builtin_amdgcn_rcpf(u));
+    return v <= 20.f ? s : v;
 }
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * v)); }
 
@@ -118,15 +138,49 @@ __device__ __forceinline__ int xcd_order(int i, int n) {
     return i < each << 3 ? (i & 7) * each + (i >> 3) : i;
 }
 
+// Streams are read and written by buffer instructions from a base that moves on with the tile: a lane's offset is the same for every
+// tile, what is not there (past the sequence's end, past the channels) is at NOWHERE, read as zero and not written.  Without
+// branches around them the loads of the next tile can stay in flight over a tile, and no wait for them waits for a store.
+typedef __amdgpu_buffer_rsrc_t Buffer;
+constexpr unsigned NOWHERE = 0x80000000u;
+__device__ __forceinline__ Buffer buffer_at(const void *p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, (int)NOWHERE, 0x00027000);
+}
+template <class T> __device__ __forceinline__ float buffer_load(Buffer b, unsigned at) {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, (int)at, 0, 0));
+    else return to_float(__builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b16(b, (int)at, 0, 0)));
+}
+template <class T> __device__ __forceinline__ void buffer_store(Buffer b, unsigned at, float v) {
+    const T t = from_float<T>(v);
+    if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, t), b, (int)at, 0, 0);
+    else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t), b, (int)at, 0, 0);
+}
+
+// one operand or result of the tiles' tokens: where the tile at hand begins, and a lane's element from there
+template <class T> struct Stream {
+    const char *at;                // of the workgroup's channels
+    long long step;                // from a tile to the next
+    unsigned lane;
+    __device__ __forceinline__ Stream(const void *p, long long offset, long long token, int own, int n, int tile)
+        : at(static_cast<const char *>(p) + (offset + tile * TILE * token) * (long long)sizeof(T)), step(TILE * token * (long long)sizeof(T)),
+          lane((unsigned)((n * token + own) * sizeof(T))) {}
+    __device__ __forceinline__ float load(bool in) const { return buffer_load<T>(buffer_at(at), in ? lane : NOWHERE); }
+    __device__ __forceinline__ void store(bool in, float v) const { buffer_store<T>(buffer_at(at), in ? lane : NOWHERE, v); }
+    __device__ __forceinline__ void next() { at += step; }
+    __device__ __forceinline__ void back() { at -= step; }
+};
+
 // Where a workgroup is, and the B and C of its tiles on their way through LDS
-template <class T, int J, int WAVES, bool NEEDS_C>
+template <class T, int J, int WAVES, bool NEEDS_B, bool NEEDS_C>
 struct Work {
     static constexpr int THREADS = 64 * WAVES, CHANNELS = 4 * WAVES, STATES = 16 * J;
     static constexpr int PIECES = (TILE * STATES + THREADS - 1) / THREADS;
     const Call &k;
-    int tid, row, n, wave, b, g, ct, seg, channel, len, first, last;      // channel: within all D; first .. last: tiles
-    bool live;                                                             // the lane's channel exists
+    int tid, row, n, wave, own, b, g, ct, seg, channel, len, first, last, end;      // own: the channel within the workgroup's, channel: within all D
+    bool live;                                                                      // it exists
+    unsigned at_b[PIECES], at_c[PIECES];
     float pb[PIECES], pc[PIECES];
+    const char *from_b, *from_c;                // of the tile that fetch takes next
 
     __device__ __forceinline__ Work(const Call &k_) : k(k_) {
         tid = threadIdx.x;
@@ -136,16 +190,26 @@ struct Work {
         ct = i % cts; i /= cts;
         g = i % k.G; i /= k.G;
         b = i % k.B; seg = k.seg0 + i / k.B;
-        const int c = ct * CHANNELS + wave * 4 + row;
-        live = c < k.Dg;
-        channel = g * k.Dg + (live ? c : k.Dg - 1);
+        own = wave * 4 + row;
+        live = ct * CHANNELS + own < k.Dg;
+        channel = live ? base_channel() + own : 0;
         len = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
         first = seg * k.seg_tiles;
         last = min(first + k.seg_tiles, k.tiles);
+        end = max(first, min(last, (len + TILE - 1) / TILE));          // first .. end: tiles with tokens, end .. last: those without
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+            const int at = tid + p * THREADS, token = at / STATES, state = at % STATES;
+            const bool in = token < TILE && state < k.N;
+            at_b[p] = in ? (unsigned)((token * k.b.token + state) * sizeof(T)) : NOWHERE;
+            at_c[p] = in ? (unsigned)((token * k.c.token + state) * sizeof(T)) : NOWHERE;
+        }
     }
-    __device__ __forceinline__ float stream(const Rows &r, int t) const {
-        return t < len ? to_float(static_cast<const T *>(r.p)[b * r.batch + t * r.token + channel]) : 0.f;
-    }
+    __device__ __forceinline__ int base_channel() const { return g * k.Dg + ct * CHANNELS; }
+    __device__ __forceinline__ Stream<T> stream(const Rows &r, int tile) const { return Stream<T>(r.p, b * r.batch + base_channel(), r.token, own, n, tile); }
+    __device__ __forceinline__ Stream<T> packed(const void *p, int tile) const { return Stream<T>(p, (long long)b * k.T * k.D + base_channel(), k.D, own, n, tile); }
+    __device__ __forceinline__ bool in(int tile) const { return live && n < len - tile * TILE; }
+    __device__ __forceinline__ bool exists(int tile) const { return live && n < k.T - tile * TILE; }
     __device__ __forceinline__ float param(const float *p, float other) const { return p ? p[channel] : other; }
     __device__ __forceinline__ size_t state_at(int state) const { return ((size_t)b * k.D + channel) * k.N + state; }
     __device__ __forceinline__ void load_a(float (&a2)[J]) const {
@@ -161,23 +225,53 @@ struct Work {
         for (int j = 0; j < J; j++)
             if (live && n + 16 * j < k.N) s[state_at(n + 16 * j)] = h[j];
     }
-    __device__ __forceinline__ float *wide(float *s, size_t index) const { return s + (index * k.D + channel) * STATES + n; }
-    __device__ __forceinline__ void fetch(int tile) {
+    // (. , D, 16 J) arrays: the workgroup's first channel, and the lane's element from there
+    __device__ __forceinline__ Buffer wide(const float *s, size_t index) const { return buffer_at(s + (index * k.D + base_channel()) * STATES); }
+    __device__ __forceinline__ unsigned wide_lane() const { return live ? (unsigned)((own * STATES + n) * 4) : NOWHERE; }
+    __device__ __forceinline__ void load_wide(const float *s, size_t index, float (&h)[J]) const {
+        const Buffer from = wide(s, index);
+        const unsigned at = wide_lane();
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const int at = tid + i * THREADS, token = at / STATES, state = at % STATES, t = tile * TILE + token;
-            const bool in = (TILE * STATES % THREADS == 0 || token < TILE) && t < len && state < k.N && tile >= 0;
-            pb[i] = in ? to_float(static_cast<const T *>(k.b.p)[b * k.b.batch + t * k.b.token + g * k.b.group + state]) : 0.f;
-            if (NEEDS_C) pc[i] = in ? to_float(static_cast<const T *>(k.c.p)[b * k.c.batch + t * k.c.token + g * k.c.group + state]) : 0.f;
+        for (int j = 0; j < J; j++) h[j] = buffer_load<float>(from, at + 64 * j);
+    }
+    __device__ __forceinline__ void store_wide(float *s, size_t index, const float (&h)[J]) const {
+        const Buffer to = wide(s, index);
+        const unsigned at = wide_lane();
+#pragma unroll
+        for (int j = 0; j < J; j++) buffer_store<float>(to, at + 64 * j, h[j]);
+    }
+    // what the segments on one side make of an incoming state (or its gradient): v <- decay v + theirs
+    __device__ __forceinline__ void pass(int s, const float (&a2)[J], float (&v)[J]) const {
+        const size_t at = (size_t)b * k.segments + s;
+        const float dt = k.seg_dt[at * k.D + channel];
+        float theirs[J];
+        load_wide(k.seg_state, at, theirs);
+#pragma unroll
+        for (int j = 0; j < J; j++) v[j] = fmaf(exp2_fast(dt * a2[j]), v[j], theirs[j]);
+    }
+    __device__ __forceinline__ void from(int tile) {
+        from_b = static_cast<const char *>(k.b.p) + (b * k.b.batch + tile * TILE * k.b.token + g * k.b.group) * (long long)sizeof(T);
+        from_c = static_cast<const char *>(k.c.p) + (b * k.c.batch + tile * TILE * k.c.token + g * k.c.group) * (long long)sizeof(T);
+    }
+    // a tile's B and C, `step` tokens on from there next
+    __device__ __forceinline__ void fetch(int left, int step) {
+        const Buffer fb = buffer_at(from_b), fc = buffer_at(from_c);
+        from_b += step * k.b.token * (long long)sizeof(T);
+        from_c += step * k.c.token * (long long)sizeof(T);
+#pragma unroll
+        for (int p = 0; p < PIECES; p++) {
+            const bool there = (tid + p * THREADS) / STATES < left;
+            if (NEEDS_B) pb[p] = buffer_load<T>(fb, there ? at_b[p] : NOWHERE);
+            if (NEEDS_C) pc[p] = buffer_load<T>(fc, there ? at_c[p] : NOWHERE);
         }
     }
     __device__ __forceinline__ void stage(float *sb, float *sc) const {
 #pragma unroll
-        for (int i = 0; i < PIECES; i++) {
-            const int at = tid + i * THREADS, token = at / STATES, state = at % STATES;
+        for (int p = 0; p < PIECES; p++) {
+            const int at = tid + p * THREADS, token = at / STATES, state = at % STATES;
             if (TILE * STATES % THREADS == 0 || token < TILE) {
-                sb[state * PITCH + token] = pb[i];
-                if (NEEDS_C) sc[state * PITCH + token] = pc[i];
+                if (NEEDS_B) sb[state * PITCH + token] = pb[p];
+                if (NEEDS_C) sc[state * PITCH + token] = pc[p];
             }
         }
     }
@@ -200,216 +294,254 @@ __device__ __forceinline__ float row_sum(float v) {
 // OUT: the outputs of every token; without it a segment's summary (its state from nothing, its total step) alone
 template <class T, int J, bool OUT>
 __global__ __launch_bounds__(256) void forward(const Call k) {
-    typedef Work<T, J, 4, OUT> W;
+    typedef Work<T, J, 4, true, OUT> W;
     __shared__ __align__(16) float bc[2][OUT ? 2 : 1][W::STATES * PITCH];
     W w(k);
     float a2[J], h[J];
     w.load_a(a2);
     const float bias = w.param(k.bias, 0.f), skip = w.param(k.skip, 0.f);
+    const bool gated = OUT && k.z.p;
+    Stream<T> sx = w.stream(k.x, w.first), sdt = w.stream(k.dt, w.first), sz = w.stream(gated ? k.z : k.x, w.first), sy = w.packed(k.y, w.first);
     if (OUT) {
         w.load_state(k.state_in, h);
-        for (int s = 0; s < w.seg; s++) {          // what the segments before this one make of it
-            const size_t at = (size_t)w.b * k.segments + s;
-            const float dt = k.seg_dt[at * k.D + w.channel];
-#pragma unroll
-            for (int j = 0; j < J; j++) h[j] = fmaf(exp2_fast(dt * a2[j]), h[j], w.wide(k.seg_state, at)[16 * j]);
-        }
+        for (int s = 0; s < w.seg; s++) w.pass(s, a2, h);
     } else {
 #pragma unroll
         for (int j = 0; j < J; j++) h[j] = 0.f;
     }
-    float total = 0.f;
-    w.fetch(w.first);
-    int t = w.first * TILE + w.n;
-    float x = w.stream(k.x, t), raw = w.stream(k.dt, t), z = OUT && k.z.p ? w.stream(k.z, t) : 0.f;
-    for (int tile = w.first; tile < w.last; tile++) {
+    float total = 0.f, x, raw, z = 0.f;
+    auto fetch = [&](int tile) {
+        const bool in = w.in(tile);
+        w.fetch(w.len - tile * TILE, TILE);
+        x = sx.load(in);
+        raw = sdt.load(in);
+        if (gated) z = sz.load(in);
+        sx.next(); sdt.next(); sz.next();
+    };
+    w.from(w.first);
+    fetch(w.first);
+    for (int tile = w.first; tile < w.end; tile++) {
         float *sb = bc[tile & 1][0], *sc = bc[tile & 1][OUT ? 1 : 0];
         w.stage(sb, sc);
         lds_barrier();
-        const float xn = x, zn = z, dt = t < w.len ? softplus(raw + bias) : 0.f, dtx = dt * x;
-        const int tn = t;
-        t += TILE;
-        w.fetch(tile + 1);
-        x = w.stream(k.x, t); raw = w.stream(k.dt, t);
-        if (OUT && k.z.p) z = w.stream(k.z, t);
-        if (OUT && k.checkpoints && w.live) {
-            float *to = w.wide(k.checkpoints, (size_t)w.b * k.tiles + tile);
-#pragma unroll
-            for (int j = 0; j < J; j++) to[16 * j] = h[j];
-        }
+        const bool in = w.in(tile);
+        const float xn = x, zn = z, dt = in ? softplus(raw + bias) : 0.f, dtx = dt * x;
+        fetch(tile + 1);          // (past the end: nothing is there)
+        if (OUT && k.checkpoints) w.store_wide(k.checkpoints, (size_t)w.b * k.tiles + tile, h);
         float y[TILE];
 #pragma unroll
         for (int j = 0; j < J; j++) {
             float vb[TILE], vc[TILE];
             w.read(sb, j, vb);
             if (OUT) w.read(sc, j, vc);
+            const float dtj = again(dt), dtxj = again(dtx);
             unrolled<TILE>([&](auto i) {
                 constexpr int I = decltype(i)::value;
-                const float a = exp2_fast(row_lane<I>(dt) * a2[j]);
-                h[j] = fmaf(a, h[j], row_lane<I>(dtx) * vb[I]);
+                const float a = exp2_fast(row_lane<I>(dtj) * a2[j]);
+                h[j] = fmaf(a, h[j], row_lane<I>(dtxj) * vb[I]);
                 if (OUT) y[I] = j == 0 ? vc[I] * h[j] : fmaf(vc[I], h[j], y[I]);
             });
         }
         if (OUT) {
-            float out = fmaf(skip, xn, reduce_row(y, w.n));
-            if (k.z.p) out *= zn * sigmoid(zn);
-            if (w.live && tn < k.T) static_cast<T *>(k.y)[((size_t)w.b * k.T + tn) * k.D + w.channel] = from_float<T>(tn < w.len ? out : 0.f);
+            float out = fmaf(skip, xn, reduce_row(y));
+            if (gated) out *= zn * sigmoid(zn);
+            sy.store(w.exists(tile), in ? out : 0.f);
+            sy.next();
         } else {
             total += dt;
         }
     }
     if (OUT) {
+        for (int tile = w.end; tile < w.last; tile++, sy.next()) sy.store(w.exists(tile), 0.f);
         if (w.last == k.tiles) w.store_state(k.state_out, h);
-    } else if (w.live) {
+    } else {
         total = row_sum(total);
         const size_t at = (size_t)w.b * k.segments + w.seg;
-#pragma unroll
-        for (int j = 0; j < J; j++) w.wide(k.seg_state, at)[16 * j] = h[j];
-        if (w.n == 0) k.seg_dt[at * k.D + w.channel] = total;
+        w.store_wide(k.seg_state, at, h);
+        if (w.live && w.n == 0) k.seg_dt[at * k.D + w.channel] = total;
     }
 }
 
 // The state's gradient that a segment hands to the one before it if none comes in: the backward's summary
 template <class T, int J>
 __global__ __launch_bounds__(256) void backward_summary(const Call k) {
-    typedef Work<T, J, 4, true> W;
-    __shared__ __align__(16) float bc[2][2][W::STATES * PITCH];
+    typedef Work<T, J, 4, false, true> W;
+    __shared__ __align__(16) float cs[2][W::STATES * PITCH];
     W w(k);
     float a2[J], g[J];
     w.load_a(a2);
     const float bias = w.param(k.bias, 0.f);
+    const bool gated = k.z.p;
+    const int begin = max(w.end - 1, w.first);
+    Stream<T> sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin), sg = w.packed(k.gy, begin);
 #pragma unroll
     for (int j = 0; j < J; j++) g[j] = 0.f;
-    float total = 0.f;
-    for (int tile = w.last - 1; tile >= w.first; tile--) {
-        const int t = tile * TILE + w.n;
-        w.fetch(tile);
-        const float raw = w.stream(k.dt, t);
-        float gy = t < w.len ? to_float(static_cast<const T *>(k.gy)[((size_t)w.b * k.T + t) * k.D + w.channel]) : 0.f;
-        if (k.z.p) {
-            const float z = w.stream(k.z, t);
-            gy *= z * sigmoid(z);
-        }
-        float *sb = bc[tile & 1][0], *sc = bc[tile & 1][1];
-        w.stage(sb, sc);
+    float total = 0.f, raw, go, z = 0.f;
+    auto fetch = [&](int tile) {
+        const bool there = tile >= w.first, in = there && w.in(tile);
+        w.fetch(there ? w.len - tile * TILE : 0, -TILE);
+        raw = sdt.load(in);
+        go = sg.load(in);
+        if (gated) z = sz.load(in);
+        sdt.back(); sz.back(); sg.back();
+    };
+    w.from(begin);
+    fetch(w.end - 1);
+    for (int tile = w.end - 1; tile >= w.first; tile--) {
+        w.stage(nullptr, cs[tile & 1]);
         lds_barrier();
-        const float dt = t < w.len ? softplus(raw + bias) : 0.f;
+        const float dt = w.in(tile) ? softplus(raw + bias) : 0.f, gy = gated ? go * (z * sigmoid(z)) : go;
         total += dt;
+        fetch(tile - 1);
 #pragma unroll
         for (int j = 0; j < J; j++) {
             float vc[TILE];
-            w.read(sc, j, vc);
+            w.read(cs[tile & 1], j, vc);
+            const float dtj = again(dt), gyj = again(gy);
             unrolled<TILE>([&](auto i) {
                 constexpr int I = TILE - 1 - decltype(i)::value;
-                g[j] = fmaf(row_lane<I>(gy), vc[I], g[j]) * exp2_fast(row_lane<I>(dt) * a2[j]);
+                g[j] = fmaf(row_lane<I>(gyj), vc[I], g[j]) * exp2_fast(row_lane<I>(dtj) * a2[j]);
             });
         }
     }
-    if (w.live) {
-        total = row_sum(total);
-        const size_t at = (size_t)w.b * k.segments + w.seg;
-#pragma unroll
-        for (int j = 0; j < J; j++) w.wide(k.seg_state, at)[16 * j] = g[j];
-        if (w.n == 0) k.seg_dt[at * k.D + w.channel] = total;
-    }
+    total = row_sum(total);
+    const size_t at = (size_t)w.b * k.segments + w.seg;
+    w.store_wide(k.seg_state, at, g);
+    if (w.live && w.n == 0) k.seg_dt[at * k.D + w.channel] = total;
 }
 
 // Tiles from the last to the first.  Within a tile the state runs forward again from its checkpoint, leaving every token's decay a
-// and what is left of the state p in registers, then the gradient runs back over them.
+// and the state before it in registers, then the gradient runs back over them.  A tile's shares of gB and gC are added up over the
+// workgroup's channels in LDS after the next tile's barrier.
 constexpr int BACK_WAVES = 8;
 template <class T, int J>
-__global__ __launch_bounds__(64 * BACK_WAVES) void backward(const Call k) {
-    typedef Work<T, J, BACK_WAVES, true> W;
+__global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(const Call k) {
+    typedef Work<T, J, BACK_WAVES, true, true> W;
+    constexpr int TURNS = J == 1 ? 2 : 1;
     __shared__ __align__(16) float bc[2][2][W::STATES * PITCH];
-    __shared__ __align__(16) float part[BACK_WAVES][2][16 * PITCH];
+    __shared__ __align__(16) float part[TURNS][BACK_WAVES][2][16 * PITCH];
+    static_assert(W::THREADS == 512, "a thread per element of both sums");
     W w(k);
     float a2[J], g[J], ga[J];
     w.load_a(a2);
     w.load_state(k.gstate_out, g);
-    for (int s = k.segments - 1; s > w.seg; s--) {
-        const size_t at = (size_t)w.b * k.segments + s;
-        const float dt = k.seg_dt[at * k.D + w.channel];
-#pragma unroll
-        for (int j = 0; j < J; j++) g[j] = fmaf(exp2_fast(dt * a2[j]), g[j], w.wide(k.seg_state, at)[16 * j]);
-    }
+    for (int s = k.segments - 1; s > w.seg; s--) w.pass(s, a2, g);
 #pragma unroll
     for (int j = 0; j < J; j++) ga[j] = 0.f;
     const float bias = w.param(k.bias, 0.f), skip = w.param(k.skip, 0.f);
+    const bool gated = k.z.p;
     float gskip = 0.f, gbias = 0.f;
-    const T *gout = static_cast<const T *>(k.gy);
-    const size_t bt = (size_t)w.b * k.T;
-    for (int tile = w.last - 1; tile >= w.first; tile--) {
-        const int t = tile * TILE + w.n;
-        w.fetch(tile);
-        const float x = w.stream(k.x, t), raw = w.stream(k.dt, t) + bias, z = k.z.p ? w.stream(k.z, t) : 0.f;
-        const float go = t < w.len ? to_float(gout[(bt + t) * k.D + w.channel]) : 0.f;
-        float h0[J];
-        const float *from = w.wide(k.checkpoints, (size_t)w.b * k.tiles + tile);
+    const int begin = max(w.end - 1, w.first);
+    Stream<T> sx = w.stream(k.x, begin), sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin), sg = w.packed(k.gy, begin);
+    Stream<T> tx = w.packed(k.gx, w.last - 1), tdt = w.packed(k.gdt, w.last - 1), tz = w.packed(gated ? k.gz : k.gx, w.last - 1);
+    // this thread's element of the workgroup's gB or gC
+    const int which = w.tid >> 8, token = (w.tid >> 4) & 15, state = w.tid & 15;
+    float *vectors = (which ? k.gc_part : k.gb_part) + (((size_t)w.ct * k.B + w.b) * k.T * k.G + w.g) * k.N;
+    auto add_up = [&](const float (&p)[BACK_WAVES][2][16 * PITCH], int tile, int j) {
+        float s = 0.f;
 #pragma unroll
-        for (int j = 0; j < J; j++) h0[j] = from[16 * j];
+        for (int i = 0; i < BACK_WAVES; i++) s += p[i][which][state * PITCH + token];
+        const int t = tile * TILE + token;
+        if (t < k.T && state + 16 * j < k.N) vectors[(size_t)t * k.G * k.N + state + 16 * j] = s;
+    };
+    auto nothing = [&](int tile) {
+        const int t = tile * TILE + token;
+        for (int j = 0; j < J; j++)
+            if (t < k.T && state + 16 * j < k.N) vectors[(size_t)t * k.G * k.N + state + 16 * j] = 0.f;
+        const bool there = w.exists(tile);
+        tx.store(there, 0.f);
+        tdt.store(there, 0.f);
+        if (gated) tz.store(there, 0.f);
+        tx.back(); tdt.back(); tz.back();
+    };
+    for (int tile = w.last - 1; tile >= w.end; tile--) nothing(tile);
+    float x, raw, go, z = 0.f, h0[J];
+    auto fetch = [&](int tile) {
+        const bool there = tile >= w.first, in = there && w.in(tile);
+        w.fetch(there ? w.len - tile * TILE : 0, -TILE);
+        x = sx.load(in);
+        raw = sdt.load(in);
+        go = sg.load(in);
+        if (gated) z = sz.load(in);
+        w.load_wide(k.checkpoints, (size_t)w.b * k.tiles + max(tile, w.first), h0);
+        sx.back(); sdt.back(); sz.back(); sg.back();
+    };
+    w.from(begin);
+    fetch(w.end - 1);
+    for (int tile = w.end - 1; tile >= w.first; tile--) {
         float *sb = bc[tile & 1][0], *sc = bc[tile & 1][1];
         w.stage(sb, sc);
         lds_barrier();
-        const float dt = t < w.len ? softplus(raw) : 0.f, dtx = dt * x;
-        const float sig = k.z.p ? sigmoid(z) : 1.f, gate = k.z.p ? z * sig : 1.f, gy = go * gate;
-        float y[TILE], sx[TILE], sd[TILE];
+        const bool in = w.in(tile), there = w.exists(tile);
+        const float xn = x, rawn = raw + bias, gon = go, zn = z, dt = in ? softplus(rawn) : 0.f, dtx = dt * xn;
+        const float sig = gated ? sigmoid(zn) : 1.f, gate = gated ? zn * sig : 1.f, gy = gon * gate;
+        float hn[J];
+#pragma unroll
+        for (int j = 0; j < J; j++) hn[j] = h0[j];
+        fetch(tile - 1);
+        if (J == 1 && tile + 1 < w.end) add_up(part[(tile + 1) & 1], tile + 1, 0);
+        float y[TILE], sums[TILE], slopes[TILE], ysum = 0.f;
 #pragma unroll
         for (int j = 0; j < J; j++) {
-            float vb[TILE], vc[TILE], a[TILE], p[TILE], gb[TILE], gc[TILE];
-            w.read(sb, j, vb);
-            w.read(sc, j, vc);
-            float h = h0[j];
-            unrolled<TILE>([&](auto i) {
-                constexpr int I = decltype(i)::value;
-                a[I] = exp2_fast(row_lane<I>(dt) * a2[j]);
-                p[I] = a[I] * h;
-                h = fmaf(row_lane<I>(dtx), vb[I], p[I]);
-                y[I] = j == 0 ? vc[I] * h : fmaf(vc[I], h, y[I]);
-                gc[I] = row_lane<I>(gy) * h;
-            });
-            const float an = a2[j] * LN2;
-            unrolled<TILE>([&](auto i) {
-                constexpr int I = TILE - 1 - decltype(i)::value;
-                g[j] = fmaf(row_lane<I>(gy), vc[I], g[j]);
-                gb[I] = row_lane<I>(dtx) * g[j];
-                const float q = g[j] * p[I];
-                sx[I] = j == 0 ? g[j] * vb[I] : fmaf(g[j], vb[I], sx[I]);
-                sd[I] = j == 0 ? q * an : fmaf(q, an, sd[I]);
-                ga[j] = fmaf(row_lane<I>(dt), q, ga[j]);
-                g[j] *= a[I];
-            });
-            if (!w.live) {          // (its lanes repeat another channel)
-#pragma unroll
-                for (int i = 0; i < TILE; i++) gb[i] = gc[i] = 0.f;
+            float a[TILE], before[TILE];
+            float h = hn[j];
+            {
+                float vb[TILE], vc[TILE], gc[TILE], r[4];
+                w.read(sb, j, vb);
+                w.read(sc, j, vc);
+                const float gy1 = again(gy), dt1 = again(dt), dtx1 = again(dtx);
+                unrolled<TILE>([&](auto i) {
+                    constexpr int I = decltype(i)::value;
+                    before[I] = h;
+                    a[I] = exp2_fast(row_lane<I>(dt1) * a2[j]);
+                    h = fmaf(a[I], h, row_lane<I>(dtx1) * vb[I]);
+                    y[I] = j == 0 ? vc[I] * h : fmaf(vc[I], h, y[I]);
+                    gc[I] = row_lane<I>(gy1) * h;
+                });
+                reduce_rows(gc, r);
+                if (j) lds_barrier();
+                *reinterpret_cast<float4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][1][w.n * PITCH + 4 * w.row]) = make_float4(r[0], r[1], r[2], r[3]);
             }
-            float rb[4], rc[4];
-            reduce_rows(gb, rb);
-            reduce_rows(gc, rc);
-            if (j) lds_barrier();
-            *reinterpret_cast<float4 *>(&part[w.wave][0][w.n * PITCH + 4 * w.row]) = make_float4(rb[0], rb[1], rb[2], rb[3]);
-            *reinterpret_cast<float4 *>(&part[w.wave][1][w.n * PITCH + 4 * w.row]) = make_float4(rc[0], rc[1], rc[2], rc[3]);
-            lds_barrier();
-            static_assert(W::THREADS == 512, "a thread per element of both sums");
-            const int which = w.tid >> 8, token = (w.tid >> 4) & 15, state = w.tid & 15, tt = tile * TILE + token;
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < BACK_WAVES; i++) s += part[i][which][state * PITCH + token];
-            if (tt < k.T && state + 16 * j < k.N)
-                (which ? k.gc_part : k.gb_part)[((((size_t)w.ct * k.B + w.b) * k.T + tt) * k.G + w.g) * k.N + state + 16 * j] = s;
+            if (j == J - 1) ysum = reduce_row(y);
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                float vb[TILE], vc[TILE], gb[TILE], r[4];
+                w.read(sb, j, vb);
+                w.read(sc, j, vc);
+                const float an = a2[j] * LN2, gy2 = again(gy), dt2 = again(dt), dtx2 = again(dtx);
+                unrolled<TILE>([&](auto i) {
+                    constexpr int I = TILE - 1 - decltype(i)::value;
+                    g[j] = fmaf(row_lane<I>(gy2), vc[I], g[j]);
+                    gb[I] = row_lane<I>(dtx2) * g[j];
+                    sums[I] = j == 0 ? g[j] * vb[I] : fmaf(g[j], vb[I], sums[I]);
+                    g[j] *= a[I];
+                    const float q = g[j] * before[I];
+                    slopes[I] = j == 0 ? q * an : fmaf(q, an, slopes[I]);
+                    ga[j] = fmaf(row_lane<I>(dt2), q, ga[j]);
+                });
+                reduce_rows(gb, r);
+                *reinterpret_cast<float4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][0][w.n * PITCH + 4 * w.row]) = make_float4(r[0], r[1], r[2], r[3]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (J > 1) {
+                lds_barrier();
+                add_up(part[0], tile, j);
+            }
         }
-        const float ypre = fmaf(skip, x, reduce_row(y, w.n)), u = reduce_row(sx, w.n), d = reduce_row(sd, w.n);
-        const float graw = fmaf(u, x, d) * sigmoid(raw), gx = fmaf(u, dt, gy * skip);
-        if (t < w.len) {
-            gskip = fmaf(gy, x, gskip);
+        const float ypre = fmaf(skip, xn, ysum), u = reduce_row(sums), d = reduce_row(slopes);
+        const float graw = fmaf(u, xn, d) * sigmoid(rawn), gx = fmaf(u, dt, gy * skip);
+        if (in) {
+            gskip = fmaf(gy, xn, gskip);
             gbias += graw;
         }
-        if (w.live && t < k.T) {
-            const size_t at = (bt + t) * k.D + w.channel;
-            const bool in = t < w.len;
-            static_cast<T *>(k.gx)[at] = from_float<T>(in ? gx : 0.f);
-            static_cast<T *>(k.gdt)[at] = from_float<T>(in ? graw : 0.f);
-            if (k.z.p) static_cast<T *>(k.gz)[at] = from_float<T>(in ? go * ypre * (sig + gate * (1.f - sig)) : 0.f);
-        }
+        tx.store(there, in ? gx : 0.f);
+        tdt.store(there, in ? graw : 0.f);
+        if (gated) tz.store(there, in ? gon * ypre * (sig + gate * (1.f - sig)) : 0.f);
+        tx.back(); tdt.back(); tz.back();
+    }
+    if (J == 1 && w.end > w.first) {
+        lds_barrier();
+        add_up(part[w.first & 1], w.first, 0);
     }
     gskip = row_sum(gskip);
     gbias = row_sum(gbias);
