@@ -10,10 +10,14 @@
 //     gB = sum over channels of dt x g     gC = sum over channels of gy h     gA = sum over tokens of dt g p
 //
 // Layout.  A row of 16 lanes (the unit of a DPP) is one channel, its lanes are 16 states, and over a tile of 16 tokens
-// the same lanes are the tokens: a lane reads, converts and finishes one token's values, the recurrence takes them from
-// there by row broadcasts that ride on the multiplications, and the sums over the states come out one token per lane
-// (reduce_row).  So nothing of a token's own arithmetic is done twice, and there are as many wavefronts as a quarter of
-// the channels.  N above 16 takes J = 2 or 4 states per lane.  B[t] and C[t] go through LDS in fp32, [state][token].
+// the same lanes are the tokens: the recurrence takes a token's values from its lane by row broadcasts that ride on the
+// multiplications, and the sums over the states come out one token per lane (reduce_row).  So nothing of a token's own
+// arithmetic is done twice, and there are as many wavefronts as a quarter of the channels.  N above 16 takes J = 2 or 4
+// states per lane.  B[t] and C[t] go through LDS in fp32, [state][token].
+//
+// That arithmetic (softplus, gate, what leaves) is done in the order of memory instead, lane 4 token + channel, so that four neighbouring lanes
+// touch one line: in the order of the rows every lane of an access is an L1 access of its own, and those were what
+// bounded the forward.  to_rows and to_memory are the two permutations between the orders.
 //
 // What bounds it: the exponentials and fp32 multiply-adds, an exponential and four to five instructions per token, channel
 // and state, not the memory (which would take a third of the time).
@@ -61,15 +65,11 @@ template <int N, int I = 0, class F> __device__ __forceinline__ void unrolled(F 
 template <int I> __device__ __forceinline__ float row_lane(float x) {
     return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x150 + I, 0xf, 0xf, true));
 }
-template <int CTRL> __device__ __forceinline__ float dpp(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
-}
 // (a value the compiler does not connect with `v`: a broadcast of it is made where it is used and held in no register)
 __device__ __forceinline__ float again(float v) {
     asm volatile("" : "+v"(v));
     return v;
 }
-constexpr int ROR8 = 0x128, ROR4 = 0x124, SWAP2 = 0x4e, SWAP1 = 0xb1;      // row_ror:n, quad_perm [2,3,0,1], [1,0,3,2]
 
 // v[i] of 16 lanes summed over the row, the sum of v[n] in lane n: each step adds two registers' halves into one.  A DPP's bank mask
 // writes a register's groups of four lanes one by one, so the steps of eight and four lanes need no selection: 33 instructions
@@ -163,7 +163,7 @@ template <class T> struct Stream {
     unsigned lane;
     __device__ __forceinline__ Stream(const void *p, long long offset, long long token, int own, int n, int tile)
         : at(static_cast<const char *>(p) + (offset + tile * TILE * token) * (long long)sizeof(T)), step(TILE * token * (long long)sizeof(T)),
-          lane((unsigned)((n * token + own) * sizeof(T))) {}
+          lane((unsigned)((n * token + own) * sizeof(T))) {}          // n, own: the lane's token and channel
     __device__ __forceinline__ float load(bool in) const { return buffer_load<T>(buffer_at(at), in ? lane : NOWHERE); }
     __device__ __forceinline__ void store(bool in, float v) const { buffer_store<T>(buffer_at(at), in ? lane : NOWHERE, v); }
     __device__ __forceinline__ void next() { at += step; }
@@ -176,8 +176,10 @@ struct Work {
     static constexpr int THREADS = 64 * WAVES, CHANNELS = 4 * WAVES, STATES = 16 * J;
     static constexpr int PIECES = (TILE * STATES + THREADS - 1) / THREADS;
     const Call &k;
-    int tid, row, n, wave, own, b, g, ct, seg, channel, len, first, last, end;      // own: the channel within the workgroup's, channel: within all D
-    bool live;                                                                      // it exists
+    int tid, row, n, wave, own, b, g, ct, seg, channel, len, first, last, end;      // own: the row's channel within the workgroup's, channel: within all D
+    int token, other, mine;                                                         // in the order of memory: the lane's token, its channel likewise
+    bool live, mine_live;                                                           // they exist
+    int from_row, from_memory;
     unsigned at_b[PIECES], at_c[PIECES];
     float pb[PIECES], pc[PIECES];
     const char *from_b, *from_c;                // of the tile that fetch takes next
@@ -193,6 +195,12 @@ struct Work {
         own = wave * 4 + row;
         live = ct * CHANNELS + own < k.Dg;
         channel = live ? base_channel() + own : 0;
+        token = (tid & 63) >> 2;
+        other = wave * 4 + (tid & 3);
+        mine_live = ct * CHANNELS + other < k.Dg;
+        mine = mine_live ? base_channel() + other : 0;
+        from_memory = 4 * (n * 4 + row);
+        from_row = 4 * ((tid & 3) * 16 + token);
         len = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
         first = seg * k.seg_tiles;
         last = min(first + k.seg_tiles, k.tiles);
@@ -206,11 +214,13 @@ struct Work {
         }
     }
     __device__ __forceinline__ int base_channel() const { return g * k.Dg + ct * CHANNELS; }
-    __device__ __forceinline__ Stream<T> stream(const Rows &r, int tile) const { return Stream<T>(r.p, b * r.batch + base_channel(), r.token, own, n, tile); }
-    __device__ __forceinline__ Stream<T> packed(const void *p, int tile) const { return Stream<T>(p, (long long)b * k.T * k.D + base_channel(), k.D, own, n, tile); }
-    __device__ __forceinline__ bool in(int tile) const { return live && n < len - tile * TILE; }
-    __device__ __forceinline__ bool exists(int tile) const { return live && n < k.T - tile * TILE; }
-    __device__ __forceinline__ float param(const float *p, float other) const { return p ? p[channel] : other; }
+    __device__ __forceinline__ Stream<T> stream(const Rows &r, int tile) const { return Stream<T>(r.p, b * r.batch + base_channel(), r.token, other, token, tile); }
+    __device__ __forceinline__ Stream<T> packed(const void *p, int tile) const { return Stream<T>(p, (long long)b * k.T * k.D + base_channel(), k.D, other, token, tile); }
+    __device__ __forceinline__ bool in(int tile) const { return mine_live && token < len - tile * TILE; }
+    __device__ __forceinline__ bool exists(int tile) const { return mine_live && token < k.T - tile * TILE; }
+    __device__ __forceinline__ float param(const float *p) const { return p ? p[mine] : 0.f; }
+    __device__ __forceinline__ float to_rows(float v) const { return __int_as_float(__builtin_amdgcn_ds_bpermute(from_memory, __float_as_int(v))); }
+    __device__ __forceinline__ float to_memory(float v) const { return __int_as_float(__builtin_amdgcn_ds_bpermute(from_row, __float_as_int(v))); }
     __device__ __forceinline__ size_t state_at(int state) const { return ((size_t)b * k.D + channel) * k.N + state; }
     __device__ __forceinline__ void load_a(float (&a2)[J]) const {
 #pragma unroll
@@ -284,11 +294,11 @@ struct Work {
     }
 };
 
-__device__ __forceinline__ float row_sum(float v) {
-    v += dpp<ROR8>(v);
-    v += dpp<ROR4>(v);
-    v += dpp<SWAP2>(v);
-    return v + dpp<SWAP1>(v);
+// over a channel's lanes in the order of memory
+__device__ __forceinline__ float token_sum(float v) {
+#pragma unroll
+    for (int m = 4; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    return v;
 }
 
 // OUT: the outputs of every token; without it a segment's summary (its state from nothing, its total step) alone
@@ -299,7 +309,7 @@ __global__ __launch_bounds__(256) void forward(const Call k) {
     W w(k);
     float a2[J], h[J];
     w.load_a(a2);
-    const float bias = w.param(k.bias, 0.f), skip = w.param(k.skip, 0.f);
+    const float bias = w.param(k.bias), skip = w.param(k.skip);
     const bool gated = OUT && k.z.p;
     Stream<T> sx = w.stream(k.x, w.first), sdt = w.stream(k.dt, w.first), sz = w.stream(gated ? k.z : k.x, w.first), sy = w.packed(k.y, w.first);
     if (OUT) {
@@ -325,7 +335,7 @@ __global__ __launch_bounds__(256) void forward(const Call k) {
         w.stage(sb, sc);
         lds_barrier();
         const bool in = w.in(tile);
-        const float xn = x, zn = z, dt = in ? softplus(raw + bias) : 0.f, dtx = dt * x;
+        const float xn = x, zn = z, step = in ? softplus(raw + bias) : 0.f, dt = w.to_rows(step), dtx = w.to_rows(step * x);
         fetch(tile + 1);          // (past the end: nothing is there)
         if (OUT && k.checkpoints) w.store_wide(k.checkpoints, (size_t)w.b * k.tiles + tile, h);
         float y[TILE];
@@ -343,22 +353,22 @@ __global__ __launch_bounds__(256) void forward(const Call k) {
             });
         }
         if (OUT) {
-            float out = fmaf(skip, xn, reduce_row(y));
+            float out = fmaf(skip, xn, w.to_memory(reduce_row(y)));
             if (gated) out *= zn * sigmoid(zn);
             sy.store(w.exists(tile), in ? out : 0.f);
             sy.next();
         } else {
-            total += dt;
+            total += step;
         }
     }
     if (OUT) {
         for (int tile = w.end; tile < w.last; tile++, sy.next()) sy.store(w.exists(tile), 0.f);
         if (w.last == k.tiles) w.store_state(k.state_out, h);
     } else {
-        total = row_sum(total);
+        total = token_sum(total);
         const size_t at = (size_t)w.b * k.segments + w.seg;
         w.store_wide(k.seg_state, at, h);
-        if (w.live && w.n == 0) k.seg_dt[at * k.D + w.channel] = total;
+        if (w.mine_live && w.token == 0) k.seg_dt[at * k.D + w.mine] = total;
     }
 }
 
@@ -370,7 +380,7 @@ __global__ __launch_bounds__(256) void backward_summary(const Call k) {
     W w(k);
     float a2[J], g[J];
     w.load_a(a2);
-    const float bias = w.param(k.bias, 0.f);
+    const float bias = w.param(k.bias);
     const bool gated = k.z.p;
     const int begin = max(w.end - 1, w.first);
     Stream<T> sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin), sg = w.packed(k.gy, begin);
@@ -390,8 +400,8 @@ __global__ __launch_bounds__(256) void backward_summary(const Call k) {
     for (int tile = w.end - 1; tile >= w.first; tile--) {
         w.stage(nullptr, cs[tile & 1]);
         lds_barrier();
-        const float dt = w.in(tile) ? softplus(raw + bias) : 0.f, gy = gated ? go * (z * sigmoid(z)) : go;
-        total += dt;
+        const float step = w.in(tile) ? softplus(raw + bias) : 0.f, dt = w.to_rows(step), gy = w.to_rows(gated ? go * (z * sigmoid(z)) : go);
+        total += step;
         fetch(tile - 1);
 #pragma unroll
         for (int j = 0; j < J; j++) {
@@ -404,10 +414,10 @@ __global__ __launch_bounds__(256) void backward_summary(const Call k) {
             });
         }
     }
-    total = row_sum(total);
+    total = token_sum(total);
     const size_t at = (size_t)w.b * k.segments + w.seg;
     w.store_wide(k.seg_state, at, g);
-    if (w.live && w.n == 0) k.seg_dt[at * k.D + w.channel] = total;
+    if (w.mine_live && w.token == 0) k.seg_dt[at * k.D + w.mine] = total;
 }
 
 // Tiles from the last to the first.  Within a tile the state runs forward again from its checkpoint, leaving every token's decay a
@@ -428,7 +438,7 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
     for (int s = k.segments - 1; s > w.seg; s--) w.pass(s, a2, g);
 #pragma unroll
     for (int j = 0; j < J; j++) ga[j] = 0.f;
-    const float bias = w.param(k.bias, 0.f), skip = w.param(k.skip, 0.f);
+    const float bias = w.param(k.bias), skip = w.param(k.skip);
     const bool gated = k.z.p;
     float gskip = 0.f, gbias = 0.f;
     const int begin = max(w.end - 1, w.first);
@@ -473,8 +483,9 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
         w.stage(sb, sc);
         lds_barrier();
         const bool in = w.in(tile), there = w.exists(tile);
-        const float xn = x, rawn = raw + bias, gon = go, zn = z, dt = in ? softplus(rawn) : 0.f, dtx = dt * xn;
-        const float sig = gated ? sigmoid(zn) : 1.f, gate = gated ? zn * sig : 1.f, gy = gon * gate;
+        const float xn = x, rawn = raw + bias, gon = go, zn = z, step = in ? softplus(rawn) : 0.f;
+        const float sig = gated ? sigmoid(zn) : 1.f, gate = gated ? zn * sig : 1.f, gyn = gon * gate;
+        const float dt = w.to_rows(step), dtx = w.to_rows(step * xn), gy = w.to_rows(gyn);
         float hn[J];
 #pragma unroll
         for (int j = 0; j < J; j++) hn[j] = h0[j];
@@ -528,10 +539,10 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
                 add_up(part[0], tile, j);
             }
         }
-        const float ypre = fmaf(skip, xn, ysum), u = reduce_row(sums), d = reduce_row(slopes);
-        const float graw = fmaf(u, xn, d) * sigmoid(rawn), gx = fmaf(u, dt, gy * skip);
+        const float ypre = fmaf(skip, xn, w.to_memory(ysum)), u = w.to_memory(reduce_row(sums)), d = w.to_memory(reduce_row(slopes));
+        const float graw = fmaf(u, xn, d) * sigmoid(rawn), gx = fmaf(u, step, gyn * skip);
         if (in) {
-            gskip = fmaf(gy, xn, gskip);
+            gskip = fmaf(gyn, xn, gskip);
             gbias += graw;
         }
         tx.store(there, in ? gx : 0.f);
@@ -543,17 +554,16 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
         lds_barrier();
         add_up(part[w.first & 1], w.first, 0);
     }
-    gskip = row_sum(gskip);
-    gbias = row_sum(gbias);
-    if (w.live) {
-        const size_t at = ((size_t)w.b * k.segments + w.seg) * k.D + w.channel;
+    gskip = token_sum(gskip);
+    gbias = token_sum(gbias);
+    const size_t at = (size_t)w.b * k.segments + w.seg;
+    if (w.live)
 #pragma unroll
         for (int j = 0; j < J; j++)
-            if (w.n + 16 * j < k.N) k.ga_part[at * k.N + w.n + 16 * j] = ga[j];
-        if (w.n == 0) {
-            k.gskip_part[at] = gskip;
-            k.gbias_part[at] = gbias;
-        }
+            if (w.n + 16 * j < k.N) k.ga_part[(at * k.D + w.channel) * k.N + w.n + 16 * j] = ga[j];
+    if (w.mine_live && w.token == 0) {
+        k.gskip_part[at * k.D + w.mine] = gskip;
+        k.gbias_part[at * k.D + w.mine] = gbias;
     }
     if (k.gstate_in && w.seg == 0) w.store_state(k.gstate_in, g);
 }
