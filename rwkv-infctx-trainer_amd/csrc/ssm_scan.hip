@@ -106,9 +106,12 @@ __device__ __forceinline__ float reduce_row(float (&v)[TILE]) {
     return v[0];
 }
 
-// v[i] summed over the wavefront's four rows: out[i] holds token i + 4 row, state n
-__device__ __forceinline__ void reduce_rows(const float (&v)[TILE], float (&out)[4]) {
+// v[i] summed over the wavefront's four rows: out[i] holds token 4 row + i.  (As a matrix product with one-hot operands, which would take the
+// broadcast along, it cost more: an fp32 MFMA keeps the vector unit from issuing, 1600 us for the backward of B8 T2048 D4096 against 1250.)
+typedef float f4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f4 reduce_rows(const float (&v)[TILE]) {
     float a[8];
+    f4 out;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + 8]), false, false);
@@ -119,6 +122,12 @@ __device__ __forceinline__ void reduce_rows(const float (&v)[TILE], float (&out)
         const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[i]), __float_as_uint(a[i + 4]), false, false);
         out[i] = __uint_as_float(s[0]) + __uint_as_float(s[1]);
     }
+    return out;
+}
+// v += (lane I of every row of w) u.  (The compiler makes the broadcast a move of its own here.  The s_nop: a register is not to be read by a DPP
+// within two instructions of its write.)
+template <int I> __device__ __forceinline__ void add_lane(float &v, float w, float u) {
+    asm("s_nop 1\nv_fmac_f32_dpp %0, %1, %2 row_newbcast:%3 row_mask:0xf bank_mask:0xf" : "+v"(v) : "v"(w), "v"(u), "n"(I));
 }
 
 // log(1 + e^v): e^v with what v log2(e) rounds away, the logarithm with what 1 + e^v does
@@ -156,16 +165,27 @@ template <class T> __device__ __forceinline__ void buffer_store(Buffer b, unsign
     else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, t), b, (int)at, 0, 0);
 }
 
-// one operand or result of the tiles' tokens: where the tile at hand begins, and a lane's element from there
+// an operand with strides: where the tile at hand begins, and a lane's element from there
 template <class T> struct Stream {
     const char *at;                // of the workgroup's channels
-    long long step;                // from a tile to the next
+    int step;                      // from a tile to the next (below 2^31 by MAX_TOKEN_STRIDE)
     unsigned lane;
-    __device__ __forceinline__ Stream(const void *p, long long offset, long long token, int own, int n, int tile)
-        : at(static_cast<const char *>(p) + (offset + tile * TILE * token) * (long long)sizeof(T)), step(TILE * token * (long long)sizeof(T)),
-          lane((unsigned)((n * token + own) * sizeof(T))) {}          // n, own: the lane's token and channel
+    __device__ __forceinline__ Stream(const void *p, long long offset, long long token, int own, int n, int tile)          // n, own: the lane's token and channel
+        : at(static_cast<const char *>(p) + (offset + tile * TILE * token) * (long long)sizeof(T)), step((int)(TILE * token * (long long)sizeof(T))),
+          lane((unsigned)((n * token + own) * sizeof(T))) {}
     __device__ __forceinline__ float load(bool in) const { return buffer_load<T>(buffer_at(at), in ? lane : NOWHERE); }
-    __device__ __forceinline__ void store(bool in, float v) const { buffer_store<T>(buffer_at(at), in ? lane : NOWHERE, v); }
+    __device__ __forceinline__ void next() { at += step; }
+    __device__ __forceinline__ void back() { at -= step; }
+};
+// the same of all contiguous (B, T, D) operands and results
+template <class T> struct Packed {
+    long long at;
+    int step;
+    unsigned lane;
+    __device__ __forceinline__ Packed(long long offset, int D, int own, int n, int tile)
+        : at((offset + (long long)tile * TILE * D) * (long long)sizeof(T)), step(TILE * D * (int)sizeof(T)), lane((unsigned)((n * D + own) * sizeof(T))) {}
+    __device__ __forceinline__ float load(const void *p, bool in) const { return buffer_load<T>(buffer_at(static_cast<const char *>(p) + at), in ? lane : NOWHERE); }
+    __device__ __forceinline__ void store(void *p, bool in, float v) const { buffer_store<T>(buffer_at(static_cast<char *>(p) + at), in ? lane : NOWHERE, v); }
     __device__ __forceinline__ void next() { at += step; }
     __device__ __forceinline__ void back() { at -= step; }
 };
@@ -215,7 +235,7 @@ struct Work {
     }
     __device__ __forceinline__ int base_channel() const { return g * k.Dg + ct * CHANNELS; }
     __device__ __forceinline__ Stream<T> stream(const Rows &r, int tile) const { return Stream<T>(r.p, b * r.batch + base_channel(), r.token, other, token, tile); }
-    __device__ __forceinline__ Stream<T> packed(const void *p, int tile) const { return Stream<T>(p, (long long)b * k.T * k.D + base_channel(), k.D, other, token, tile); }
+    __device__ __forceinline__ Packed<T> packed(int tile) const { return Packed<T>((long long)b * k.T * k.D + base_channel(), k.D, other, token, tile); }
     __device__ __forceinline__ bool in(int tile) const { return mine_live && token < len - tile * TILE; }
     __device__ __forceinline__ bool exists(int tile) const { return mine_live && token < k.T - tile * TILE; }
     __device__ __forceinline__ float param(const float *p) const { return p ? p[mine] : 0.f; }
@@ -303,7 +323,7 @@ __device__ __forceinline__ float token_sum(float v) {
 
 // OUT: the outputs of every token; without it a segment's summary (its state from nothing, its total step) alone
 template <class T, int J, bool OUT>
-__global__ __launch_bounds__(256) void forward(const Call k) {
+__global__ __launch_bounds__(256, J == 1 ? 8 : 4) void forward(const Call k) {
     typedef Work<T, J, 4, true, OUT> W;
     __shared__ __align__(16) float bc[2][OUT ? 2 : 1][W::STATES * PITCH];
     W w(k);
@@ -311,7 +331,8 @@ __global__ __launch_bounds__(256) void forward(const Call k) {
     w.load_a(a2);
     const float bias = w.param(k.bias), skip = w.param(k.skip);
     const bool gated = OUT && k.z.p;
-    Stream<T> sx = w.stream(k.x, w.first), sdt = w.stream(k.dt, w.first), sz = w.stream(gated ? k.z : k.x, w.first), sy = w.packed(k.y, w.first);
+    Stream<T> sx = w.stream(k.x, w.first), sdt = w.stream(k.dt, w.first), sz = w.stream(gated ? k.z : k.x, w.first);
+    Packed<T> out_at = w.packed(w.first);
     if (OUT) {
         w.load_state(k.state_in, h);
         for (int s = 0; s < w.seg; s++) w.pass(s, a2, h);
@@ -355,14 +376,14 @@ __global__ __launch_bounds__(256) void forward(const Call k) {
         if (OUT) {
             float out = fmaf(skip, xn, w.to_memory(reduce_row(y)));
             if (gated) out *= zn * sigmoid(zn);
-            sy.store(w.exists(tile), in ? out : 0.f);
-            sy.next();
+            out_at.store(k.y, w.exists(tile), in ? out : 0.f);
+            out_at.next();
         } else {
             total += step;
         }
     }
     if (OUT) {
-        for (int tile = w.end; tile < w.last; tile++, sy.next()) sy.store(w.exists(tile), 0.f);
+        for (int tile = w.end; tile < w.last; tile++, out_at.next()) out_at.store(k.y, w.exists(tile), 0.f);
         if (w.last == k.tiles) w.store_state(k.state_out, h);
     } else {
         total = token_sum(total);
@@ -383,7 +404,8 @@ __global__ __launch_bounds__(256) void backward_summary(const Call k) {
     const float bias = w.param(k.bias);
     const bool gated = k.z.p;
     const int begin = max(w.end - 1, w.first);
-    Stream<T> sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin), sg = w.packed(k.gy, begin);
+    Stream<T> sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin);
+    Packed<T> in_at = w.packed(begin);
 #pragma unroll
     for (int j = 0; j < J; j++) g[j] = 0.f;
     float total = 0.f, raw, go, z = 0.f;
@@ -391,9 +413,9 @@ __global__ __launch_bounds__(256) void backward_summary(const Call k) {
         const bool there = tile >= w.first, in = there && w.in(tile);
         w.fetch(there ? w.len - tile * TILE : 0, -TILE);
         raw = sdt.load(in);
-        go = sg.load(in);
+        go = in_at.load(k.gy, in);
         if (gated) z = sz.load(in);
-        sdt.back(); sz.back(); sg.back();
+        sdt.back(); sz.back(); in_at.back();
     };
     w.from(begin);
     fetch(w.end - 1);
@@ -442,8 +464,8 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
     const bool gated = k.z.p;
     float gskip = 0.f, gbias = 0.f;
     const int begin = max(w.end - 1, w.first);
-    Stream<T> sx = w.stream(k.x, begin), sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin), sg = w.packed(k.gy, begin);
-    Stream<T> tx = w.packed(k.gx, w.last - 1), tdt = w.packed(k.gdt, w.last - 1), tz = w.packed(gated ? k.gz : k.gx, w.last - 1);
+    Stream<T> sx = w.stream(k.x, begin), sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin);
+    Packed<T> in_at = w.packed(begin), out_at = w.packed(w.last - 1);
     // this thread's element of the workgroup's gB or gC
     const int which = w.tid >> 8, token = (w.tid >> 4) & 15, state = w.tid & 15;
     float *vectors = (which ? k.gc_part : k.gb_part) + (((size_t)w.ct * k.B + w.b) * k.T * k.G + w.g) * k.N;
@@ -459,10 +481,10 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
         for (int j = 0; j < J; j++)
             if (t < k.T && state + 16 * j < k.N) vectors[(size_t)t * k.G * k.N + state + 16 * j] = 0.f;
         const bool there = w.exists(tile);
-        tx.store(there, 0.f);
-        tdt.store(there, 0.f);
-        if (gated) tz.store(there, 0.f);
-        tx.back(); tdt.back(); tz.back();
+        out_at.store(k.gx, there, 0.f);
+        out_at.store(k.gdt, there, 0.f);
+        if (gated) out_at.store(k.gz, there, 0.f);
+        out_at.back();
     };
     for (int tile = w.last - 1; tile >= w.end; tile--) nothing(tile);
     float x, raw, go, z = 0.f, h0[J];
@@ -471,10 +493,10 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
         w.fetch(there ? w.len - tile * TILE : 0, -TILE);
         x = sx.load(in);
         raw = sdt.load(in);
-        go = sg.load(in);
+        go = in_at.load(k.gy, in);
         if (gated) z = sz.load(in);
         w.load_wide(k.checkpoints, (size_t)w.b * k.tiles + max(tile, w.first), h0);
-        sx.back(); sdt.back(); sz.back(); sg.back();
+        sx.back(); sdt.back(); sz.back(); in_at.back();
     };
     w.from(begin);
     fetch(w.end - 1);
@@ -497,41 +519,41 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
             float a[TILE], before[TILE];
             float h = hn[j];
             {
-                float vb[TILE], vc[TILE], gc[TILE], r[4];
+                float vb[TILE], vc[TILE];
                 w.read(sb, j, vb);
                 w.read(sc, j, vc);
-                const float gy1 = again(gy), dt1 = again(dt), dtx1 = again(dtx);
+                float gc[TILE];
+                const float dt1 = again(dt), dtx1 = again(dtx);
                 unrolled<TILE>([&](auto i) {
                     constexpr int I = decltype(i)::value;
                     before[I] = h;
                     a[I] = exp2_fast(row_lane<I>(dt1) * a2[j]);
                     h = fmaf(a[I], h, row_lane<I>(dtx1) * vb[I]);
                     y[I] = j == 0 ? vc[I] * h : fmaf(vc[I], h, y[I]);
-                    gc[I] = row_lane<I>(gy1) * h;
+                    gc[I] = row_lane<I>(gy) * h;
                 });
-                reduce_rows(gc, r);
                 if (j) lds_barrier();
-                *reinterpret_cast<float4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][1][w.n * PITCH + 4 * w.row]) = make_float4(r[0], r[1], r[2], r[3]);
+                *reinterpret_cast<f4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][1][w.n * PITCH + 4 * w.row]) = reduce_rows(gc);
             }
             if (j == J - 1) ysum = reduce_row(y);
             __builtin_amdgcn_sched_barrier(0);
             {
-                float vb[TILE], vc[TILE], gb[TILE], r[4];
+                float vb[TILE], vc[TILE];
                 w.read(sb, j, vb);
                 w.read(sc, j, vc);
-                const float an = a2[j] * LN2, gy2 = again(gy), dt2 = again(dt), dtx2 = again(dtx);
+                float gb[TILE];
+                const float an = a2[j] * LN2, dtx2 = again(dtx);
                 unrolled<TILE>([&](auto i) {
                     constexpr int I = TILE - 1 - decltype(i)::value;
-                    g[j] = fmaf(row_lane<I>(gy2), vc[I], g[j]);
+                    add_lane<I>(g[j], gy, vc[I]);
                     gb[I] = row_lane<I>(dtx2) * g[j];
                     sums[I] = j == 0 ? g[j] * vb[I] : fmaf(g[j], vb[I], sums[I]);
                     g[j] *= a[I];
                     const float q = g[j] * before[I];
                     slopes[I] = j == 0 ? q * an : fmaf(q, an, slopes[I]);
-                    ga[j] = fmaf(row_lane<I>(dt2), q, ga[j]);
+                    add_lane<I>(ga[j], dt, q);
                 });
-                reduce_rows(gb, r);
-                *reinterpret_cast<float4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][0][w.n * PITCH + 4 * w.row]) = make_float4(r[0], r[1], r[2], r[3]);
+                *reinterpret_cast<f4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][0][w.n * PITCH + 4 * w.row]) = reduce_rows(gb);
             }
             __builtin_amdgcn_sched_barrier(0);
             if (J > 1) {
@@ -545,10 +567,10 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
             gskip = fmaf(gyn, xn, gskip);
             gbias += graw;
         }
-        tx.store(there, in ? gx : 0.f);
-        tdt.store(there, in ? graw : 0.f);
-        if (gated) tz.store(there, in ? gon * ypre * (sig + gate * (1.f - sig)) : 0.f);
-        tx.back(); tdt.back(); tz.back();
+        out_at.store(k.gx, there, in ? gx : 0.f);
+        out_at.store(k.gdt, there, in ? graw : 0.f);
+        if (gated) out_at.store(k.gz, there, in ? gon * ypre * (sig + gate * (1.f - sig)) : 0.f);
+        out_at.back();
     }
     if (J == 1 && w.end > w.first) {
         lds_barrier();
