@@ -44,10 +44,10 @@ conv::Call conv_call(int B, int T, int D, int param_dtype, int silu, const wkv_r
     k.weight = weight; k.bias = bias; k.state_in = state_in; k.lengths = lengths;
     return k;
 }
-// whether a lane may take 16 bytes of channels at once
+// whether a lane may take four channels at once
 bool conv_wide(const wkv_rows *x, int D, int dtype) {
-    const int v = conv::vector_of(dtype, D);
-    return v > 1 && aligned16(x->p) && x->batch % v == 0 && x->token % v == 0;
+    const int v = conv::vector_of(D);
+    return v > 1 && aligned_to(x->p, v * element(dtype)) && x->batch % v == 0 && x->token % v == 0;
 }
 
 // ---- scan
@@ -109,7 +109,7 @@ int wkv_causal_conv_forward(void *stream, int B, int T, int D, int W, int dtype,
 }
 
 size_t wkv_causal_conv_backward_workspace(int B, int T, int D, int W, int dtype) {
-    return check_conv(B, T, D, W, dtype, WKV_F32) ? 0 : conv::backward_scratch(B, T, D, W, dtype);
+    return check_conv(B, T, D, W, dtype, WKV_F32) ? 0 : conv::backward_scratch(B, T, D, W);
 }
 
 int wkv_causal_conv_backward(void *stream, int B, int T, int D, int W, int dtype, int param_dtype, int silu, const wkv_rows *x, const void *weight,
@@ -121,7 +121,7 @@ int wkv_causal_conv_backward(void *stream, int B, int T, int D, int W, int dtype
                           (const void *)workspace})
         if (!aligned16(p)) return WKV_ERR_ALIGN;
     if (!aligned_to(x->p, element(dtype))) return WKV_ERR_ALIGN;
-    if (workspace_bytes < conv::backward_scratch(B, T, D, W, dtype)) return WKV_ERR_WORKSPACE;
+    if (workspace_bytes < conv::backward_scratch(B, T, D, W)) return WKV_ERR_WORKSPACE;
     if (overlaps(gstate_out, gstate_in, (size_t)B * (W - 1) * D * element(dtype))) return WKV_ERR_ALIAS;
     conv::Call k = conv_call(B, T, D, param_dtype, silu, x, weight, bias, state_in, lengths);
     k.gy = gy; k.gstate_out = gstate_out; k.gx = gx; k.gstate_in = gstate_in;

@@ -5,7 +5,7 @@
 // where xx continues x to the left by the state, the W-1 inputs before it; the last W-1 of xx are the new state.  Backwards, with
 // gp[t] = gy[t] silu'(pre[t]):   gx[s] = sum over k of w[k] gp[s + W-1 - k],   gw[k] = sum over t of gp[t] xx[t - (W-1) + k].
 //
-// Bound by memory: each input is to be read once and each output written once.  A lane holds 16 bytes of channels and walks
+// Bound by memory: each input is to be read once and each output written once.  A lane holds four channels and walks
 // a run of tokens with the window in registers; the W-1 inputs (backwards also the W-1 gp) on a run's edge are read again, from
 // the cache.  The filter's gradient is summed along the run in registers, over the workgroup's four runs in LDS, and over
 // the workgroups by sum_rows.
@@ -16,7 +16,7 @@
 namespace wkv {
 namespace conv {
 
-constexpr int MIN_TAPS = 2, MAX_TAPS = 4, RUNS = 4;         // runs per workgroup: one per wavefront
+constexpr int MIN_TAPS = 2, MAX_TAPS = 4, RUNS = 4, WIDE = 4;         // runs per workgroup: one per wavefront
 
 struct Call {
     int B, T, D, run;                         // run: tokens per lane
@@ -87,7 +87,7 @@ template <int W, int V> __device__ __forceinline__ void push(float (&win)[W][V],
 constexpr int AHEAD = 4;                      // tokens asked for together
 template <class T, int W, int V>
 __global__ __launch_bounds__(64 * RUNS) void forward(const Call k) {
-    const int run_index = blockIdx.y * RUNS + (threadIdx.x >> 6);
+    const int run_index = blockIdx.y * RUNS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);          // (the same for a wavefront: its tokens are scalars)
     Lane<T, W, V> l(k, run_index);
     if (!l.live) return;
     float win[W][V];
@@ -126,7 +126,7 @@ __global__ __launch_bounds__(64 * RUNS) void forward(const Call k) {
 template <class T, int W, int V>
 __global__ __launch_bounds__(64 * RUNS) void backward(const Call k) {
     __shared__ float sums[RUNS][64 * V];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, run_index = blockIdx.y * RUNS + wave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, run_index = blockIdx.y * RUNS + wave;
     Lane<T, W, V> l(k, run_index);
     float gw[W][V], gb[V];
 #pragma unroll
@@ -226,11 +226,11 @@ static inline int run_for(int B, int T, int D, int V) {
     return run;
 }
 static inline int run_groups(int T, int run) { return (T + RUNS * run - 1) / (RUNS * run); }
-static inline int vector_of(int dtype, int D) { return D % (dtype == 0 ? 4 : 8) == 0 ? (dtype == 0 ? 4 : 8) : 1; }
+static inline int vector_of(int D) { return D % WIDE == 0 ? WIDE : 1; }
 // (the largest of what the two widths of a lane need: which one a call takes depends on its pointers)
-static inline size_t backward_scratch(int B, int T, int D, int W, int dtype) {
+static inline size_t backward_scratch(int B, int T, int D, int W) {
     size_t n = 0;
-    for (int V : {1, vector_of(dtype, D)}) n = std::max(n, (size_t)B * run_groups(T, run_for(B, T, D, V)));
+    for (int V : {1, vector_of(D)}) n = std::max(n, (size_t)B * run_groups(T, run_for(B, T, D, V)));
     return n * (W + 1) * D * 4;
 }
 
@@ -247,12 +247,12 @@ template <class T, int V, bool BACK> static hipError_t launch(hipStream_t s, int
     return hipGetLastError();
 }
 template <class T> static hipError_t forward_t(hipStream_t s, int W, const Call &k, bool wide) {
-    return wide ? launch<T, 16 / sizeof(T), false>(s, W, k) : launch<T, 1, false>(s, W, k);
+    return wide ? launch<T, WIDE, false>(s, W, k) : launch<T, 1, false>(s, W, k);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, int W, const Call &k, bool wide, void *gweight, void *gbias) {
-    const hipError_t e = wide ? launch<T, 16 / sizeof(T), true>(s, W, k) : launch<T, 1, true>(s, W, k);
+    const hipError_t e = wide ? launch<T, WIDE, true>(s, W, k) : launch<T, 1, true>(s, W, k);
     if (e != hipSuccess) return e;
-    const int rows = k.B * run_groups(k.T, run_for(k.B, k.T, k.D, wide ? 16 / (int)sizeof(T) : 1));
+    const int rows = k.B * run_groups(k.T, run_for(k.B, k.T, k.D, wide ? WIDE : 1));
     const size_t n = (size_t)(W + 1) * k.D;
     if (k.w32) sum_rows_launch(s, rows, n, k.part, ToFilter<float>{static_cast<float *>(gweight), static_cast<float *>(gbias), W, k.D});
     else sum_rows_launch(s, rows, n, k.part, ToFilter<T>{static_cast<T *>(gweight), static_cast<T *>(gbias), W, k.D});

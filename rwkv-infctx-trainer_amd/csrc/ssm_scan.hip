@@ -107,7 +107,7 @@ __device__ __forceinline__ float reduce_row(float (&v)[TILE]) {
 }
 
 // v[i] summed over the wavefront's four rows: out[i] holds token 4 row + i.  (As a matrix product with one-hot operands, which would take the
-// broadcast along, it cost more: an fp32 MFMA keeps the vector unit from issuing, 1600 us for the backward of B8 T2048 D4096 against 1250.)
+// broadcast along, it cost more: an fp32 MFMA keeps the vector unit from issuing, 1602 us for the backward of B8 T2048 D4096 against 1203.)
 typedef float f4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ f4 reduce_rows(const float (&v)[TILE]) {
     float a[8];
