@@ -11,7 +11,6 @@
 // the workgroups by sum_rows.
 #include "common.h"
 #include "row_sums.h"
-#include "vec.h"
 
 namespace wkv {
 namespace conv {
@@ -30,21 +29,65 @@ struct Call {
     float *part;                              // (workgroups per channel, W + 1, D)
 };
 
-template <class T, int V> __device__ __forceinline__ void zero(float (&o)[V]) {
+template <int V> __device__ __forceinline__ void zero(float (&o)[V]) {
 #pragma unroll
     for (int i = 0; i < V; i++) o[i] = 0.f;
 }
 
+// A row's V elements of one lane as they lie in memory, read and written by buffer instructions whose range is a scalar: of a row that is not there it
+// is nothing, which reads as zero and is not written.  So no branch stands between a load and its use a group of tokens later.
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+template <int BYTES> struct RawOf;
+template <> struct RawOf<2> { typedef unsigned short type; };
+template <> struct RawOf<4> { typedef unsigned type; };
+template <> struct RawOf<8> { typedef u2 type; };
+template <> struct RawOf<16> { typedef u4 type; };
+template <class T, int V> struct Row {
+    typedef typename RawOf<V * sizeof(T)>::type Raw;
+    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void *p, bool there) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, there ? (int)0x80000000u : 0, 0x00027000);
+    }
+    static __device__ __forceinline__ Raw load(const T *p, bool there, int at) {
+        const __amdgpu_buffer_rsrc_t b = range(p, there);
+        if constexpr (sizeof(Raw) == 2) return __builtin_amdgcn_raw_buffer_load_b16(b, at, 0, 0);
+        else if constexpr (sizeof(Raw) == 4) return __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
+        else if constexpr (sizeof(Raw) == 8) return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0));
+        else return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
+    }
+    static __device__ __forceinline__ void store(T *p, bool there, int at, const float (&v)[V]) {
+        T e[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) e[i] = from_float<T>(v[i]);
+        Raw raw;
+        __builtin_memcpy(&raw, e, sizeof(raw));
+        const __amdgpu_buffer_rsrc_t b = range(p, there);
+        if constexpr (sizeof(Raw) == 2) __builtin_amdgcn_raw_buffer_store_b16(raw, b, at, 0, 0);
+        else if constexpr (sizeof(Raw) == 4) __builtin_amdgcn_raw_buffer_store_b32(raw, b, at, 0, 0);
+        else if constexpr (sizeof(Raw) == 8) __builtin_amdgcn_raw_buffer_store_b64(raw, b, at, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b128(raw, b, at, 0, 0);
+    }
+    static __device__ __forceinline__ void floats(const Raw &raw, float (&o)[V]) {
+        T e[V];
+        __builtin_memcpy(e, &raw, sizeof(raw));
+#pragma unroll
+        for (int i = 0; i < V; i++) o[i] = to_float(e[i]);
+    }
+};
+
 // one lane's channels of one sequence
 template <class T, int W, int V> struct Lane {
+    typedef Row<T, V> R;
+    typedef typename R::Raw Raw;
     const Call &k;
-    int b, d, run0, len;           // run0: the run's first token
+    int b, d, at, run0, len;           // at: d in bytes; run0: the run's first token
     bool live;
     float w[W][V], bias[V];
 
     __device__ __forceinline__ Lane(const Call &k_, int run_index) : k(k_) {
         b = blockIdx.z;
         d = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
+        at = d * (int)sizeof(T);
         live = d < k.D && (long long)run_index * k.run < k.T;
         run0 = run_index * k.run;
         len = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
@@ -60,12 +103,12 @@ template <class T, int W, int V> struct Lane {
         return k.w32 ? static_cast<const float *>(p)[i] : to_float(static_cast<const T *>(p)[i]);
     }
     // xx[t]: the state's tokens are -(W-1) .. -1; nothing from the length on
-    __device__ __forceinline__ void input(int t, float (&o)[V]) const {
-        if (t >= len) zero<T>(o);
-        else if (t >= 0) load_vec(static_cast<const T *>(k.x) + b * k.batch + t * k.token + d, o);
-        else if (k.state_in) load_vec(static_cast<const T *>(k.state_in) + ((size_t)b * (W - 1) + t + W - 1) * k.D + d, o);
-        else zero<T>(o);
+    __device__ __forceinline__ Raw input(int t) const {
+        const T *x = static_cast<const T *>(k.x) + b * k.batch + t * k.token;
+        const T *state = static_cast<const T *>(k.state_in) + ((long long)b * (W - 1) + t + W - 1) * k.D;
+        return R::load(t >= 0 ? x : state, t < len && (t >= 0 || k.state_in), at);
     }
+    __device__ __forceinline__ void input(int t, float (&o)[V]) const { R::floats(input(t), o); }
     __device__ __forceinline__ float before(const float (&win)[W][V], int v) const {
         float p = bias[v];
 #pragma unroll
@@ -84,33 +127,41 @@ template <int W, int V> __device__ __forceinline__ void push(float (&win)[W][V],
     }
 }
 
-constexpr int AHEAD = 4;                      // tokens asked for together
+constexpr int AHEAD = 4;                      // tokens asked for together, a group before they are used
 template <class T, int W, int V>
 __global__ __launch_bounds__(64 * RUNS) void forward(const Call k) {
+    typedef Row<T, V> R;
     const int run_index = blockIdx.y * RUNS + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);          // (the same for a wavefront: its tokens are scalars)
     Lane<T, W, V> l(k, run_index);
     if (!l.live) return;
     float win[W][V];
-    zero<T>(win[0]);
+    typename R::Raw next[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; i++) next[i] = l.input(l.run0 + i);
+    zero(win[0]);
 #pragma unroll
     for (int i = 0; i + 1 < W; i++) l.input(l.run0 - (W - 1) + i, win[i + 1]);
     const int end = min(l.run0 + k.run, k.T);
-    T *y = static_cast<T *>(k.y) + ((size_t)l.b * k.T) * k.D + l.d;
+    T *y = static_cast<T *>(k.y) + (size_t)l.b * k.T * k.D;
     for (int t0 = l.run0; t0 < end; t0 += AHEAD) {
-        float x[AHEAD][V];
+        typename R::Raw now[AHEAD];
 #pragma unroll
-        for (int i = 0; i < AHEAD; i++) l.input(t0 + i, x[i]);
+        for (int i = 0; i < AHEAD; i++) {
+            now[i] = next[i];
+            next[i] = l.input(t0 + AHEAD + i);
+        }
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
             const int t = t0 + i;
-            push(win, x[i]);
-            float o[V];
+            float x[V], o[V];
+            R::floats(now[i], x);
+            push(win, x);
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 const float p = l.before(win, v);
                 o[v] = t >= l.len ? 0.f : k.silu ? p * sigmoid(p) : p;
             }
-            if (t < end) store_vec(y + (size_t)t * k.D, o);
+            R::store(y + (size_t)t * k.D, t < end, l.at, o);
         }
     }
     // the run that the sequence ends in (its first one if there is nothing) leaves the new state
@@ -120,57 +171,67 @@ __global__ __launch_bounds__(64 * RUNS) void forward(const Call k) {
 #pragma unroll
     for (int i = 0; i + 1 < W; i++) l.input(l.len - (W - 1) + i, row[i]);
 #pragma unroll
-    for (int i = 0; i + 1 < W; i++) store_vec(static_cast<T *>(k.state_out) + ((size_t)l.b * (W - 1) + i) * k.D + l.d, row[i]);
+    for (int i = 0; i + 1 < W; i++) R::store(static_cast<T *>(k.state_out) + ((size_t)l.b * (W - 1) + i) * k.D, true, l.at, row[i]);
 }
 
 template <class T, int W, int V>
 __global__ __launch_bounds__(64 * RUNS) void backward(const Call k) {
+    typedef Row<T, V> R;
     __shared__ float sums[RUNS][64 * V];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, run_index = blockIdx.y * RUNS + wave;
     Lane<T, W, V> l(k, run_index);
     float gw[W][V], gb[V];
 #pragma unroll
-    for (int i = 0; i < W; i++) zero<T>(gw[i]);
-    zero<T>(gb);
+    for (int i = 0; i < W; i++) zero(gw[i]);
+    zero(gb);
     if (l.live) {
         float win[W][V], gp[W][V];          // gp[i]: of token t - (W-1) + i
-        zero<T>(win[0]);
+        const T *gy = static_cast<const T *>(k.gy) + (size_t)l.b * k.T * k.D;
+        T *gx = static_cast<T *>(k.gx) + (size_t)l.b * k.T * k.D;
+        typename R::Raw next_x[AHEAD], next_g[AHEAD];
+        auto ask = [&](int t0) {
 #pragma unroll
-        for (int i = 0; i < W; i++) zero<T>(gp[i]);
+            for (int i = 0; i < AHEAD; i++) {
+                next_x[i] = l.input(t0 + i);
+                next_g[i] = R::load(gy + (long long)(t0 + i) * k.D, t0 + i < l.len, l.at);
+            }
+        };
+        ask(l.run0);
+        zero(win[0]);
+#pragma unroll
+        for (int i = 0; i < W; i++) zero(gp[i]);
 #pragma unroll
         for (int i = 0; i + 1 < W; i++) l.input(l.run0 - (W - 1) + i, win[i + 1]);
         const int end = min(l.run0 + k.run, k.T), begin = l.run0 == 0 ? -(W - 1) : l.run0;
-        const T *gy = static_cast<const T *>(k.gy) + (size_t)l.b * k.T * k.D + l.d;
-        T *gx = static_cast<T *>(k.gx) + (size_t)l.b * k.T * k.D + l.d;
         for (int t0 = l.run0; t0 < end + W - 1; t0 += AHEAD) {
-            float x[AHEAD][V], g[AHEAD][V];
+            typename R::Raw now_x[AHEAD], now_g[AHEAD];
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
-                l.input(t0 + i, x[i]);
-                if (t0 + i < l.len) load_vec(gy + (size_t)(t0 + i) * k.D, g[i]);
-                else zero<T>(g[i]);
+                now_x[i] = next_x[i];
+                now_g[i] = next_g[i];
             }
+            ask(t0 + AHEAD);
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
                 const int t = t0 + i, s = t - (W - 1);          // gx[s] is complete with gp[t]
-                push(win, x[i]);
-                float d[V];
-#pragma unroll
-                for (int v = 0; v < V; v++) {
-                    const float p = l.before(win, v), sig = sigmoid(p);
-                    d[v] = k.silu ? g[i][v] * fmaf(p * sig, 1.f - sig, sig) : g[i][v];
-                    if (t >= l.len) d[v] = 0.f;
-                }
-                push(gp, d);
-                if (t < end)
+                float x[V], d[V], o[V];
+                R::floats(now_x[i], x);
+                R::floats(now_g[i], d);                         // (zero from the length on)
+                push(win, x);
+                if (k.silu)
 #pragma unroll
                     for (int v = 0; v < V; v++) {
-                        gb[v] += d[v];
-#pragma unroll
-                        for (int j = 0; j < W; j++) gw[j][v] = fmaf(d[v], win[j][v], gw[j][v]);
+                        const float p = l.before(win, v), sig = sigmoid(p);
+                        d[v] = t < l.len ? d[v] * fmaf(p * sig, 1.f - sig, sig) : 0.f;
                     }
-                if (s < begin || s >= end) continue;
-                float o[V];
+                push(gp, d);
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    const float e = t < end ? d[v] : 0.f;          // (the next run's tokens are counted there)
+                    gb[v] += e;
+#pragma unroll
+                    for (int j = 0; j < W; j++) gw[j][v] = fmaf(e, win[j][v], gw[j][v]);
+                }
 #pragma unroll
                 for (int v = 0; v < V; v++) {
                     o[v] = 0.f;
@@ -178,14 +239,14 @@ __global__ __launch_bounds__(64 * RUNS) void backward(const Call k) {
                     for (int j = 0; j < W; j++) o[v] = fmaf(l.w[j][v], gp[W - 1 - j][v], o[v]);
                 }
                 const int kept = s - (l.len - (W - 1));           // the new state's row that token s went into
-                if (k.gstate_out && kept >= 0 && s < l.len) {
+                if (k.gstate_out && kept >= 0 && s < l.len && s >= begin && s < end) {
                     float e[V];
-                    load_vec(static_cast<const T *>(k.gstate_out) + ((size_t)l.b * (W - 1) + kept) * k.D + l.d, e);
+                    R::floats(R::load(static_cast<const T *>(k.gstate_out) + ((long long)l.b * (W - 1) + kept) * k.D, true, l.at), e);
 #pragma unroll
                     for (int v = 0; v < V; v++) o[v] += e[v];
                 }
-                if (s >= 0) store_vec(gx + (size_t)s * k.D, o);
-                else if (k.gstate_in) store_vec(static_cast<T *>(k.gstate_in) + ((size_t)l.b * (W - 1) + s + W - 1) * k.D + l.d, o);
+                if (s < 0 && k.gstate_in && s >= begin) R::store(static_cast<T *>(k.gstate_in) + ((long long)l.b * (W - 1) + s + W - 1) * k.D, true, l.at, o);
+                R::store(gx + (long long)s * k.D, s >= 0 && s >= begin && s < end, l.at, o);
             }
         }
     }
