@@ -11,6 +11,7 @@
 // the workgroups by sum_rows.
 #include "common.h"
 #include "row_sums.h"
+#include "vec.h"
 
 namespace wkv {
 namespace conv {
@@ -92,15 +93,20 @@ template <class T, int W, int V> struct Lane {
         run0 = run_index * k.run;
         len = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
         if (!live) return;
-#pragma unroll
-        for (int v = 0; v < V; v++) {
-#pragma unroll
-            for (int i = 0; i < W; i++) w[i][v] = parameter(k.weight, (d + v) * W + i);
-            bias[v] = k.bias ? parameter(k.bias, d + v) : 0.f;
-        }
+        if (k.w32) parameters(static_cast<const float *>(k.weight), static_cast<const float *>(k.bias));
+        else parameters(static_cast<const T *>(k.weight), static_cast<const T *>(k.bias));
     }
-    __device__ __forceinline__ float parameter(const void *p, int i) const {
-        return k.w32 ? static_cast<const float *>(p)[i] : to_float(static_cast<const T *>(p)[i]);
+    // (V taps' worth of a channel at a time: whole 8 or 16 bytes)
+    template <class P> __device__ __forceinline__ void parameters(const P *pw, const P *pb) {
+        float flat[W][V];
+#pragma unroll
+        for (int i = 0; i < W; i++) load_vec(pw + (size_t)d * W + i * V, flat[i]);
+#pragma unroll
+        for (int v = 0; v < V; v++)
+#pragma unroll
+            for (int i = 0; i < W; i++) w[i][v] = flat[(v * W + i) / V][(v * W + i) % V];
+        if (pb) load_vec(pb + d, bias);
+        else zero(bias);
     }
     // xx[t]: the state's tokens are -(W-1) .. -1; nothing from the length on
     __device__ __forceinline__ Raw input(int t) const {
@@ -141,6 +147,11 @@ __global__ __launch_bounds__(64 * RUNS) void forward(const Call k) {
     zero(win[0]);
 #pragma unroll
     for (int i = 0; i + 1 < W; i++) l.input(l.run0 - (W - 1) + i, win[i + 1]);
+    // the run that the sequence ends in (its first one if there is nothing) leaves the new state
+    const bool ends = run_index == (l.len > 0 ? (l.len - 1) / k.run : 0);
+    typename R::Raw state[W - 1];
+#pragma unroll
+    for (int i = 0; i + 1 < W; i++) state[i] = l.input(ends ? l.len - (W - 1) + i : l.len);
     const int end = min(l.run0 + k.run, k.T);
     T *y = static_cast<T *>(k.y) + (size_t)l.b * k.T * k.D;
     for (int t0 = l.run0; t0 < end; t0 += AHEAD) {
@@ -164,14 +175,12 @@ __global__ __launch_bounds__(64 * RUNS) void forward(const Call k) {
             R::store(y + (size_t)t * k.D, t < end, l.at, o);
         }
     }
-    // the run that the sequence ends in (its first one if there is nothing) leaves the new state
-    const int last = l.len > 0 ? (l.len - 1) / k.run : 0;
-    if (run_index != last) return;
-    float row[W][V];
 #pragma unroll
-    for (int i = 0; i + 1 < W; i++) l.input(l.len - (W - 1) + i, row[i]);
-#pragma unroll
-    for (int i = 0; i + 1 < W; i++) R::store(static_cast<T *>(k.state_out) + ((size_t)l.b * (W - 1) + i) * k.D, true, l.at, row[i]);
+    for (int i = 0; i + 1 < W; i++) {
+        float row[V];
+        R::floats(state[i], row);
+        R::store(static_cast<T *>(k.state_out) + ((size_t)l.b * (W - 1) + i) * k.D, ends, l.at, row);
+    }
 }
 
 template <class T, int W, int V>
@@ -270,13 +279,13 @@ __global__ __launch_bounds__(64 * RUNS) void backward(const Call k) {
 }
 
 // gradients (W + 1, D) to the weight's (D, W) and the bias
-template <class P> struct ToFilter {
-    P *weight, *bias;
+template <class T> struct ToFilter {
+    ToRow<T> weight, bias;
     int W, D;
     __device__ __forceinline__ void operator()(size_t i, float v) const {
         const int tap = (int)(i / D), d = (int)(i % D);
-        if (tap < W) weight[(size_t)d * W + tap] = from_float<P>(v);
-        else if (bias) bias[d] = from_float<P>(v);
+        if (tap < W) weight((size_t)d * W + tap, v);
+        else if (bias.out) bias(d, v);
     }
 };
 
@@ -313,10 +322,10 @@ template <class T> static hipError_t forward_t(hipStream_t s, int W, const Call 
 template <class T> static hipError_t backward_t(hipStream_t s, int W, const Call &k, bool wide, void *gweight, void *gbias) {
     const hipError_t e = wide ? launch<T, WIDE, true>(s, W, k) : launch<T, 1, true>(s, W, k);
     if (e != hipSuccess) return e;
-    const int rows = k.B * run_groups(k.T, run_for(k.B, k.T, k.D, wide ? WIDE : 1));
-    const size_t n = (size_t)(W + 1) * k.D;
-    if (k.w32) sum_rows_launch(s, rows, n, k.part, ToFilter<float>{static_cast<float *>(gweight), static_cast<float *>(gbias), W, k.D});
-    else sum_rows_launch(s, rows, n, k.part, ToFilter<T>{static_cast<T *>(gweight), static_cast<T *>(gbias), W, k.D});
+    Sums<ToFilter<T>> sums;
+    sums.add(k.B * run_groups(k.T, run_for(k.B, k.T, k.D, wide ? WIDE : 1)), (size_t)(W + 1) * k.D, k.part,
+             {{gweight, k.w32 != 0}, {gbias, k.w32 != 0}, W, k.D});
+    sum_rows_launch(s, sums);
     return hipGetLastError();
 }
 

@@ -261,8 +261,9 @@ template <class T, class R> static hipError_t backward_t(hipStream_t s, const Ca
 #define WKV_NORM(V, N, W) hipLaunchKernelGGL((backward<T, R, V, N, W>), dim3(groups), dim3(64 * W), 0, s, k)
     WKV_NORM_SHAPES(WKV_NORM);
 #undef WKV_NORM
-    if (k.w32) sum_rows_launch(s, groups, (size_t)k.C, k.part, ToRow<float>{static_cast<float *>(gweight)});
-    else sum_rows_launch(s, groups, (size_t)k.C, k.part, ToRow<T>{static_cast<T *>(gweight)});
+    Sums<ToRow<T>> sums;
+    sums.add(groups, (size_t)k.C, k.part, {gweight, k.w32 != 0});
+    sum_rows_launch(s, sums);
     return hipGetLastError();
 }
 

@@ -23,6 +23,7 @@
 // and state, not the memory (which would take a third of the time).
 #include "common.h"
 #include "row_sums.h"
+#include "vec.h"
 
 namespace wkv {
 namespace scan {
@@ -591,49 +592,71 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
 }
 
 // One token: bound by the states, read once and written once.  Q lanes per channel with four states each (N = 4 Q), or, for
-// other N, a row of lanes as above.  state_out may be state_in: a lane writes what it has read.
-template <class T, int Q>
+// other N, a row of lanes as above; a lane takes NB sequences, whose loads are all in flight together, with one read of its A.  VEC: four of
+// B or C are one load.  state_out may be state_in: a lane writes what it has read.
+template <class T, int Q, int NB, bool VEC>
 __global__ __launch_bounds__(256) void decode(const Call k) {
     constexpr int V = Q ? 4 : 1, LANES = Q ? Q : 16, STEPS = Q ? 1 : (MAX_STATES + 15) / 16;
-    const long long item = ((long long)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int lane = threadIdx.x % LANES;
-    if (item >= (long long)k.B * k.D) return;
-    const int b = (int)(item / k.D), d = (int)(item % k.D), g = d / k.Dg;
-    const bool in = !k.lengths || k.lengths[b] > 0;
-    const float x = in ? to_float(static_cast<const T *>(k.x.p)[b * k.x.batch + d]) : 0.f;
-    const float dt = in ? softplus(to_float(static_cast<const T *>(k.dt.p)[b * k.dt.batch + d]) + (k.bias ? k.bias[d] : 0.f)) : 0.f;
-    const T *pb = static_cast<const T *>(k.b.p) + b * k.b.batch + g * k.b.group, *pc = static_cast<const T *>(k.c.p) + b * k.c.batch + g * k.c.group;
-    float y = 0.f;
+    const int d = (int)(((long long)blockIdx.x * 256 + threadIdx.x) / LANES), lane = threadIdx.x % LANES, b0 = blockIdx.y * NB;
+    if (d >= k.D) return;
+    const int g = d / k.Dg;
+    const float bias = k.bias ? k.bias[d] : 0.f, skip = k.skip ? k.skip[d] : 0.f;
+    float x[NB], raw[NB], z[NB], y[NB], step[NB];
+    bool in[NB];
+#pragma unroll
+    for (int i = 0; i < NB; i++) {
+        const int b = min(b0 + i, k.B - 1);
+        in[i] = !k.lengths || k.lengths[b] > 0;
+        x[i] = in[i] ? to_float(static_cast<const T *>(k.x.p)[b * k.x.batch + d]) : 0.f;
+        raw[i] = in[i] ? to_float(static_cast<const T *>(k.dt.p)[b * k.dt.batch + d]) : 0.f;
+        z[i] = in[i] && k.z.p ? to_float(static_cast<const T *>(k.z.p)[b * k.z.batch + d]) : 0.f;
+        y[i] = 0.f;
+    }
 #pragma unroll
     for (int s = 0; s < STEPS; s++) {
         const int n = V * lane + 16 * s;
         if (n >= k.N) break;
-        float a[V], h[V] = {};
-        if constexpr (Q != 0) {
-            load4(k.A + (size_t)d * k.N + n, a);
-            if (k.state_in) load4(k.state_in + item * k.N + n, h);
-        } else {
-            a[0] = k.A[(size_t)d * k.N + n];
-            if (k.state_in) h[0] = k.state_in[item * k.N + n];
+        float a[V], h[NB][V], vb[NB][V], vc[NB][V];
+        load_vec(k.A + (size_t)d * k.N + n, a);
+#pragma unroll
+        for (int i = 0; i < NB; i++) {
+            const int b = min(b0 + i, k.B - 1);
+            const T *pb = static_cast<const T *>(k.b.p) + b * k.b.batch + g * k.b.group + n, *pc = static_cast<const T *>(k.c.p) + b * k.c.batch + g * k.c.group + n;
+#pragma unroll
+            for (int v = 0; v < V; v++) h[i][v] = 0.f;
+            if (k.state_in) load_vec(k.state_in + ((size_t)b * k.D + d) * k.N + n, h[i]);
+            if constexpr (VEC) {
+                load_vec(pb, vb[i]);
+                load_vec(pc, vc[i]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < V; v++) {
+                    vb[i][v] = to_float(pb[v]);
+                    vc[i][v] = to_float(pc[v]);
+                }
+            }
         }
 #pragma unroll
-        for (int v = 0; v < V; v++) {
-            const float vb = in ? to_float(pb[n + v]) : 0.f, vc = in ? to_float(pc[n + v]) : 0.f;
-            h[v] = fmaf(exp2_fast(dt * (a[v] * LOG2E)), h[v], dt * x * vb);
-            y = fmaf(vc, h[v], y);
+        for (int i = 0; i < NB; i++) {
+            if (s == 0) step[i] = in[i] ? softplus(raw[i] + bias) : 0.f;
+            const float dtx = step[i] * x[i];
+#pragma unroll
+            for (int v = 0; v < V; v++) {
+                h[i][v] = fmaf(exp2_fast(step[i] * (a[v] * LOG2E)), h[i][v], in[i] ? dtx * vb[i][v] : 0.f);
+                y[i] = fmaf(in[i] ? vc[i][v] : 0.f, h[i][v], y[i]);
+            }
+            if (b0 + i < k.B) store_vec(k.state_out + ((size_t)(b0 + i) * k.D + d) * k.N + n, h[i]);
         }
-        if constexpr (Q != 0) store4(k.state_out + item * k.N + n, h);
-        else k.state_out[item * k.N + n] = h[0];
     }
 #pragma unroll
-    for (int m = LANES / 2; m > 0; m >>= 1) y += __shfl_xor(y, m);
-    if (lane == 0) {
-        y = fmaf(k.skip ? k.skip[d] : 0.f, x, y);
-        if (k.z.p) {
-            const float z = in ? to_float(static_cast<const T *>(k.z.p)[b * k.z.batch + d]) : 0.f;
-            y *= z * sigmoid(z);
+    for (int i = 0; i < NB; i++) {
+#pragma unroll
+        for (int m = LANES / 2; m > 0; m >>= 1) y[i] += __shfl_xor(y[i], m);
+        if (lane == 0 && b0 + i < k.B) {
+            float out = fmaf(skip, x[i], y[i]);
+            if (k.z.p) out *= z[i] * sigmoid(z[i]);
+            static_cast<T *>(k.y)[(size_t)(b0 + i) * k.D + d] = from_float<T>(in[i] ? out : 0.f);
         }
-        static_cast<T *>(k.y)[(size_t)b * k.D + d] = from_float<T>(in ? y : 0.f);
     }
 }
 
@@ -682,9 +705,20 @@ template <class T> static hipError_t forward_t(hipStream_t s, Call k, void *scra
     const int J = states_per_lane(k.N);
     if (k.T == 1 && !k.checkpoints) {
         const bool four = k.N % 4 == 0 && (k.N & (k.N - 1)) == 0;
+        auto whole = [](const Rows &r) { return reinterpret_cast<uintptr_t>(r.p) % (4 * sizeof(T)) == 0 && r.batch % 4 == 0 && r.group % 4 == 0; };
+        const bool vec = whole(k.b) && whole(k.c);
         const int lanes = four ? k.N / 4 : 16;
-        const long long blocks = ((long long)k.B * k.D * lanes + 255) / 256;
-#define WKV_DECODE_SCAN(Q) hipLaunchKernelGGL((decode<T, Q>), dim3((unsigned)blocks), dim3(256), 0, s, k)
+        const unsigned blocks = (unsigned)(((long long)k.D * lanes + 255) / 256);
+        // four sequences per lane where that leaves every compute unit its wavefronts (B64 D5120: 17.2 us with one, 12.8 with four; below that
+        // one token's latency counts and the lanes are spread)
+        const bool many = (long long)blocks * ((k.B + 3) / 4) >= 2ll * cu_count();
+#define WKV_DECODE_SCAN(Q)                                                                                                         \
+    do {                                                                                                                           \
+        if (many && vec) hipLaunchKernelGGL((decode<T, Q, 4, true>), dim3(blocks, (k.B + 3) / 4), dim3(256), 0, s, k);             \
+        else if (many) hipLaunchKernelGGL((decode<T, Q, 4, false>), dim3(blocks, (k.B + 3) / 4), dim3(256), 0, s, k);              \
+        else if (vec) hipLaunchKernelGGL((decode<T, Q, 1, true>), dim3(blocks, k.B), dim3(256), 0, s, k);                          \
+        else hipLaunchKernelGGL((decode<T, Q, 1, false>), dim3(blocks, k.B), dim3(256), 0, s, k);                                  \
+    } while (0)
         switch (four ? lanes : 0) {
             case 1: WKV_DECODE_SCAN(1); break;
             case 2: WKV_DECODE_SCAN(2); break;
@@ -736,13 +770,15 @@ template <class T> static hipError_t backward_t(hipStream_t s, Call k, const Gra
     k.gskip_part = rows == 1 && to.gskip ? to.gskip : take(rows * k.D);
     k.gbias_part = rows == 1 && to.gbias ? to.gbias : take(rows * k.D);
     WKV_SCAN_J(backward, workgroups(k.B, k.D, k.G, 4 * BACK_WAVES) * p.segments, 64 * BACK_WAVES, );
-    sum_rows_launch(s, (int)cts, vectors, k.gb_part, ToRow<T>{static_cast<T *>(to.gb)});
-    sum_rows_launch(s, (int)cts, vectors, k.gc_part, ToRow<T>{static_cast<T *>(to.gc)});
+    Sums<ToRow<T>> sums;
+    sums.add((int)cts, vectors, k.gb_part, {to.gb, false});
+    sums.add((int)cts, vectors, k.gc_part, {to.gc, false});
     if (rows > 1) {
-        sum_rows_launch(s, (int)rows, (size_t)k.D * k.N, k.ga_part, ToRow<float>{to.ga});
-        if (to.gskip) sum_rows_launch(s, (int)rows, (size_t)k.D, k.gskip_part, ToRow<float>{to.gskip});
-        if (to.gbias) sum_rows_launch(s, (int)rows, (size_t)k.D, k.gbias_part, ToRow<float>{to.gbias});
+        sums.add((int)rows, (size_t)k.D * k.N, k.ga_part, {to.ga, true});
+        if (to.gskip) sums.add((int)rows, (size_t)k.D, k.gskip_part, {to.gskip, true});
+        if (to.gbias) sums.add((int)rows, (size_t)k.D, k.gbias_part, {to.gbias, true});
     }
+    sum_rows_launch(s, sums);
     return hipGetLastError();
 }
 
