@@ -10,8 +10,10 @@
 // The weights are whole numbers so that every sum is exact: no order of adding, no split over lanes changes a token.
 //
 // A workgroup of 16 wavefronts holds a row's s in registers (65536 elements; wider rows are read again for every pass) and
-// never sorts: the two cuts are found from counts and weights in 1024 bins of s, then in 1024 bins of the bin with the cut, then, between the
-// elements left there (for 16-bit logits mostly one value), by bisection of the value's bits.
+// never sorts.  Each of the two cuts is found from a histogram over 1024 bins of s, of tokens for top_k and of weights for top_p, and
+// then among the elements of the bin it falls into, which one wavefront searches by the bits of s.  What bounds it is the passes over
+// the registers and the histograms' atomics in LDS, so these take only what a cut can reach: for top_k what is not
+// below every lane's best (1024 such there are), for top_p what the rest of the vocabulary could not outweigh.
 #include "common.h"
 
 namespace wkv {
@@ -37,21 +39,23 @@ struct Call {
     float *logprob;
 };
 
-__device__ __forceinline__ u64 shfl_up(u64 v, int d) {
-    const unsigned lo = __shfl_up((unsigned)v, d), hi = __shfl_up((unsigned)(v >> 32), d);
+// v of the lane that a DPP names, 0 where there is none
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 from_lane(u64 v) {
+    const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)(unsigned)v, CTRL, ROWS, 0xf, false);
+    const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(unsigned)(v >> 32), CTRL, ROWS, 0xf, false);
     return (u64)hi << 32 | lo;
 }
 __device__ __forceinline__ u64 up_to(u64 v) {          // inclusive sum over the wavefront's lanes
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const u64 o = shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    v += from_lane<0x111, 0xf>(v);                     // row_shr:1, 2, 4, 8
+    v += from_lane<0x112, 0xf>(v);
+    v += from_lane<0x114, 0xf>(v);
+    v += from_lane<0x118, 0xf>(v);
+    v += from_lane<0x142, 0xa>(v);                     // row_bcast:15 to the second and the fourth row
+    v += from_lane<0x143, 0xc>(v);                     // row_bcast:31 to the upper two
     return v;
 }
 __device__ __forceinline__ u64 last_lane(u64 v) {
-    return (u64)__builtin_amdgcn_readlane((unsigned)(v >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((unsigned)v, 63);
+    return (u64)(unsigned)__builtin_amdgcn_readlane((int)(unsigned)(v >> 32), 63) << 32 | (unsigned)__builtin_amdgcn_readlane((int)(unsigned)v, 63);
 }
 
 // N chunks of a row in registers, as s; N = 0: read again for every pass
@@ -110,16 +114,20 @@ template <class T, int N> struct Row {
 
 __device__ __forceinline__ unsigned weight(float s) { return (unsigned)rintf(exp2_fast(-s) * (float)ONE); }
 
+constexpr int LIST = 1024;                     // elements of one bin that one wavefront searches
 struct Shared {
-    u64 bin_weight[2][BINS];
-    unsigned bin_count[2][BINS];
+    u64 bin_weight[BINS];
+    unsigned bin_count[BINS];
+    float list[LIST];
+    unsigned listed;
     u64 sums[WAVES * MAX_CHUNKS];          // by chunk and wavefront
     unsigned ties[WAVES * MAX_CHUNKS];
     u64 red[2][WAVES];
     float redf[2][WAVES];
-    // what a scan found
+    // what a search found
     int bin;
-    u64 before;
+    unsigned key;
+    u64 before, equal, total;
 };
 
 // sum over the workgroup; `turn` alternates between two barriers
@@ -134,122 +142,148 @@ __device__ __forceinline__ u64 over_all(u64 v, Shared &sh, int &turn) {
     return s;
 }
 
-// The first bin at which the sum of `in` reaches `need` (1 <= need <= the sum of all), and the sum before it
-template <class E> __device__ __forceinline__ void find_bin(const E *in, u64 need, Shared &sh, int &bin, u64 &before) {
-    if (threadIdx.x < 64) {
-        constexpr int EACH = BINS / 64;
-        u64 own = 0;
-        for (int i = 0; i < EACH; i++) own += in[threadIdx.x * EACH + i];
-        const u64 upto = up_to(own);
-        if (upto >= need && upto - own < need) {
-            u64 s = upto - own;
-            int i = threadIdx.x * EACH;
-            while (s + in[i] < need) s += in[i++];
-            sh.bin = i;
-            sh.before = s;
-        }
+// The first bin at which the sum of `in` reaches `need` (at least 1), and the sum before it; false if it does not
+template <class E> __device__ __forceinline__ bool find_bin(const E *in, u64 need, Shared &sh, int &turn, int &bin, u64 &before) {
+    static_assert(BINS == THREADS, "a bin per thread");
+    const int wave = threadIdx.x >> 6;
+    const u64 own = in[threadIdx.x];
+    u64 upto = up_to(own), total = 0;
+    if ((threadIdx.x & 63) == 63) sh.red[turn][wave] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+        if (i < wave) upto += sh.red[turn][i];
+        total += sh.red[turn][i];
+    }
+    turn ^= 1;
+    if (total < need) return false;
+    if (upto >= need && upto - own < need) {
+        sh.bin = threadIdx.x;
+        sh.before = upto - own;
     }
     __syncthreads();
     bin = sh.bin;
     before = sh.before;
-    __syncthreads();
+    return true;
 }
 
 struct Cut {
     unsigned key;          // kept: the values below, and the first `ties` of those equal
     u64 ties;
-    u64 before;            // what the values below come to
-    u64 here;              // what all the equal ones do
+    u64 before;            // the weight (tokens) of the values below
+    u64 equal;             // how many are equal
 };
 
-// Where the first `need` (of tokens, or of weight) in the order of s end; the first level's bins are filled.
-// limit: tokens of larger s do not count
-template <bool WEIGHT, class R>
-__device__ __forceinline__ Cut find_cut(R &row, u64 need, float limit, Shared &sh, int &turn) {
-    int b1, b2;
-    u64 before, inner;
-    if (WEIGHT) find_bin(sh.bin_weight[0], need, sh, b1, before);
-    else find_bin(sh.bin_count[0], need, sh, b1, before);
-    for (int i = threadIdx.x; i < BINS; i += THREADS) {
-        sh.bin_weight[1][i] = 0;
-        sh.bin_count[1][i] = 0;
-    }
-    __syncthreads();
-    const float base = (float)b1;
-    row.each([&](int, const float (&s)[PIECE]) {
-#pragma unroll
-        for (int i = 0; i < PIECE; i++) {
-            const float x = s[i] * PER_OCTAVE - base;
-            if (x >= 0.f && x < 1.f && s[i] <= limit) {
-                const int b = (int)(x * BINS);
-                if (WEIGHT) atomicAdd(&sh.bin_weight[1][b], (u64)weight(s[i]));
-                else atomicAdd(&sh.bin_count[1][b], 1u);
-            }
-        }
-    });
-    __syncthreads();
-    if (WEIGHT) find_bin(sh.bin_weight[1], need - before, sh, b2, inner);
-    else find_bin(sh.bin_count[1], need - before, sh, b2, inner);
-    before += inner;
-    // the values left: those with x in [b2, b2 + 1) / BINS; their smallest and largest bits
-    auto inside = [&](float s) {
-        const float x = s * PER_OCTAVE - base;
-        return x >= 0.f && x < 1.f && s <= limit && (int)(x * BINS) == b2;
-    };
-    unsigned lo = 0xffffffffu, hi = 0;
+// Where the first `need` (of tokens, or of weight) in the order of s end, from the histogram `in` of the elements that count; false if
+// there is less than that.  counts(s): whether an element does.
+template <bool WEIGHT, class E, class R, class F>
+__device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, F counts, Shared &sh, int &turn, Cut &cut) {
+    int bin;
+    u64 before;
+    if (threadIdx.x == 0) sh.listed = 0;
+    if (!find_bin(in, need, sh, turn, bin, before)) return false;
+    const float lo_s = bin * (1.f / PER_OCTAVE), hi_s = (bin + 1) * (1.f / PER_OCTAVE);
+    auto inside = [&](float s) { return s >= lo_s && s < hi_s && counts(s); };
     row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
         for (int i = 0; i < PIECE; i++)
             if (inside(s[i])) {
-                lo = min(lo, __float_as_uint(s[i]));
-                hi = max(hi, __float_as_uint(s[i]));
+                const unsigned at = atomicAdd(&sh.listed, 1u);
+                if (at < LIST) sh.list[at] = s[i];
             }
     });
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) {
-        lo = min(lo, (unsigned)__shfl_xor((int)lo, m));
-        hi = max(hi, (unsigned)__shfl_xor((int)hi, m));
-    }
-    if ((threadIdx.x & 63) == 0) sh.red[turn][threadIdx.x >> 6] = (u64)hi << 32 | lo;
     __syncthreads();
+    const unsigned m = sh.listed;
+    if (m <= LIST) {
+        if (threadIdx.x < 64) {
+            constexpr int EACH = LIST / 64;
+            unsigned v[EACH], w[EACH], lo = 0xffffffffu, hi = 0;
 #pragma unroll
-    for (int i = 0; i < WAVES; i++) {
-        const u64 r = sh.red[turn][i];
-        lo = min(lo, (unsigned)r);
-        hi = max(hi, (unsigned)(r >> 32));
-    }
-    turn ^= 1;
-    // the smallest value up to which there is enough
-    auto upto = [&](unsigned key) {
-        u64 n = 0;
+            for (int i = 0; i < EACH; i++) {
+                const bool there = i * 64 + threadIdx.x < m;
+                const float s = there ? sh.list[i * 64 + threadIdx.x] : 0.f;
+                v[i] = there ? __float_as_uint(s) : 0xffffffffu;
+                w[i] = there ? (WEIGHT ? weight(s) : 1u) : 0u;
+                lo = min(lo, v[i]);
+                hi = there ? max(hi, v[i]) : hi;
+            }
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) {
+                lo = min(lo, (unsigned)__shfl_xor((int)lo, d));
+                hi = max(hi, (unsigned)__shfl_xor((int)hi, d));
+            }
+            auto upto = [&](unsigned key) {          // the weight of the values up to it
+                u64 n = 0;
+#pragma unroll
+                for (int i = 0; i < EACH; i++)
+                    if (i * 64 < m) n += v[i] <= key ? w[i] : 0u;
+                return last_lane(up_to(n));
+            };
+            while (lo < hi) {
+                const unsigned mid = lo + ((hi - lo) >> 1);
+                if (before + upto(mid) >= need) hi = mid;
+                else lo = mid + 1;
+            }
+            u64 n = 0;
+#pragma unroll
+            for (int i = 0; i < EACH; i++) n += v[i] == lo;
+            n = last_lane(up_to(n));
+            const u64 below = lo ? upto(lo - 1) : 0;
+            if (threadIdx.x == 0) {
+                sh.key = lo;
+                sh.equal = n;
+                sh.total = before + below;
+            }
+        }
+        __syncthreads();
+        cut.key = sh.key;
+        cut.equal = sh.equal;
+        cut.before = sh.total;
+    } else {          // too many for that, most likely equal ones: the same search by all, over the registers
+        unsigned lo = 0xffffffffu, hi = 0;
         row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
             for (int i = 0; i < PIECE; i++)
-                if (__float_as_uint(s[i]) <= key && inside(s[i])) n += WEIGHT ? weight(s[i]) : 1;
+                if (inside(s[i])) {
+                    lo = min(lo, __float_as_uint(s[i]));
+                    hi = max(hi, __float_as_uint(s[i]));
+                }
         });
-        return over_all(n, sh, turn);
-    };
-    while (lo < hi) {
-        const unsigned mid = lo + ((hi - lo) >> 1);
-        if (before + upto(mid) >= need) hi = mid;
-        else lo = mid + 1;
-    }
-    Cut cut;
-    cut.key = lo;
-    u64 below = 0, equal = 0;
-    row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
-        for (int i = 0; i < PIECE; i++)
-            if (inside(s[i])) {
-                if (__float_as_uint(s[i]) < lo) below += WEIGHT ? weight(s[i]) : 1;
-                if (__float_as_uint(s[i]) == lo) equal += 1;
-            }
-    });
-    cut.before = before + over_all(below, sh, turn);
-    cut.here = over_all(equal, sh, turn);
-    const u64 left = need - cut.before, each = WEIGHT ? max(weight(__uint_as_float(lo)), 1u) : 1u;
+        for (int d = 32; d > 0; d >>= 1) {
+            lo = min(lo, (unsigned)__shfl_xor((int)lo, d));
+            hi = max(hi, (unsigned)__shfl_xor((int)hi, d));
+        }
+        if ((threadIdx.x & 63) == 0) sh.red[turn][threadIdx.x >> 6] = (u64)hi << 32 | lo;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < WAVES; i++) {
+            const u64 r = sh.red[turn][i];
+            lo = min(lo, (unsigned)r);
+            hi = max(hi, (unsigned)(r >> 32));
+        }
+        turn ^= 1;
+        auto sum = [&](unsigned from, unsigned to, bool weights) {          // of the values from .. to
+            u64 n = 0;
+            row.each([&](int, const float (&s)[PIECE]) {
+#pragma unroll
+                for (int i = 0; i < PIECE; i++)
+                    if (__float_as_uint(s[i]) >= from && __float_as_uint(s[i]) <= to && inside(s[i])) n += weights ? weight(s[i]) : 1;
+            });
+            return over_all(n, sh, turn);
+        };
+        while (lo < hi) {
+            const unsigned mid = lo + ((hi - lo) >> 1);
+            if (before + sum(0, mid, WEIGHT) >= need) hi = mid;
+            else lo = mid + 1;
+        }
+        cut.key = lo;
+        cut.equal = sum(lo, lo, false);
+        cut.before = before + (lo ? sum(0, lo - 1, WEIGHT) : 0);
+    }
+    const u64 left = need - cut.before, each = WEIGHT ? max(weight(__uint_as_float(cut.key)), 1u) : 1u;
     cut.ties = (left + each - 1) / each;
-    return cut;
+    return true;
 }
 
 template <class T, int N>
@@ -262,32 +296,40 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     const float top_p = k.top_p ? k.top_p[r] : k.top_p_value, min_p = k.min_p ? k.min_p[r] : k.min_p_value;
     const bool warm = temperature >= 1e-6f;
     const int top_k = !warm ? 1 : k.top_k ? k.top_k[r] : k.top_k_value;
-    // the largest logit
-    float top = -INFINITY;
+    // the largest logit of the lane and of all
+    float best = -INFINITY;
     if constexpr (N > 0) {
 #pragma unroll
         for (int c = 0; c < N; c++) {
             row.raw(c, row.s[c]);
 #pragma unroll
-            for (int i = 0; i < PIECE; i++) top = fmaxf(top, row.s[c][i]);
+            for (int i = 0; i < PIECE; i++) best = fmaxf(best, row.s[c][i]);
         }
     } else {
         for (int c = 0; c < row.chunks; c++) {
             row.raw(c, row.s[0]);
 #pragma unroll
-            for (int i = 0; i < PIECE; i++) top = fmaxf(top, row.s[0][i]);
+            for (int i = 0; i < PIECE; i++) best = fmaxf(best, row.s[0][i]);
         }
     }
+    float top = best, least_best = best;
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-    if (lane == 0) sh.redf[0][wave] = top;
-    for (int i = tid; i < BINS; i += THREADS) {
-        sh.bin_weight[0][i] = 0;
-        sh.bin_count[0][i] = 0;
+    for (int m = 32; m > 0; m >>= 1) {
+        top = fmaxf(top, __shfl_xor(top, m));
+        least_best = fminf(least_best, __shfl_xor(least_best, m));
     }
+    if (lane == 0) {
+        sh.redf[0][wave] = top;
+        sh.redf[1][wave] = least_best;
+    }
+    sh.bin_weight[tid] = 0;
+    sh.bin_count[tid] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < WAVES; i++) top = fmaxf(top, sh.redf[0][i]);
+    for (int i = 0; i < WAVES; i++) {
+        top = fmaxf(top, sh.redf[0][i]);
+        least_best = fminf(least_best, sh.redf[1][i]);
+    }
     if (top == -INFINITY) {
         if (tid == 0) {
             k.token[r] = -1;
@@ -301,55 +343,71 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
 #pragma unroll
         for (int c = 0; c < N; c++) row.place(row.s[c]);
     }
-    // counts and weights in bins of s; a token lighter than `least` does not count
+    // a token counts from a weight of 1, or of min_p's share; `reach` is a little more than the s of that
     const double share = (double)min_p * ONE;
     const unsigned least = share > 1.0 ? share < ONE ? (unsigned)ceil(share) : (unsigned)ONE : 1u;
+    const float reach = fminf(MOST, 31.01f - __builtin_amdgcn_logf((float)least - 0.5f));
     int turn = 0;
-    u64 own = 0, count = 0;
-    float limit = 0.f;          // the largest s that counts (weights fall with s)
-    row.each([&](int, const float (&s)[PIECE]) {
-#pragma unroll
-        for (int i = 0; i < PIECE; i++)
-            if (s[i] < MOST) {
-                const unsigned w = weight(s[i]);
-                if (w >= least) {
-                    const int b = (int)(s[i] * PER_OCTAVE);
-                    atomicAdd(&sh.bin_weight[0][b], (u64)w);
-                    atomicAdd(&sh.bin_count[0][b], 1u);
-                    own += w;
-                    count++;
-                    limit = fmaxf(limit, s[i]);
-                }
-            }
-    });
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) limit = fmaxf(limit, __shfl_xor(limit, m));
-    if (lane == 0) sh.redf[1][wave] = limit;
-    u64 total = over_all(own, sh, turn);
-    count = over_all(count, sh, turn);
-#pragma unroll
-    for (int i = 0; i < WAVES; i++) limit = fmaxf(limit, sh.redf[1][i]);
-    unsigned key = __float_as_uint(limit);
+    unsigned key = 0x7f800000u;          // (the bits of infinity: all that count)
     u64 ties = ~0ull;
-    if (top_k > 0 && (u64)top_k < count) {
-        const Cut c = find_cut<false>(row, (u64)top_k, limit, sh, turn);
-        u64 lighter = 0;          // the weight of what is kept
+    auto counts = [&](float s) { return s < reach && (least == 1 || weight(s) >= least); };
+    bool cut_k = false;
+    if (top_k > 0 && top_k < k.V) {
+        // every lane has an element within `bound`: the first 1024 are there
+        float far[PIECE] = {least_best, least_best, least_best, least_best, least_best, least_best, least_best, least_best};
+        row.place(far);
+        const float bound = top_k <= THREADS ? far[0] : INFINITY;
+        auto near = [&](float s) { return s <= bound && counts(s); };
         row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
             for (int i = 0; i < PIECE; i++)
-                if (__float_as_uint(s[i]) < c.key) lighter += weight(s[i]);
+                if (near(s[i])) atomicAdd(&sh.bin_count[(int)(s[i] * PER_OCTAVE)], 1u);
         });
-        total = over_all(lighter, sh, turn) + c.ties * weight(__uint_as_float(c.key));
-        key = c.key;
-        ties = c.ties < c.here ? c.ties : ~0ull;
+        __syncthreads();
+        Cut c;
+        if (find_cut<false>(row, sh.bin_count, (u64)top_k, near, sh, turn, c)) {
+            cut_k = true;
+            key = c.key;
+            ties = c.ties < c.equal ? c.ties : ~0ull;
+        }
     }
     if (top_p < 1.f) {
+        // the weight of what is left; where top_k has left little, its histogram too
+        u64 own = 0;
+        row.each([&](int, const float (&s)[PIECE]) {
+#pragma unroll
+            for (int i = 0; i < PIECE; i++) {
+                const unsigned bits = __float_as_uint(s[i]);
+                if (bits <= key && counts(s[i])) {
+                    const unsigned w = weight(s[i]);
+                    if (cut_k) atomicAdd(&sh.bin_weight[(int)(s[i] * PER_OCTAVE)], (u64)w);
+                    if (bits < key || ties == ~0ull) own += w;
+                }
+            }
+        });
+        u64 total = over_all(own, sh, turn);
+        if (ties != ~0ull) total += ties * weight(__uint_as_float(key));
         const double share_p = ceil((double)top_p * (double)total);
         const u64 need = share_p > 1.0 ? (u64)share_p : 1;
         if (need < total) {
-            const Cut c = find_cut<true>(row, need, limit, sh, turn);
-            key = c.key;
-            ties = c.ties < c.here ? c.ties : ~0ull;
+            float bound = INFINITY;
+            if (!cut_k) {
+                // what lies beyond `bound` weighs less than what top_p leaves out, even if all of the vocabulary lies there
+                const float each = (float)(total - need) / (float)k.V - 1.f;
+                if (each > 1.f) bound = 31.01f - __builtin_amdgcn_logf(each);
+                row.each([&](int, const float (&s)[PIECE]) {
+#pragma unroll
+                    for (int i = 0; i < PIECE; i++)
+                        if (s[i] <= bound && counts(s[i])) atomicAdd(&sh.bin_weight[(int)(s[i] * PER_OCTAVE)], (u64)weight(s[i]));
+                });
+                __syncthreads();
+            }
+            Cut c;
+            auto near = [&](float s) { return s <= bound && __float_as_uint(s) <= key && counts(s); };
+            if (find_cut<true>(row, sh.bin_weight, need, near, sh, turn, c)) {
+                key = c.key;
+                ties = c.ties < c.equal ? c.ties : ~0ull;
+            }
         }
     }
     // ties by index: how many of the values equal to the cut lie before each wavefront's piece of each chunk
@@ -387,7 +445,7 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
 #pragma unroll
         for (int i = 0; i < PIECE; i++) {
             const unsigned bits = __float_as_uint(s[i]);
-            w[i] = bits <= key && (bits < key || rank++ < ties) ? weight(s[i]) : 0;
+            w[i] = bits <= key && counts(s[i]) && (bits < key || rank++ < ties) ? weight(s[i]) : 0;
             all += w[i];
         }
         return all;
@@ -408,7 +466,7 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
         }
     }
     __syncthreads();
-    total = sh.sums[entries - 1];
+    const u64 total = sh.sums[entries - 1];
     const float u = k.u[r];
     u64 target = u > 0.f ? (u64)fmin((double)u * (double)total, 9007199254740991.0) : 0;
     target = target < total ? target : total - 1;
