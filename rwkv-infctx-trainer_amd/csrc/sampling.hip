@@ -91,35 +91,62 @@ template <class T, int N> struct Row {
             for (int i = 0; i < PIECE; i++) o[i] = at + i >= 0 && at + i < V ? to_float(p[at + i]) : -INFINITY;
         }
 #pragma unroll
-        for (int i = 0; i < PIECE; i++) o[i] = o[i] != o[i] ? -INFINITY : o[i];
+        for (int i = 0; i < PIECE; i++) o[i] = fmaxf(o[i], -INFINITY);          // (of a NaN and a number the number)
     }
     __device__ __forceinline__ void place(float (&o)[PIECE]) const {
+        if (top == INFINITY) {
 #pragma unroll
-        for (int i = 0; i < PIECE; i++) o[i] = o[i] == -INFINITY ? INFINITY : o[i] == top ? 0.f : (top - o[i]) * scale;
+            for (int i = 0; i < PIECE; i++) o[i] = o[i] == INFINITY ? 0.f : INFINITY;
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECE; i++) o[i] = (top - o[i]) * scale;          // (-infinity: infinity)
+        }
     }
-    // f(chunk, its piece's s)
+    // f(chunk, its piece's s), from the registers where they hold it
     template <class F> __device__ __forceinline__ void each(F f) {
         if constexpr (N > 0) {
 #pragma unroll
             for (int c = 0; c < N; c++) f(c, s[c]);
         } else {
-            for (int c = 0; c < chunks; c++) {
-                raw(c, s[0]);
-                place(s[0]);
-                f(c, s[0]);
-            }
+            each_again(f);
         }
+    }
+    // the same read again, in a short loop: for what is rare
+    template <class F> __device__ __forceinline__ void each_again(F f) const {
+#pragma unroll 1
+        for (int c = 0; c < chunks; c++) {
+            float o[PIECE];
+            read(c, o);
+            f(c, o);
+        }
+    }
+    __device__ __forceinline__ void read(int c, float (&o)[PIECE]) const {
+        raw(c, o);
+        place(o);
     }
 };
 
 __device__ __forceinline__ unsigned weight(float s) { return (unsigned)rintf(exp2_fast(-s) * (float)ONE); }
+
+// the largest bits of s whose weight is at least `least`: 64 of them tried at once
+__device__ __forceinline__ unsigned last_of_weight(unsigned least) {
+    unsigned lo = 0, hi = __float_as_uint(MOST);          // it lies in [lo, hi)
+    while (hi - lo > 1) {
+        const unsigned step = (hi - lo + 63) / 64, at = lo + (threadIdx.x & 63) * step;
+        const u64 reached = __ballot(at < hi && weight(__uint_as_float(at)) >= least);
+        const int last = 63 - __clzll((long long)reached);          // (lane 0's does: that of lo)
+        hi = min(hi, lo + (last + 1) * step);
+        lo += last * step;
+    }
+    return lo;
+}
 
 constexpr int LIST = 1024;                     // elements of one bin that one wavefront searches
 struct Shared {
     u64 bin_weight[BINS];
     unsigned bin_count[BINS];
     float list[LIST];
-    unsigned listed;
+    unsigned list_weight[LIST], listed;
     u64 sums[WAVES * MAX_CHUNKS];          // by chunk and wavefront
     unsigned ties[WAVES * MAX_CHUNKS];
     u64 red[2][WAVES];
@@ -174,16 +201,17 @@ struct Cut {
     u64 equal;             // how many are equal
 };
 
-// Where the first `need` (of tokens, or of weight) in the order of s end, from the histogram `in` of the elements that count; false if
-// there is less than that.  counts(s): whether an element does.
-template <bool WEIGHT, class E, class R, class F>
-__device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, F counts, Shared &sh, int &turn, Cut &cut) {
+// Where the first `need` (of tokens, or of weight) in the order of s end, from the histogram `in` of the elements up to `most` (bits of s); false if
+// there is less than that
+template <bool WEIGHT, class E, class R>
+__device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, unsigned most, Shared &sh, int &turn, Cut &cut) {
     int bin;
     u64 before;
     if (threadIdx.x == 0) sh.listed = 0;
     if (!find_bin(in, need, sh, turn, bin, before)) return false;
-    const float lo_s = bin * (1.f / PER_OCTAVE), hi_s = (bin + 1) * (1.f / PER_OCTAVE);
-    auto inside = [&](float s) { return s >= lo_s && s < hi_s && counts(s); };
+    // the bin's values (the products are exact)
+    const unsigned first = __float_as_uint(bin * (1.f / PER_OCTAVE)), span = min(__float_as_uint((bin + 1) * (1.f / PER_OCTAVE)) - 1, most) - first;
+    auto inside = [&](float s) { return __float_as_uint(s) - first <= span; };
     row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
         for (int i = 0; i < PIECE; i++)
@@ -196,39 +224,32 @@ __device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, F counts
     const unsigned m = sh.listed;
     if (m <= LIST) {
         if (threadIdx.x < 64) {
-            constexpr int EACH = LIST / 64;
-            unsigned v[EACH], w[EACH], lo = 0xffffffffu, hi = 0;
-#pragma unroll
-            for (int i = 0; i < EACH; i++) {
-                const bool there = i * 64 + threadIdx.x < m;
-                const float s = there ? sh.list[i * 64 + threadIdx.x] : 0.f;
-                v[i] = there ? __float_as_uint(s) : 0xffffffffu;
-                w[i] = there ? (WEIGHT ? weight(s) : 1u) : 0u;
-                lo = min(lo, v[i]);
-                hi = there ? max(hi, v[i]) : hi;
+            unsigned lo = 0xffffffffu, hi = 0;
+            for (unsigned i = threadIdx.x; i < m; i += 64) {
+                const float s = sh.list[i];
+                if (WEIGHT) sh.list_weight[i] = weight(s);
+                lo = min(lo, __float_as_uint(s));
+                hi = max(hi, __float_as_uint(s));
             }
 #pragma unroll
             for (int d = 32; d > 0; d >>= 1) {
                 lo = min(lo, (unsigned)__shfl_xor((int)lo, d));
                 hi = max(hi, (unsigned)__shfl_xor((int)hi, d));
             }
-            auto upto = [&](unsigned key) {          // the weight of the values up to it
+            auto sum = [&](unsigned from, unsigned to, bool weights) {          // of the values from .. to (a lane reads what it has written)
                 u64 n = 0;
-#pragma unroll
-                for (int i = 0; i < EACH; i++)
-                    if (i * 64 < m) n += v[i] <= key ? w[i] : 0u;
+                for (unsigned i = threadIdx.x; i < m; i += 64) {
+                    const unsigned bits = __float_as_uint(sh.list[i]);
+                    n += bits >= from && bits <= to ? (weights ? sh.list_weight[i] : 1u) : 0u;
+                }
                 return last_lane(up_to(n));
             };
             while (lo < hi) {
                 const unsigned mid = lo + ((hi - lo) >> 1);
-                if (before + upto(mid) >= need) hi = mid;
+                if (before + sum(0, mid, WEIGHT) >= need) hi = mid;
                 else lo = mid + 1;
             }
-            u64 n = 0;
-#pragma unroll
-            for (int i = 0; i < EACH; i++) n += v[i] == lo;
-            n = last_lane(up_to(n));
-            const u64 below = lo ? upto(lo - 1) : 0;
+            const u64 n = sum(lo, lo, false), below = lo ? sum(0, lo - 1, WEIGHT) : 0;
             if (threadIdx.x == 0) {
                 sh.key = lo;
                 sh.equal = n;
@@ -241,7 +262,7 @@ __device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, F counts
         cut.before = sh.total;
     } else {          // too many for that, most likely equal ones: the same search by all, over the registers
         unsigned lo = 0xffffffffu, hi = 0;
-        row.each([&](int, const float (&s)[PIECE]) {
+        row.each_again([&](int, const float (&s)[PIECE]) {
 #pragma unroll
             for (int i = 0; i < PIECE; i++)
                 if (inside(s[i])) {
@@ -265,7 +286,7 @@ __device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, F counts
         turn ^= 1;
         auto sum = [&](unsigned from, unsigned to, bool weights) {          // of the values from .. to
             u64 n = 0;
-            row.each([&](int, const float (&s)[PIECE]) {
+            row.each_again([&](int, const float (&s)[PIECE]) {
 #pragma unroll
                 for (int i = 0; i < PIECE; i++)
                     if (__float_as_uint(s[i]) >= from && __float_as_uint(s[i]) <= to && inside(s[i])) n += weights ? weight(s[i]) : 1;
@@ -343,25 +364,25 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
 #pragma unroll
         for (int c = 0; c < N; c++) row.place(row.s[c]);
     }
-    // a token counts from a weight of 1, or of min_p's share; `reach` is a little more than the s of that
+    // a token counts from a weight of 1, or of min_p's share: up to the bits `most` of s
     const double share = (double)min_p * ONE;
     const unsigned least = share > 1.0 ? share < ONE ? (unsigned)ceil(share) : (unsigned)ONE : 1u;
-    const float reach = fminf(MOST, 31.01f - __builtin_amdgcn_logf((float)least - 0.5f));
+    const unsigned most = least == 1 ? __float_as_uint(MOST) - 1 : last_of_weight(least);
     int turn = 0;
-    unsigned key = 0x7f800000u;          // (the bits of infinity: all that count)
+    unsigned key = most;
     u64 ties = ~0ull;
-    auto counts = [&](float s) { return s < reach && (least == 1 || weight(s) >= least); };
     bool cut_k = false;
     if (top_k > 0 && top_k < k.V) {
-        // every lane has an element within `bound`: the first 1024 are there
-        float far[PIECE] = {least_best, least_best, least_best, least_best, least_best, least_best, least_best, least_best};
+        // every lane has an element within `far`: the first 1024 are there
+        float far[PIECE];
+#pragma unroll
+        for (int i = 0; i < PIECE; i++) far[i] = least_best;
         row.place(far);
-        const float bound = top_k <= THREADS ? far[0] : INFINITY;
-        auto near = [&](float s) { return s <= bound && counts(s); };
+        const unsigned near = top_k <= THREADS ? min(most, __float_as_uint(far[0])) : most;
         row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
             for (int i = 0; i < PIECE; i++)
-                if (near(s[i])) atomicAdd(&sh.bin_count[(int)(s[i] * PER_OCTAVE)], 1u);
+                if (__float_as_uint(s[i]) <= near) atomicAdd(&sh.bin_count[(int)(s[i] * PER_OCTAVE)], 1u);
         });
         __syncthreads();
         Cut c;
@@ -374,36 +395,41 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     if (top_p < 1.f) {
         // the weight of what is left; where top_k has left little, its histogram too
         u64 own = 0;
-        row.each([&](int, const float (&s)[PIECE]) {
+        if (cut_k) {
+            row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
-            for (int i = 0; i < PIECE; i++) {
-                const unsigned bits = __float_as_uint(s[i]);
-                if (bits <= key && counts(s[i])) {
-                    const unsigned w = weight(s[i]);
-                    if (cut_k) atomicAdd(&sh.bin_weight[(int)(s[i] * PER_OCTAVE)], (u64)w);
-                    if (bits < key || ties == ~0ull) own += w;
-                }
-            }
-        });
+                for (int i = 0; i < PIECE; i++)
+                    if (__float_as_uint(s[i]) <= key) {
+                        const unsigned w = weight(s[i]);
+                        atomicAdd(&sh.bin_weight[(int)(s[i] * PER_OCTAVE)], (u64)w);
+                        if (__float_as_uint(s[i]) < key || ties == ~0ull) own += w;
+                    }
+            });
+        } else {
+            row.each([&](int, const float (&s)[PIECE]) {
+#pragma unroll
+                for (int i = 0; i < PIECE; i++)
+                    if (__float_as_uint(s[i]) <= key) own += weight(s[i]);
+            });
+        }
         u64 total = over_all(own, sh, turn);
         if (ties != ~0ull) total += ties * weight(__uint_as_float(key));
         const double share_p = ceil((double)top_p * (double)total);
         const u64 need = share_p > 1.0 ? (u64)share_p : 1;
         if (need < total) {
-            float bound = INFINITY;
+            unsigned near = key;
             if (!cut_k) {
-                // what lies beyond `bound` weighs less than what top_p leaves out, even if all of the vocabulary lies there
+                // what lies beyond weighs less than what top_p leaves out, even if all of the vocabulary lies there
                 const float each = (float)(total - need) / (float)k.V - 1.f;
-                if (each > 1.f) bound = 31.01f - __builtin_amdgcn_logf(each);
+                if (each > 1.f) near = min(near, __float_as_uint(31.01f - __builtin_amdgcn_logf(each)));
                 row.each([&](int, const float (&s)[PIECE]) {
 #pragma unroll
                     for (int i = 0; i < PIECE; i++)
-                        if (s[i] <= bound && counts(s[i])) atomicAdd(&sh.bin_weight[(int)(s[i] * PER_OCTAVE)], (u64)weight(s[i]));
+                        if (__float_as_uint(s[i]) <= near) atomicAdd(&sh.bin_weight[(int)(s[i] * PER_OCTAVE)], (u64)weight(s[i]));
                 });
                 __syncthreads();
             }
             Cut c;
-            auto near = [&](float s) { return s <= bound && __float_as_uint(s) <= key && counts(s); };
             if (find_cut<true>(row, sh.bin_weight, need, near, sh, turn, c)) {
                 key = c.key;
                 ties = c.ties < c.equal ? c.ties : ~0ull;
@@ -420,9 +446,9 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
         return n;
     };
     if (some_ties) {
-        row.each([&](int c, const float (&s)[PIECE]) {
+        row.each_again([&](int c, const float (&s)[PIECE]) {
             const u64 all = last_lane(up_to(equal(s)));
-            if (lane == 0 && c < row.chunks) sh.ties[c * WAVES + wave] = (unsigned)all;
+            if (lane == 0) sh.ties[c * WAVES + wave] = (unsigned)all;
         });
         __syncthreads();
         if (wave == 0) {
@@ -437,23 +463,32 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     }
     // the kept weights by index
     auto kept = [&](int c, const float (&s)[PIECE], unsigned (&w)[PIECE]) {
-        u64 rank = 0, all = 0;
-        if (some_ties && c < row.chunks) {
-            const int n = equal(s);
-            rank = sh.ties[c * WAVES + wave] + up_to(n) - n;
-        }
+        const int n = equal(s);
+        u64 rank = sh.ties[c * WAVES + wave] + up_to(n) - n, all = 0;
 #pragma unroll
         for (int i = 0; i < PIECE; i++) {
-            const unsigned bits = __float_as_uint(s[i]);
-            w[i] = bits <= key && counts(s[i]) && (bits < key || rank++ < ties) ? weight(s[i]) : 0;
+            // (selections: as branches around weight() the compiler lost the weight of the ties that stay)
+            const unsigned bits = __float_as_uint(s[i]), each = weight(fminf(s[i], MOST));
+            const bool tie = bits == key, stays = (bits < key) | (tie & (!some_ties | (rank < ties)));
+            rank += tie;
+            w[i] = stays ? each : 0;
             all += w[i];
         }
         return all;
     };
     row.each([&](int c, const float (&s)[PIECE]) {
-        unsigned w[PIECE];
-        const u64 all = last_lane(up_to(kept(c, s, w)));
-        if (lane == 0 && c < row.chunks) sh.sums[c * WAVES + wave] = all;
+        if (c >= row.chunks) return;
+        u64 all = 0;
+        if (some_ties) {
+            unsigned w[PIECE];
+            all = kept(c, s, w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < PIECE; i++)
+                if (__float_as_uint(s[i]) <= key) all += weight(s[i]);
+        }
+        all = last_lane(up_to(all));
+        if (lane == 0) sh.sums[c * WAVES + wave] = all;
     });
     __syncthreads();
     // the entry with the target, by wavefront 0
@@ -470,14 +505,15 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     const float u = k.u[r];
     u64 target = u > 0.f ? (u64)fmin((double)u * (double)total, 9007199254740991.0) : 0;
     target = target < total ? target : total - 1;
-    row.each([&](int c, const float (&s)[PIECE]) {
-        if (c >= row.chunks) return;
+    for (int c = 0; c < row.chunks; c++) {
         const int e = c * WAVES + wave;
         const u64 before = e ? sh.sums[e - 1] : 0;
-        if (target < before || target >= sh.sums[e]) return;          // (the wavefront's)
+        if (target < before || target >= sh.sums[e]) continue;          // (the same for the wavefront)
+        float s[PIECE];
         unsigned w[PIECE];
+        row.read(c, s);
         const u64 own = kept(c, s, w), upto = up_to(own) + before;
-        if (target < upto - own || target >= upto) return;            // one lane is left
+        if (target < upto - own || target >= upto) break;               // one lane is left
         u64 at = upto - own;
         bool done = false;
 #pragma unroll
@@ -489,7 +525,8 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
                 k.logprob[r] = (float)log((double)w[i] / (double)total);
             }
         }
-    });
+        break;
+    }
 }
 
 template <class T> static hipError_t launch(hipStream_t s, const Call &k) {
