@@ -316,7 +316,7 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     const float temperature = k.temperature ? k.temperature[r] : k.temperature_value;
     const float top_p = k.top_p ? k.top_p[r] : k.top_p_value, min_p = k.min_p ? k.min_p[r] : k.min_p_value;
     const bool warm = temperature >= 1e-6f;
-    const int top_k = !warm ? 1 : k.top_k ? k.top_k[r] : k.top_k_value;
+    const int top_k = k.top_k ? k.top_k[r] : k.top_k_value;
     // the largest logit of the lane and of all
     float best = -INFINITY;
     if constexpr (N > 0) {
@@ -363,6 +363,24 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     if constexpr (N > 0) {
 #pragma unroll
         for (int c = 0; c < N; c++) row.place(row.s[c]);
+    }
+    if (!warm) {          // the first of the likeliest
+        unsigned at = ~0u;
+        row.each([&](int c, const float (&s)[PIECE]) {
+#pragma unroll
+            for (int i = 0; i < PIECE; i++)
+                if (s[i] == 0.f) at = min(at, (unsigned)(row.first(c) + i));
+        });
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) at = min(at, (unsigned)__shfl_xor((int)at, m));
+        if (lane == 0) sh.red[0][wave] = at;
+        __syncthreads();
+        if (tid == 0) {
+            for (int i = 1; i < WAVES; i++) at = min(at, (unsigned)sh.red[0][i]);
+            k.token[r] = at;
+            k.logprob[r] = 0.f;
+        }
+        return;
     }
     // a token counts from a weight of 1, or of min_p's share: up to the bits `most` of s
     const double share = (double)min_p * ONE;
