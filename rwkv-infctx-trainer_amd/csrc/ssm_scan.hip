@@ -664,18 +664,20 @@ __global__ __launch_bounds__(256) void decode(const Call k) {
 static inline int states_per_lane(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4; }
 static inline long long workgroups(int B, int D, int G, int channels) { return (long long)B * G * ((D / G + channels - 1) / channels); }
 
-// Segments of a sequence: as many as give every compute unit `per_cu` workgroups, none shorter than eight tiles (a segment's
-// start costs it one summary per segment before it)
+// Segments of a sequence: as many as give every compute unit `per_cu` workgroups, of eight tiles or more (of four up to four segments).
+// A cut costs a pass over the inputs without outputs, so it pays where workgroups are few: forward B1 T4096 D4096 281 us with one per compute unit,
+// 230 with two, 173 with four, but B4 T777 D4096 96 us uncut and 114 in two segments; forward and backward B1 T4096 D4096 (128 workgroups of
+// the backward) 815, 707 and 706 us with one, two and four of them, B1 T2048 D1536 (48) 177, 170, 144, B4 T1024 D4096 (512) 438 uncut, 501 in two.
 static inline int segments_for(long long groups, int tiles, int per_cu) {
-    if (tiles < 16) return 1;
     const long long want = ((long long)per_cu * cu_count() + groups - 1) / groups;
-    return (int)std::max(1ll, std::min({want, (long long)tiles / 8, 64ll}));
+    return (int)std::max(1ll, std::min({want, (long long)std::max(tiles / 8, std::min(4, tiles / 4)), 64ll}));
 }
 struct Plan { int tiles, segments, seg_tiles; };
 static inline Plan plan(int B, int T, int D, int G, bool backward) {
     Plan p;
     p.tiles = (T + TILE - 1) / TILE;
-    p.segments = segments_for(workgroups(B, D, G, backward ? 4 * BACK_WAVES : 16), p.tiles, backward ? 1 : 2);
+    const long long groups = workgroups(B, D, G, backward ? 4 * BACK_WAVES : 16);
+    p.segments = segments_for(groups, p.tiles, !backward || 2 * groups < cu_count() ? 4 : 2);
     p.seg_tiles = (p.tiles + p.segments - 1) / p.segments;
     p.segments = (p.tiles + p.seg_tiles - 1) / p.seg_tiles;
     return p;
