@@ -9,7 +9,9 @@
 #include <Python.h>
 #include <ATen/ATen.h>
 #include <ATen/TracerMode.h>
+#include <ATen/EmptyTensor.h>
 #include <ATen/autocast_mode.h>
+#include <ATen/hip/HIPContextLight.h>
 #include <c10/hip/HIPGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>

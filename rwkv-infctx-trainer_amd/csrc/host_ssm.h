@@ -1,6 +1,14 @@
 // The state space operators and sampling: checks, allocation and autograd nodes over the entry points of csrc/ssm_api.hip.
 // (Part of host.cpp.)
 
+// A new tensor on the current device, straight from its caching allocator: through the dispatcher it takes half as long again, and
+// a single token's call makes two or three of them.
+Tensor fresh(at::IntArrayRef sizes, at::ScalarType type) {
+    static c10::Allocator *const allocator = at::cuda::getCUDADeviceAllocator();
+    return at::detail::empty_generic(sizes, allocator, c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
+Tensor fresh_bytes(size_t n) { return fresh({(int64_t)std::max<size_t>(n, 16)}, at::kByte); }
+
 // ---- operands
 void same_device(const Tensor &x, std::initializer_list<const Tensor *> others) {
     on_gpu(x);
@@ -64,7 +72,7 @@ public:
         const Tensor b = bias.defined() ? plain(as_type(bias, w.scalar_type())) : bias, s = plain(state);
         const int B = fits_int(x.size(0)), T = fits_int(x.size(1)), D = fits_int(x.size(2)), W = fits_int(w.size(1)), dt = dtype_code(x);
         OnDevice dev(x);
-        const Tensor y = at::empty({B, T, D}, x.options()), out = out_state.defined() ? out_state : at::empty({B, W - 1, D}, x.options());
+        const Tensor y = fresh({B, T, D}, x.scalar_type()), out = out_state.defined() ? out_state : fresh({B, W - 1, D}, x.scalar_type());
         const wkv_rows rows = rows_of(x);
         check(abi.wkv_causal_conv_forward(dev.stream(), B, T, D, W, dt, dtype_code(w), silu, &rows, ptr(w), ptr(b), ptr(s), iptr(lengths), ptr(y), ptr(out)),
               "wkv_causal_conv_forward");
@@ -83,8 +91,8 @@ public:
         const int B = x.size(0), T = x.size(1), D = x.size(2), W = w.size(1), dt = dtype_code(x);
         OnDevice dev(x);
         const Tensor gy = grads[0].defined() ? plain(grads[0]) : at::zeros({B, T, D}, x.options()), gout = plain(grads[1]);
-        const Tensor gx = at::empty({B, T, D}, x.options()), gw = at::empty_like(w), gb = b.defined() ? at::empty_like(b) : Tensor();
-        const Tensor gs = s.defined() ? at::empty_like(s) : Tensor(), ws = bytes(abi.wkv_causal_conv_backward_workspace(B, T, D, W, dt), x);
+        const Tensor gx = fresh({B, T, D}, x.scalar_type()), gw = fresh(w.sizes(), w.scalar_type()), gb = b.defined() ? fresh(b.sizes(), b.scalar_type()) : Tensor();
+        const Tensor gs = s.defined() ? fresh(s.sizes(), s.scalar_type()) : Tensor(), ws = fresh_bytes(abi.wkv_causal_conv_backward_workspace(B, T, D, W, dt));
         const wkv_rows rows = rows_of(x);
         check(abi.wkv_causal_conv_backward(dev.stream(), B, T, D, W, dt, dtype_code(w), c[0], &rows, ptr(w), ptr(b), ptr(s), iptr(v[4]), ptr(gy), ptr(gout),
                                            ptr(gx), ptr(gw), ptr(gb), ptr(gs), ptr(ws), ws.numel()), "wkv_causal_conv_backward");
@@ -132,10 +140,10 @@ public:
         const Tensor b = strided(B_.dim() == 3 ? B_.unsqueeze(2) : B_), c = strided(C_.dim() == 3 ? C_.unsqueeze(2) : C_), s = plain_float(state_);
         const int B = fits_int(x.size(0)), T = fits_int(x.size(1)), D = fits_int(x.size(2)), N = fits_int(A.size(1)), G = fits_int(b.size(2)), t = dtype_code(x);
         OnDevice dev(x);
-        const Tensor y = at::empty({B, T, D}, x.options()), out = out_state.defined() ? out_state : at::empty({B, D, N}, A.options());
-        const Tensor kept = ctx ? bytes(abi.wkv_selective_scan_checkpoint_bytes(B, T, D, N, G, t), x) : Tensor();
+        const Tensor y = fresh({B, T, D}, x.scalar_type()), out = out_state.defined() ? out_state : fresh({B, D, N}, at::kFloat);
+        const Tensor kept = ctx ? fresh_bytes(abi.wkv_selective_scan_checkpoint_bytes(B, T, D, N, G, t)) : Tensor();
         const size_t need = abi.wkv_selective_scan_forward_workspace(B, T, D, N, G, t);
-        const Tensor ws = need ? bytes(need, x) : Tensor();
+        const Tensor ws = need ? fresh_bytes(need) : Tensor();
         const wkv_rows rx = rows_of(x), rdt = rows_of(dt), rz = rows_of(z), rb = rows_of(b), rc = rows_of(c);
         check(abi.wkv_selective_scan_forward(dev.stream(), B, T, D, N, G, t, &rx, &rdt, fptr(A), &rb, &rc, fptr(skip), z.defined() ? &rz : nullptr, fptr(bias),
                                              fptr(s), iptr(lengths), ptr(y), fptr(out), fptr(kept), ptr(ws), need), "wkv_selective_scan_forward");
@@ -154,13 +162,13 @@ public:
         const Tensor &x = v[0], &dt = v[1], &A = v[2], &b = v[3], &c = v[4], &skip = v[5], &z = v[6], &bias = v[7], &lengths = v[8], &kept = v[9];
         const int B = x.size(0), T = x.size(1), D = x.size(2), N = A.size(1), G = b.size(2), t = dtype_code(x);
         OnDevice dev(x);
-        auto like_x = [&] { return at::empty({B, T, D}, x.options()); };
+        auto like_x = [&] { return fresh({B, T, D}, x.scalar_type()); };
         const Tensor gy = grads[0].defined() ? plain(grads[0]) : at::zeros({B, T, D}, x.options()), gout = plain_float(grads[1]);
-        const Tensor gx = like_x(), gdt = like_x(), gz = z.defined() ? like_x() : Tensor(), gA = at::empty_like(A);
-        const Tensor gb = at::empty({B, T, G, N}, x.options()), gc = at::empty({B, T, G, N}, x.options());
-        const Tensor gskip = skip.defined() ? at::empty_like(skip) : Tensor(), gbias = bias.defined() ? at::empty_like(bias) : Tensor();
-        const Tensor gs = k[5] ? at::empty({B, D, N}, A.options()) : Tensor();
-        const Tensor ws = bytes(abi.wkv_selective_scan_backward_workspace(B, T, D, N, G, t), x);
+        const Tensor gx = like_x(), gdt = like_x(), gz = z.defined() ? like_x() : Tensor(), gA = fresh(A.sizes(), at::kFloat);
+        const Tensor gb = fresh({B, T, G, N}, x.scalar_type()), gc = fresh({B, T, G, N}, x.scalar_type());
+        const Tensor gskip = skip.defined() ? fresh(skip.sizes(), at::kFloat) : Tensor(), gbias = bias.defined() ? fresh(bias.sizes(), at::kFloat) : Tensor();
+        const Tensor gs = k[5] ? fresh({B, D, N}, at::kFloat) : Tensor();
+        const Tensor ws = fresh_bytes(abi.wkv_selective_scan_backward_workspace(B, T, D, N, G, t));
         const wkv_rows rx = rows_of(x), rdt = rows_of(dt), rz = rows_of(z), rb = rows_of(b), rc = rows_of(c);
         check(abi.wkv_selective_scan_backward(dev.stream(), B, T, D, N, G, t, &rx, &rdt, fptr(A), &rb, &rc, fptr(skip), z.defined() ? &rz : nullptr, fptr(bias),
                                               iptr(lengths), fptr(kept), ptr(gy), fptr(gout), ptr(gx), ptr(gdt), fptr(gA), ptr(gb), ptr(gc), fptr(gskip),
@@ -232,8 +240,8 @@ public:
         const Tensor residual = given(residual_);
         const NormOperands v(x, weight, residual);
         OnDevice dev(v.x);
-        const Tensor y = at::empty(x.sizes(), x.options()), sum = residual.defined() ? at::empty(residual.sizes(), residual.options()) : Tensor();
-        const Tensor rstd = ctx ? at::empty({v.rows}, x.options().dtype(at::kFloat)) : Tensor();
+        const Tensor y = fresh(x.sizes(), x.scalar_type()), sum = residual.defined() ? fresh(residual.sizes(), residual.scalar_type()) : Tensor();
+        const Tensor rstd = ctx ? fresh({v.rows}, at::kFloat) : Tensor();
         check(abi.wkv_rms_norm_forward(dev.stream(), v.rows, v.C, v.dt, v.rt, v.wt, (float)eps, ptr(v.x), row_stride(v.x), ptr(v.residual),
                                        row_stride(v.residual), ptr(v.weight), ptr(y), nullptr, nullptr, ptr(sum), fptr(rstd)), "wkv_rms_norm_forward");
         if (ctx) {
@@ -255,13 +263,13 @@ public:
         const Tensor &weight = saved[2], &rstd = saved[3], &some = saved[0].defined() ? saved[0] : saved[1];
         const Tensor x = as_rows(saved[0]), residual = as_rows(saved[1]);
         OnDevice dev(some);
-        const auto options = some.options().dtype(type), wide = some.options().dtype(has_residual ? saved[1].scalar_type() : type);
+        const auto options = some.options().dtype(type);
         const Tensor gy = grads[0].defined() ? plain(grads[0]) : at::zeros(some.sizes(), options), gsum = has_residual ? plain(grads[1]) : Tensor();
-        const Tensor gx = at::empty(some.sizes(), options), gw = at::empty_like(weight);
+        const Tensor gx = fresh(some.sizes(), type), gw = fresh(weight.sizes(), weight.scalar_type());
         const bool two = has_residual && saved[1].scalar_type() != type;
-        const Tensor gres = two ? at::empty(some.sizes(), wide) : has_residual ? gx : Tensor();
+        const Tensor gres = two ? fresh(some.sizes(), saved[1].scalar_type()) : has_residual ? gx : Tensor();
         const int C = weight.size(0), R = rstd.size(0);
-        const Tensor ws = bytes(abi.wkv_rms_norm_backward_workspace(R, C), some);
+        const Tensor ws = fresh_bytes(abi.wkv_rms_norm_backward_workspace(R, C));
         check(abi.wkv_rms_norm_backward(dev.stream(), R, C, dtype_code(gx), has_residual ? dtype_code(saved[1]) : dtype_code(gx), dtype_code(weight), ptr(x),
                                         row_stride(x), ptr(residual), row_stride(residual), ptr(weight), fptr(rstd), ptr(gy), ptr(gsum), ptr(gx),
                                         two ? ptr(gres) : nullptr, ptr(gw), ptr(ws), ws.numel()), "wkv_rms_norm_backward");
@@ -320,9 +328,9 @@ PyObject *py_rms_norm_fp8(PyObject *, PyObject *const *a, Py_ssize_t n) {
         OnDevice dev(v.x);
         std::vector<int64_t> one = x.sizes().vec();
         one.back() = 1;
-        q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-        scale = at::empty(one, x.options().dtype(at::kFloat));
-        sum = r.defined() ? at::empty(r.sizes(), r.options()) : Tensor();
+        q = fresh(x.sizes(), at::kFloat8_e4m3fn);
+        scale = fresh(one, at::kFloat);
+        sum = r.defined() ? fresh(r.sizes(), r.scalar_type()) : Tensor();
         check(abi.wkv_rms_norm_forward(dev.stream(), v.rows, v.C, v.dt, v.rt, v.wt, (float)eps, ptr(v.x), row_stride(v.x), ptr(v.residual),
                                        row_stride(v.residual), ptr(v.weight), nullptr, ptr(q), fptr(scale), ptr(sum), nullptr), "wkv_rms_norm_forward");
     }
@@ -366,8 +374,8 @@ PyObject *py_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
         for (Setting *s : {&temperature, &top_p, &min_p}) s->settle(l, at::kFloat);
         top_k.settle(l, at::kInt);
         const int rows = fits_int(l.size(0));
-        token = at::empty({rows}, l.options().dtype(at::kLong));
-        logprob = at::empty({rows}, l.options().dtype(at::kFloat));
+        token = fresh({rows}, at::kLong);
+        logprob = fresh({rows}, at::kFloat);
         check(abi.wkv_sample(dev.stream(), rows, fits_int(l.size(1)), dt, ptr(l), l.stride(0), fptr(u), fptr(temperature.rows), (float)temperature.value,
                              iptr(top_k.rows), (int)std::max(0.0, std::min(top_k.value, 2147483647.0)), fptr(top_p.rows), (float)top_p.value, fptr(min_p.rows),
                              (float)min_p.value, static_cast<long long *>(ptr(token)), fptr(logprob)), "wkv_sample");
