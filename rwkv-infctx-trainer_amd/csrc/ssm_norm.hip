@@ -223,10 +223,11 @@ __global__ __launch_bounds__(64 * WAVES) void backward(const Call k) {
         });
 }
 
-// Wavefronts per row and pieces per lane: one wavefront up to 1024 elements (no barrier), else four, 8192 elements in registers
+// Wavefronts per row and pieces per lane: one wavefront up to 1024 elements (no barrier), else four, 8192 elements in registers; rows that are not in
+// whole 8-element pieces go element by element, by four wavefronts (in registers too: read again, 5424 rows of 646 fp8 20 us, so 12)
 struct Shape { int waves, n; };
 static inline Shape shape_of(int C, bool wide) {
-    if (!wide) return {4, 0};
+    if (!wide) return {4, C <= 1024 ? 4 : C <= 4096 ? 16 : C <= 8192 ? 32 : 0};
     const int v = C / 8;
     if (v <= 64) return {1, 1};
     if (v <= 128) return {1, 2};
@@ -237,7 +238,10 @@ static inline int backward_groups(int rows, int C) { return std::max(1, std::min
 #define WKV_NORM_SHAPES(LAUNCH)                                          \
     do {                                                                 \
         const Shape f = shape_of(k.C, wide);                             \
-        if (!wide) LAUNCH(1, 0, 4);                                      \
+        if (!wide && f.n == 4) LAUNCH(1, 4, 4);                          \
+        else if (!wide && f.n == 16) LAUNCH(1, 16, 4);                   \
+        else if (!wide && f.n == 32) LAUNCH(1, 32, 4);                   \
+        else if (!wide) LAUNCH(1, 0, 4);                                 \
         else if (f.waves == 1 && f.n == 1) LAUNCH(8, 1, 1);              \
         else if (f.waves == 1) LAUNCH(8, 2, 1);                          \
         else if (f.n == 1) LAUNCH(8, 1, 4);                              \
