@@ -446,14 +446,16 @@ __global__ __launch_bounds__(256) void backward_summary(const Call k) {
 // Tiles from the last to the first.  Within a tile the state runs forward again from its checkpoint, leaving every token's decay a
 // and the state before it in registers, then the gradient runs back over them.  A tile's shares of gB and gC are added up over the
 // workgroup's channels in LDS after the next tile's barrier.
-constexpr int BACK_WAVES = 8;
+// Eight wavefronts share a workgroup's sums, two workgroups a compute unit (128 registers) up to 16 states; with four states per lane
+// 256 registers do not hold a tile (B2 T2048 D4096 N64: 3658 us), so four wavefronts have 512 each.
+constexpr int back_waves(int J) { return J == 4 ? 4 : 8; }
 template <class T, int J>
-__global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(const Call k) {
+__global__ __launch_bounds__(64 * back_waves(J), J == 1 ? 4 : J == 2 ? 2 : 1) void backward(const Call k) {
+    constexpr int BACK_WAVES = back_waves(J);
     typedef Work<T, J, BACK_WAVES, true, true> W;
     constexpr int TURNS = J == 1 ? 2 : 1;
     __shared__ __align__(16) float bc[2][2][W::STATES * PITCH];
     __shared__ __align__(16) float part[TURNS][BACK_WAVES][2][16 * PITCH];
-    static_assert(W::THREADS == 512, "a thread per element of both sums");
     W w(k);
     float a2[J], g[J], ga[J];
     w.load_a(a2);
@@ -467,20 +469,26 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
     const int begin = max(w.end - 1, w.first);
     Stream<T> sx = w.stream(k.x, begin), sdt = w.stream(k.dt, begin), sz = w.stream(gated ? k.z : k.x, begin);
     Packed<T> in_at = w.packed(begin), out_at = w.packed(w.last - 1);
-    // this thread's element of the workgroup's gB or gC
-    const int which = w.tid >> 8, token = (w.tid >> 4) & 15, state = w.tid & 15;
-    float *vectors = (which ? k.gc_part : k.gb_part) + (((size_t)w.ct * k.B + w.b) * k.T * k.G + w.g) * k.N;
-    auto add_up = [&](const float (&p)[BACK_WAVES][2][16 * PITCH], int tile, int j) {
-        float s = 0.f;
+    // the elements of the workgroup's gB and gC: 256 of each per tile and 16 states
+    auto elements = [&](int tile, int j, auto f) {
 #pragma unroll
-        for (int i = 0; i < BACK_WAVES; i++) s += p[i][which][state * PITCH + token];
-        const int t = tile * TILE + token;
-        if (t < k.T && state + 16 * j < k.N) vectors[(size_t)t * k.G * k.N + state + 16 * j] = s;
+        for (int e = w.tid; e < 512; e += W::THREADS) {
+            const int which = e >> 8, token = (e >> 4) & 15, state = e & 15, t = tile * TILE + token;
+            const float v = f(which, token, state);
+            if (t < k.T && state + 16 * j < k.N)
+                (which ? k.gc_part : k.gb_part)[((((size_t)w.ct * k.B + w.b) * k.T + t) * k.G + w.g) * k.N + state + 16 * j] = v;
+        }
+    };
+    auto add_up = [&](const float (&p)[BACK_WAVES][2][16 * PITCH], int tile, int j) {
+        elements(tile, j, [&](int which, int token, int state) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < BACK_WAVES; i++) s += p[i][which][state * PITCH + token];
+            return s;
+        });
     };
     auto nothing = [&](int tile) {
-        const int t = tile * TILE + token;
-        for (int j = 0; j < J; j++)
-            if (t < k.T && state + 16 * j < k.N) vectors[(size_t)t * k.G * k.N + state + 16 * j] = 0.f;
+        for (int j = 0; j < J; j++) elements(tile, j, [](int, int, int) { return 0.f; });
         const bool there = w.exists(tile);
         out_at.store(k.gx, there, 0.f);
         out_at.store(k.gdt, there, 0.f);
@@ -524,14 +532,14 @@ __global__ __launch_bounds__(64 * BACK_WAVES, J == 1 ? 4 : 2) void backward(cons
                 w.read(sb, j, vb);
                 w.read(sc, j, vc);
                 float gc[TILE];
-                const float dt1 = again(dt), dtx1 = again(dtx);
+                const float gy1 = again(gy), dt1 = again(dt), dtx1 = again(dtx);
                 unrolled<TILE>([&](auto i) {
                     constexpr int I = decltype(i)::value;
                     before[I] = h;
                     a[I] = exp2_fast(row_lane<I>(dt1) * a2[j]);
                     h = fmaf(a[I], h, row_lane<I>(dtx1) * vb[I]);
                     y[I] = j == 0 ? vc[I] * h : fmaf(vc[I], h, y[I]);
-                    gc[I] = row_lane<I>(gy) * h;
+                    gc[I] = row_lane<I>(gy1) * h;
                 });
                 if (j) lds_barrier();
                 *reinterpret_cast<f4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][1][w.n * PITCH + 4 * w.row]) = reduce_rows(gc);
@@ -673,10 +681,10 @@ static inline int segments_for(long long groups, int tiles, int per_cu) {
     return (int)std::max(1ll, std::min({want, (long long)std::max(tiles / 8, std::min(4, tiles / 4)), 64ll}));
 }
 struct Plan { int tiles, segments, seg_tiles; };
-static inline Plan plan(int B, int T, int D, int G, bool backward) {
+static inline Plan plan(int B, int T, int D, int N, int G, bool backward) {
     Plan p;
     p.tiles = (T + TILE - 1) / TILE;
-    const long long groups = workgroups(B, D, G, backward ? 4 * BACK_WAVES : 16);
+    const long long groups = workgroups(B, D, G, backward ? 4 * back_waves(states_per_lane(N)) : 16);
     p.segments = segments_for(groups, p.tiles, !backward || 2 * groups < cu_count() ? 4 : 2);
     p.seg_tiles = (p.tiles + p.segments - 1) / p.segments;
     p.segments = (p.tiles + p.seg_tiles - 1) / p.seg_tiles;
@@ -687,10 +695,11 @@ static inline size_t summary_bytes(int B, int D, int N, int segments) {
     return segments > 1 ? rounded((size_t)B * segments * D * 16 * states_per_lane(N) * 4) + rounded((size_t)B * segments * D * 4) : 0;
 }
 static inline size_t checkpoint_bytes(int B, int T, int D, int N) { return (size_t)B * ((T + TILE - 1) / TILE) * D * 16 * states_per_lane(N) * 4; }
-static inline size_t forward_scratch(int B, int T, int D, int N, int G) { return T == 1 ? 0 : summary_bytes(B, D, N, plan(B, T, D, G, false).segments); }
+static inline size_t forward_scratch(int B, int T, int D, int N, int G) { return T == 1 ? 0 : summary_bytes(B, D, N, plan(B, T, D, N, G, false).segments); }
 static inline size_t backward_scratch(int B, int T, int D, int N, int G) {
-    const Plan p = plan(B, T, D, G, true);
-    const size_t cts = (D / G + 4 * BACK_WAVES - 1) / (4 * BACK_WAVES), rows = (size_t)B * p.segments;
+    const Plan p = plan(B, T, D, N, G, true);
+    const int channels = 4 * back_waves(states_per_lane(N));
+    const size_t cts = (D / G + channels - 1) / channels, rows = (size_t)B * p.segments;
     return summary_bytes(B, D, N, p.segments) + 2 * rounded(cts * B * T * G * N * 4) + rounded(rows * D * N * 4) + 2 * rounded(rows * D * 4);
 }
 
@@ -732,7 +741,7 @@ template <class T> static hipError_t forward_t(hipStream_t s, Call k, void *scra
 #undef WKV_DECODE_SCAN
         return hipGetLastError();
     }
-    const Plan p = plan(k.B, k.T, k.D, k.G, false);
+    const Plan p = plan(k.B, k.T, k.D, k.N, k.G, false);
     k.tiles = p.tiles; k.segments = p.segments; k.seg_tiles = p.seg_tiles;
     const long long groups = workgroups(k.B, k.D, k.G, 16);
     if (p.segments > 1) {
@@ -749,7 +758,7 @@ template <class T> static hipError_t forward_t(hipStream_t s, Call k, void *scra
 struct Gradients { void *gb, *gc; float *ga, *gskip, *gbias; };
 template <class T> static hipError_t backward_t(hipStream_t s, Call k, const Gradients &to, void *scratch) {
     const int J = states_per_lane(k.N);
-    const Plan p = plan(k.B, k.T, k.D, k.G, true);
+    const Plan p = plan(k.B, k.T, k.D, k.N, k.G, true);
     k.tiles = p.tiles; k.segments = p.segments; k.seg_tiles = p.seg_tiles;
     char *at = static_cast<char *>(scratch);
     auto take = [&](size_t floats) {
@@ -757,7 +766,8 @@ template <class T> static hipError_t backward_t(hipStream_t s, Call k, const Gra
         at += rounded(floats * 4);
         return f;
     };
-    const size_t rows = (size_t)k.B * p.segments, cts = (k.Dg + 4 * BACK_WAVES - 1) / (4 * BACK_WAVES), vectors = (size_t)k.B * k.T * k.G * k.N;
+    const int channels = 4 * back_waves(J);
+    const size_t rows = (size_t)k.B * p.segments, cts = (k.Dg + channels - 1) / channels, vectors = (size_t)k.B * k.T * k.G * k.N;
     if (p.segments > 1) {
         k.seg_state = take(rows * k.D * 16 * J);
         k.seg_dt = take(rows * k.D);
@@ -771,7 +781,7 @@ template <class T> static hipError_t backward_t(hipStream_t s, Call k, const Gra
     k.ga_part = rows == 1 ? to.ga : take(rows * k.D * k.N);
     k.gskip_part = rows == 1 && to.gskip ? to.gskip : take(rows * k.D);
     k.gbias_part = rows == 1 && to.gbias ? to.gbias : take(rows * k.D);
-    WKV_SCAN_J(backward, workgroups(k.B, k.D, k.G, 4 * BACK_WAVES) * p.segments, 64 * BACK_WAVES, );
+    WKV_SCAN_J(backward, workgroups(k.B, k.D, k.G, channels) * p.segments, 16 * channels, );
     Sums<ToRow<T>> sums;
     sums.add((int)cts, vectors, k.gb_part, {to.gb, false});
     sums.add((int)cts, vectors, k.gc_part, {to.gc, false});
