@@ -10,7 +10,7 @@
 // The weights are whole numbers so that every sum is exact: no order of adding, no split over lanes changes a token.
 //
 // A workgroup of 16 wavefronts holds a row's s in registers (65536 elements; wider rows are read again for every pass) and
-// never sorts.  Each of the two cuts is found from a histogram over 1024 bins of s, of tokens for top_k and of weights for top_p, and
+// never sorts.  Each of the two cuts is found from a histogram over 4096 bins of s, of tokens for top_k and of weights for top_p, and
 // then among the elements of the bin it falls into, which one wavefront searches by the bits of s.  What bounds it is the passes over
 // the registers and the histograms' atomics in LDS, so these take only what a cut can reach: for top_k what is not
 // below every lane's best (1024 such there are), for top_p what the rest of the vocabulary could not outweigh.
@@ -20,8 +20,8 @@ namespace wkv {
 namespace sampling {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64, PIECE = 8, CHUNK = THREADS * PIECE;
-constexpr int BINS = 1024;
-constexpr float MOST = 32.f, PER_OCTAVE = 32.f;      // weights vanish at s = 32, in bin BINS; a power of two: products with it are exact
+constexpr int BINS = 4096, PER_THREAD = BINS / THREADS;
+constexpr float MOST = 32.f, PER_OCTAVE = 128.f;     // weights vanish at s = 32, in bin BINS; a power of two: products with it are exact
 constexpr int MAX_VOCABULARY = 1 << 20;        // totals stay below 2^53: exact in fp64
 constexpr int MAX_CHUNKS = MAX_VOCABULARY / CHUNK + 1;
 typedef unsigned long long u64;
@@ -171,9 +171,10 @@ __device__ __forceinline__ u64 over_all(u64 v, Shared &sh, int &turn) {
 
 // The first bin at which the sum of `in` reaches `need` (at least 1), and the sum before it; false if it does not
 template <class E> __device__ __forceinline__ bool find_bin(const E *in, u64 need, Shared &sh, int &turn, int &bin, u64 &before) {
-    static_assert(BINS == THREADS, "a bin per thread");
     const int wave = threadIdx.x >> 6;
-    const u64 own = in[threadIdx.x];
+    u64 own = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; i++) own += in[threadIdx.x * PER_THREAD + i];
     u64 upto = up_to(own), total = 0;
     if ((threadIdx.x & 63) == 63) sh.red[turn][wave] = upto;
     __syncthreads();
@@ -185,8 +186,11 @@ template <class E> __device__ __forceinline__ bool find_bin(const E *in, u64 nee
     turn ^= 1;
     if (total < need) return false;
     if (upto >= need && upto - own < need) {
-        sh.bin = threadIdx.x;
-        sh.before = upto - own;
+        u64 sum = upto - own;
+        int i = threadIdx.x * PER_THREAD;
+        while (sum + in[i] < need) sum += in[i++];
+        sh.bin = i;
+        sh.before = sum;
     }
     __syncthreads();
     bin = sh.bin;
@@ -222,7 +226,31 @@ __device__ __forceinline__ bool find_cut(R &row, const E *in, u64 need, unsigned
     });
     __syncthreads();
     const unsigned m = sh.listed;
-    if (m <= LIST) {
+    if (m <= 64) {          // an element per lane of one wavefront: each is held against all
+        if (threadIdx.x < 64) {
+            const bool there = threadIdx.x < m;
+            const float s = there ? sh.list[threadIdx.x] : 0.f;
+            const unsigned own = __float_as_uint(s), w = WEIGHT ? weight(s) : 1;
+            u64 below = 0;
+            unsigned equal = 0;
+            for (unsigned i = 0; i < m; i++) {
+                const unsigned bits = __builtin_amdgcn_readlane(own, i), each = __builtin_amdgcn_readlane(w, i);
+                below += bits < own ? each : 0u;
+                equal += bits == own;
+            }
+            below += before;
+            // (equal ones agree, so whichever writes)
+            if (there && below < need && below + (u64)equal * w >= need) {
+                sh.key = own;
+                sh.equal = equal;
+                sh.total = below;
+            }
+        }
+        __syncthreads();
+        cut.key = sh.key;
+        cut.equal = sh.equal;
+        cut.before = sh.total;
+    } else if (m <= LIST) {
         if (threadIdx.x < 64) {
             unsigned lo = 0xffffffffu, hi = 0;
             for (unsigned i = threadIdx.x; i < m; i += 64) {
@@ -343,8 +371,11 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
         sh.redf[0][wave] = top;
         sh.redf[1][wave] = least_best;
     }
-    sh.bin_weight[tid] = 0;
-    sh.bin_count[tid] = 0;
+#pragma unroll
+    for (int i = 0; i < PER_THREAD; i++) {
+        sh.bin_weight[tid + i * THREADS] = 0;
+        sh.bin_count[tid + i * THREADS] = 0;
+    }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < WAVES; i++) {
