@@ -148,7 +148,7 @@ struct Shared {
     float list[LIST];
     unsigned list_weight[LIST], listed;
     u64 sums[WAVES * MAX_CHUNKS];          // by chunk and wavefront
-    unsigned ties[WAVES * MAX_CHUNKS];
+    unsigned ties[WAVES * MAX_CHUNKS + 1];
     u64 red[2][WAVES];
     float redf[2][WAVES];
     // what a search found
@@ -495,9 +495,11 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
         return n;
     };
     if (some_ties) {
-        row.each_again([&](int c, const float (&s)[PIECE]) {
-            const u64 all = last_lane(up_to(equal(s)));
-            if (lane == 0) sh.ties[c * WAVES + wave] = (unsigned)all;
+        row.each([&](int c, const float (&s)[PIECE]) {
+            unsigned n = 0;
+#pragma unroll
+            for (int i = 0; i < PIECE; i++) n += __popcll(__ballot(__float_as_uint(s[i]) == key));
+            if (lane == 0 && c < row.chunks) sh.ties[c * WAVES + wave] = n;
         });
         __syncthreads();
         if (wave == 0) {
@@ -507,6 +509,7 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
                 if (e0 + lane < entries) sh.ties[e0 + lane] = (unsigned)(upto - v);
                 carried = last_lane(upto);
             }
+            if (lane == 0) sh.ties[entries] = (unsigned)carried;
         }
         __syncthreads();
     }
@@ -527,17 +530,25 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     };
     row.each([&](int c, const float (&s)[PIECE]) {
         if (c >= row.chunks) return;
+        // of the wavefront's equal ones all stay, or none, or (in one place of the row) some
+        const int e = c * WAVES + wave;
         u64 all = 0;
-        if (some_ties) {
-            unsigned w[PIECE];
-            all = kept(c, s, w);
-        } else {
+        unsigned below = key + 1;
+        if (some_ties && sh.ties[e + 1] > ties) {
+            below = key;
+            if (sh.ties[e] < ties) {
+                unsigned w[PIECE];
+                all = kept(c, s, w);
+                below = 0;
+            }
+        }
+        if (below) {
 #pragma unroll
             for (int i = 0; i < PIECE; i++)
-                if (__float_as_uint(s[i]) <= key) all += weight(s[i]);
+                if (__float_as_uint(s[i]) < below) all += weight(s[i]);
         }
         all = last_lane(up_to(all));
-        if (lane == 0) sh.sums[c * WAVES + wave] = all;
+        if (lane == 0) sh.sums[e] = all;
     });
     __syncthreads();
     // the entry with the target, by wavefront 0
