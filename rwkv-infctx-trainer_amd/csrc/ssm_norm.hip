@@ -6,7 +6,8 @@
 // Backwards, with w = gy weight and xhat = r rstd:   gr = gresidual + rstd (w - xhat mean(w xhat)),   gweight = sum over rows of gy xhat;
 // gr is the gradient of x and of the incoming residual alike.
 //
-// Bound by memory: a row is read once and stays in registers between its sum of squares (and its largest value) and its output.
+// Bound by memory (32768 rows of 2560 bf16, residual fp32: forward 171 us = 5.9 TB/s, backward 262 us = 5.1 TB/s; 4096 rows of 4096 to 8 bits
+// 28 us = 6.6 TB/s): a row is read once and stays in registers between its sum of squares (and its largest value) and its output.
 // A row belongs to one wavefront or to four; wider rows than those hold are read again, from the cache.  The norm is that of the sum before it is
 // rounded to the residual's type, also backwards: there r is the forward's fp32 sum, or added up again.
 #include "common.h"

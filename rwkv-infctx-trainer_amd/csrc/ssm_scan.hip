@@ -19,8 +19,10 @@
 // touch one line: in the order of the rows every lane of an access is an L1 access of its own, and those were what
 // bounded the forward.  to_rows and to_memory are the two permutations between the orders.
 //
-// What bounds it: the exponentials and fp32 multiply-adds, an exponential and four to five instructions per token, channel
-// and state, not the memory (which would take a third of the time).
+// What bounds it: vector instructions, not the memory.  Per token, channel and state the forward takes an exponential (two issue
+// slots) and four multiplications or multiply-adds, the backward an exponential and twelve; with the sums over the rows and a token's own arithmetic
+// that is 165 and 456 instructions per wavefront and tile, and the vector unit is busy 83 % and 81 % of the time (B8 T2048 D4096 N16 bf16: 450 us
+// forward with checkpoints, 0.8 GB, which memory alone would take 160 us for; 1190 us backward).
 #include "common.h"
 #include "row_sums.h"
 #include "vec.h"
@@ -599,7 +601,7 @@ __global__ __launch_bounds__(64 * back_waves(J), J == 1 ? 4 : J == 2 ? 2 : 1) vo
     if (k.gstate_in && w.seg == 0) w.store_state(k.gstate_in, g);
 }
 
-// One token: bound by the states, read once and written once.  Q lanes per channel with four states each (N = 4 Q), or, for
+// One token: bound by the states, read once and written once (B64 D5120: 42 MB in 12.8 us; B1 D4096: 3.5 us, a launch).  Q lanes per channel with four states each (N = 4 Q), or, for
 // other N, a row of lanes as above; a lane takes NB sequences, whose loads are all in flight together, with one read of its A.  VEC: four of
 // B or C are one load.  state_out may be state_in: a lane writes what it has read.
 template <class T, int Q, int NB, bool VEC>
