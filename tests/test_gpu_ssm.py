@@ -438,3 +438,35 @@ def test_single_tokens_in_a_graph():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, want)
+
+
+def test_offsets_beyond_32_bits():
+    """Sequences, rows and tokens that lie more than 2^32 bytes apart in one buffer give what their copies side by side give."""
+    from rwkv_wkv_hip import sampling, ssm as K
+    free, _ = torch.cuda.mem_get_info()
+    if free < 24 << 30:
+        pytest.skip("needs 24 GB")
+    D, N, far = 64, 16, (1 << 31) + 24            # elements of two bytes: 4 GiB and a little between two sequences
+    buffer = torch.empty(far + 64 * 1024, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    view = lambda *s: buffer.as_strided(s, (far,) + tuple(torch.empty(s[1:], device="meta").stride()))
+    for T in (1, 40):
+        x = view(2, T, 6 * D)
+        x.copy_(torch.randn(2, T, 6 * D, device="cuda", generator=g))
+        part = lambda t, i, n=D: t[..., i * D:i * D + n]
+        A = -torch.rand(D, N, device="cuda", generator=g)
+        run = lambda t: K.selective_scan(part(t, 0), part(t, 1), A, part(t, 2, N), part(t, 3, N), z=part(t, 4))
+        w = torch.randn(D, 4, device="cuda", generator=g).bfloat16()
+        for f in (run, lambda t: K.causal_conv(part(t, 5), w)):
+            assert all(torch.equal(a, b) for a, b in zip(f(x), f(x.contiguous())))
+    rows = view(2, 300)
+    rows.copy_(torch.randn(2, 300, device="cuda", generator=g))
+    weight, u = torch.ones(300, device="cuda"), torch.tensor([0.3, 0.8], device="cuda")
+    for f in (lambda t: K.rms_norm(t, weight, 1e-5, t), lambda t: sampling.sample(t, u, top_p=0.9)):
+        assert all(torch.equal(a, b) for a, b in zip(f(rows), f(rows.contiguous())))
+    # 300 tokens of 16 MiB: offsets within one sequence, and those of the result, pass 2^32 bytes
+    B, T, D = 1, 300, 1 << 23
+    x = torch.randn(B, T, 8, device="cuda", generator=g).bfloat16().repeat_interleave(D // 8, -1)
+    y, s = K.causal_conv(x, w[:1].expand(D, 4))
+    small, end = K.causal_conv(x[..., ::D // 8].contiguous(), w[:1].expand(8, 4))
+    assert torch.equal(y[..., ::D // 8], small) and torch.equal(y[..., D // 8 - 1::D // 8], small) and torch.equal(s[..., ::D // 8], end)
