@@ -84,8 +84,10 @@ int check_norm(int rows, int C, int dtype, int residual_dtype, int weight_dtype)
     if (residual_dtype != WKV_F32 && residual_dtype != dtype) return WKV_ERR_DTYPE;
     return weight_dtype == WKV_F32 || weight_dtype == dtype ? WKV_OK : WKV_ERR_DTYPE;
 }
-bool norm_wide(int C, long long xs, long long rs, const void *x, const void *residual) {
-    return C % 8 == 0 && xs % 8 == 0 && rs % 8 == 0 && aligned16(x) && aligned16(residual);
+// elements per piece of a row, as its width, its strides and the addresses allow
+int norm_piece(int C, long long xs, long long rs, const void *x, const void *residual, int dtype, int residual_dtype) {
+    if (C % 8 == 0 && xs % 8 == 0 && rs % 8 == 0 && aligned16(x) && aligned16(residual)) return 8;
+    return C % 2 == 0 && xs % 2 == 0 && rs % 2 == 0 && aligned_to(x, 2 * element(dtype)) && aligned_to(residual, 2 * element(residual_dtype)) ? 2 : 1;
 }
 
 }  // namespace
@@ -198,8 +200,8 @@ int wkv_rms_norm_forward(void *stream, int rows, int C, int dtype, int residual_
     k.xs = x_stride; k.rs = residual_stride; k.eps = eps;
     k.x = x; k.residual = residual; k.weight = weight;
     k.y = q ? nullptr : y; k.q = q; k.scale = scale; k.out = residual_out; k.rstd = rstd;
-    const bool wide = norm_wide(C, x_stride, residual ? residual_stride : 0, x, residual);
-#define CALL(TY) (residual_dtype == WKV_F32 ? norm::forward_t<TY, float>((hipStream_t)stream, k, wide) : norm::forward_t<TY, TY>((hipStream_t)stream, k, wide))
+    const int piece = norm_piece(C, x_stride, residual ? residual_stride : 0, x, residual, dtype, residual_dtype);
+#define CALL(TY) (residual_dtype == WKV_F32 ? norm::forward_t<TY, float>((hipStream_t)stream, k, piece) : norm::forward_t<TY, TY>((hipStream_t)stream, k, piece))
     return finished(BY_DTYPE(dtype, CALL));
 #undef CALL
 }
@@ -223,8 +225,8 @@ int wkv_rms_norm_backward(void *stream, int rows, int C, int dtype, int residual
     k.x = x; k.residual = residual; k.weight = weight; k.rstd = const_cast<float *>(rstd);
     k.gy = gy; k.gout = gresidual_out; k.gx = gx; k.gres = gresidual;
     k.part = static_cast<float *>(workspace);
-    const bool wide = norm_wide(C, x ? x_stride : 0, residual ? residual_stride : 0, x, residual);
-#define CALL(TY) (residual_dtype == WKV_F32 ? norm::backward_t<TY, float>((hipStream_t)stream, k, wide, gweight) : norm::backward_t<TY, TY>((hipStream_t)stream, k, wide, gweight))
+    const int piece = norm_piece(C, x ? x_stride : 0, residual ? residual_stride : 0, x, residual, dtype, residual_dtype);
+#define CALL(TY) (residual_dtype == WKV_F32 ? norm::backward_t<TY, float>((hipStream_t)stream, k, piece, gweight) : norm::backward_t<TY, TY>((hipStream_t)stream, k, piece, gweight))
     return finished(BY_DTYPE(dtype, CALL));
 #undef CALL
 }

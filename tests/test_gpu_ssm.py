@@ -470,3 +470,16 @@ def test_offsets_beyond_32_bits():
     y, s = K.causal_conv(x, w[:1].expand(D, 4))
     small, end = K.causal_conv(x[..., ::D // 8].contiguous(), w[:1].expand(8, 4))
     assert torch.equal(y[..., ::D // 8], small) and torch.equal(y[..., D // 8 - 1::D // 8], small) and torch.equal(s[..., ::D // 8], end)
+
+
+@pytest.mark.parametrize("dtype,residual", [(torch.bfloat16, None), (torch.bfloat16, torch.float32), (torch.float32, torch.float32)])
+@pytest.mark.parametrize("rows,C", [(1, 16), (37, 24), (33, 64), (517, 72), (16, 128), (1023, 136), (9, 256), (77, 264), (4999, 512), (70, 520), (600, 1024), (9, 1),
+                                    (700, 255), (41, 257), (3, 1023), (30000, 128), (50, 2), (81, 100), (30, 250), (19, 646), (7, 1022), (5, 2050), (3, 4098)])
+def test_rms_norm_of_narrow_rows(dtype, residual, rows, C):
+    """Several rows to a wavefront or workgroup, the last ones short of a whole one."""
+    test_rms_norm(dtype, residual, rows, C)
+
+
+@pytest.mark.parametrize("rows,C", [(37, 24), (1023, 128), (517, 256), (45, 511), (700, 777), (21, 90), (9, 646), (3, 2050)])
+def test_rms_norm_fp8_of_narrow_rows(rows, C):
+    test_rms_norm_fp8(torch.bfloat16, rows, C)
