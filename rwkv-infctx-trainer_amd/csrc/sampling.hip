@@ -590,16 +590,25 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
     }
 }
 
-template <class T> static hipError_t launch(hipStream_t s, const Call &k) {
+constexpr int ROWS_PER_LAUNCH = 1 << 21;          // (a grid has fewer than 2^32 threads)
+template <class T> static hipError_t launch(hipStream_t s, const Call &all) {
     // (a row may start anywhere in its first piece unless all of them start on one)
-    const bool whole = k.stride % PIECE == 0 && reinterpret_cast<uintptr_t>(k.logits) % (PIECE * sizeof(T)) == 0;
-    const int chunks = (k.V + (whole ? 0 : PIECE - 1) + CHUNK - 1) / CHUNK;
-    const dim3 grid(k.rows), block(THREADS);
-    if (chunks <= 1) hipLaunchKernelGGL((sample<T, 1>), grid, block, 0, s, k);
-    else if (chunks <= 2) hipLaunchKernelGGL((sample<T, 2>), grid, block, 0, s, k);
-    else if (chunks <= 4) hipLaunchKernelGGL((sample<T, 4>), grid, block, 0, s, k);
-    else if (chunks <= 8) hipLaunchKernelGGL((sample<T, 8>), grid, block, 0, s, k);
-    else hipLaunchKernelGGL((sample<T, 0>), grid, block, 0, s, k);
+    const bool whole = all.stride % PIECE == 0 && reinterpret_cast<uintptr_t>(all.logits) % (PIECE * sizeof(T)) == 0;
+    const int chunks = (all.V + (whole ? 0 : PIECE - 1) + CHUNK - 1) / CHUNK;
+    for (int done = 0; done < all.rows; done += std::min(all.rows - done, ROWS_PER_LAUNCH)) {
+        Call k = all;
+        auto on = [&](auto *p) { return p ? p + done : p; };
+        k.rows = std::min(all.rows - done, ROWS_PER_LAUNCH);
+        k.logits = static_cast<const T *>(all.logits) + done * all.stride;
+        k.u = on(all.u); k.temperature = on(all.temperature); k.top_p = on(all.top_p); k.min_p = on(all.min_p); k.top_k = on(all.top_k);
+        k.token = on(all.token); k.logprob = on(all.logprob);
+        const dim3 grid(k.rows), block(THREADS);
+        if (chunks <= 1) hipLaunchKernelGGL((sample<T, 1>), grid, block, 0, s, k);
+        else if (chunks <= 2) hipLaunchKernelGGL((sample<T, 2>), grid, block, 0, s, k);
+        else if (chunks <= 4) hipLaunchKernelGGL((sample<T, 4>), grid, block, 0, s, k);
+        else if (chunks <= 8) hipLaunchKernelGGL((sample<T, 8>), grid, block, 0, s, k);
+        else hipLaunchKernelGGL((sample<T, 0>), grid, block, 0, s, k);
+    }
     return hipGetLastError();
 }
 

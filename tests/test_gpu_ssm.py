@@ -483,3 +483,27 @@ def test_rms_norm_of_narrow_rows(dtype, residual, rows, C):
 @pytest.mark.parametrize("rows,C", [(37, 24), (1023, 128), (517, 256), (45, 511), (700, 777), (21, 90), (9, 646), (3, 2050)])
 def test_rms_norm_fp8_of_narrow_rows(rows, C):
     test_rms_norm_fp8(torch.bfloat16, rows, C)
+
+
+def test_more_rows_than_a_grid_of_threads():
+    """Rows whose threads pass 2^32, from one row that stands for all: each gives what it gives alone."""
+    from rwkv_wkv_hip import sampling, ssm as K
+    free, _ = torch.cuda.mem_get_info()
+    if free < 64 << 30:
+        pytest.skip("needs 64 GB")
+    rows, C = (1 << 24) + 5, 1032
+    x, w = torch.randn(1, C, device="cuda").bfloat16(), torch.randn(C, device="cuda")
+    q, scale, _ = K.rms_norm_fp8(x.expand(rows, C), w)
+    one, s, _ = K.rms_norm_fp8(x, w)
+    assert (scale == s).all()
+    bits = one.view(torch.uint8)
+    for part in q.view(torch.uint8).split(1 << 21):
+        assert (part == bits).all()
+    rows = (1 << 22) + 5
+    u = torch.rand(rows, device="cuda")
+    logits = torch.randn(1, 9, device="cuda")
+    token, logprob = sampling.sample(logits.expand(rows, 9), u)
+    for at in (0, rows // 2 - 7, rows - 20):
+        a, b = sampling.sample(logits.expand(20, 9).contiguous(), u[at:at + 20].clone())
+        assert torch.equal(token[at:at + 20], a) and torch.equal(logprob[at:at + 20], b)
+    assert token.min() >= 0 and token.max() < 9
