@@ -44,10 +44,11 @@ conv::Call conv_call(int B, int T, int D, int param_dtype, int silu, const wkv_r
     k.weight = weight; k.bias = bias; k.state_in = state_in; k.lengths = lengths;
     return k;
 }
-// whether a lane may take four channels at once
-bool conv_wide(const wkv_rows *x, int D, int dtype) {
-    const int v = conv::vector_of(D);
-    return v > 1 && aligned_to(x->p, v * element(dtype)) && x->batch % v == 0 && x->token % v == 0;
+// how many channels a lane may take at once
+int conv_piece(const wkv_rows *x, int D, int dtype) {
+    for (int v : {4, 2})
+        if (D % v == 0 && aligned_to(x->p, v * element(dtype)) && x->batch % v == 0 && x->token % v == 0) return v;
+    return 1;
 }
 
 // ---- scan
@@ -104,8 +105,8 @@ int wkv_causal_conv_forward(void *stream, int B, int T, int D, int W, int dtype,
     if (overlaps(state_in, state_out, (size_t)B * (W - 1) * D * element(dtype)) && !(T == 1 && state_in == state_out)) return WKV_ERR_ALIAS;
     conv::Call k = conv_call(B, T, D, param_dtype, silu, x, weight, bias, state_in, lengths);
     k.y = y; k.state_out = state_out;
-    const bool wide = conv_wide(x, D, dtype);
-#define CALL(TY) conv::forward_t<TY>((hipStream_t)stream, W, k, wide)
+    const int piece = conv_piece(x, D, dtype);
+#define CALL(TY) conv::forward_t<TY>((hipStream_t)stream, W, k, piece)
     return finished(BY_DTYPE(dtype, CALL));
 #undef CALL
 }
@@ -128,8 +129,8 @@ int wkv_causal_conv_backward(void *stream, int B, int T, int D, int W, int dtype
     conv::Call k = conv_call(B, T, D, param_dtype, silu, x, weight, bias, state_in, lengths);
     k.gy = gy; k.gstate_out = gstate_out; k.gx = gx; k.gstate_in = gstate_in;
     k.part = static_cast<float *>(workspace);
-    const bool wide = conv_wide(x, D, dtype);
-#define CALL(TY) conv::backward_t<TY>((hipStream_t)stream, W, k, wide, gweight, gbias)
+    const int piece = conv_piece(x, D, dtype);
+#define CALL(TY) conv::backward_t<TY>((hipStream_t)stream, W, k, piece, gweight, gbias)
     return finished(BY_DTYPE(dtype, CALL));
 #undef CALL
 }

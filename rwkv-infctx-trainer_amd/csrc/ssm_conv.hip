@@ -5,8 +5,8 @@
 // where xx continues x to the left by the state, the W-1 inputs before it; the last W-1 of xx are the new state.  Backwards, with
 // gp[t] = gy[t] silu'(pre[t]):   gx[s] = sum over k of w[k] gp[s + W-1 - k],   gw[k] = sum over t of gp[t] xx[t - (W-1) + k].
 //
-// Bound by memory (B8 T4096 D4096 bf16: forward 103 us = 5.2 TB/s, backward 185 us = 4.4 TB/s): each input is to be read once and each output written once.  A lane holds four channels and walks
-// a run of tokens with the window in registers; the W-1 inputs (backwards also the W-1 gp) on a run's edge are read again, from
+// Bound by memory (B8 T4096 D4096 bf16: forward 103 us = 5.2 TB/s, backward 185 us = 4.4 TB/s): each input is to be read once and each output written once.  A lane holds four channels
+// (two or one where four are not aligned) and walks a run of tokens with the window in registers; the W-1 inputs (backwards also the W-1 gp) on a run's edge are read again, from
 // the cache.  The filter's gradient is summed along the run in registers, over the workgroup's four runs in LDS, and over
 // the workgroups by sum_rows.
 #include "common.h"
@@ -16,7 +16,7 @@
 namespace wkv {
 namespace conv {
 
-constexpr int MIN_TAPS = 2, MAX_TAPS = 4, RUNS = 4, WIDE = 4;         // runs per workgroup: one per wavefront
+constexpr int MIN_TAPS = 2, MAX_TAPS = 4, RUNS = 4;         // runs per workgroup: one per wavefront
 
 struct Call {
     int B, T, D, run;                         // run: tokens per lane
@@ -296,11 +296,10 @@ static inline int run_for(int B, int T, int D, int V) {
     return run;
 }
 static inline int run_groups(int T, int run) { return (T + RUNS * run - 1) / (RUNS * run); }
-static inline int vector_of(int D) { return D % WIDE == 0 ? WIDE : 1; }
-// (the largest of what the two widths of a lane need: which one a call takes depends on its pointers)
+// (the largest of what a lane's possible channels need: how many a call takes depends on its pointers)
 static inline size_t backward_scratch(int B, int T, int D, int W) {
     size_t n = 0;
-    for (int V : {1, vector_of(D)}) n = std::max(n, (size_t)B * run_groups(T, run_for(B, T, D, V)));
+    for (int V : {1, 2, 4}) n = std::max(n, (size_t)B * run_groups(T, run_for(B, T, D, V)));
     return n * (W + 1) * D * 4;
 }
 
@@ -316,14 +315,16 @@ template <class T, int V, bool BACK> static hipError_t launch(hipStream_t s, int
 #undef WKV_CONV
     return hipGetLastError();
 }
-template <class T> static hipError_t forward_t(hipStream_t s, int W, const Call &k, bool wide) {
-    return wide ? launch<T, WIDE, false>(s, W, k) : launch<T, 1, false>(s, W, k);
+// v: channels per lane, 4, or 2 or 1 where widths, strides or addresses allow no more (B8 T4096 bf16, forward and backward: D 4096 111 and 193 us by four,
+// D 4094 171 and 259 by two, 196 and 345 by one)
+template <class T> static hipError_t forward_t(hipStream_t s, int W, const Call &k, int v) {
+    return v == 4 ? launch<T, 4, false>(s, W, k) : v == 2 ? launch<T, 2, false>(s, W, k) : launch<T, 1, false>(s, W, k);
 }
-template <class T> static hipError_t backward_t(hipStream_t s, int W, const Call &k, bool wide, void *gweight, void *gbias) {
-    const hipError_t e = wide ? launch<T, WIDE, true>(s, W, k) : launch<T, 1, true>(s, W, k);
+template <class T> static hipError_t backward_t(hipStream_t s, int W, const Call &k, int v, void *gweight, void *gbias) {
+    const hipError_t e = v == 4 ? launch<T, 4, true>(s, W, k) : v == 2 ? launch<T, 2, true>(s, W, k) : launch<T, 1, true>(s, W, k);
     if (e != hipSuccess) return e;
     Sums<ToFilter<T>> sums;
-    sums.add(k.B * run_groups(k.T, run_for(k.B, k.T, k.D, wide ? WIDE : 1)), (size_t)(W + 1) * k.D, k.part,
+    sums.add(k.B * run_groups(k.T, run_for(k.B, k.T, k.D, v)), (size_t)(W + 1) * k.D, k.part,
              {{gweight, k.w32 != 0}, {gbias, k.w32 != 0}, W, k.D});
     sum_rows_launch(s, sums);
     return hipGetLastError();

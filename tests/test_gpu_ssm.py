@@ -507,3 +507,22 @@ def test_more_rows_than_a_grid_of_threads():
         a, b = sampling.sample(logits.expand(20, 9).contiguous(), u[at:at + 20].clone())
         assert torch.equal(token[at:at + 20], a) and torch.equal(logprob[at:at + 20], b)
     assert token.min() >= 0 and token.max() < 9
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,T,D,W", [(2, 37, 2, 4), (3, 50, 130, 3), (1, 300, 646, 4), (2, 9, 258, 2), (1, 1, 66, 4), (2, 70, 131, 4)])
+def test_causal_conv_of_widths_not_in_fours(dtype, B, T, D, W):
+    from rwkv_wkv_hip import ssm as K
+    v, grads = _conv_inputs(dtype, B, T, D, W)
+    _compare(lambda **k: K.causal_conv(**k), lambda **k: O.causal_conv(**k), v, grads, ["y", "state"])
+
+
+@pytest.mark.parametrize("from_,step", [(2, 2), (1, 2), (2, 3), (4, 2), (0, 2)])
+def test_causal_conv_of_slices_that_begin_anywhere(from_, step):
+    """A slice of a wider tensor whose address or row distance allows four channels to a lane, two or one."""
+    from rwkv_wkv_hip import ssm as K
+    x = torch.randn(2, 40, 64 * step + 2 * step, generator=_g(from_, step)).bfloat16().cuda()
+    w = torch.randn(64, 4, generator=_g(3)).cuda()
+    part = x[..., from_:from_ + 64]
+    for a, b in zip(K.causal_conv(part, w), K.causal_conv(part.contiguous(), w)):
+        assert torch.equal(a, b)
