@@ -63,6 +63,12 @@ template <int LANES, bool MAX> __device__ __forceinline__ float over_row(float v
 // threads of a workgroup: rows of up to one wavefront share it
 template <int LANES> constexpr int forward_threads() { return LANES < 64 ? 256 : LANES; }
 template <int LANES> constexpr int backward_threads() { return LANES <= 64 ? 512 : LANES; }
+// which of the workgroup's rows a lane is at: a scalar unless a wavefront has several
+template <int LANES, int THREADS> __device__ __forceinline__ int row_of() {
+    if constexpr (LANES == THREADS) return 0;
+    else if constexpr (LANES == 64) return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64);
+    else return (int)threadIdx.x / LANES;
+}
 
 // a row's elements in registers, N pieces of V per lane, or (N = 0) read again for every use
 template <int V, int N, int LANES> struct Pieces {
@@ -84,8 +90,8 @@ template <class T, class R, int V, int N, int LANES, bool Q>
 __global__ __launch_bounds__(forward_threads<LANES>()) void forward(const Call k) {
     typedef Pieces<V, N, LANES> P;
     __shared__ float red[2][4];
-    const size_t row = (size_t)blockIdx.x * (forward_threads<LANES>() / LANES) + threadIdx.x / LANES;
-    const int lane = threadIdx.x % LANES;
+    const size_t row = (size_t)blockIdx.x * (forward_threads<LANES>() / LANES) + row_of<LANES, forward_threads<LANES>()>();
+    const int lane = LANES == forward_threads<LANES>() ? threadIdx.x : threadIdx.x % LANES;
     if (LANES < 64 && row >= (size_t)k.rows) return;
     const T *x = static_cast<const T *>(k.x) + row * k.xs;
     const R *residual = k.residual ? static_cast<const R *>(k.residual) + row * k.rs : nullptr;
@@ -160,7 +166,7 @@ __global__ __launch_bounds__(backward_threads<LANES>()) void backward(const Call
     constexpr int THREADS = backward_threads<LANES>(), ROWS = THREADS / LANES, WIDTH = V * N * LANES;
     __shared__ float red[2][4];
     __shared__ float sums[ROWS > 1 ? THREADS / 64 : 1][ROWS > 1 ? WIDTH : 1];
-    const int lane = threadIdx.x % LANES;
+    const int lane = LANES == THREADS ? threadIdx.x : threadIdx.x % LANES;          // (masked for nothing, a row's pieces have an address each: 114 -> 156 registers)
     float *part = k.part + (size_t)blockIdx.x * k.C;
     float gw[N ? N : 1][V];
     if constexpr (N > 0) {
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(backward_threads<LANES>()) void backward(const Call
         });
     }
     int turn = 0;
-    for (size_t row = (size_t)blockIdx.x * ROWS + threadIdx.x / LANES; row < (size_t)k.rows; row += (size_t)gridDim.x * ROWS, turn ^= 1) {
+    for (size_t row = (size_t)blockIdx.x * ROWS + row_of<LANES, THREADS>(); row < (size_t)k.rows; row += (size_t)gridDim.x * ROWS, turn ^= 1) {
         const float rstd = k.rstd[row];
         float xh[N ? N : 1][V], w[N ? N : 1][V];
         auto take = [&](int i, int c, bool sum_weight) {
@@ -246,7 +252,7 @@ __global__ __launch_bounds__(backward_threads<LANES>()) void backward(const Call
 // (no barrier), else by four, 8192 elements in registers
 struct Shape { int v, n, lanes; };
 static inline Shape shape_of(int C, int v) {
-    if (v == 2 && C <= 4096) return C <= 256 ? Shape{2, 2, 64} : Shape{2, 8, C <= 1024 ? 64 : 256};
+    if (v == 2 && C <= 8192) return C <= 256 ? Shape{2, 2, 64} : C <= 4096 ? Shape{2, 8, C <= 1024 ? 64 : 256} : Shape{2, 16, 256};
     if (v < 8) return C <= 256 ? Shape{1, 4, 64} : Shape{1, C <= 1024 ? 4 : C <= 4096 ? 16 : C <= 8192 ? 32 : 0, 256};
     const int p = C / 8;
     if (p <= 64) return {8, 1, p <= 8 ? 8 : p <= 16 ? 16 : p <= 32 ? 32 : 64};
@@ -267,7 +273,8 @@ static inline int backward_groups(int rows, int C) { return std::max(1, std::min
         else if (f.v == 1) LAUNCH(1, 0, 256);                                             \
         else if (is(2, 2, 64)) LAUNCH(2, 2, 64);                                          \
         else if (is(2, 8, 64)) LAUNCH(2, 8, 64);                                          \
-        else if (f.v == 2) LAUNCH(2, 8, 256);                                             \
+        else if (is(2, 8, 256)) LAUNCH(2, 8, 256);                                        \
+        else if (f.v == 2) LAUNCH(2, 16, 256);                                            \
         else if (f.lanes == 8) LAUNCH(8, 1, 8);                                           \
         else if (f.lanes == 16) LAUNCH(8, 1, 16);                                         \
         else if (f.lanes == 32) LAUNCH(8, 1, 32);                                         \

@@ -526,3 +526,9 @@ def test_causal_conv_of_slices_that_begin_anywhere(from_, step):
     part = x[..., from_:from_ + 64]
     for a, b in zip(K.causal_conv(part, w), K.causal_conv(part.contiguous(), w)):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("rows,C", [(3, 4100), (5, 6002), (2, 8190)])
+def test_rms_norm_of_wide_rows_in_pairs(rows, C):
+    test_rms_norm(torch.bfloat16, torch.float32, rows, C)
+    test_rms_norm_fp8(torch.bfloat16, rows, C)
