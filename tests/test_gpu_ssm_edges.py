@@ -28,3 +28,26 @@ def test_rows_in_8_bits_round_once(weights, times, thousandths):
     want = weight.float().abs().max() / 448
     assert (scale.cpu() == want).all()
     assert torch.equal(q.cpu().view(torch.uint8), (weight.float() / want).to(torch.float8_e4m3fn).view(torch.uint8).expand(3, -1))
+
+
+# ---- 8 bits
+@pytest.mark.parametrize("C", [64, 100, 646, 2560, 8200])
+def test_rows_in_8_bits_that_are_not_finite(C):
+    """A row with a NaN or an infinity has the scale max |y| / 448, which is NaN (an infinity: its norm is NaN); its neighbours are what they are without it."""
+    from rwkv_wkv_hip import ssm as K
+    g = S._g(C, 3)
+    x, w = torch.randn(7, C, generator=g).bfloat16().cuda(), (torch.rand(C, generator=g) + 0.5).bfloat16().cuda()
+    q, scale, _ = K.rms_norm_fp8(x, w)
+    bad = x.clone()
+    bad[1, C // 2], bad[3, 5], bad[5, 7] = math.nan, math.inf, -math.inf
+    q2, scale2, _ = K.rms_norm_fp8(bad, w)
+    assert scale2[1::2].isnan().sum() == 3 and q2[1::2].float().isnan().all()
+    assert torch.equal(q2.view(torch.uint8)[::2], q.view(torch.uint8)[::2]) and torch.equal(scale2[::2], scale[::2])
+    # from one weight: every row's largest value
+    w2 = w.clone()
+    w2[C - 1] = math.nan
+    q2, scale2, _ = K.rms_norm_fp8(x, w2)
+    assert scale2.isnan().all() and q2.float().isnan().all()
+    w2[C - 1] = math.inf
+    q2, scale2, _ = K.rms_norm_fp8(x, w2)
+    assert scale2.isinf().all() and not q2[:, :-1].float().any() and q2[:, -1].float().isnan().all()
