@@ -23,9 +23,9 @@ template <class O> struct Sums {               // up to five arrays in one launc
 
 // 64 columns per workgroup; its wavefronts share the rows
 template <class O, int WAVES>
-static __global__ __launch_bounds__(64 * WAVES) void sum_rows(Sums<O> sums) {
+static __global__ __launch_bounds__(64 * WAVES) void sum_rows(Sums<O> sums, int first) {
     __shared__ float part[WAVES][64];
-    int block = blockIdx.x, j = 0;
+    int block = first + (int)blockIdx.x, j = 0;
     while (j + 1 < sums.count && block >= sums.job[j].blocks) block -= sums.job[j++].blocks;
     const auto &job = sums.job[j];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rows = job.rows;
@@ -48,6 +48,7 @@ static __global__ __launch_bounds__(64 * WAVES) void sum_rows(Sums<O> sums) {
         job.out(i, all);
     }
 }
+constexpr long long SUMS_PER_LAUNCH = 1 << 21;          // workgroups: a grid has fewer than 2^32 threads
 // 16 wavefronts where there are many rows: 1024 rows of 2560 columns 22 us with four, 8 with sixteen
 template <class O> static void sum_rows_launch(hipStream_t s, const Sums<O> &sums) {
     long long blocks = 0;
@@ -56,8 +57,11 @@ template <class O> static void sum_rows_launch(hipStream_t s, const Sums<O> &sum
         blocks += sums.job[j].blocks;
         rows = std::max(rows, sums.job[j].rows);
     }
-    if (rows >= 64) hipLaunchKernelGGL((sum_rows<O, 16>), dim3((unsigned)blocks), dim3(1024), 0, s, sums);
-    else hipLaunchKernelGGL((sum_rows<O, 4>), dim3((unsigned)blocks), dim3(256), 0, s, sums);
+    for (long long first = 0; first < blocks; first += SUMS_PER_LAUNCH) {
+        const dim3 grid((unsigned)std::min(blocks - first, SUMS_PER_LAUNCH));
+        if (rows >= 64) hipLaunchKernelGGL((sum_rows<O, 16>), grid, dim3(1024), 0, s, sums, (int)first);
+        else hipLaunchKernelGGL((sum_rows<O, 4>), grid, dim3(256), 0, s, sums, (int)first);
+    }
 }
 
 }  // namespace wkv

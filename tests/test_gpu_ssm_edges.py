@@ -51,3 +51,28 @@ def test_rows_in_8_bits_that_are_not_finite(C):
     w2[C - 1] = math.inf
     q2, scale2, _ = K.rms_norm_fp8(x, w2)
     assert scale2.isinf().all() and not q2[:, :-1].float().any() and q2[:, -1].float().isnan().all()
+
+
+# ---- sizes past a grid's threads
+def test_sums_of_more_columns_than_a_grid_has_threads():
+    """B and C of 2^27 elements and 64 sequences: the sum of their gradients' shares takes 2^32 threads.  Sequences are compared with calls of their own
+    (cut in time elsewhere: within the tolerances)."""
+    from rwkv_wkv_hip import ssm as K
+    free, _ = torch.cuda.mem_get_info()
+    if free < 32 << 30:
+        pytest.skip("needs 32 GB")
+    B, T, D, N = 64, 1 << 17, 16, 16
+    g = torch.Generator(device="cuda").manual_seed(1)
+    r = lambda *s: torch.empty(s, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    v = dict(x=r(B, T, D), dt=r(B, T, D), B=r(B, T, N), C=r(B, T, N))
+    A, gy = -torch.rand(D, N, device="cuda", generator=g) - 0.1, r(B, T, D)
+
+    def run(rows):
+        leaf = {n: t[rows].clone().requires_grad_(True) for n, t in v.items()}
+        y, _ = K.selective_scan(A=A, **leaf)
+        return [y, *torch.autograd.grad(y, list(leaf.values()), gy[rows])]
+
+    whole = run(slice(None))
+    for b in (0, 37, 63):
+        for got, want in zip(whole, run(slice(b, b + 1))):
+            assert_close(got[b], want[0].cpu(), RTOL[torch.bfloat16])
