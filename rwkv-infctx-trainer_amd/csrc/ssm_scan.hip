@@ -40,7 +40,8 @@ struct Rows {                               // (B, T, .) with a contiguous last 
 };
 
 struct Call {
-    int B, T, D, N, G, Dg, tiles, segments, seg_tiles, seg0;      // Dg channels per group; seg0: the launch's first segment
+    int B, T, D, N, G, Dg, tiles, segments, seg_tiles, seg0;      // Dg channels per group; seg0: the first segment there is work for
+    int first, workgroups;                                        // the launch's first workgroup, and of how many in all
     Rows x, dt, z, b, c;
     const float *A, *skip, *bias, *state_in;
     const int *lengths;
@@ -211,7 +212,7 @@ struct Work {
         tid = threadIdx.x;
         wave = tid >> 6; row = (tid >> 4) & 3; n = tid & 15;
         const int cts = (k.Dg + CHANNELS - 1) / CHANNELS;
-        int i = xcd_order(blockIdx.x, gridDim.x);
+        int i = xcd_order(k.first + (int)blockIdx.x, k.workgroups);
         ct = i % cts; i /= cts;
         g = i % k.G; i /= k.G;
         b = i % k.B; seg = k.seg0 + i / k.B;
@@ -705,12 +706,18 @@ static inline size_t backward_scratch(int B, int T, int D, int N, int G) {
     return summary_bytes(B, D, N, p.segments) + 2 * rounded(cts * B * T * G * N * 4) + rounded(rows * D * N * 4) + 2 * rounded(rows * D * 4);
 }
 
+constexpr long long WORKGROUPS_PER_LAUNCH = 1 << 22;          // (a grid has fewer than 2^32 threads)
 #define WKV_SCAN_J(KERNEL, GRID, BLOCK, ...)                                                             \
     do {                                                                                                 \
-        const dim3 grid_((unsigned)(GRID)), block_(BLOCK);                                               \
-        if (J == 1) hipLaunchKernelGGL((KERNEL<T, 1 __VA_ARGS__>), grid_, block_, 0, s, k);              \
-        else if (J == 2) hipLaunchKernelGGL((KERNEL<T, 2 __VA_ARGS__>), grid_, block_, 0, s, k);         \
-        else hipLaunchKernelGGL((KERNEL<T, 4 __VA_ARGS__>), grid_, block_, 0, s, k);                     \
+        const long long all_ = GRID;                                                                     \
+        k.workgroups = (int)all_;                                                                        \
+        for (long long at_ = 0; at_ < all_; at_ += WORKGROUPS_PER_LAUNCH) {                              \
+            const dim3 grid_((unsigned)std::min(all_ - at_, WORKGROUPS_PER_LAUNCH)), block_(BLOCK);      \
+            k.first = (int)at_;                                                                          \
+            if (J == 1) hipLaunchKernelGGL((KERNEL<T, 1 __VA_ARGS__>), grid_, block_, 0, s, k);          \
+            else if (J == 2) hipLaunchKernelGGL((KERNEL<T, 2 __VA_ARGS__>), grid_, block_, 0, s, k);     \
+            else hipLaunchKernelGGL((KERNEL<T, 4 __VA_ARGS__>), grid_, block_, 0, s, k);                 \
+        }                                                                                                \
     } while (0)
 #define WKV_COMMA ,
 

@@ -76,3 +76,26 @@ def test_sums_of_more_columns_than_a_grid_has_threads():
     for b in (0, 37, 63):
         for got, want in zip(whole, run(slice(b, b + 1))):
             assert_close(got[b], want[0].cpu(), RTOL[torch.bfloat16])
+
+
+def test_scan_of_more_workgroups_than_a_grid_has_threads():
+    """4096 sequences of 4096 channels with a B and C each: 2^24 workgroups.  A sequence gives what it gives alone."""
+    from rwkv_wkv_hip import ssm as K
+    free, _ = torch.cuda.mem_get_info()
+    if free < 32 << 30:
+        pytest.skip("needs 32 GB")
+    B, T, D = 4096, 2, 4096
+    g = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *s: torch.empty(s, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    v = dict(x=r(B, T, D), dt=r(B, T, D), B=r(B, T, D, 1), C=r(B, T, D, 1))
+    A, gy = -torch.rand(D, 1, device="cuda", generator=g) - 0.1, r(B, T, D)
+
+    def run(rows):
+        leaf = {n: t[rows].clone().requires_grad_(True) for n, t in v.items()}
+        y, s = K.selective_scan(A=A, **leaf)
+        return [y, s, *torch.autograd.grad(y, list(leaf.values()), gy[rows])]
+
+    whole = run(slice(None))
+    for b in (0, 2047, 4093):
+        for got, want in zip(whole, run(slice(b, b + 3))):
+            assert torch.equal(got[b:b + 3], want)
