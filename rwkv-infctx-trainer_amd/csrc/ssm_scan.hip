@@ -41,7 +41,6 @@ struct Rows {                               // (B, T, .) with a contiguous last 
 
 struct Call {
     int B, T, D, N, G, Dg, tiles, segments, seg_tiles, seg0;      // Dg channels per group; seg0: the first segment there is work for
-    int first, workgroups;                                        // the launch's first workgroup, and of how many in all
     Rows x, dt, z, b, c;
     const float *A, *skip, *bias, *state_in;
     const int *lengths;
@@ -56,6 +55,7 @@ struct Call {
     float *gb_part, *gc_part;               // (channel tiles, B, T, G, N)
     float *ga_part, *gskip_part, *gbias_part;   // (B segments, D, N), (B segments, D) twice
     float *gstate_in;
+    int first, workgroups;                  // the launch's first workgroup, and of how many in all (at the end: the other operands' places cost a single token 0.2 us of 11.7)
 };
 
 template <int I> struct Int { static constexpr int value = I; };
