@@ -143,6 +143,11 @@ __device__ __forceinline__ float softplus(float v) {
     return v <= 20.f ? s : v;
 }
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * v)); }
+// A as the exponentials of two take it.  An infinite one becomes the largest number: times a step of zero, as of a token that is not there, it is to be zero.
+__device__ __forceinline__ float octaves(float a) {
+    a *= LOG2E;
+    return fabsf(a) < INFINITY || a != a ? a : copysignf(3.40282347e38f, a);
+}
 
 // Workgroups are handed to the eight XCDs in turn: neighbours in channels, which share lines of the streams and all of B
 // and C, are given to one of them.
@@ -248,7 +253,7 @@ struct Work {
     __device__ __forceinline__ size_t state_at(int state) const { return ((size_t)b * k.D + channel) * k.N + state; }
     __device__ __forceinline__ void load_a(float (&a2)[J]) const {
 #pragma unroll
-        for (int j = 0; j < J; j++) a2[j] = n + 16 * j < k.N ? k.A[(size_t)channel * k.N + n + 16 * j] * LOG2E : 0.f;
+        for (int j = 0; j < J; j++) a2[j] = n + 16 * j < k.N ? octaves(k.A[(size_t)channel * k.N + n + 16 * j]) : 0.f;
     }
     __device__ __forceinline__ void load_state(const float *s, float (&h)[J]) const {
 #pragma unroll
@@ -651,11 +656,12 @@ __global__ __launch_bounds__(256) void decode(const Call k) {
         for (int i = 0; i < NB; i++) {
             if (s == 0) step[i] = in[i] ? softplus(raw[i] + bias) : 0.f;
             const float dtx = step[i] * x[i];
+            if (in[i])          // (else the state stays as it is)
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                h[i][v] = fmaf(exp2_fast(step[i] * (a[v] * LOG2E)), h[i][v], in[i] ? dtx * vb[i][v] : 0.f);
-                y[i] = fmaf(in[i] ? vc[i][v] : 0.f, h[i][v], y[i]);
-            }
+                for (int v = 0; v < V; v++) {
+                    h[i][v] = fmaf(exp2_fast(step[i] * (a[v] * LOG2E)), h[i][v], dtx * vb[i][v]);
+                    y[i] = fmaf(vc[i][v], h[i][v], y[i]);
+                }
             if (b0 + i < k.B) store_vec(k.state_out + ((size_t)(b0 + i) * k.D + d) * k.N + n, h[i]);
         }
     }

@@ -99,3 +99,18 @@ def test_scan_of_more_workgroups_than_a_grid_has_threads():
     for b in (0, 2047, 4093):
         for got, want in zip(whole, run(slice(b, b + 3))):
             assert torch.equal(got[b:b + 3], want)
+
+
+# ---- values that are not finite, decays that grow
+@pytest.mark.parametrize("N", [16, 20, 4])
+@pytest.mark.parametrize("T,lengths", [(1, [0, 1, 1]), (40, [0, 17, 40])])
+def test_a_state_that_forgets_everything(N, T, lengths):
+    """A = -infinity: nothing is left of the state before a token; where there is no token (behind a sequence's end) it stays."""
+    from rwkv_wkv_hip import ssm as K
+    v, _ = S._scan_inputs(torch.float32, 3, T, 24, N, lengths=lengths)
+    v["A"][3, 1], v["A"][7], v["A"][8, N - 1] = -math.inf, -math.inf, -math.inf
+    ref = O.selective_scan(**{n: t.double() if t.is_floating_point() else t for n, t in v.items()})
+    for a, b in zip(K.selective_scan(**S._cuda(v, leaf=False)), ref):
+        assert_close(a, b, RTOL[torch.float32])
+    for a, b in zip(K.selective_scan(**S._cuda(v, leaf=True)), ref):
+        assert_close(a, b, RTOL[torch.float32])
