@@ -279,14 +279,22 @@ struct Work {
 #pragma unroll
         for (int j = 0; j < J; j++) buffer_store<float>(to, at + 64 * j, h[j]);
     }
-    // what the segments on one side make of an incoming state (or its gradient): v <- decay v + theirs
+    // what the segments on one side make of an incoming state (or its gradient): v <- decay v + theirs.  (A > 0: a growth past 2^127 is applied in
+    // two steps and to nothing not at all, since what it makes may be finite where it itself is not.)
     __device__ __forceinline__ void pass(int s, const float (&a2)[J], float (&v)[J]) const {
         const size_t at = (size_t)b * k.segments + s;
         const float dt = k.seg_dt[at * k.D + channel];
         float theirs[J];
         load_wide(k.seg_state, at, theirs);
 #pragma unroll
-        for (int j = 0; j < J; j++) v[j] = fmaf(exp2_fast(dt * a2[j]), v[j], theirs[j]);
+        for (int j = 0; j < J; j++) {
+            float e = dt * a2[j];
+            if (e > 127.f) {
+                if (v[j] != 0.f) v[j] *= exp2_fast(e - 127.f);
+                e = 127.f;
+            }
+            v[j] = fmaf(exp2_fast(e), v[j], theirs[j]);
+        }
     }
     __device__ __forceinline__ void from(int tile) {
         from_b = static_cast<const char *>(k.b.p) + (b * k.b.batch + tile * TILE * k.b.token + g * k.b.group) * (long long)sizeof(T);

@@ -114,3 +114,25 @@ def test_a_state_that_forgets_everything(N, T, lengths):
         assert_close(a, b, RTOL[torch.float32])
     for a, b in zip(K.selective_scan(**S._cuda(v, leaf=True)), ref):
         assert_close(a, b, RTOL[torch.float32])
+
+
+def test_growth_past_what_32_bits_hold_from_nothing():
+    """A > 0 in a sequence that is cut in time: a segment's growth alone passes 2^128, but there is nothing yet that grows, and backwards no gradient."""
+    from rwkv_wkv_hip import ssm as K
+    v, grads = S._scan_inputs(torch.float32, 1, 2048, 24, 16, state=False)
+    v["A"], v["dt"], v["dt_bias"] = torch.full((24, 16), 0.5), torch.full((1, 2048, 24), 1.0), torch.full((24,), 0.2)
+    token = torch.arange(2048)[None, :, None]
+    v["x"] = v["x"] * (token >= 2048 - 60)
+    S._compare(K.selective_scan, O.selective_scan, v, [grads[0] * (token < 60), grads[1] * 0], ("y", "state"))
+
+
+def test_growth_of_a_small_state():
+    """What comes in is small enough that the growth through a segment, too large for 32 bits by itself, leaves it finite."""
+    from rwkv_wkv_hip import ssm as K
+    v, _ = S._scan_inputs(torch.float32, 1, 256, 8, 16, gate=False, skip=False, bias=False)
+    v["A"], v["dt"], v["x"] = torch.full((8, 16), 0.5), torch.full((1, 256, 8), 3.0), torch.zeros(1, 256, 8)
+    v["state"] = v["state"] * 1e-35
+    v["dt"][:, 64:] = -100.0
+    ref = O.selective_scan(**{n: t.double() for n, t in v.items()})
+    for a, b in zip(K.selective_scan(**S._cuda(v, leaf=False)), ref):
+        assert_close(a, b, RTOL[torch.float32])
