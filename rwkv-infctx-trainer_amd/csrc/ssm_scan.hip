@@ -251,13 +251,14 @@ struct Work {
     __device__ __forceinline__ float to_rows(float v) const { return __int_as_float(__builtin_amdgcn_ds_bpermute(from_memory, __float_as_int(v))); }
     __device__ __forceinline__ float to_memory(float v) const { return __int_as_float(__builtin_amdgcn_ds_bpermute(from_row, __float_as_int(v))); }
     __device__ __forceinline__ size_t state_at(int state) const { return ((size_t)b * k.D + channel) * k.N + state; }
+    // (a row without a channel has nothing, not the first channel's: what it adds to its group's gB and gC is to be zero whatever that holds)
     __device__ __forceinline__ void load_a(float (&a2)[J]) const {
 #pragma unroll
-        for (int j = 0; j < J; j++) a2[j] = n + 16 * j < k.N ? octaves(k.A[(size_t)channel * k.N + n + 16 * j]) : 0.f;
+        for (int j = 0; j < J; j++) a2[j] = live && n + 16 * j < k.N ? octaves(k.A[(size_t)channel * k.N + n + 16 * j]) : 0.f;
     }
     __device__ __forceinline__ void load_state(const float *s, float (&h)[J]) const {
 #pragma unroll
-        for (int j = 0; j < J; j++) h[j] = s && n + 16 * j < k.N ? s[state_at(n + 16 * j)] : 0.f;
+        for (int j = 0; j < J; j++) h[j] = s && live && n + 16 * j < k.N ? s[state_at(n + 16 * j)] : 0.f;
     }
     __device__ __forceinline__ void store_state(float *s, const float (&h)[J]) const {
 #pragma unroll
@@ -283,7 +284,7 @@ struct Work {
     // two steps and to nothing not at all, since what it makes may be finite where it itself is not.)
     __device__ __forceinline__ void pass(int s, const float (&a2)[J], float (&v)[J]) const {
         const size_t at = (size_t)b * k.segments + s;
-        const float dt = k.seg_dt[at * k.D + channel];
+        const float dt = live ? k.seg_dt[at * k.D + channel] : 0.f;
         float theirs[J];
         load_wide(k.seg_state, at, theirs);
 #pragma unroll

@@ -136,3 +136,23 @@ def test_growth_of_a_small_state():
     ref = O.selective_scan(**{n: t.double() for n, t in v.items()})
     for a, b in zip(K.selective_scan(**S._cuda(v, leaf=False)), ref):
         assert_close(a, b, RTOL[torch.float32])
+
+
+@pytest.mark.parametrize("T", [40, 200])
+def test_a_channel_that_is_not_finite_leaves_other_groups_alone(T):
+    """Groups of 5 channels in workgroups of more, sequences in one piece and cut in time: the first channel's state gradient, decay and step are not finite, the
+    second group's gradients are what they are without."""
+    from rwkv_wkv_hip import ssm as K
+    for N in (16, 24, 64):
+        v, grads = S._scan_inputs(torch.float32, 2, T, 10, N, 2)
+        runs = []
+        for bad in (False, True):
+            c = S._cuda(v, leaf=False)
+            gs = grads[1].cuda()
+            if bad:
+                gs[:, 0], c["A"][0, 1:], c["dt"][:, T - 9, 0] = math.inf, math.nan, math.nan
+            c = {n: t.requires_grad_(True) for n, t in c.items()}
+            runs.append((c, torch.autograd.grad(list(K.selective_scan(**c)), list(c.values()), [grads[0].cuda(), gs])))
+        for n, a, b in zip(v, *(r[1] for r in runs)):
+            if n in ("B", "C"):
+                assert torch.isfinite(a).all() and torch.equal(a[:, :, 1], b[:, :, 1]), n
