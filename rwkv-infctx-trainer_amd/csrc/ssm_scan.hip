@@ -492,8 +492,9 @@ __global__ __launch_bounds__(64 * back_waves(J), J == 1 ? 4 : J == 2 ? 2 : 1) vo
         for (int e = w.tid; e < 512; e += W::THREADS) {
             const int which = e >> 8, token = (e >> 4) & 15, state = e & 15, t = tile * TILE + token;
             const float v = f(which, token, state);
+            // (behind the sequence's end a step or gradient of zero times a state or gradient that is not finite is still to be zero)
             if (t < k.T && state + 16 * j < k.N)
-                (which ? k.gc_part : k.gb_part)[((((size_t)w.ct * k.B + w.b) * k.T + t) * k.G + w.g) * k.N + state + 16 * j] = v;
+                (which ? k.gc_part : k.gb_part)[((((size_t)w.ct * k.B + w.b) * k.T + t) * k.G + w.g) * k.N + state + 16 * j] = t < w.len ? v : 0.f;
         }
     };
     auto add_up = [&](const float (&p)[BACK_WAVES][2][16 * PITCH], int tile, int j) {

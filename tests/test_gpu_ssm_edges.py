@@ -156,3 +156,16 @@ def test_a_channel_that_is_not_finite_leaves_other_groups_alone(T):
         for n, a, b in zip(v, *(r[1] for r in runs)):
             if n in ("B", "C"):
                 assert torch.isfinite(a).all() and torch.equal(a[:, :, 1], b[:, :, 1]), n
+
+
+@pytest.mark.parametrize("N", [16, 40])
+def test_gradients_behind_a_sequence_are_zero(N):
+    """Of B and C too, in the tile the sequence ends in, whatever gradient comes in through the state."""
+    from rwkv_wkv_hip import ssm as K
+    v, grads = S._scan_inputs(torch.float32, 3, 40, 12, N, lengths=[21, 0, 40])
+    grads[1][0, 3], grads[1][1, 5, 2] = math.inf, math.nan
+    c = S._cuda(v)
+    torch.autograd.backward(list(K.selective_scan(**c)), [a.cuda() for a in grads])
+    for n in ("x", "dt", "z", "B", "C"):
+        assert not c[n].grad[0, 21:].any() and not c[n].grad[1].any(), n
+    assert torch.isfinite(c["B"].grad[2]).all()
