@@ -51,6 +51,10 @@ void check_out_state(const Tensor &out, std::initializer_list<int64_t> shape, at
     REQUIRE(!recorded);          // (a backward would need the state it replaces)
     REQUIRE(has_shape(out, shape) && out.scalar_type() == type && out.is_contiguous() && (reinterpret_cast<uintptr_t>(out.data_ptr()) & 15) == 0);
 }
+// a kernel has written the caller's buffer: whoever saved it for a backward is to notice (inference tensors have no version)
+void written(const Tensor &out) {
+    if (out.defined() && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+}
 int fits_int(int64_t n) {
     if (n > INT_MAX) raise(PyExc_ValueError, "size out of range");
     return (int)n;
@@ -123,6 +127,7 @@ PyObject *py_causal_conv(PyObject *, PyObject *const *a, Py_ssize_t n) {
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
             o = CausalConv::forward(nullptr, x, w, maybe(b), maybe(s), maybe(lengths), silu, maybe(out));
+            written(out);
         }
     }
     return tuple(o[0], o[1]);
@@ -209,6 +214,7 @@ PyObject *py_selective_scan(PyObject *, PyObject *const *a, Py_ssize_t n) {
         } else {
             at::AutoDispatchBelowADInplaceOrView below;
             o = SelectiveScan::forward(nullptr, v[0], v[1], v[2], v[3], v[4], maybe(v[5]), maybe(v[6]), maybe(v[7]), maybe(v[8]), maybe(lengths), maybe(out));
+            written(out);
         }
     }
     return tuple(o[0], o[1]);

@@ -169,3 +169,35 @@ def test_gradients_behind_a_sequence_are_zero(N):
     for n in ("x", "dt", "z", "B", "C"):
         assert not c[n].grad[0, 21:].any() and not c[n].grad[1].any(), n
     assert torch.isfinite(c["B"].grad[2]).all()
+
+
+# ---- buffers
+def test_a_state_overwritten_in_place_is_noticed():
+    """What autograd has saved and out_state has overwritten since raises in the backward pass, as after any operation in place."""
+    from rwkv_wkv_hip import ssm as K
+    r = lambda *s: torch.randn(*s, device="cuda")
+    w, window, state = r(8, 4), r(2, 3, 8), r(2, 8, 16)
+    A, one, b = -torch.rand(8, 16, device="cuda"), r(2, 1, 8), r(2, 1, 16)
+    scale = torch.ones((), device="cuda", requires_grad=True)
+
+    y, _ = K.causal_conv(r(2, 5, 8).requires_grad_(True), w, state=window)
+    before = window._version
+    with torch.no_grad():
+        K.causal_conv(one, w, state=window, out_state=window)
+    assert window._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+    z = state * scale
+    before = state._version
+    with torch.no_grad():
+        K.selective_scan(one, one, A, b, b, state=state, out_state=state)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+
+    with torch.inference_mode():          # (tensors without a version)
+        s = torch.zeros(2, 8, 16, device="cuda")
+        t = torch.zeros(2, 3, 8, device="cuda")
+        assert K.selective_scan(one, one, A, b, b, state=s, out_state=s)[1].data_ptr() == s.data_ptr()
+        assert K.causal_conv(one, w, state=t, out_state=t)[1].data_ptr() == t.data_ptr()
