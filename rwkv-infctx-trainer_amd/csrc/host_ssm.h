@@ -72,8 +72,10 @@ public:
     static variable_list forward(AutogradContext *ctx, const Tensor &x_, const Tensor &weight, const Maybe &bias_, const Maybe &state_, const Maybe &lengths_,
                                  bool silu, const Maybe &out_state_) {
         const Tensor bias = given(bias_), state = given(state_), lengths = given(lengths_), out_state = given(out_state_);
-        const Tensor x = strided(x_), w = plain_parameter(weight, x.scalar_type());
-        const Tensor b = bias.defined() ? plain(as_type(bias, w.scalar_type())) : bias, s = plain(state);
+        const Tensor x = strided(x_), s = plain(state);
+        // (the kernels take both parameters in one type: fp32 unless both have the streams')
+        const bool narrow = weight.scalar_type() == x.scalar_type() && (!bias.defined() || bias.scalar_type() == x.scalar_type());
+        const Tensor w = narrow ? plain(weight) : plain_float(weight), b = narrow ? plain(bias) : plain_float(bias);
         const int B = fits_int(x.size(0)), T = fits_int(x.size(1)), D = fits_int(x.size(2)), W = fits_int(w.size(1)), dt = dtype_code(x);
         OnDevice dev(x);
         const Tensor y = fresh({B, T, D}, x.scalar_type()), out = out_state.defined() ? out_state : fresh({B, W - 1, D}, x.scalar_type());

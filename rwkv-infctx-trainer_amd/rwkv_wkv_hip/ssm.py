@@ -44,7 +44,7 @@ def causal_conv(x, weight, bias=None, state=None, lengths=None, silu=True, out_s
         y[t] = act(bias + sum_k weight[:, k] xx[t - (W-1) + k]),   xx = x continued to the left by ``state``
 
     with act the SiLU, or nothing with ``silu=False``.  ``state`` (B,W-1,D), the W-1 inputs before x (None: zeros), and the
-    new state have x's type; weight and bias are read in x's type or in fp32.  x may be a slice of a wider
+    new state have x's type; weight and bias are read in x's type if both have it, else both in fp32.  x may be a slice of a wider
     tensor (any strides but the last).  ``lengths`` (B, integers): where each sequence ends; later tokens are not read, their y is
     zero, and the new state is the one after the sequence's last token.  ``out_state``: a buffer the new state is written
     to, without autograd; for a single token it may be ``state`` itself."""

@@ -201,3 +201,24 @@ def test_a_state_overwritten_in_place_is_noticed():
         t = torch.zeros(2, 3, 8, device="cuda")
         assert K.selective_scan(one, one, A, b, b, state=s, out_state=s)[1].data_ptr() == s.data_ptr()
         assert K.causal_conv(one, w, state=t, out_state=t)[1].data_ptr() == t.data_ptr()
+
+
+# ---- types that differ
+@pytest.mark.parametrize("x,weight,bias", [(torch.bfloat16, torch.bfloat16, torch.float32), (torch.float16, torch.float16, torch.float32), (torch.bfloat16, torch.float32, torch.bfloat16),
+                                           (torch.float32, torch.bfloat16, torch.float32), (torch.float16, torch.bfloat16, torch.float16)])
+def test_causal_conv_of_parameters_in_two_types(x, weight, bias):
+    """Neither parameter is held in fewer bits than it has: the fp32 one's gradient is right to fp32."""
+    from rwkv_wkv_hip import ssm as K
+    v, grads = S._conv_inputs(x, 2, 37, 48, 4, parameters=torch.float32)
+    v["weight"], v["bias"] = v["weight"].to(weight), v["bias"].to(bias)
+    S._compare(K.causal_conv, O.causal_conv, v, grads, ("y", "state"))
+
+
+@pytest.mark.parametrize("dtype,value", [(torch.bfloat16, 100.0625), (torch.float16, 70000.0)])
+def test_causal_conv_reads_a_bias_in_its_own_bits(dtype, value):
+    """bias - value + x: what a bias of 16 bits would lose is all that is left."""
+    from rwkv_wkv_hip import ssm as K
+    whole = 100.0 if dtype == torch.bfloat16 else 65504.0
+    x = torch.ones(1, 3, 8, dtype=dtype, device="cuda")
+    y, _ = K.causal_conv(x, torch.tensor([0.0, -whole], dtype=dtype, device="cuda").expand(8, 2), torch.full((8,), value, device="cuda"), silu=False)
+    assert (y.float() == value - whole).all()
