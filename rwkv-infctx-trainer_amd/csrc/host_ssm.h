@@ -160,7 +160,7 @@ public:
             ctx->saved_data["call"] = std::vector<int64_t>{type(A_), type(D_), type(bias_), type(state_), B_.dim(), state_.defined() && state_.requires_grad()};
             ctx->save_for_backward({x, dt, A, b, c, skip, z, bias, lengths, kept});
         }
-        return {y, state_.defined() && !out_state.defined() ? as_type(out, state_.scalar_type()) : out};
+        return {y, out};
     }
     static variable_list backward(AutogradContext *ctx, variable_list grads) {
         const std::vector<int64_t> k = ctx->saved_data["call"].toIntVector();

@@ -60,7 +60,7 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, state=None, len
 
     G groups of D/G consecutive channels have a B and C of their own.  D, dt_bias (D), the gate z (B,T,D) and the incoming ``state``
     may be left out.  x, dt, z, B and C share one type and may be slices of wider tensors (any strides but the last); A, D,
-    dt_bias and the state are read in fp32.  ``lengths`` and ``out_state`` as in ``causal_conv``."""
+    dt_bias and the state are read in fp32 whatever their type, and the new state is fp32.  ``lengths`` and ``out_state`` as in ``causal_conv``."""
     return _call("selective_scan", x, dt, A, B, C, D, z, dt_bias, state, lengths, out_state)
 
 

@@ -222,3 +222,23 @@ def test_causal_conv_reads_a_bias_in_its_own_bits(dtype, value):
     x = torch.ones(1, 3, 8, dtype=dtype, device="cuda")
     y, _ = K.causal_conv(x, torch.tensor([0.0, -whole], dtype=dtype, device="cuda").expand(8, 2), torch.full((8,), value, device="cuda"), silu=False)
     assert (y.float() == value - whole).all()
+
+
+@pytest.mark.parametrize("T", [1, 40])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float64])
+def test_a_state_leaves_in_32_bits(T, dtype):
+    """Whatever type the state comes in; its gradient goes back in that type."""
+    from rwkv_wkv_hip import ssm as K
+    v, grads = S._scan_inputs(torch.float32, 2, T, 24, 16)
+    v["state"] = v["state"].to(dtype)
+    c = S._cuda(v, leaf=False)
+    y, s = K.selective_scan(**c)
+    ref = O.selective_scan(**{n: t.double() for n, t in v.items()})
+    assert s.dtype == torch.float32
+    assert_close(s, ref[1], RTOL[torch.float32])
+    assert_close(y, ref[0], RTOL[torch.float32])
+    got, want = S._cuda(v), S._double(v)
+    torch.autograd.backward(list(K.selective_scan(**got)), [a.cuda() for a in grads])
+    torch.autograd.backward(list(O.selective_scan(**want)), [a.double() for a in grads])
+    assert got["state"].grad.dtype == dtype
+    assert_close(got["state"].grad, want["state"].grad, RTOL[torch.bfloat16 if dtype == torch.bfloat16 else torch.float32])
