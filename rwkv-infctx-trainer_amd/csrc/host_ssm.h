@@ -372,8 +372,9 @@ PyObject *py_sample(PyObject *, PyObject *const *a, Py_ssize_t n) {
     Tensor token, logprob;
     {
         NoLock no_lock;
-        at::AutoDispatchBelowADInplaceOrView below;
         same_device(l, {&u});
+        if (seen_by_autograd({&l})) raise(wkv_error, "sample has no gradient: call it under torch.no_grad() or with logits.detach()");
+        at::AutoDispatchBelowADInplaceOrView below;
         const int dt = dtype_code(l);
         REQUIRE(l.dim() == 2 && has_shape(u, {l.size(0)}));
         OnDevice dev(l);

@@ -14,5 +14,6 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
     kept weights passes u times their total.  logprobs: the logs of the probabilities they were drawn with.
 
     A temperature below 1e-6 takes the likeliest token.  NaN counts as -infinity; a row of nothing else gives token -1 and
-    -infinity.  The sums are of whole numbers, so a token depends on its row, u and settings alone.  No gradient."""
+    -infinity.  The sums are of whole numbers, so a token depends on its row, u and settings alone.  Without autograd only (logits that want a
+    gradient are refused: the logprobs would have none)."""
     return _call("sample", logits, u, temperature, top_k, top_p, min_p)

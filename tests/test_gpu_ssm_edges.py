@@ -242,3 +242,14 @@ def test_a_state_leaves_in_32_bits(T, dtype):
     torch.autograd.backward(list(O.selective_scan(**want)), [a.double() for a in grads])
     assert got["state"].grad.dtype == dtype
     assert_close(got["state"].grad, want["state"].grad, RTOL[torch.bfloat16 if dtype == torch.bfloat16 else torch.float32])
+
+
+# ---- sampling
+def test_sampling_refuses_logits_that_want_a_gradient():
+    from rwkv_wkv_hip import WKVError, sampling
+    l, u = torch.randn(2, 9, device="cuda", requires_grad=True), torch.rand(2, device="cuda")
+    with pytest.raises(WKVError):
+        sampling.sample(l, u)
+    want = sampling.sample(l.detach(), u)
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(sampling.sample(l, u), want))
