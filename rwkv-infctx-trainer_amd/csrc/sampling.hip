@@ -369,7 +369,7 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
         least_best = fminf(least_best, __shfl_xor(least_best, m));
     }
     if (lane == 0) {
-        sh.redf[0][wave] = top;
+        sh.redf[0][wave] = top + 0.f;          // (-0, which a maximum of zeros of both signs may be, is +0 from here on: less +0 it would be -0, whose bits lie past every cut)
         sh.redf[1][wave] = least_best;
     }
 #pragma unroll
@@ -378,6 +378,7 @@ __global__ __launch_bounds__(THREADS) void sample(const Call k) {
         sh.bin_count[tid + i * THREADS] = 0;
     }
     __syncthreads();
+    top = sh.redf[0][0];
 #pragma unroll
     for (int i = 0; i < WAVES; i++) {
         top = fmaxf(top, sh.redf[0][i]);

@@ -253,3 +253,21 @@ def test_sampling_refuses_logits_that_want_a_gradient():
     want = sampling.sample(l.detach(), u)
     with torch.no_grad():
         assert all(torch.equal(a, b) for a, b in zip(sampling.sample(l, u), want))
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
+def test_zeros_of_both_signs_are_the_likeliest_alike(dtype):
+    """In every order, within a lane's piece and in different lanes' and wavefronts'."""
+    from tests.test_gpu_sampling import _check
+    rows = []
+    for zeros in ([0.0, -0.0, -1.0], [-0.0, 0.0, -1.0], [-0.0, -1.0, -0.0], [-1.0, -0.0, 0.0]):
+        for apart in (1, 8, 512, 3000):
+            row = torch.full((9001,), -5.0)
+            row[0:3 * apart:apart] = torch.tensor(zeros)
+            rows.append(row)
+    l = torch.stack(rows).to(dtype)
+    assert torch.signbit(l[l == 0]).any() and not torch.signbit(l[l == 0]).all()
+    u = torch.linspace(0, 0.999, len(l))
+    for k in (dict(), dict(top_k=2), dict(top_p=0.5), dict(temperature=0.0)):
+        _check(l, u, **k)
+        _check(l, u.flip(0), **k)
