@@ -271,3 +271,56 @@ def test_zeros_of_both_signs_are_the_likeliest_alike(dtype):
     for k in (dict(), dict(top_k=2), dict(top_p=0.5), dict(temperature=0.0)):
         _check(l, u, **k)
         _check(l, u.flip(0), **k)
+
+
+# ---- the forms that many rows, tokens and sequences take
+@pytest.mark.parametrize("dtype,N,apart", [(torch.bfloat16, 16, 0), (torch.bfloat16, 16, 1), (torch.float32, 16, 0), (torch.float16, 20, 0), (torch.bfloat16, 8, 3)])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_single_tokens_of_many_sequences(dtype, N, apart, ragged):
+    """Four sequences to a lane, the last lanes with two; B and C at an offset that allows no whole loads; sequences without a token; the state in place."""
+    from rwkv_wkv_hip import ssm as K
+    B, D = 66, 8200 if N == 8 else 4100
+    v, _ = S._scan_inputs(dtype, B, 1, D, N, lengths=[i % 3 != 1 for i in range(B)] if ragged else None)
+    ref = O.selective_scan(**{n: t.double() if t.is_floating_point() else t for n, t in v.items()})
+    c = S._cuda(v, leaf=False)
+    wide = torch.zeros(B, 1, 2 * N + 4, dtype=dtype, device="cuda")
+    for n, at in (("B", apart), ("C", apart + N)):
+        wide[..., at:at + N] = c[n][:, :, 0]
+        c[n] = wide[..., at:at + N]
+    for out in K.selective_scan(**c), K.selective_scan(**c, out_state=c["state"]):
+        for a, b in zip(out, ref):
+            assert_close(a, b, RTOL[a.dtype])
+    assert out[1].data_ptr() == c["state"].data_ptr()
+
+
+def _conv_in_64_bits(x, weight, bias, state, lengths):
+    W, T = weight.shape[1], x.shape[1]
+    live = (torch.arange(T, device=x.device) < lengths[:, None])[..., None]
+    xx = torch.cat([state, torch.where(live, x, 0.0)], 1)
+    pre = bias + sum(weight[:, k] * xx[:, k:k + T] for k in range(W))
+    rows = (lengths[:, None] + torch.arange(W - 1, device=x.device))[..., None].expand_as(state)
+    return torch.where(live, pre * torch.sigmoid(pre), 0.0), xx.gather(1, rows)
+
+
+@pytest.mark.parametrize("dtype,B,T,D,W", [(torch.bfloat16, 8, 1061, 4096, 4), (torch.float32, 8, 1000, 2046, 3), (torch.float16, 8, 1061, 1023, 4), (torch.bfloat16, 8, 300, 4096, 2),
+                                           (torch.bfloat16, 8, 530, 4096, 4)])
+def test_causal_conv_by_long_runs(dtype, B, T, D, W):
+    """16 to 64 tokens to a lane, the sequences' ends and the last run's anywhere in a run; forward and backward, of four channels to a lane, two and one."""
+    from rwkv_wkv_hip import ssm as K
+    g = S._g(B, T, D, W)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()
+    v = dict(x=r(B, T, D), weight=r(D, W) * 0.5, bias=r(D), state=r(B, W - 1, D))
+    lengths = torch.tensor([T, 0, 1, 63, 64, 129, T - 1, T], device="cuda")
+    gy, gs = r(B, T, D), r(B, W - 1, D)
+    leaf, want = ({n: f(t).detach().requires_grad_(True) for n, t in v.items()} for f in (torch.clone, torch.Tensor.double))
+    out, ref = K.causal_conv(**leaf, lengths=lengths), _conv_in_64_bits(**want, lengths=lengths)
+    got, exact = (torch.autograd.grad(list(o), list(l.values()), [gy.to(o[0].dtype), gs.to(o[0].dtype)]) for o, l in ((out, leaf), (ref, want)))
+    for a, b, n in zip([*out, *got], [*ref, *exact], ["y", "state", *v]):
+        # (a parameter's gradient is a sum over 8 T tokens: fp32 errors of their magnitudes, not of the sum's)
+        assert_close(a, b, RTOL[a.dtype] if n not in ("weight", "bias") else max(RTOL[a.dtype], 2e-4), n)
+
+
+@pytest.mark.parametrize("rows,C", [(2500, 1032), (2500, 1030), (2500, 1029), (2500, 777), (2500, 2048), (1100, 2560), (1100, 6002), (1100, 4097), (1100, 8200), (5000, 1000)])
+def test_rms_norm_of_more_rows_than_workgroups(rows, C):
+    """Each workgroup of the backward takes several rows, one after another."""
+    S.test_rms_norm(torch.bfloat16, torch.float32, rows, C)
