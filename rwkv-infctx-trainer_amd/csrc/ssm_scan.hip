@@ -568,7 +568,7 @@ __global__ __launch_bounds__(64 * back_waves(J), J == 1 ? 4 : J == 2 ? 2 : 1) vo
                 float vb[TILE], vc[TILE];
                 w.read(sb, j, vb);
                 w.read(sc, j, vc);
-                float gb[TILE];
+                float gb[TILE], share = 0.f;          // share: a tile's of gA, so that its sum over the tokens rounds T / 16 + 16 times in a row, not T
                 const float an = a2[j] * LN2, dtx2 = again(dtx);
                 unrolled<TILE>([&](auto i) {
                     constexpr int I = TILE - 1 - decltype(i)::value;
@@ -578,8 +578,9 @@ __global__ __launch_bounds__(64 * back_waves(J), J == 1 ? 4 : J == 2 ? 2 : 1) vo
                     g[j] *= a[I];
                     const float q = g[j] * before[I];
                     slopes[I] = j == 0 ? q * an : fmaf(q, an, slopes[I]);
-                    add_lane<I>(ga[j], dt, q);
+                    add_lane<I>(share, dt, q);
                 });
+                ga[j] += share;
                 *reinterpret_cast<f4 *>(&part[J == 1 ? tile & 1 : 0][w.wave][0][w.n * PITCH + 4 * w.row]) = reduce_rows(gb);
             }
             __builtin_amdgcn_sched_barrier(0);

@@ -324,3 +324,28 @@ def test_causal_conv_by_long_runs(dtype, B, T, D, W):
 def test_rms_norm_of_more_rows_than_workgroups(rows, C):
     """Each workgroup of the backward takes several rows, one after another."""
     S.test_rms_norm(torch.bfloat16, torch.float32, rows, C)
+
+
+# ---- sums over many tokens
+def test_gradient_of_A_over_many_tokens():
+    """2048 tokens that are all alike, of a width at which no sequence is cut: every token adds the same to gA, so that a running sum's roundings go one way.  A tile's
+    16 are added up first: 16 + 128 roundings in a row, of 2^-24 each, are 8.6e-6 at the most; the terms themselves, whose state and gradient are fixed points of
+    recurrences that forget three quarters and more per token, have some 2e-6.  One after another they would have 2048 roundings."""
+    from rwkv_wkv_hip import ssm as K
+    T, D, N = 2048, 16384, 16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.rand(*s, device="cuda", generator=g)
+    x, raw, gy, b, c = r(1, 1, D) + 0.5, r(1, 1, D) + 1.0, r(1, 1, D) + 0.5, r(1, 1, N) + 0.5, r(1, 1, N) + 0.5
+    A = (-1.0 - r(D, N)).requires_grad_(True)
+    wide = lambda t: t.expand(1, T, -1)
+    y, _ = K.selective_scan(wide(x), wide(raw), A, wide(b), wide(c))
+    got, = torch.autograd.grad(y, A, wide(gy))
+    with torch.no_grad():
+        step = torch.nn.functional.softplus(raw[0, 0].double())[:, None]
+        a = torch.exp(step * A.double())
+        u, v = step * x[0, 0].double()[:, None] * b[0, 0].double(), c[0, 0].double() * gy[0, 0].double()[:, None]
+        # h[t] = u (1 - a^t) / (1 - a), its gradient v (1 - a^(T-t+1)) / (1 - a); gA = step sum over t of g[t] a h[t-1]
+        t = torch.arange(1, T + 1, device="cuda", dtype=torch.float64)
+        terms = sum(((1 - a ** (T - k + 1)) * (1 - a ** (k - 1)) for k in t.tolist()[:40] + t.tolist()[-40:])) + (T - 80)          # (a^40 < 2^-53)
+        want = step * u * v * a * terms / (1 - a) ** 2
+    assert_close(got / want, torch.ones_like(want), 6e-6)          # (taken twice: of the value and of the root mean square)
