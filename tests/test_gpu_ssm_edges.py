@@ -349,3 +349,18 @@ def test_gradient_of_A_over_many_tokens():
         terms = sum(((1 - a ** (T - k + 1)) * (1 - a ** (k - 1)) for k in t.tolist()[:40] + t.tolist()[-40:])) + (T - 80)          # (a^40 < 2^-53)
         want = step * u * v * a * terms / (1 - a) ** 2
     assert_close(got / want, torch.ones_like(want), 6e-6)          # (taken twice: of the value and of the root mean square)
+
+
+def test_gradients_of_a_state_that_forgets_everything():
+    """A = -infinity gives what an A gives that is finite and whose every exponential is zero: autograd through the definition would multiply zeros by infinities."""
+    from rwkv_wkv_hip import ssm as K
+    runs = []
+    for a in (-math.inf, -1e30):
+        v, grads = S._scan_inputs(torch.float32, 2, 40, 24, 16, lengths=[23, 40])
+        v["A"][3, 1], v["A"][7] = a, a
+        c = S._cuda(v)
+        out = K.selective_scan(**c)
+        torch.autograd.backward(list(out), [g.cuda() for g in grads])
+        runs.append([*out, *(c[n].grad for n in c if n != "lengths")])
+    for a, b in zip(*runs):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
