@@ -374,7 +374,8 @@ int wkv_causal_conv_backward(void *stream, int B, int T, int D, int W, int dtype
 /* The selective state space scan, N states (1 to 64) per channel, G groups of D / G channels:
  *   step = softplus(dt + dt_bias),  h[t] = exp(step A) h[t-1] + step x b[t],  y[t] = (c[t] . h[t] + skip x[t]) silu(z[t])
  * x, dt, z (or NULL: no gate), y (B,T,D), b, c (B,T,G,N) in `dtype`; A (D,N), skip, dt_bias (D; or NULL) fp32; state (B,D,N) fp32,
- * state_in NULL: zeros.  checkpoints: NULL, or wkv_selective_scan_checkpoint_bytes for a backward call.  workspace:
+ * state_in NULL: zeros.  checkpoints: NULL, or wkv_selective_scan_checkpoint_bytes (4 bytes per token and channel up to 16 states, 8 up to 32, 16
+ * above) for a backward call.  workspace:
  * wkv_selective_scan_forward_workspace bytes (none are needed for a single token without checkpoints, where state_out may be state_in). */
 size_t wkv_selective_scan_checkpoint_bytes(int B, int T, int D, int N, int G, int dtype);
 size_t wkv_selective_scan_forward_workspace(int B, int T, int D, int N, int G, int dtype);
@@ -382,7 +383,7 @@ int wkv_selective_scan_forward(void *stream, int B, int T, int D, int N, int G, 
                                const wkv_rows *b, const wkv_rows *c, const float *skip, const wkv_rows *z, const float *dt_bias, const float *state_in,
                                const int *lengths, void *y, float *state_out, float *checkpoints, void *workspace, size_t workspace_bytes);
 
-/* Its backward, from the forward call's checkpoints: gx, gdt, gz (B,T,D), gb, gc (B,T,G,N) contiguous in `dtype`, gA, gskip, gdt_bias and gstate_in fp32;
+/* Its backward, from the forward call's checkpoints, with a workspace of about N / 4 bytes per token and channel (N / 2 above 32 states): gx, gdt, gz (B,T,D), gb, gc (B,T,G,N) contiguous in `dtype`, gA, gskip, gdt_bias and gstate_in fp32;
  * gstate_out, gskip, gdt_bias and gstate_in may be NULL. */
 size_t wkv_selective_scan_backward_workspace(int B, int T, int D, int N, int G, int dtype);
 int wkv_selective_scan_backward(void *stream, int B, int T, int D, int N, int G, int dtype, const wkv_rows *x, const wkv_rows *dt, const float *A,
@@ -394,7 +395,7 @@ int wkv_selective_scan_backward(void *stream, int B, int T, int D, int N, int G,
  *   r = x + residual (NULL: x),   y = r / sqrt(mean(r^2) + eps) * weight
  * x, y in `dtype`; residual, residual_out (r; or NULL) in `residual_dtype`, weight in `weight_dtype`, each fp32 or `dtype`.  Row strides in
  * elements; outputs are contiguous.  q, scale non-NULL instead of y: y in 8 bits (e4m3), y = q scale[row], scale = max|y| / 448 (1 for a row of
- * zeros).  rstd: (rows), for a backward call, or NULL. */
+ * zeros, NaN for a row with one).  rstd: (rows), for a backward call, or NULL. */
 int wkv_rms_norm_forward(void *stream, int rows, int C, int dtype, int residual_dtype, int weight_dtype, float eps, const void *x, long long x_stride,
                          const void *residual, long long residual_stride, const void *weight, void *y, void *q, float *scale, void *residual_out,
                          float *rstd);

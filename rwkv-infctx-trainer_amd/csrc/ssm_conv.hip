@@ -5,7 +5,7 @@
 // where xx continues x to the left by the state, the W-1 inputs before it; the last W-1 of xx are the new state.  Backwards, with
 // gp[t] = gy[t] silu'(pre[t]):   gx[s] = sum over k of w[k] gp[s + W-1 - k],   gw[k] = sum over t of gp[t] xx[t - (W-1) + k].
 //
-// Bound by memory (B8 T4096 D4096 bf16: forward 103 us = 5.2 TB/s, backward 185 us = 4.4 TB/s): each input is to be read once and each output written once.  A lane holds four channels
+// Bound by memory (B8 T4096 D4096 bf16: forward 103 us = 5.2 TB/s, backward 187 us = 4.3 TB/s; single tokens of 64 sequences, the same kernel, 4.4 us): each input is to be read once and each output written once.  A lane holds four channels
 // (two or one where four are not aligned) and walks a run of tokens with the window in registers; the W-1 inputs (backwards also the W-1 gp) on a run's edge are read again, from
 // the cache.  The filter's gradient is summed along the run in registers, over the workgroup's four runs in LDS, and over
 // the workgroups by sum_rows.
@@ -315,8 +315,8 @@ template <class T, int V, bool BACK> static hipError_t launch(hipStream_t s, int
 #undef WKV_CONV
     return hipGetLastError();
 }
-// v: channels per lane, 4, or 2 or 1 where widths, strides or addresses allow no more (B8 T4096 bf16, forward and backward: D 4096 111 and 193 us by four,
-// D 4094 171 and 259 by two, 196 and 345 by one)
+// v: channels per lane, 4, or 2 or 1 where widths, strides or addresses allow no more (B8 T4096 bf16, forward and backward: D 4096 103 and 187 us by four,
+// D 4094 158 and 282 by two, D 4095 186 and 345 by one)
 template <class T> static hipError_t forward_t(hipStream_t s, int W, const Call &k, int v) {
     return v == 4 ? launch<T, 4, false>(s, W, k) : v == 2 ? launch<T, 2, false>(s, W, k) : launch<T, 1, false>(s, W, k);
 }

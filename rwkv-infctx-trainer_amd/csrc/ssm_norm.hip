@@ -145,7 +145,7 @@ __global__ __launch_bounds__(forward_threads<LANES>()) void forward(const Call k
         // (a scale below the smallest normal number would have no reciprocal.)  The quotient by the reciprocal and what that leaves is the rounded quotient
         // (Markstein); without the second step it is rounded twice, which moves elements in the middle of two 8-bit values.  A division's own
         // instructions took up to 7 % longer (5424 rows of 646 10.3 us against 9.8, 2000 of 9000 43.5 against 40.3).  What is left is that another order of the
-        // row's sum moves y by a step of fp32, and with it three in 100000 elements that lie that close to such a middle, by one of their steps.
+        // row's sum moves y by a step of fp32, and with it up to three in 100000 elements that lie that close to such a middle, by one of their steps.
         // per: an infinite scale leaves nothing.
         const float scale = top != top ? top : top > 0.f ? fmaxf(top / 448.f, 1.17549435e-38f) : 1.f, by = 1.f / scale, per = scale < INFINITY ? scale : 0.f;
         if (lane == 0) k.scale[row] = scale;

@@ -21,8 +21,9 @@
 //
 // What bounds it: vector instructions, not the memory.  Per token, channel and state the forward takes an exponential (two issue
 // slots) and four multiplications or multiply-adds, the backward an exponential and twelve; with the sums over the rows and a token's own arithmetic
-// that is 165 and 456 instructions per wavefront and tile, and the vector unit is busy 83 % and 81 % of the time (B8 T2048 D4096 N16 bf16: 450 us
-// forward with checkpoints, 0.8 GB, which memory alone would take 160 us for; 1190 us backward).
+// that is 165 and 472 instructions per wavefront and tile, and the vector unit is busy 83 % of the time in both (B8 T2048 D4096 N16 bf16: 455 us
+// forward with checkpoints, 0.8 GB, which memory alone would take 160 us for; 1188 us backward).  The recurrence by itself has 5 and 13 of them per token,
+// 80 and 208 per tile; the rest are the sums over states and channels (33 and 99 + 48) and a token's own arithmetic.
 #include "common.h"
 #include "row_sums.h"
 #include "vec.h"
@@ -693,9 +694,9 @@ static inline int states_per_lane(int N) { return N <= 16 ? 1 : N <= 32 ? 2 : 4;
 static inline long long workgroups(int B, int D, int G, int channels) { return (long long)B * G * ((D / G + channels - 1) / channels); }
 
 // Segments of a sequence: as many as give every compute unit `per_cu` workgroups, of eight tiles or more (of four up to four segments).
-// A cut costs a pass over the inputs without outputs, so it pays where workgroups are few: forward B1 T4096 D4096 281 us with one per compute unit,
-// 230 with two, 173 with four, but B4 T777 D4096 96 us uncut and 114 in two segments; forward and backward B1 T4096 D4096 (128 workgroups of
-// the backward) 815, 707 and 706 us with one, two and four of them, B1 T2048 D1536 (48) 177, 170, 144, B4 T1024 D4096 (512) 438 uncut, 501 in two.
+// A cut costs a pass over the inputs without outputs, so it pays where workgroups are few: forward B1 T4096 D4096 271 us with one per compute unit,
+// 221 with two, 159 with four, but B4 T777 D4096 84 us uncut and 101 in two segments; forward and backward B1 T4096 D4096 (128 workgroups of
+// the backward) 847, 666 and 562 us with one, two and four of them, B1 T2048 D1536 (48) 203, 163, 132, B4 T1024 D4096 (512) 431 uncut, 487 in two.
 static inline int segments_for(long long groups, int tiles, int per_cu) {
     const long long want = ((long long)per_cu * cu_count() + groups - 1) / groups;
     return (int)std::max(1ll, std::min({want, (long long)std::max(tiles / 8, std::min(4, tiles / 4)), 64ll}));
