@@ -418,6 +418,52 @@ int wkv_sample(void *stream, int rows, int V, int dtype, const void *logits, lon
                float temperature_value, const int *top_k, int top_k_value, const float *top_p, float top_p_value, const float *min_p, float min_p_value,
                long long *token, float *logprob);
 
+/* ---- The operators of a gated recurrence model (no counterpart in the reference). */
+
+/* The gated linear recurrence, a state per channel:
+ *   a[t] = exp(-scale softplus(decay) sigmoid(r[t])),  h[t] = a[t] h[t-1] + sqrt(1 - a[t]^2) sigmoid(i[t]) x[t],  y[t] = h[t] silu(z[t])
+ * x, r, i, z (or NULL: y = h), y (B,T,D) in `dtype` (wkv_rows: any strides of batch and token); decay (D), state_in (NULL: zeros), state_out (B,D) fp32;
+ * lengths as above.  checkpoints: NULL, or wkv_gated_recurrence_checkpoint_bytes (an fp32 state per 64 tokens) for a backward call.  state_out may be
+ * state_in for a single token without checkpoints. */
+size_t wkv_gated_recurrence_checkpoint_bytes(int B, int T, int D, int dtype);
+size_t wkv_gated_recurrence_forward_workspace(int B, int T, int D, int dtype);
+int wkv_gated_recurrence_forward(void *stream, int B, int T, int D, int dtype, float scale, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i,
+                                 const float *decay, const wkv_rows *z, const float *state_in, const int *lengths, void *y, float *state_out,
+                                 float *checkpoints, void *workspace, size_t workspace_bytes);
+
+/* Its backward: gx, gr, gi, gz (B,T,D) contiguous in `dtype`, gdecay (D) and gstate_in (B,D) fp32; gstate_out and gstate_in may be NULL. */
+size_t wkv_gated_recurrence_backward_workspace(int B, int T, int D, int dtype);
+int wkv_gated_recurrence_backward(void *stream, int B, int T, int D, int dtype, float scale, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i,
+                                  const float *decay, const wkv_rows *z, const int *lengths, const float *checkpoints, const void *gy, const float *gstate_out,
+                                  void *gx, void *gr, void *gi, float *gdecay, void *gz, float *gstate_in, void *workspace, size_t workspace_bytes);
+
+/* Rows of a table (V, C) by token:  out[n] = scale table[tokens[n]], n below count; tokens of 4 or 8 bytes (index_bytes).  A token below zero or from V on
+ * is a place without one: a row of zeros.  out (count, C) and the table contiguous in `dtype`. */
+int wkv_embedding_forward(void *stream, long long count, int V, int C, int dtype, int index_bytes, float scale, const void *tokens, const void *table,
+                          void *out);
+
+/* The table's gradient, written whole: gtable[v] = scale times the sum, in fp32 and the places' order, of gout's rows (a row stride in elements) whose token is v. */
+size_t wkv_embedding_backward_workspace(long long count, int V, int C);
+int wkv_embedding_backward(void *stream, long long count, int V, int C, int dtype, int index_bytes, float scale, const void *tokens, const void *gout,
+                           long long gout_stride, void *gtable, void *workspace, size_t workspace_bytes);
+
+/* The first half of a gated feed-forward block, for rows of C elements and two weights (F, C):
+ *   h = act(x w_gate') * (x w_up'),   act: 0 silu, 1 gelu (its tanh form), 2 relu
+ * x (rows, C) with a row stride in elements, weights and h (rows, F) contiguous, all in `dtype`; sums in fp32, h rounded once.  Where C is whole pieces of
+ * 16 bytes x, its stride and the weights are aligned to 16 bytes.  kept: NULL, or wkv_gated_product_kept_bytes (both products in fp32) for a backward call.
+ * workspace: wkv_gated_product_forward_workspace bytes (none where C is whole pieces or rows are few).  rows up to 2^21, C and F below 2^20. */
+size_t wkv_gated_product_kept_bytes(int rows, int C, int F, int dtype);
+size_t wkv_gated_product_forward_workspace(int rows, int C, int F, int dtype);
+int wkv_gated_product_forward(void *stream, int rows, int C, int F, int dtype, int activation, const void *x, long long x_stride, const void *w_gate,
+                              const void *w_up, void *h, float *kept, void *workspace, size_t workspace_bytes);
+
+/* Its backward, from the forward call's kept: gh (rows, F); gx (rows, C), gw_gate, gw_up (F, C) contiguous in `dtype`.  gx, or both of the weights' gradients, may be
+ * NULL: not wanted (want_x, want_w 0 in the query). */
+size_t wkv_gated_product_backward_workspace(int rows, int C, int F, int dtype, int want_x, int want_w);
+int wkv_gated_product_backward(void *stream, int rows, int C, int F, int dtype, int activation, const void *x, long long x_stride, const void *w_gate,
+                               const void *w_up, const float *kept, const void *gh, void *gx, void *gw_gate, void *gw_up, void *workspace,
+                               size_t workspace_bytes);
+
 #ifdef __cplusplus
 }
 #endif

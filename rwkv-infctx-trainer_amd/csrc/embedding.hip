@@ -1,0 +1,358 @@
+// Rows of a table by token, scaled, and the table's gradient:
+//
+//     out[n] = scale table[token[n]],      gtable[v] = scale (sum over the n with token[n] = v of gout[n])
+//
+// A token outside the table is a place without one: a row of zeros, no gradient.  Both directions are bound by memory.  The gradient is written
+// whole (V C, most of it zeros) from the places sorted by token, so that each row of it is summed by one wavefront in the places' order, in fp32: no
+// atomics, the same bits every time.  Sorting: stable passes over ten bits of the token at a most, counts per tile of 4096 places, then each tile's places to
+// where the tiles and digits before leave off; up to one tile's worth in a single launch.  A token that many places have is summed by runs of 64 places
+// first, whoever they belong to, so that no wavefront walks more than 126 places and the runs' sums.
+#include "common.h"
+#include "vec.h"
+
+namespace wkv {
+namespace embedding {
+
+// ---- lookup: 16 bytes (or an element) per lane
+struct Lookup { size_t count; int V, C; long long ws; float scale; const void *tokens, *table; void *out; };
+template <class I> __device__ __forceinline__ long long token_at(const void *p, size_t n) { return static_cast<const I *>(p)[n]; }
+
+constexpr int EACH = 4;                       // pieces per lane
+template <class T, class I, int W> __global__ __launch_bounds__(256) void lookup(const Lookup k) {
+    const unsigned pieces = k.C / W;
+    const size_t first = (size_t)blockIdx.x * (256 * EACH), n0 = first / pieces, total = k.count * pieces;
+    const unsigned start = (unsigned)(first - n0 * pieces);
+    float v[EACH][W];
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const unsigned at = start + e * 256 + threadIdx.x, r = at / pieces, c = at - r * pieces;
+#pragma unroll
+        for (int w = 0; w < W; w++) v[e][w] = 0.f;
+        if (first + e * 256 + threadIdx.x >= total) continue;
+        const long long t = token_at<I>(k.tokens, n0 + r);
+        if (t >= 0 && t < k.V) load_vec(static_cast<const T *>(k.table) + t * k.ws + c * W, v[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; e++) {
+        const size_t at = first + e * 256 + threadIdx.x;
+        if (at >= total) continue;
+#pragma unroll
+        for (int w = 0; w < W; w++) v[e][w] *= k.scale;
+        store_vec(static_cast<T *>(k.out) + at * W, v[e]);
+    }
+}
+
+// ---- sorting
+constexpr int TILE = 4096, SORT_THREADS = 1024, SORT_WAVES = 16, ROUNDS = TILE / SORT_THREADS, MAX_BITS = 10, BINS = 1 << MAX_BITS;
+struct Sort {
+    int count, V;                             // keys: tokens, V for none
+    const void *tokens;                       // the first pass's keys; their places are 0, 1, ..
+    const int *keys, *places;                 // the later passes'
+    int *to_keys, *to_places, *counts;        // counts (tiles, BINS)
+    int shift, bits;
+};
+template <class I> __device__ __forceinline__ int key_at(const Sort &k, int n) {
+    if (!k.tokens) return k.keys[n];
+    const long long t = token_at<I>(k.tokens, n);
+    return t >= 0 && t < k.V ? (int)t : k.V;
+}
+template <class I> __global__ __launch_bounds__(SORT_THREADS) void count(const Sort k) {
+    __shared__ int bin[BINS];
+    bin[threadIdx.x] = 0;
+    __syncthreads();
+    const int mask = (1 << k.bits) - 1;
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++) {
+        const long long n = (long long)blockIdx.x * TILE + j * SORT_THREADS + threadIdx.x;
+        if (n < k.count) atomicAdd(&bin[key_at<I>(k, (int)n) >> k.shift & mask], 1);          // (whole numbers: the order is nothing)
+    }
+    __syncthreads();
+    k.counts[(size_t)blockIdx.x * BINS + threadIdx.x] = bin[threadIdx.x];
+}
+
+struct SortLds {
+    int base[BINS];                           // where the tile's first place of a digit goes
+    int wave_sum[SORT_WAVES];
+    unsigned short seen[SORT_WAVES][BINS];    // places of a digit in a wavefront, then in those before it
+};
+// an exclusive sum over the workgroup's 1024 values
+__device__ __forceinline__ int sum_before(SortLds &m, int v) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int o = __shfl_up(s, d);
+        s += lane >= d ? o : 0;
+    }
+    if (lane == 63) m.wave_sum[wave] = s;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; w++) before += m.wave_sum[w];
+    return before + s - v;
+}
+// One tile's stable ranks by digit: keys[j] is place wave * 256 + j * 64 + lane of it, `there` of them exist.  rank[j]: the places of the same digit before it
+// in its wavefront; seen: those in the wavefronts before.  total: of digit threadIdx.x in the tile.
+__device__ __forceinline__ void ranks(SortLds &m, const int (&digit)[ROUNDS], const bool (&there)[ROUNDS], int bits, int (&rank)[ROUNDS], int &total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; w++) m.seen[w][threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++) {
+        unsigned long long same = __ballot(there[j]);
+        for (int b = 0; b < bits; b++) {
+            const unsigned long long set = __ballot(digit[j] >> b & 1);
+            same &= digit[j] >> b & 1 ? set : ~set;
+        }
+        const int before = __popcll(same & ((1ull << lane) - 1));
+        if (there[j]) {
+            rank[j] = m.seen[wave][digit[j]] + before;
+            // (the digit's last place in this round, after all of them have read: a wavefront's LDS accesses are in order)
+            if (__popcll(same >> lane) == 1) m.seen[wave][digit[j]] = (unsigned short)(rank[j] + 1);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < SORT_WAVES; w++) {
+        const int n = m.seen[w][threadIdx.x];
+        m.seen[w][threadIdx.x] = (unsigned short)total;
+        total += n;
+    }
+}
+template <class I> __global__ __launch_bounds__(SORT_THREADS) void scatter(const Sort k, int tiles) {
+    __shared__ SortLds m;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mask = (1 << k.bits) - 1;
+    int key[ROUNDS], place[ROUNDS], digit[ROUNDS], rank[ROUNDS], total;
+    bool there[ROUNDS];
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++) {
+        const long long n = (long long)blockIdx.x * TILE + wave * (64 * ROUNDS) + j * 64 + lane;
+        there[j] = n < k.count;
+        key[j] = there[j] ? key_at<I>(k, (int)n) : 0;
+        place[j] = k.tokens || !there[j] ? (int)n : k.places[n];
+        digit[j] = key[j] >> k.shift & mask;
+        rank[j] = 0;
+    }
+    // of digit threadIdx.x: in the tiles before, and in all
+    int before = 0, all = 0;
+    for (int t = 0; t < tiles; t++) {
+        const int n = k.counts[(size_t)t * BINS + threadIdx.x];
+        before += t < (int)blockIdx.x ? n : 0;
+        all += n;
+    }
+    m.base[threadIdx.x] = sum_before(m, all) + before;
+    ranks(m, digit, there, k.bits, rank, total);
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++)
+        if (there[j]) {
+            const int to = m.base[digit[j]] + m.seen[wave][digit[j]] + rank[j];
+            k.to_keys[to] = key[j];
+            k.to_places[to] = place[j];
+        }
+}
+// up to one tile: every pass in one launch
+template <class I> __global__ __launch_bounds__(SORT_THREADS) void sort_few(const Sort k, int passes) {
+    __shared__ SortLds m;
+    __shared__ int keys[TILE], places[TILE];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mask = (1 << k.bits) - 1;
+    for (int p = 0; p < passes; p++) {
+        int key[ROUNDS], place[ROUNDS], digit[ROUNDS], rank[ROUNDS], total;
+        bool there[ROUNDS];
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++) {
+            const int n = wave * (64 * ROUNDS) + j * 64 + lane;
+            there[j] = n < k.count;
+            key[j] = !there[j] ? 0 : p ? keys[n] : key_at<I>(k, n);
+            place[j] = p ? places[n] : n;
+            digit[j] = key[j] >> (p * k.bits) & mask;
+            rank[j] = 0;
+        }
+        __syncthreads();
+        ranks(m, digit, there, k.bits, rank, total);
+        m.base[threadIdx.x] = sum_before(m, total);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++)
+            if (there[j]) {
+                const int to = m.base[digit[j]] + m.seen[wave][digit[j]] + rank[j];
+                keys[to] = key[j];
+                places[to] = place[j];
+            }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int j = 0; j < ROUNDS; j++) {
+        const int n = j * SORT_THREADS + threadIdx.x;
+        if (n < k.count) {
+            k.to_keys[n] = keys[n];
+            k.to_places[n] = places[n];
+        }
+    }
+}
+// starts[v]: the first place whose token is v or later, v up to V (what has no token lies behind)
+static __global__ __launch_bounds__(256) void find_starts(const int *keys, int count, int V, int *starts) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v > V) return;
+    int lo = 0, hi = count;
+    while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (keys[mid] < v) lo = mid + 1;
+        else hi = mid;
+    }
+    starts[v] = lo;
+}
+
+// ---- sums
+constexpr int RUN = 64;                       // places of a run
+struct Gradient {
+    int count, V, C;
+    long long gs;                             // gout's row stride
+    float scale;
+    const int *keys, *places, *starts;
+    const void *gout;
+    float *runs;                              // (count / RUN, C)
+    void *out;
+};
+template <int W> __device__ __forceinline__ void add(float (&s)[W], const float (&v)[W]) {
+#pragma unroll
+    for (int w = 0; w < W; w++) s[w] += v[w];
+}
+// a run of places that all have one token: its sum
+template <class T, int W> __global__ __launch_bounds__(256) void sum_runs(const Gradient k) {
+    const int run = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * W;
+    const int *place = k.places + run * RUN, key = k.keys[run * RUN];
+    if (key == k.V || key != k.keys[run * RUN + RUN - 1] || c >= k.C) return;
+    float s[W];
+#pragma unroll
+    for (int w = 0; w < W; w++) s[w] = 0.f;
+    for (int j = 0; j < RUN; j += 4) {
+        float v[4][W];
+#pragma unroll
+        for (int q = 0; q < 4; q++) load_vec(static_cast<const T *>(k.gout) + place[j + q] * k.gs + c, v[q]);
+#pragma unroll
+        for (int q = 0; q < 4; q++) add(s, v[q]);
+    }
+    float *to = k.runs + (size_t)run * k.C + c;
+#pragma unroll
+    for (int w = 0; w < W; w++) to[w] = s[w];
+}
+// a row of the table per wavefront: its places up to the first whole run, the runs, the rest
+template <class T, int W> __global__ __launch_bounds__(256) void sum_rows_of(const Gradient k) {
+    const int v = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (v >= k.V) return;
+    const int from = k.starts[v], to = k.starts[v + 1];
+    int run0 = (from + RUN - 1) / RUN, run1 = to / RUN;
+    if (run1 <= run0) run0 = run1 = -1;
+    const int head = run0 < 0 ? to : run0 * RUN, tail = run0 < 0 ? to : run1 * RUN;
+    T *out = static_cast<T *>(k.out) + (size_t)v * k.C;
+    for (int c = lane * W; c < k.C; c += 64 * W) {
+        float s[W];
+#pragma unroll
+        for (int w = 0; w < W; w++) s[w] = 0.f;
+        auto places = [&](int n, int end) {
+            for (; n + 4 <= end; n += 4) {
+                float g[4][W];
+#pragma unroll
+                for (int q = 0; q < 4; q++) load_vec(static_cast<const T *>(k.gout) + k.places[n + q] * k.gs + c, g[q]);
+#pragma unroll
+                for (int q = 0; q < 4; q++) add(s, g[q]);
+            }
+            for (; n < end; n++) {
+                float g[W];
+                load_vec(static_cast<const T *>(k.gout) + k.places[n] * k.gs + c, g);
+                add(s, g);
+            }
+        };
+        places(from, head);
+        for (int r = run0; r < run1; r++) {
+            const float *p = k.runs + (size_t)r * k.C + c;
+#pragma unroll
+            for (int w = 0; w < W; w++) s[w] += p[w];
+        }
+        places(tail, to);
+#pragma unroll
+        for (int w = 0; w < W; w++) s[w] *= k.scale;
+        store_vec(out + c, s);
+    }
+}
+
+// ---- launches
+static inline int tiles_of(int count) { return (count + TILE - 1) / TILE; }
+struct Regions { size_t keys[2], places[2], counts, starts, runs, all; };
+static inline Regions regions(int count, int V, int C) {
+    Regions r;
+    size_t at = 0;
+    auto take = [&](size_t n) { const size_t was = at; at += (n + 255) / 256 * 256; return was; };
+    for (int i = 0; i < 2; i++) {
+        r.keys[i] = take((size_t)count * 4);
+        r.places[i] = take((size_t)count * 4);
+    }
+    r.counts = take((size_t)tiles_of(count) * BINS * 4);
+    r.starts = take(((size_t)V + 1) * 4);
+    r.runs = take((size_t)(count / RUN) * C * 4);
+    r.all = at;
+    return r;
+}
+// elements per lane: 16 bytes where rows are whole pieces, else one
+template <class T, class I> static hipError_t forward_t(hipStream_t s, const Lookup &k, bool whole) {
+    constexpr int W = 16 / sizeof(T);
+    const size_t pieces = k.count * (whole ? k.C / W : k.C);
+    const dim3 grid((unsigned)((pieces + 256 * EACH - 1) / (256 * EACH)));
+    if (whole) hipLaunchKernelGGL((lookup<T, I, W>), grid, dim3(256), 0, s, k);
+    else hipLaunchKernelGGL((lookup<T, I, 1>), grid, dim3(256), 0, s, k);
+    return hipGetLastError();
+}
+template <class I> static void sort(hipStream_t s, int count_, int V, const void *tokens, char *ws, const Regions &r, int &at) {
+    int bits = 1;
+    while ((V >> bits) != 0) bits++;          // V itself is a key
+    const int passes = (bits + MAX_BITS - 1) / MAX_BITS, tiles = tiles_of(count_);
+    Sort k = {};
+    k.count = count_; k.V = V; k.tokens = tokens;
+    k.bits = (bits + passes - 1) / passes;
+    k.counts = reinterpret_cast<int *>(ws + r.counts);
+    auto region = [&](size_t o) { return reinterpret_cast<int *>(ws + o); };
+    at = 0;
+    if (tiles == 1) {
+        k.to_keys = region(r.keys[0]);
+        k.to_places = region(r.places[0]);
+        hipLaunchKernelGGL(sort_few<I>, dim3(1), dim3(SORT_THREADS), 0, s, k, passes);
+        return;
+    }
+    for (int p = 0; p < passes; p++) {
+        k.shift = p * k.bits;
+        k.to_keys = region(r.keys[p & 1]);
+        k.to_places = region(r.places[p & 1]);
+        hipLaunchKernelGGL(count<I>, dim3(tiles), dim3(SORT_THREADS), 0, s, k);
+        hipLaunchKernelGGL(scatter<I>, dim3(tiles), dim3(SORT_THREADS), 0, s, k, tiles);
+        k.tokens = nullptr;
+        k.keys = k.to_keys;
+        k.places = k.to_places;
+        at = p & 1;
+    }
+}
+template <class T, int W> static void sums_w(hipStream_t s, const Gradient &k) {
+    if (k.count >= RUN) hipLaunchKernelGGL((sum_runs<T, W>), dim3(k.count / RUN, (k.C + 256 * W - 1) / (256 * W)), dim3(256), 0, s, k);
+    hipLaunchKernelGGL((sum_rows_of<T, W>), dim3((k.V + 3) / 4), dim3(256), 0, s, k);
+}
+template <class T> static hipError_t backward_t(hipStream_t s, Gradient k, const void *tokens, bool wide, bool whole, void *workspace) {
+    char *ws = static_cast<char *>(workspace);
+    const Regions r = regions(k.count, k.V, k.C);
+    int at;
+    if (wide) sort<long long>(s, k.count, k.V, tokens, ws, r, at);
+    else sort<int>(s, k.count, k.V, tokens, ws, r, at);
+    int *starts = reinterpret_cast<int *>(ws + r.starts);
+    k.keys = reinterpret_cast<int *>(ws + r.keys[at]);
+    k.places = reinterpret_cast<int *>(ws + r.places[at]);
+    k.starts = starts;
+    k.runs = reinterpret_cast<float *>(ws + r.runs);
+    hipLaunchKernelGGL(find_starts, dim3(k.V / 256 + 1), dim3(256), 0, s, k.keys, k.count, k.V, starts);
+    if (whole) sums_w<T, 16 / sizeof(T)>(s, k);
+    else sums_w<T, 1>(s, k);
+    return hipGetLastError();
+}
+
+}  // namespace embedding
+}  // namespace wkv

@@ -38,7 +38,11 @@ namespace {
     X(wkv_sigmoid_mul_forward) X(wkv_sigmoid_mul_backward) X(wkv_causal_conv_forward) X(wkv_causal_conv_backward)             \
     X(wkv_causal_conv_backward_workspace) X(wkv_selective_scan_checkpoint_bytes) X(wkv_selective_scan_forward_workspace)      \
     X(wkv_selective_scan_forward) X(wkv_selective_scan_backward_workspace) X(wkv_selective_scan_backward)                     \
-    X(wkv_rms_norm_forward) X(wkv_rms_norm_backward_workspace) X(wkv_rms_norm_backward) X(wkv_sample)
+    X(wkv_rms_norm_forward) X(wkv_rms_norm_backward_workspace) X(wkv_rms_norm_backward) X(wkv_sample) X(wkv_gated_product_kept_bytes) X(wkv_gated_product_forward_workspace) \
+    X(wkv_gated_product_forward) X(wkv_gated_product_backward_workspace) X(wkv_gated_product_backward)                           \
+    X(wkv_gated_recurrence_checkpoint_bytes) X(wkv_gated_recurrence_forward_workspace) X(wkv_gated_recurrence_forward)        \
+    X(wkv_gated_recurrence_backward_workspace) X(wkv_gated_recurrence_backward) X(wkv_embedding_forward)                      \
+    X(wkv_embedding_backward_workspace) X(wkv_embedding_backward)
 struct {
 #define X(name) decltype(&::name) name = nullptr;
     WKV_ABI(X)
@@ -422,6 +426,7 @@ PyObject *py_wkv4(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #include "host_layers.h"
 #include "host_ssm.h"
+#include "host_gated.h"
 
 // bind(path of the kernel library, WKVError, torch.nn.Linear, torch.nn.GroupNorm, (the dictionaries of hooks on all modules))
 PyObject *py_bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
@@ -445,7 +450,8 @@ PyObject *py_bind(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void *>(py_##name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(wkv56), METHOD(forward56), METHOD(backward56), METHOD(decay_operand), METHOD(wkv4), METHOD(timemix),
-                         METHOD(channelmix), METHOD(causal_conv), METHOD(selective_scan), METHOD(rms_norm), METHOD(rms_norm_fp8), METHOD(sample),
+                         METHOD(channelmix), METHOD(causal_conv), METHOD(selective_scan), METHOD(rms_norm), METHOD(rms_norm_fp8), METHOD(sample), METHOD(gated_recurrence), METHOD(gated_product),
+                         METHOD(embedding),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", "native host side of rwkv_wkv_hip", -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,134 @@
+// Products  out[m][n] = sum over k of A[m][k] B[n][k]  of operands whose k is contiguous, tile by tile on the matrix cores: the loop that the
+// gated feed-forward's products share.  A workgroup makes BM x BN outputs; 128 bytes of every row of A and B at a time (64 16-bit elements, 32 of
+// fp32) go from memory straight to LDS, the next 128 while these are multiplied.
+//
+// In LDS a row's eight pieces of 16 bytes are exchanged by the row's low three bits, so that sixteen rows' equal pieces, which the
+// matrix instructions take, lie over all banks.  A piece is a matrix instruction's whole operand of one lane: eight 16-bit elements for
+// v_mfma_f32_16x16x32, four fp32 ones for four v_mfma_f32_16x16x4_f32 (whatever the order of k, it is A's and B's alike).
+#pragma once
+#include "common.h"
+
+namespace wkv {
+namespace tiles {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+template <class T> constexpr int piece() { return 16 / (int)sizeof(T); }             // elements in 16 bytes
+template <class T> constexpr int depth() { return 128 / (int)sizeof(T); }            // of k at a time
+
+template <class T> __device__ __forceinline__ f4 mma(i4 a, i4 b, f4 c);
+template <> __device__ __forceinline__ f4 mma<bf16>(i4 a, i4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f4 mma<f16>(i4 a, i4 b, f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ f4 mma<float>(i4 a, i4 b, f4 c) {
+    const f4 x = __builtin_bit_cast(f4, a), y = __builtin_bit_cast(f4, b);
+#pragma unroll
+    for (int e = 0; e < 4; e++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+    return c;
+}
+
+// 16 bytes per lane from memory to LDS, the lanes' side by side from `lds` on; nothing waits for them here.  What lies outside the range comes as zeros.
+__device__ __forceinline__ void to_lds(i4 range, unsigned offset, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(range) : "memory");
+}
+__device__ __forceinline__ i4 range_of(const void *p, long long bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    const unsigned n = (unsigned)__builtin_amdgcn_readfirstlane((int)(bytes < 0 ? 0 : bytes > 0x7fffffff ? 0x7fffffff : bytes));
+    return i4{__builtin_amdgcn_readfirstlane((int)a), __builtin_amdgcn_readfirstlane((int)((a >> 32) & 0xffff)), (int)n, 0x00027000};
+}
+constexpr unsigned NOWHERE = 0xfffffff0u;
+
+// One operand's share of a workgroup's tile: ROWS rows of K elements from `p` on, `ld` apart, of which `live` are there.
+template <class T, int ROWS, int THREADS> struct Side {
+    static constexpr int ROUNDS = ROWS * 8 / THREADS;
+    const char *p;
+    long long bytes;                  // from p to the last live row's end
+    unsigned at[ROUNDS];
+    int column;                       // of the lane's piece, in elements
+    __device__ __forceinline__ void place(const T *base, long long ld, int K, int live) {
+        p = reinterpret_cast<const char *>(base);
+        bytes = live > 0 ? ((long long)(live - 1) * ld + K) * (long long)sizeof(T) : 0;
+        const int row = threadIdx.x >> 3, c = (threadIdx.x & 7) ^ (row & 7);
+        column = c * piece<T>();
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++) at[j] = (unsigned)((row + j * (THREADS / 8)) * ld * (long long)sizeof(T)) + c * 16;
+    }
+    // the tile of k from `k` on into LDS at `lds`
+    __device__ __forceinline__ void fetch(int k, int K, unsigned lds) const {
+        const long long skip = (long long)k * sizeof(T);
+        const i4 r = range_of(p + skip, bytes - skip);
+        const bool there = k + column < K;                      // (K is whole pieces)
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++) to_lds(r, there ? at[j] : NOWHERE, lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
+    }
+};
+
+// A launch's tiles in the order in which they are worked: the eight XCDs (a workgroup's number modulo 8) each take a run of
+// tiles, and a run goes down eight rows of tiles before it goes on to the next column, so that the workgroups that share an L2 share operands.
+__device__ __forceinline__ void tile_of(int index, int rows, int columns, int &row, int &column) {
+    const int all = rows * columns, x = index & 7, i = index >> 3, q = all >> 3, rest = all & 7;
+    const int t = x * q + (x < rest ? x : rest) + i;
+    const int band = 8 * columns, b = t / band, first = b * 8, high = rows - first < 8 ? rows - first : 8, in = t - b * band;
+    row = first + in % high;
+    column = in / high;
+}
+
+// The loop over k of a workgroup of WM x WN wavefronts: acc[i][j] is the sum of 16 rows of A and 16 of B, a lane's element e the one of A's row
+// (lane & 15) and B's row 4 (lane >> 4) + e.  B's rows come in PARTS parts of BN / PARTS rows; a wavefront takes its share of each.
+template <class T, int BM, int BN, int WM, int WN, int PARTS> struct Loop {
+    static constexpr int THREADS = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, BYTES = (BM + BN) * 128;
+    static constexpr int LDS = 2 * BYTES;
+    Side<T, BM, THREADS> a;
+    Side<T, BN / PARTS, THREADS> b[PARTS];
+    f4 acc[MT][NT];
+
+    __device__ __forceinline__ void fetch(int k, int K, unsigned lds) const {
+        a.fetch(k, K, lds);
+#pragma unroll
+        for (int p = 0; p < PARTS; p++) b[p].fetch(k, K, lds + (BM + p * (BN / PARTS)) * 128);
+    }
+    // k from k0 (whole tiles) to k1
+    __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
+        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+        const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+        const int row = lane & 15, first = row * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+        fetch(k0, K, base);
+        int which = 0;
+        for (int k = k0; k < k1; k += depth<T>()) {
+            // this tile is there, and every wavefront is done with the one before it
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (k + depth<T>() < k1) fetch(k + depth<T>(), K, base + (which ^ 1) * BYTES);
+            const char *A = lds + which * BYTES + wm * (MT * 16 * 128), *B = lds + which * BYTES + BM * 128;
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                const int off = first ^ (s * 64);
+                i4 y[NT];
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    const int part = j / (NT / PARTS), jj = j % (NT / PARTS);
+                    y[j] = *reinterpret_cast<const i4 *>(B + (part * (BN / PARTS) + (wn * (NT / PARTS) + jj) * 16) * 128 + off);
+                }
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    const i4 x = *reinterpret_cast<const i4 *>(A + i * 16 * 128 + off);
+#pragma unroll
+                    for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(y[j], x, acc[i][j]);
+                }
+            }
+            which ^= 1;
+        }
+    }
+};
+
+}  // namespace tiles
+}  // namespace wkv

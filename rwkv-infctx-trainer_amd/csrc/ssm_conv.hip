@@ -10,6 +10,7 @@
 // the cache.  The filter's gradient is summed along the run in registers, over the workgroup's four runs in LDS, and over
 // the workgroups by sum_rows.
 #include "common.h"
+#include "row_access.h"
 #include "row_sums.h"
 #include "vec.h"
 
@@ -34,47 +35,6 @@ template <int V> __device__ __forceinline__ void zero(float (&o)[V]) {
 #pragma unroll
     for (int i = 0; i < V; i++) o[i] = 0.f;
 }
-
-// A row's V elements of one lane as they lie in memory, read and written by buffer instructions whose range is a scalar: of a row that is not there it
-// is nothing, which reads as zero and is not written.  So no branch stands between a load and its use a group of tokens later.
-typedef unsigned u2 __attribute__((ext_vector_type(2)));
-typedef unsigned u4 __attribute__((ext_vector_type(4)));
-template <int BYTES> struct RawOf;
-template <> struct RawOf<2> { typedef unsigned short type; };
-template <> struct RawOf<4> { typedef unsigned type; };
-template <> struct RawOf<8> { typedef u2 type; };
-template <> struct RawOf<16> { typedef u4 type; };
-template <class T, int V> struct Row {
-    typedef typename RawOf<V * sizeof(T)>::type Raw;
-    static __device__ __forceinline__ __amdgpu_buffer_rsrc_t range(const void *p, bool there) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), (short)0, there ? (int)0x80000000u : 0, 0x00027000);
-    }
-    static __device__ __forceinline__ Raw load(const T *p, bool there, int at) {
-        const __amdgpu_buffer_rsrc_t b = range(p, there);
-        if constexpr (sizeof(Raw) == 2) return __builtin_amdgcn_raw_buffer_load_b16(b, at, 0, 0);
-        else if constexpr (sizeof(Raw) == 4) return __builtin_amdgcn_raw_buffer_load_b32(b, at, 0, 0);
-        else if constexpr (sizeof(Raw) == 8) return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b64(b, at, 0, 0));
-        else return __builtin_bit_cast(Raw, __builtin_amdgcn_raw_buffer_load_b128(b, at, 0, 0));
-    }
-    static __device__ __forceinline__ void store(T *p, bool there, int at, const float (&v)[V]) {
-        T e[V];
-#pragma unroll
-        for (int i = 0; i < V; i++) e[i] = from_float<T>(v[i]);
-        Raw raw;
-        __builtin_memcpy(&raw, e, sizeof(raw));
-        const __amdgpu_buffer_rsrc_t b = range(p, there);
-        if constexpr (sizeof(Raw) == 2) __builtin_amdgcn_raw_buffer_store_b16(raw, b, at, 0, 0);
-        else if constexpr (sizeof(Raw) == 4) __builtin_amdgcn_raw_buffer_store_b32(raw, b, at, 0, 0);
-        else if constexpr (sizeof(Raw) == 8) __builtin_amdgcn_raw_buffer_store_b64(raw, b, at, 0, 0);
-        else __builtin_amdgcn_raw_buffer_store_b128(raw, b, at, 0, 0);
-    }
-    static __device__ __forceinline__ void floats(const Raw &raw, float (&o)[V]) {
-        T e[V];
-        __builtin_memcpy(e, &raw, sizeof(raw));
-#pragma unroll
-        for (int i = 0; i < V; i++) o[i] = to_float(e[i]);
-    }
-};
 
 // one lane's channels of one sequence
 template <class T, int W, int V> struct Lane {

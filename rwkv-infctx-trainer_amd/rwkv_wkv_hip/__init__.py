@@ -6,6 +6,7 @@ from .ops import (WKV_5, WKV_6, RUN_WKV5_CUDA, RUN_WKV6STATE_CUDA, wkv_op, cumsu
 
 from . import blocks  # noqa: E402,F401  (token shift + mixing, ln_x * gate, channel-mix activations, L2Wrap)
 from . import ssm, sampling  # noqa: E402,F401  (state space block: convolution, selective scan, residual norm; next tokens)
+from . import gated  # noqa: E402,F401  (gated recurrence model: recurrence, feed-forward, embedding)
 
 # the reference's class names, same in-place calling convention as its RUN_* wrappers
 class WKV5_CUDA:
@@ -17,4 +18,4 @@ class WKV6STATE_CUDA:
 
 
 __all__ = ["WKV_5", "WKV_6", "WKV5_CUDA", "WKV6STATE_CUDA", "RUN_WKV5_CUDA", "RUN_WKV6STATE_CUDA", "wkv_op",
-           "cumsum_decay", "blocks", "ssm", "sampling", "set_algo", "RecomputeCache", "recompute_cache", "call_key", "stats", "WKVError", "LIB_PATH"]
+           "cumsum_decay", "blocks", "ssm", "sampling", "gated", "set_algo", "RecomputeCache", "recompute_cache", "call_key", "stats", "WKVError", "LIB_PATH"]

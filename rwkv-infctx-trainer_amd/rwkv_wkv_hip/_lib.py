@@ -79,6 +79,19 @@ SIGNATURES = {
     "wkv_rms_norm_forward": (_I, [_P] + [_I] * 5 + [c_float, _P, c_longlong, _P, c_longlong] + [_P] * 6),
     "wkv_rms_norm_backward_workspace": (c_size_t, [_I] * 2),
     "wkv_rms_norm_backward": (_I, [_P] + [_I] * 5 + [_P, c_longlong, _P, c_longlong] + [_P] * 7 + [_P, c_size_t]),
+    "wkv_gated_recurrence_checkpoint_bytes": (c_size_t, [_I] * 4),
+    "wkv_gated_recurrence_forward_workspace": (c_size_t, [_I] * 4),
+    "wkv_gated_recurrence_forward": (_I, [_P] + [_I] * 4 + [c_float] + [_P] * 11 + [c_size_t]),
+    "wkv_gated_recurrence_backward_workspace": (c_size_t, [_I] * 4),
+    "wkv_gated_recurrence_backward": (_I, [_P] + [_I] * 4 + [c_float] + [_P] * 16 + [c_size_t]),
+    "wkv_embedding_forward": (_I, [_P, c_longlong] + [_I] * 4 + [c_float] + [_P] * 3),
+    "wkv_embedding_backward_workspace": (c_size_t, [c_longlong, _I, _I]),
+    "wkv_embedding_backward": (_I, [_P, c_longlong] + [_I] * 4 + [c_float, _P, _P, c_longlong, _P, _P, c_size_t]),
+    "wkv_gated_product_kept_bytes": (c_size_t, [_I] * 4),
+    "wkv_gated_product_forward_workspace": (c_size_t, [_I] * 4),
+    "wkv_gated_product_forward": (_I, [_P] + [_I] * 5 + [_P, c_longlong] + [_P] * 5 + [c_size_t]),
+    "wkv_gated_product_backward_workspace": (c_size_t, [_I] * 6),
+    "wkv_gated_product_backward": (_I, [_P] + [_I] * 5 + [_P, c_longlong] + [_P] * 8 + [c_size_t]),
     "wkv_sample": (_I, [_P, _I, _I, _I, _P, c_longlong, _P, _P, c_float, _P, _I, _P, c_float, _P, c_float, _P, _P]),
 }
 
