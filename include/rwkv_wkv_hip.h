@@ -422,7 +422,7 @@ int wkv_sample(void *stream, int rows, int V, int dtype, const void *logits, lon
 
 /* The gated linear recurrence, a state per channel:
  *   a[t] = exp(-scale softplus(decay) sigmoid(r[t])),  h[t] = a[t] h[t-1] + sqrt(1 - a[t]^2) sigmoid(i[t]) x[t],  y[t] = h[t] silu(z[t])
- * x, r, i, z (or NULL: y = h), y (B,T,D) in `dtype` (wkv_rows: any strides of batch and token); decay (D), state_in (NULL: zeros), state_out (B,D) fp32;
+ * x, r, i, z (or NULL: y = h), y (B,T,D) in `dtype` (wkv_rows: any stride of batch, a token's from D up to 2^24); decay (D), state_in (NULL: zeros), state_out (B,D) fp32;
  * lengths as above.  checkpoints: NULL, or wkv_gated_recurrence_checkpoint_bytes (an fp32 state per 64 tokens) for a backward call.  state_out may be
  * state_in for a single token without checkpoints. */
 size_t wkv_gated_recurrence_checkpoint_bytes(int B, int T, int D, int dtype);

@@ -24,15 +24,16 @@ bool overlaps(const void *a, const void *b, size_t bytes) {
 
 // ---- gated recurrence
 int check_recurrence(int B, int T, int D, int dtype) {
-    if (B <= 0 || T <= 0 || D <= 0 || B > 65535 || T > (1 << 24) || D > (1 << 24)) return WKV_ERR_DIMS;
+    if (B <= 0 || T <= 0 || D <= 0 || B > 65535 || T > (1 << 24) || D >= gated::MAX_TOKEN_STRIDE) return WKV_ERR_DIMS;
     if ((long long)B * T * D >= (1ll << 40) || (long long)B * D >= (1ll << 30)) return WKV_ERR_DIMS;
     return dtype_ok(dtype);
 }
-int check_operands(int dtype, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i, const wkv_rows *z, const float *decay) {
+int check_operands(int T, int D, int dtype, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i, const wkv_rows *z, const float *decay) {
     if (!x || !r || !i || !decay) return WKV_ERR_NULL;
     for (const wkv_rows *o : {x, r, i, z}) {
         if (o && !o->p) return WKV_ERR_NULL;
         if (o && !aligned_to(o->p, element(dtype))) return WKV_ERR_ALIGN;
+        if (o && T > 1 && (o->token < D || o->token >= gated::MAX_TOKEN_STRIDE)) return WKV_ERR_DIMS;
     }
     return aligned16(decay) ? WKV_OK : WKV_ERR_ALIGN;
 }
@@ -92,7 +93,7 @@ int wkv_gated_recurrence_forward(void *stream, int B, int T, int D, int dtype, f
                                  const float *decay, const wkv_rows *z, const float *state_in, const int *lengths, void *y, float *state_out,
                                  float *checkpoints, void *workspace, size_t workspace_bytes) {
     if (int st = check_recurrence(B, T, D, dtype)) return st;
-    if (int st = check_operands(dtype, x, r, i, z, decay)) return st;
+    if (int st = check_operands(T, D, dtype, x, r, i, z, decay)) return st;
     if (!y || !state_out) return WKV_ERR_NULL;
     for (const void *p : {(const void *)state_in, (const void *)y, (const void *)state_out, (const void *)checkpoints, (const void *)workspace})
         if (!aligned16(p)) return WKV_ERR_ALIGN;
@@ -116,7 +117,7 @@ int wkv_gated_recurrence_backward(void *stream, int B, int T, int D, int dtype, 
                                   const float *decay, const wkv_rows *z, const int *lengths, const float *checkpoints, const void *gy, const float *gstate_out,
                                   void *gx, void *gr, void *gi, float *gdecay, void *gz, float *gstate_in, void *workspace, size_t workspace_bytes) {
     if (int st = check_recurrence(B, T, D, dtype)) return st;
-    if (int st = check_operands(dtype, x, r, i, z, decay)) return st;
+    if (int st = check_operands(T, D, dtype, x, r, i, z, decay)) return st;
     if (!checkpoints || !gy || !gx || !gr || !gi || !gdecay || (z && !gz) || !workspace) return WKV_ERR_NULL;
     for (const void *p : {(const void *)checkpoints, gy, (const void *)gstate_out, (const void *)gx, (const void *)gr, (const void *)gi, (const void *)gdecay,
                           (const void *)gz, (const void *)gstate_in, (const void *)workspace})

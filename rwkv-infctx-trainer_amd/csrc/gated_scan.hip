@@ -14,7 +14,7 @@
 // and inputs alone leaves every segment's pair first.  Backwards a step runs both ways at once: the states again, from one kept
 // before every CHECK tokens, and their gradients.
 //
-// 1 - a^2 loses its digits where a is near one, the very channels that remember long: below 2 log a = -1/4 it is formed from the series of exp(2 log a) - 1.
+// 1 - a^2 loses its digits where a is near one, the very channels that remember long: there it is formed from log a.
 #include "common.h"
 #include "row_access.h"
 #include "row_sums.h"
@@ -40,20 +40,19 @@ struct Call {
     float *pairs;
 };
 
-constexpr int WAVES = 16, CHECK = 64, STEP = 128;         // STEP: tokens of a forward step, and what a segment is a multiple of
+constexpr int WAVES = 16, BACK_WAVES = 16, CHECK = 64, STEP = 128;         // STEP: tokens of a forward step, and what a segment is a multiple of
+constexpr int MAX_TOKEN_STRIDE = 1 << 24;               // a wavefront's tokens lie within 32-bit offsets
 constexpr int OUTSIDE = (int)0x80000000u;                 // a lane's offset that is in no row's range
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * v)); }
 
-// 1 - a^2 of a = 2^l
+// 1 - a^2 of a = 2^l: near one the polynomial of degree 4 in l nearest to (1 - 4^l) / l where 4^l is above exp(-1/2), right to 2^-22.5 of the value
 __device__ __forceinline__ float one_less_square(float l, float a) {
-    const float s = -2.f * LN2 * l;
-    float p = fmaf(s, -1.f / 6, 1.f);
-    p = fmaf(p * s, -1.f / 5, 1.f);
-    p = fmaf(p * s, -1.f / 4, 1.f);
-    p = fmaf(p * s, -1.f / 3, 1.f);
-    p = fmaf(p * s, -1.f / 2, 1.f);
-    return s < 0.25f ? s * p : fmaf(-a, a, 1.f);
+    float p = fmaf(l, -0.03474162146449089f, -0.1514858603477478f);
+    p = fmaf(p, l, -0.4437292814254761f);
+    p = fmaf(p, l, -0.9608924984931946f);
+    p = fmaf(p, l, -1.3862942457199097f);
+    return l > -0.36067376f ? l * p : fmaf(-a, a, 1.f);
 }
 // log2 of a at an open gate; finite, so that a shut gate keeps the state whatever the decay is
 __device__ __forceinline__ float rate_of(float decay, float scale) {
@@ -61,6 +60,8 @@ __device__ __forceinline__ float rate_of(float decay, float scale) {
     const float rate = -scale * soft * LOG2E;
     return rate < -3e38f ? -3e38f : rate;
 }
+
+template <bool B> struct Bool { static constexpr bool value = B; };
 
 // one lane's channels of one sequence
 template <class T, int V> struct Lane {
@@ -74,15 +75,25 @@ template <class T, int V> struct Lane {
         d = (blockIdx.x * 64 + (threadIdx.x & 63)) * V;
         at = d < k.D ? d * (int)sizeof(T) : OUTSIDE;
         at32 = d < k.D ? d * 4 : OUTSIDE;
-        len = k.lengths ? min(max(k.lengths[b], 0), k.T) : k.T;
+        len = k.lengths ? min(max(__builtin_amdgcn_readfirstlane(k.lengths[b]), 0), k.T) : k.T;
 #pragma unroll
         for (int v = 0; v < V; v++) rate[v] = d < k.D ? rate_of(k.decay[d + v], k.scale) : 0.f;
     }
-    __device__ __forceinline__ Raw load(const Rows &s, int t) const { return R::load(static_cast<const T *>(s.p) + b * s.batch + t * s.token, t < len, at); }
-    __device__ __forceinline__ Raw load(const void *p, int t) const { return R::load(static_cast<const T *>(p) + ((size_t)b * k.T + t) * k.D, t < len, at); }
-    __device__ __forceinline__ void store(void *p, int t, const float (&v)[V]) const {
-        R::store(static_cast<T *>(p) + ((size_t)b * k.T + t) * k.D, t < k.T, at, v);
+    // a stream of this sequence, and up to `count` tokens of it from t on, those that there are before `end`: one range for all of them
+    struct Stream { const char *p; int step; };
+    struct Tokens { __amdgpu_buffer_rsrc_t range; int step; };
+    __device__ __forceinline__ Stream in(const Rows &s) const {
+        return {static_cast<const char *>(s.p) + (long long)b * s.batch * (long long)sizeof(T), (int)s.token * (int)sizeof(T)};
     }
+    __device__ __forceinline__ Stream whole(const void *p) const { return in(Rows{p, (long long)k.T * k.D, k.D}); }
+    __device__ __forceinline__ Tokens tokens(const Stream &s, int t, int count, int end) const {
+        const int n = min(end - t, count);
+        // (a scalar, which the compiler's choice of instructions loses: a range in vector registers is walked lane by lane)
+        const int bytes = __builtin_amdgcn_readfirstlane(n > 0 ? (n - 1) * s.step + k.D * (int)sizeof(T) : 0);
+        return {__builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(s.p + (long long)t * s.step), (short)0, bytes, 0x00027000), s.step};
+    }
+    __device__ __forceinline__ Raw load(const Tokens &s, int j) const { return R::load(s.range, at, j * s.step); }
+    __device__ __forceinline__ void store(const Tokens &s, int j, const float (&v)[V]) const { R::store(s.range, at, j * s.step, v); }
     // V floats of a row of D, zeros where there is none
     __device__ __forceinline__ void floats(const float *row, float (&o)[V]) const { Row<float, V>::floats(Row<float, V>::load(row, row != nullptr, at32), o); }
     __device__ __forceinline__ void put(float *row, const float (&o)[V]) const { Row<float, V>::store(row, true, at32, o); }
@@ -103,17 +114,20 @@ __global__ __launch_bounds__(64 * WAVES) void forward(const Call k) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), segment = blockIdx.z;
     const int begin = segment * k.span, end = min(begin + k.span, k.T);
     Raw x[K], r[K], i[K], z[K];
-    auto ask = [&](int t0) {
+    typedef typename Lane<T, V>::Stream Stream;
+    typedef typename Lane<T, V>::Tokens Tokens;
+    const Stream xs = l.in(k.x), rs = l.in(k.r), is = l.in(k.i), zs = l.in(k.z), ys = l.whole(k.y);
+    {
+        const int t = begin + wave * K;
+        const Tokens nx = l.tokens(xs, t, K, l.len), nr = l.tokens(rs, t, K, l.len), ni = l.tokens(is, t, K, l.len), nz = l.tokens(zs, t, K, l.len);
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            const int t = t0 + wave * K + j;
-            x[j] = l.load(k.x, t);
-            r[j] = l.load(k.r, t);
-            i[j] = l.load(k.i, t);
-            if (GATE && MODE == FORWARD) z[j] = l.load(k.z, t);
+            x[j] = l.load(nx, j);
+            r[j] = l.load(nr, j);
+            i[j] = l.load(ni, j);
+            if (GATE && MODE == FORWARD) z[j] = l.load(nz, j);
         }
-    };
-    ask(begin);
+    }
     float h[V], all[V];                       // the state before the step; PAIRS: from nothing, with the product of all a
 #pragma unroll
     for (int v = 0; v < V; v++) h[v] = 0.f, all[v] = 1.f;
@@ -127,19 +141,26 @@ __global__ __launch_bounds__(64 * WAVES) void forward(const Call k) {
             for (int v = 0; v < V; v++) h[v] = fmaf(a[v], h[v], e[v]);
         }
     }
-    int which = 0;
-    for (int t0 = begin; t0 < end; t0 += STEP, which ^= 1) {
+    // WHOLE: all of the wavefront's tokens are there (as they are but at a sequence's end)
+    auto step = [&](auto whole, int t0, int which) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const int t = t0 + wave * K;
         float a[K][V], u[K][V];
         Pair mine;
 #pragma unroll
         for (int v = 0; v < V; v++) mine.a[v] = 1.f, mine.h[v] = 0.f;
+        const Tokens nx = l.tokens(xs, t + STEP, K, l.len), nr = l.tokens(rs, t + STEP, K, l.len), ni = l.tokens(is, t + STEP, K, l.len);
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            const bool there = t0 + wave * K + j < l.len;
+            const bool there = WHOLE || t + j < l.len;
             float xf[V], rf[V], jf[V];
             R::floats(x[j], xf);
             R::floats(r[j], rf);
             R::floats(i[j], jf);
+            // the next step's token into the place of this one's: as much is on its way at any time as a step takes
+            x[j] = l.load(nx, j);
+            r[j] = l.load(nr, j);
+            i[j] = l.load(ni, j);
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 const float lg = l.rate[v] * sigmoid(rf[v]), e = exp2_fast(lg);
@@ -149,40 +170,47 @@ __global__ __launch_bounds__(64 * WAVES) void forward(const Call k) {
                 mine.h[v] = fmaf(a[j][v], mine.h[v], u[j][v]);
             }
         }
-        float gate[K][V];
-        if (GATE && MODE == FORWARD)
-#pragma unroll
-            for (int j = 0; j < K; j++) R::floats(z[j], gate[j]);
-        ask(t0 + STEP);
         pairs[which][wave][lane] = mine;
         lds_barrier();
         float before[V];
+        auto join = [&](int from, int to) {
+#pragma unroll 4
+            for (int w = from; w < to; w++) {
+                const Pair p = pairs[which][w][lane];
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const Pair p = pairs[which][w][lane];
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                if (w == wave) before[v] = h[v];
-                h[v] = fmaf(p.a[v], h[v], p.h[v]);
-                if (MODE == PAIRS) all[v] *= p.a[v];
+                for (int v = 0; v < V; v++) {
+                    h[v] = fmaf(p.a[v], h[v], p.h[v]);
+                    if (MODE == PAIRS) all[v] *= p.a[v];
+                }
             }
-        }
-        if (MODE == PAIRS) continue;
-        if (k.checkpoints && wave * K % CHECK == 0 && t0 + wave * K < k.T)
-            l.put(k.checkpoints + ((size_t)l.b * ((k.T + CHECK - 1) / CHECK) + (t0 + wave * K) / CHECK) * k.D, before);
+        };
+        join(0, wave);
+#pragma unroll
+        for (int v = 0; v < V; v++) before[v] = h[v];
+        join(wave, WAVES);
+        if (MODE == PAIRS) return;
+        if (k.checkpoints && wave * K % CHECK == 0 && t < k.T)
+            l.put(k.checkpoints + ((size_t)l.b * ((k.T + CHECK - 1) / CHECK) + t / CHECK) * k.D, before);
+        const Tokens y = l.tokens(ys, t, K, k.T), nz = l.tokens(zs, t + STEP, K, l.len);
 #pragma unroll
         for (int j = 0; j < K; j++) {
-            const int t = t0 + wave * K + j;
-            float o[V];
+            const bool there = WHOLE || t + j < l.len;
+            float o[V], zf[V];
+            if (GATE) {
+                R::floats(z[j], zf);
+                z[j] = l.load(nz, j);
+            }
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 before[v] = fmaf(a[j][v], before[v], u[j][v]);
-                o[v] = GATE ? before[v] * gate[j][v] * sigmoid(gate[j][v]) : before[v];
-                o[v] = t < l.len ? o[v] : 0.f;
+                o[v] = there ? GATE ? before[v] * (zf[v] * sigmoid(zf[v])) : before[v] : 0.f;
             }
-            l.store(k.y, t, o);
+            l.store(y, j, o);
         }
-    }
+    };
+    int which = 0, t0 = begin;
+    for (; t0 < end && t0 + STEP <= l.len; t0 += STEP, which ^= 1) step(Bool<true>(), t0, which);
+    for (; t0 < end; t0 += STEP, which ^= 1) step(Bool<false>(), t0, which);
     if (wave != 0) return;
     if (MODE == PAIRS) {
         l.put(l.pair(segment), all);
@@ -193,33 +221,44 @@ __global__ __launch_bounds__(64 * WAVES) void forward(const Call k) {
 }
 
 template <class T, int V, bool GATE, int MODE>
-__global__ __launch_bounds__(64 * WAVES) void backward(const Call k) {
-    constexpr int K = CHECK / WAVES;
+__global__ __launch_bounds__(64 * BACK_WAVES) void backward(const Call k) {
+    constexpr int K = CHECK / BACK_WAVES;
     typedef Row<T, V> R;
     typedef typename R::Raw Raw;
     struct Pair { float a[V], h[V], g[V]; };          // a run's product of a, its state from nothing, what it hands to the token before it from nothing
-    __shared__ Pair pairs[2][WAVES][64];
+    __shared__ Pair pairs[2][BACK_WAVES][64];
     const Lane<T, V> l(k);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), segment = blockIdx.z;
     const int begin = segment * k.span, end = min(begin + k.span, k.T), checks = (k.T + CHECK - 1) / CHECK;
     Raw x[K], r[K], i[K], z[K], gy[K];
     float start[V];
-    auto ask = [&](int t0) {
-        t0 = max(t0, begin);
-#pragma unroll
-        for (int j = 0; j < K; j++) {
-            const int t = t0 + wave * K + j;
-            r[j] = l.load(k.r, t);
-            gy[j] = l.load(k.gy, t);
-            if (GATE) z[j] = l.load(k.z, t);
-            if (MODE == PAIRS) continue;
-            x[j] = l.load(k.x, t);
-            i[j] = l.load(k.i, t);
-        }
-        if (MODE != PAIRS) l.floats(k.checkpoints + ((size_t)l.b * checks + t0 / CHECK) * k.D, start);
+    typedef typename Lane<T, V>::Stream Stream;
+    typedef typename Lane<T, V>::Tokens Tokens;
+    const Stream xs = l.in(k.x), rs = l.in(k.r), is = l.in(k.i), zs = l.in(k.z), gs = l.whole(k.gy);
+    const Stream xo = l.whole(k.gx), ro = l.whole(k.gr), io = l.whole(k.gi), zo = l.whole(k.gz);
+    Tokens nx, nr, ni, nz, ng;
+    auto streams = [&](int t0) {
+        const int t = max(t0, begin) + wave * K;
+        nr = l.tokens(rs, t, K, l.len);
+        ng = l.tokens(gs, t, K, l.len);
+        if (GATE) nz = l.tokens(zs, t, K, l.len);
+        if (MODE == PAIRS) return;
+        nx = l.tokens(xs, t, K, l.len);
+        ni = l.tokens(is, t, K, l.len);
+        l.floats(k.checkpoints + ((size_t)l.b * checks + max(t0, begin) / CHECK) * k.D, start);
+    };
+    auto ask = [&](int j) {
+        r[j] = l.load(nr, j);
+        gy[j] = l.load(ng, j);
+        if (GATE) z[j] = l.load(nz, j);
+        if (MODE == PAIRS) return;
+        x[j] = l.load(nx, j);
+        i[j] = l.load(ni, j);
     };
     const int last = begin + (end - begin - 1) / CHECK * CHECK;
-    ask(last);
+    streams(last);
+#pragma unroll
+    for (int j = 0; j < K; j++) ask(j);
     float c[V], all[V], sum[V];               // c: what the tokens behind the step hand to its last one
 #pragma unroll
     for (int v = 0; v < V; v++) c[v] = sum[v] = 0.f, all[v] = 1.f;
@@ -233,99 +272,128 @@ __global__ __launch_bounds__(64 * WAVES) void backward(const Call k) {
             for (int v = 0; v < V; v++) c[v] = fmaf(a[v], c[v], e[v]);
         }
     }
-    int which = 0;
-    for (int t0 = last; t0 >= begin; t0 -= CHECK, which ^= 1) {
-        float a[K][V], lg[K][V], rs[K][V], is[K][V], ix[K][V], b[K][V], go[K][V], gv[K][V], zf[K][V], zs[K][V], h[V];
+    float slope[V];                           // of log a by sigmoid(r)
+#pragma unroll
+    for (int v = 0; v < V; v++) slope[v] = l.rate[v] * LN2;
+    auto step = [&](auto whole, int t0, int which) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        const int t = t0 + wave * K;
+        // what the tokens' second half takes from the first; u: beta sigmoid(i) x
+        float a[K][V], beta[K][V], u[K][V], rs[K][V], is[K][V], zs[K][V], hs[K + 1][V];
+        Raw zk[K], gk[K];
         Pair mine;
 #pragma unroll
-        for (int v = 0; v < V; v++) mine.a[v] = 1.f, mine.h[v] = mine.g[v] = 0.f, h[v] = start[v];
+        for (int v = 0; v < V; v++) mine.a[v] = 1.f, mine.h[v] = mine.g[v] = 0.f, hs[0][v] = start[v];
+        streams(t0 - CHECK);
 #pragma unroll
-        for (int j = 0; j < K; j++) {
-            const bool there = t0 + wave * K + j < l.len;
-            float xf[V], rf[V], jf[V];
+        for (int j = K - 1; j >= 0; j--) {
+            const bool there = WHOLE || t + j < l.len;
+            float xf[V], rf[V], jf[V], zf[V], gf[V];
             R::floats(r[j], rf);
-            R::floats(gy[j], gv[j]);
-            if (GATE) R::floats(z[j], zf[j]);
+            R::floats(gy[j], gf);
+            if (GATE) R::floats(z[j], zf);
             if (MODE == FORWARD) {
                 R::floats(x[j], xf);
                 R::floats(i[j], jf);
+                gk[j] = gy[j];
+                if (GATE) zk[j] = z[j];
             }
+            ask(j);          // the next step's token into the place of this one's
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 rs[j][v] = sigmoid(rf[v]);
-                lg[j][v] = there ? l.rate[v] * rs[j][v] : 0.f;
-                a[j][v] = exp2_fast(lg[j][v]);
-                if (GATE) zs[j][v] = sigmoid(zf[j][v]);
-                go[j][v] = !there ? 0.f : GATE ? gv[j][v] * zf[j][v] * zs[j][v] : gv[j][v];
+                const float lg = there ? l.rate[v] * rs[j][v] : 0.f;
+                a[j][v] = exp2_fast(lg);
+                if (GATE) zs[j][v] = sigmoid(zf[v]);
+                mine.g[v] = a[j][v] * (GATE ? fmaf(gf[v], zf[v] * zs[j][v], mine.g[v]) : gf[v] + mine.g[v]);          // (what is not there came as zeros)
                 mine.a[v] *= a[j][v];
                 if (MODE == PAIRS) continue;
-                b[j][v] = one_less_square(lg[j][v], a[j][v]);
+                const float b = one_less_square(lg, a[j][v]);
                 is[j][v] = sigmoid(jf[v]);
-                ix[j][v] = is[j][v] * xf[v];
-                mine.h[v] = fmaf(a[j][v], mine.h[v], there ? __builtin_amdgcn_sqrtf(b[j][v]) * ix[j][v] : 0.f);
+                beta[j][v] = __builtin_amdgcn_sqrtf(b);
+                u[j][v] = beta[j][v] * is[j][v] * xf[v];
             }
+            __builtin_amdgcn_sched_barrier(0);          // (tokens all at once take more registers than there are)
         }
+        if (MODE == FORWARD)
 #pragma unroll
-        for (int j = K - 1; j >= 0; j--)
+            for (int j = 0; j < K; j++)
 #pragma unroll
-            for (int v = 0; v < V; v++) mine.g[v] = a[j][v] * (go[j][v] + mine.g[v]);
-        ask(t0 - CHECK);
+                for (int v = 0; v < V; v++) mine.h[v] = fmaf(a[j][v], mine.h[v], u[j][v]);
         pairs[which][wave][lane] = mine;
         lds_barrier();
         float g[V];
+        auto join = [&](int from, int to) {          // runs from .. to, the later first
+#pragma unroll 4
+            for (int w = from; w >= to; w--) {
+                const Pair p = pairs[which][w][lane];
 #pragma unroll
-        for (int w = WAVES - 1; w >= 0; w--) {
-            const Pair p = pairs[which][w][lane];
-#pragma unroll
-            for (int v = 0; v < V; v++) {
-                if (w == wave) g[v] = c[v];
-                c[v] = fmaf(p.a[v], c[v], p.g[v]);
-                if (MODE == PAIRS) all[v] *= p.a[v];
+                for (int v = 0; v < V; v++) {
+                    c[v] = fmaf(p.a[v], c[v], p.g[v]);
+                    if (MODE == PAIRS) all[v] *= p.a[v];
+                }
             }
-        }
-        if (MODE == PAIRS) continue;
+        };
+        join(BACK_WAVES - 1, wave + 1);
+#pragma unroll
+        for (int v = 0; v < V; v++) g[v] = c[v];
+        join(wave, 0);
+        if (MODE == PAIRS) return;
+#pragma unroll 4
         for (int w = 0; w < wave; w++) {
             const Pair p = pairs[which][w][lane];
 #pragma unroll
-            for (int v = 0; v < V; v++) h[v] = fmaf(p.a[v], h[v], p.h[v]);
+            for (int v = 0; v < V; v++) hs[0][v] = fmaf(p.a[v], hs[0][v], p.h[v]);
         }
-        float hs[K][V];                       // the states before the tokens
+        // (kept in 16 bits over the barrier, not widened before it)
+        if constexpr (sizeof(T) == 2)
+#pragma unroll
+            for (int j = 0; j < K; j++) {
+                asm("" : "+v"(gk[j]));
+                if (GATE) asm("" : "+v"(zk[j]));
+            }
+        // hs[j]: the state before token j
 #pragma unroll
         for (int j = 0; j < K; j++)
 #pragma unroll
-            for (int v = 0; v < V; v++) {
-                hs[j][v] = h[v];
-                h[v] = fmaf(a[j][v], h[v], t0 + wave * K + j < l.len ? __builtin_amdgcn_sqrtf(b[j][v]) * ix[j][v] : 0.f);
-            }
-        float step[V];
+            for (int v = 0; v < V; v++) hs[j + 1][v] = fmaf(a[j][v], hs[j][v], u[j][v]);
+        const Tokens gx = l.tokens(xo, t, K, k.T), gr = l.tokens(ro, t, K, k.T), gi = l.tokens(io, t, K, k.T), gz = l.tokens(zo, t, K, k.T);
+        float part[V];
 #pragma unroll
-        for (int v = 0; v < V; v++) step[v] = 0.f;
+        for (int v = 0; v < V; v++) part[v] = 0.f;
 #pragma unroll
         for (int j = K - 1; j >= 0; j--) {
-            const int t = t0 + wave * K + j;
-            const bool there = t < l.len;
-            float ox[V], orr[V], oi[V], oz[V];
+            const bool there = WHOLE || t + j < l.len;
+            float ox[V], orr[V], oi[V], oz[V], zf[V], gf[V];
+            R::floats(gk[j], gf);
+            if (GATE) R::floats(zk[j], zf);
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const float gt = go[j][v] + g[v], ah = a[j][v] * hs[j][v], beta = __builtin_amdgcn_sqrtf(b[j][v]);
-                // (where a is one, as at a shut gate, beta and what it changes by are nothing)
-                const float turn = b[j][v] > 1e-37f ? a[j][v] * a[j][v] * __builtin_amdgcn_rsqf(b[j][v]) * ix[j][v] : 0.f;
-                const float gl = gt * (ah - turn);
-                ox[v] = there ? gt * beta * is[j][v] : 0.f;
-                oi[v] = there ? gt * beta * ix[j][v] * (1.f - is[j][v]) : 0.f;
-                orr[v] = there ? gl * (lg[j][v] * LN2) * (1.f - rs[j][v]) : 0.f;
-                step[v] += there ? gl * rs[j][v] : 0.f;
-                if (GATE) oz[v] = there ? gv[j][v] * fmaf(beta, ix[j][v], ah) * fmaf(zf[j][v] * zs[j][v], 1.f - zs[j][v], zs[j][v]) : 0.f;
+                const float zz = GATE ? zf[v] * zs[j][v] : 1.f, gt = fmaf(gf[v], zz, g[v]), gu = gt * u[j][v];
+                // u changes by log a as -u times a^2 / beta^2 = 1 / beta^2 - 1 (where a is one, as at a shut gate, u is zero and so is that: the largest
+                // number stands for infinity)
+                const float less = fminf(__builtin_amdgcn_rcpf(beta[j][v] * beta[j][v]), 3e38f) - 1.f;
+                const float gl = gt * fmaf(-u[j][v], less, a[j][v] * hs[j][v]) * rs[j][v];
+                ox[v] = there ? gt * (beta[j][v] * is[j][v]) : 0.f;
+                oi[v] = there ? fmaf(-gu, is[j][v], gu) : 0.f;
+                orr[v] = there ? gl * (slope[v] * (1.f - rs[j][v])) : 0.f;
+                part[v] += there ? gl : 0.f;
+                if (GATE) oz[v] = there ? gf[v] * hs[j + 1][v] * fmaf(zs[j][v], 1.f - zz, zz) : 0.f;
                 g[v] = a[j][v] * gt;
             }
-            l.store(k.gx, t, ox);
-            l.store(k.gr, t, orr);
-            l.store(k.gi, t, oi);
-            if (GATE) l.store(k.gz, t, oz);
+            l.store(gx, j, ox);
+            l.store(gr, j, orr);
+            l.store(gi, j, oi);
+            if (GATE) l.store(gz, j, oz);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
-        for (int v = 0; v < V; v++) sum[v] += step[v];
-    }
+        for (int v = 0; v < V; v++) sum[v] += part[v];
+    };
+    // (a loop of each kind: both in one take more registers than there are)
+    int which = 0, t0 = last;
+    for (; t0 >= begin && t0 + CHECK > l.len; t0 -= CHECK, which ^= 1) step(Bool<false>(), t0, which);
+    for (; t0 >= begin; t0 -= CHECK, which ^= 1) step(Bool<true>(), t0, which);
     if (MODE == PAIRS) {
         if (wave == 0) {
             l.put(l.pair(segment), all);
@@ -341,7 +409,7 @@ __global__ __launch_bounds__(64 * WAVES) void backward(const Call k) {
     __syncthreads();
     if (wave != 0) return;
 #pragma unroll
-    for (int w = 1; w < WAVES; w++)
+    for (int w = 1; w < BACK_WAVES; w++)
 #pragma unroll
         for (int v = 0; v < V; v++) sum[v] += pairs[0][w][lane].a[v];
     l.put(k.part + ((size_t)l.b * k.segments + segment) * k.D, sum);
@@ -407,20 +475,20 @@ template <class T, int V, bool GATE> static void backward_v(hipStream_t s, Call 
     k.segments = segments_of(k.T, k.span);
     k.part = k.pairs + (k.segments > 1 ? (size_t)k.B * k.segments * 2 * k.D : 0);
     const dim3 grid((k.D + 64 * V - 1) / (64 * V), k.B, k.segments);
-    if (k.segments > 1) hipLaunchKernelGGL((backward<T, V, GATE, PAIRS>), grid, dim3(64 * WAVES), 0, s, k);
-    hipLaunchKernelGGL((backward<T, V, GATE, FORWARD>), grid, dim3(64 * WAVES), 0, s, k);
+    if (k.segments > 1) hipLaunchKernelGGL((backward<T, V, GATE, PAIRS>), grid, dim3(64 * BACK_WAVES), 0, s, k);
+    hipLaunchKernelGGL((backward<T, V, GATE, FORWARD>), grid, dim3(64 * BACK_WAVES), 0, s, k);
     Sums<ToDecay> sums;
     sums.add(k.B * k.segments, k.D, k.part, ToDecay{gdecay, k.decay, k.scale});
     sum_rows_launch(s, sums);
 }
 template <class T> static hipError_t forward_t(hipStream_t s, const Call &k, int v) {
     if (k.T == 1 && !k.checkpoints) hipLaunchKernelGGL(one<T>, dim3((unsigned)(((size_t)k.B * k.D + 255) / 256)), dim3(256), 0, s, k);
-    else if (v == 2) k.z.p ? forward_v<T, 2, true>(s, k) : forward_v<T, 2, false>(s, k);
+    else if (v == 2 && sizeof(T) == 2) k.z.p ? forward_v<T, 4 / sizeof(T), true>(s, k) : forward_v<T, 4 / sizeof(T), false>(s, k);
     else k.z.p ? forward_v<T, 1, true>(s, k) : forward_v<T, 1, false>(s, k);
     return hipGetLastError();
 }
 template <class T> static hipError_t backward_t(hipStream_t s, const Call &k, int v, float *gdecay) {
-    if (v == 2) k.z.p ? backward_v<T, 2, true>(s, k, gdecay) : backward_v<T, 2, false>(s, k, gdecay);
+    if (v == 2 && sizeof(T) == 2) k.z.p ? backward_v<T, 4 / sizeof(T), true>(s, k, gdecay) : backward_v<T, 4 / sizeof(T), false>(s, k, gdecay);
     else k.z.p ? backward_v<T, 1, true>(s, k, gdecay) : backward_v<T, 1, false>(s, k, gdecay);
     return hipGetLastError();
 }

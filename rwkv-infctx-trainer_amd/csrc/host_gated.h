@@ -2,6 +2,11 @@
 // (Part of host.cpp, after host_ssm.h.)
 
 // ---- the gated linear recurrence
+// as strided(), and a token's row behind the one before it
+Tensor apart(const Tensor &t) {
+    const Tensor s = strided(t);
+    return s.defined() && s.size(1) > 1 && s.stride(1) < s.size(2) ? s.contiguous() : s;
+}
 enum { GX, GR, GI, GDECAY, GZ, GSTATE, RECURRENCE_INPUTS };
 class GatedRecurrence : public torch::autograd::Function<GatedRecurrence> {
 public:
@@ -9,7 +14,7 @@ public:
     static variable_list forward(AutogradContext *ctx, const Tensor &x_, const Tensor &r_, const Tensor &i_, const Tensor &decay_, const Maybe &z__, const Maybe &state__,
                                  const Maybe &lengths_, double scale, const Maybe &out_state_) {
         const Tensor z_ = given(z__), state_ = given(state__), lengths = given(lengths_), out_state = given(out_state_);
-        const Tensor x = strided(x_), r = strided(r_), i = strided(i_), z = strided(z_), decay = plain_float(decay_), s = plain_float(state_);
+        const Tensor x = apart(x_), r = apart(r_), i = apart(i_), z = apart(z_), decay = plain_float(decay_), s = plain_float(state_);
         const int B = fits_int(x.size(0)), T = fits_int(x.size(1)), D = fits_int(x.size(2)), dt = dtype_code(x);
         OnDevice dev(x);
         const Tensor y = fresh({B, T, D}, x.scalar_type()), out = out_state.defined() ? out_state : fresh({B, D}, at::kFloat);
