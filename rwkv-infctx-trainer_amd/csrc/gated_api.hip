@@ -48,11 +48,11 @@ gated::Call recurrence_call(int B, int T, int D, float scale, const wkv_rows *x,
     k.pairs = static_cast<float *>(workspace);
     return k;
 }
-// how many channels a lane may take at once
-int recurrence_piece(int D, int dtype, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i, const wkv_rows *z) {
+// whether a lane may take two channels at once
+bool recurrence_pairs(int D, int dtype, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i, const wkv_rows *z) {
     for (const wkv_rows *o : {x, r, i, z})
-        if (o && (D % 2 || !aligned_to(o->p, 2 * element(dtype)) || o->batch % 2 || o->token % 2)) return 1;
-    return 2;
+        if (o && (D % 2 || !aligned_to(o->p, 2 * element(dtype)) || o->batch % 2 || o->token % 2)) return false;
+    return true;
 }
 
 // ---- embedding
@@ -103,8 +103,8 @@ int wkv_gated_recurrence_forward(void *stream, int B, int T, int D, int dtype, f
     if (workspace_bytes < need) return WKV_ERR_WORKSPACE;
     gated::Call k = recurrence_call(B, T, D, scale, x, r, i, z, decay, lengths, checkpoints, workspace);
     k.state_in = state_in; k.y = y; k.state_out = state_out;
-    const int piece = recurrence_piece(D, dtype, x, r, i, z);
-#define CALL(TY) gated::forward_t<TY>((hipStream_t)stream, k, piece)
+    const bool two = recurrence_pairs(D, dtype, x, r, i, z);
+#define CALL(TY) gated::forward_t<TY>((hipStream_t)stream, k, two)
     return finished(BY_DTYPE(dtype, CALL));
 #undef CALL
 }
@@ -127,8 +127,8 @@ int wkv_gated_recurrence_backward(void *stream, int B, int T, int D, int dtype, 
     gated::Call k = recurrence_call(B, T, D, scale, x, r, i, z, decay, lengths, checkpoints, workspace);
     k.gy = gy; k.gstate_out = gstate_out;
     k.gx = gx; k.gr = gr; k.gi = gi; k.gz = gz; k.gstate_in = gstate_in;
-    const int piece = recurrence_piece(D, dtype, x, r, i, z);
-#define CALL(TY) gated::backward_t<TY>((hipStream_t)stream, k, piece, gdecay)
+    const bool two = recurrence_pairs(D, dtype, x, r, i, z);
+#define CALL(TY) gated::backward_t<TY>((hipStream_t)stream, k, two, gdecay)
     return finished(BY_DTYPE(dtype, CALL));
 #undef CALL
 }

@@ -99,6 +99,29 @@ template <class T, int V> struct Lane {
     __device__ __forceinline__ void put(float *row, const float (&o)[V]) const { Row<float, V>::store(row, true, at32, o); }
     __device__ __forceinline__ const float *state_row(const float *p) const { return p ? p + (size_t)b * k.D : nullptr; }
     __device__ __forceinline__ float *pair(int segment) const { return k.pairs + ((size_t)b * k.segments + segment) * 2 * k.D; }
+    // the pairs of the segments from `from` up to (not with) `to`, eight asked for at once
+    __device__ __forceinline__ void join_segments(int from, int to, int step, float (&h)[V]) const {
+        typedef Row<float, V> F;
+        for (int s0 = from; s0 != to;) {
+            const int n = min((to - s0) * step, 8);
+            typename F::Raw a[8], e[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                a[j] = F::load(pair(s0 + j * step), j < n, at32);
+                e[j] = F::load(pair(s0 + j * step) + k.D, j < n, at32);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                float af[V], ef[V];
+                F::floats(a[j], af);
+                F::floats(e[j], ef);
+                if (j < n)
+#pragma unroll
+                    for (int v = 0; v < V; v++) h[v] = fmaf(af[v], h[v], ef[v]);
+            }
+            s0 += n * step;
+        }
+    }
 };
 
 // FORWARD the outputs; PAIRS only the segments' pairs
@@ -133,13 +156,7 @@ __global__ __launch_bounds__(64 * WAVES) void forward(const Call k) {
     for (int v = 0; v < V; v++) h[v] = 0.f, all[v] = 1.f;
     if (MODE == FORWARD) {
         l.floats(l.state_row(k.state_in), h);
-        for (int s = 0; s < segment; s++) {
-            float a[V], e[V];
-            l.floats(l.pair(s), a);
-            l.floats(l.pair(s) + k.D, e);
-#pragma unroll
-            for (int v = 0; v < V; v++) h[v] = fmaf(a[v], h[v], e[v]);
-        }
+        l.join_segments(0, segment, 1, h);
     }
     // WHOLE: all of the wavefront's tokens are there (as they are but at a sequence's end)
     auto step = [&](auto whole, int t0, int which) {
@@ -264,13 +281,7 @@ __global__ __launch_bounds__(64 * BACK_WAVES) void backward(const Call k) {
     for (int v = 0; v < V; v++) c[v] = sum[v] = 0.f, all[v] = 1.f;
     if (MODE == FORWARD) {
         l.floats(l.state_row(k.gstate_out), c);
-        for (int s = k.segments - 1; s > segment; s--) {
-            float a[V], e[V];
-            l.floats(l.pair(s), a);
-            l.floats(l.pair(s) + k.D, e);
-#pragma unroll
-            for (int v = 0; v < V; v++) c[v] = fmaf(a[v], c[v], e[v]);
-        }
+        l.join_segments(k.segments - 1, segment, -1, c);
     }
     float slope[V];                           // of log a by sigmoid(r)
 #pragma unroll
@@ -442,20 +453,32 @@ struct ToDecay {
 };
 
 // ---- launches
-// Segments in time where whole sequences make too few workgroups
-static inline int span_of(int B, int T, int D, int V) {
-    const long long groups = (long long)B * ((D + 64 * V - 1) / (64 * V)), steps = (T + STEP - 1) / STEP;
-    long long cut = std::min<long long>(cu_count() / groups, steps / 2);
-    cut = std::max<long long>(1, std::min<long long>(cut, 64));
-    return (int)((steps + cut - 1) / cut * STEP);
+// How a call is shared out: channels per lane, and segments in time where whole sequences make too few workgroups.  A compute unit takes 5.7 us for a step of
+// two channels per lane and 3.6 us for one of one (forward, bf16; backward twice that), one workgroup after the other; a pass for the segments' pairs adds
+// two thirds, a launch and a walk over them.  Times of this rule's choice and the nearest other, forward / backward in us: B4 T777 D4096 one channel 31 / 54, two
+// in two segments 52 / 78; B1 T4096 D4096 two in eight 57 / 91, one in four 60 / 104; B5 T2048 D4096 two 113 / 213, one 145 / 256; B12 T2048
+// D4096 one 237 / 429, two 248 / 450; B1 T8192 D512 one in 32 27 / 37, two in 32 36 / 50.
+struct Plan { int v, span; };
+static inline Plan plan_of(int B, int T, int D, bool two) {
+    const long long cus = cu_count(), steps = (T + STEP - 1) / STEP;
+    Plan best = {1, (int)(steps * STEP)};
+    double least = 1e30;
+    for (int v = 1; v <= (two ? 2 : 1); v++) {
+        const long long groups = (long long)B * ((D + 64 * v - 1) / (64 * v));
+        for (long long cut = 1; cut <= std::min<long long>(steps, 64); cut++) {
+            const long long each = (steps + cut - 1) / cut, rounds = (groups * ((steps + each - 1) / each) + cus - 1) / cus;
+            const double cost = (double)(rounds * each) * (v == 2 ? 5.7 : 3.6) * (cut > 1 ? 1.65 : 1.) + (cut > 1 ? 4. + 0.1 * (double)cut : 0.);
+            if (cost < least) least = cost, best = {v, (int)(each * STEP)};
+            if (groups * cut >= 2 * cus) break;
+        }
+    }
+    return best;
 }
 static inline int segments_of(int T, int span) { return (T + span - 1) / span; }
 static inline size_t checkpoint_bytes(int B, int T, int D) { return (size_t)B * ((T + CHECK - 1) / CHECK) * D * 4; }
-// (the larger of what a lane's possible channels need: how many a call takes depends on its pointers)
+// (the more of what a lane's possible channels need: whether two are possible depends on a call's pointers)
 static inline size_t most_segments(int B, int T, int D) {
-    size_t n = 1;
-    for (int V : {1, 2}) n = std::max<size_t>(n, segments_of(T, span_of(B, T, D, V)));
-    return n;
+    return std::max(segments_of(T, plan_of(B, T, D, false).span), segments_of(T, plan_of(B, T, D, true).span));
 }
 static inline size_t forward_scratch(int B, int T, int D) {
     const size_t n = most_segments(B, T, D);
@@ -463,15 +486,15 @@ static inline size_t forward_scratch(int B, int T, int D) {
 }
 static inline size_t backward_scratch(int B, int T, int D) { return (size_t)B * most_segments(B, T, D) * 3 * D * 4; }
 
-template <class T, int V, bool GATE> static void forward_v(hipStream_t s, Call k) {
-    k.span = span_of(k.B, k.T, k.D, V);
+template <class T, int V, bool GATE> static void forward_v(hipStream_t s, Call k, int span) {
+    k.span = span;
     k.segments = segments_of(k.T, k.span);
     const dim3 grid((k.D + 64 * V - 1) / (64 * V), k.B, k.segments);
     if (k.segments > 1) hipLaunchKernelGGL((forward<T, V, GATE, PAIRS>), grid, dim3(64 * WAVES), 0, s, k);
     hipLaunchKernelGGL((forward<T, V, GATE, FORWARD>), grid, dim3(64 * WAVES), 0, s, k);
 }
-template <class T, int V, bool GATE> static void backward_v(hipStream_t s, Call k, float *gdecay) {
-    k.span = span_of(k.B, k.T, k.D, V);
+template <class T, int V, bool GATE> static void backward_v(hipStream_t s, Call k, int span, float *gdecay) {
+    k.span = span;
     k.segments = segments_of(k.T, k.span);
     k.part = k.pairs + (k.segments > 1 ? (size_t)k.B * k.segments * 2 * k.D : 0);
     const dim3 grid((k.D + 64 * V - 1) / (64 * V), k.B, k.segments);
@@ -481,15 +504,20 @@ template <class T, int V, bool GATE> static void backward_v(hipStream_t s, Call 
     sums.add(k.B * k.segments, k.D, k.part, ToDecay{gdecay, k.decay, k.scale});
     sum_rows_launch(s, sums);
 }
-template <class T> static hipError_t forward_t(hipStream_t s, const Call &k, int v) {
+// two: a lane may take two channels, which those of 16 bits do
+template <class T> static hipError_t forward_t(hipStream_t s, const Call &k, bool two) {
+    constexpr int PAIR = 4 / sizeof(T);
+    const Plan p = plan_of(k.B, k.T, k.D, two && PAIR == 2);
     if (k.T == 1 && !k.checkpoints) hipLaunchKernelGGL(one<T>, dim3((unsigned)(((size_t)k.B * k.D + 255) / 256)), dim3(256), 0, s, k);
-    else if (v == 2 && sizeof(T) == 2) k.z.p ? forward_v<T, 4 / sizeof(T), true>(s, k) : forward_v<T, 4 / sizeof(T), false>(s, k);
-    else k.z.p ? forward_v<T, 1, true>(s, k) : forward_v<T, 1, false>(s, k);
+    else if (p.v == 2) k.z.p ? forward_v<T, PAIR, true>(s, k, p.span) : forward_v<T, PAIR, false>(s, k, p.span);
+    else k.z.p ? forward_v<T, 1, true>(s, k, p.span) : forward_v<T, 1, false>(s, k, p.span);
     return hipGetLastError();
 }
-template <class T> static hipError_t backward_t(hipStream_t s, const Call &k, int v, float *gdecay) {
-    if (v == 2 && sizeof(T) == 2) k.z.p ? backward_v<T, 4 / sizeof(T), true>(s, k, gdecay) : backward_v<T, 4 / sizeof(T), false>(s, k, gdecay);
-    else k.z.p ? backward_v<T, 1, true>(s, k, gdecay) : backward_v<T, 1, false>(s, k, gdecay);
+template <class T> static hipError_t backward_t(hipStream_t s, const Call &k, bool two, float *gdecay) {
+    constexpr int PAIR = 4 / sizeof(T);
+    const Plan p = plan_of(k.B, k.T, k.D, two && PAIR == 2);
+    if (p.v == 2) k.z.p ? backward_v<T, PAIR, true>(s, k, p.span, gdecay) : backward_v<T, PAIR, false>(s, k, p.span, gdecay);
+    else k.z.p ? backward_v<T, 1, true>(s, k, p.span, gdecay) : backward_v<T, 1, false>(s, k, p.span, gdecay);
     return hipGetLastError();
 }
 
