@@ -3,10 +3,11 @@
 //     out[n] = scale table[token[n]],      gtable[v] = scale (sum over the n with token[n] = v of gout[n])
 //
 // A token outside the table is a place without one: a row of zeros, no gradient.  Both directions are bound by memory.  The gradient is written
-// whole (V C, most of it zeros) from the places sorted by token, so that each row of it is summed by one wavefront in the places' order, in fp32: no
-// atomics, the same bits every time.  Sorting: stable passes over ten bits of the token at a most, counts per tile of 4096 places, then each tile's places to
-// where the tiles and digits before leave off; up to one tile's worth in a single launch.  A token that many places have is summed by runs of 64 places
-// first, whoever they belong to, so that no wavefront walks more than 126 places and the runs' sums.
+// whole (V C, most of it zeros) from the places sorted by token: no atomics, fp32 sums in the places' order, the same bits every time.  Sorting: stable
+// passes over ten bits of the token at a most, counts per tile of places, then each tile's places to where the tiles and digits before leave off; up
+// to one tile's worth in a single launch.  Sums: a workgroup takes 64 sorted places, whoever they belong to, so that it does not matter how often a token
+// comes; a token that lies within them is written as it ends, one that crosses their border leaves a part for a second launch.  The same launch
+// writes the zeros, which keeps memory busy beside the gathers' latency.
 #include "common.h"
 #include "vec.h"
 
@@ -137,10 +138,15 @@ template <class I> __global__ __launch_bounds__(SORT_THREADS) void scatter(const
     }
     // of digit threadIdx.x: in the tiles before, and in all
     int before = 0, all = 0;
-    for (int t = 0; t < tiles; t++) {
-        const int n = k.counts[(size_t)t * BINS + threadIdx.x];
-        before += t < (int)blockIdx.x ? n : 0;
-        all += n;
+    for (int t0 = 0; t0 < tiles; t0 += 8) {
+        int n[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) n[j] = t0 + j < tiles ? k.counts[(size_t)(t0 + j) * BINS + threadIdx.x] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            before += t0 + j < (int)blockIdx.x ? n[j] : 0;
+            all += n[j];
+        }
     }
     m.base[threadIdx.x] = sum_before(m, all) + before;
     ranks(m, digit, there, k.bits, rank, total);
@@ -206,82 +212,114 @@ static __global__ __launch_bounds__(256) void find_starts(const int *keys, int c
 }
 
 // ---- sums
-constexpr int RUN = 64;                       // places of a run
+constexpr int CHUNK = 64, AHEAD = 8;          // places of a chunk, and of those asked for together
 struct Gradient {
-    int count, V, C;
+    int count, V, C, slices, chunks;          // slices: of the channels, one per workgroup
     long long gs;                             // gout's row stride
     float scale;
     const int *keys, *places, *starts;
     const void *gout;
-    float *runs;                              // (count / RUN, C)
+    float *parts;                             // (chunks, 2, C): sums of a chunk's first token where it began before, and of its last where it goes on behind
     void *out;
 };
-template <int W> __device__ __forceinline__ void add(float (&s)[W], const float (&v)[W]) {
+template <class T, int W> __device__ __forceinline__ void put_row(const Gradient &k, int v, int c, float (&s)[W]) {
 #pragma unroll
-    for (int w = 0; w < W; w++) s[w] += v[w];
+    for (int w = 0; w < W; w++) s[w] *= k.scale;
+    store_vec(static_cast<T *>(k.out) + (size_t)v * k.C + c, s);
 }
-// a run of places that all have one token: its sum
-template <class T, int W> __global__ __launch_bounds__(256) void sum_runs(const Gradient k) {
-    const int run = blockIdx.x, c = (blockIdx.y * 256 + threadIdx.x) * W;
-    const int *place = k.places + run * RUN, key = k.keys[run * RUN];
-    if (key == k.V || key != k.keys[run * RUN + RUN - 1] || c >= k.C) return;
+// a chunk's tokens, W channels per lane
+template <class T, int W> __device__ __forceinline__ void sum_chunk(const Gradient &k, int chunk, int c) {
+    __shared__ int keys[CHUNK + 2], places[CHUNK];          // keys[0], keys[n + 1]: the neighbours'
+    const int p0 = chunk * CHUNK, n = min(CHUNK, k.count - p0);
+    if (threadIdx.x < CHUNK + 2) {
+        const int p = p0 - 1 + (int)threadIdx.x;
+        keys[threadIdx.x] = p >= 0 && p < k.count ? k.keys[p] : -1;
+        if (threadIdx.x < n) places[threadIdx.x] = k.places[p0 + threadIdx.x];
+    }
+    __syncthreads();
+    if (c >= k.C) return;
     float s[W];
+    int begun = 0;                            // where the token in hand begins
+    for (int g = 0; g < n; g += AHEAD) {
+        float v[AHEAD][W];
 #pragma unroll
-    for (int w = 0; w < W; w++) s[w] = 0.f;
-    for (int j = 0; j < RUN; j += 4) {
-        float v[4][W];
+        for (int j = 0; j < AHEAD; j++) load_vec(static_cast<const T *>(k.gout) + places[min(g + j, n - 1)] * k.gs + c, v[j]);
 #pragma unroll
-        for (int q = 0; q < 4; q++) load_vec(static_cast<const T *>(k.gout) + place[j + q] * k.gs + c, v[q]);
+        for (int j = 0; j < AHEAD; j++) {
+            const int at = g + j, key = __builtin_amdgcn_readfirstlane(keys[min(at, n - 1) + 1]);
+            if (at >= n || key == k.V) break;
+            if (at == 0 || key != keys[at]) {
+                begun = at;
 #pragma unroll
-        for (int q = 0; q < 4; q++) add(s, v[q]);
-    }
-    float *to = k.runs + (size_t)run * k.C + c;
-#pragma unroll
-    for (int w = 0; w < W; w++) to[w] = s[w];
-}
-// a row of the table per wavefront: its places up to the first whole run, the runs, the rest
-template <class T, int W> __global__ __launch_bounds__(256) void sum_rows_of(const Gradient k) {
-    const int v = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (v >= k.V) return;
-    const int from = k.starts[v], to = k.starts[v + 1];
-    int run0 = (from + RUN - 1) / RUN, run1 = to / RUN;
-    if (run1 <= run0) run0 = run1 = -1;
-    const int head = run0 < 0 ? to : run0 * RUN, tail = run0 < 0 ? to : run1 * RUN;
-    T *out = static_cast<T *>(k.out) + (size_t)v * k.C;
-    for (int c = lane * W; c < k.C; c += 64 * W) {
-        float s[W];
-#pragma unroll
-        for (int w = 0; w < W; w++) s[w] = 0.f;
-        auto places = [&](int n, int end) {
-            for (; n + 4 <= end; n += 4) {
-                float g[4][W];
-#pragma unroll
-                for (int q = 0; q < 4; q++) load_vec(static_cast<const T *>(k.gout) + k.places[n + q] * k.gs + c, g[q]);
-#pragma unroll
-                for (int q = 0; q < 4; q++) add(s, g[q]);
+                for (int w = 0; w < W; w++) s[w] = 0.f;
             }
-            for (; n < end; n++) {
-                float g[W];
-                load_vec(static_cast<const T *>(k.gout) + k.places[n] * k.gs + c, g);
-                add(s, g);
-            }
-        };
-        places(from, head);
-        for (int r = run0; r < run1; r++) {
-            const float *p = k.runs + (size_t)r * k.C + c;
 #pragma unroll
-            for (int w = 0; w < W; w++) s[w] += p[w];
+            for (int w = 0; w < W; w++) s[w] += v[j][w];
+            const bool ends = keys[at + 2] != key;
+            if (!ends && at + 1 < n) continue;
+            const bool before = begun == 0 && keys[0] == key;
+            if (before || !ends) {
+                float *to = k.parts + ((size_t)chunk * 2 + !before) * k.C + c;
+#pragma unroll
+                for (int w = 0; w < W; w++) to[w] = s[w];
+            } else {
+                put_row<T>(k, key, c, s);
+            }
         }
-        places(tail, to);
-#pragma unroll
-        for (int w = 0; w < W; w++) s[w] *= k.scale;
-        store_vec(out + c, s);
     }
+}
+// the zeros of the tokens that no place has: 16 bytes per lane of the table as one row of elements, whatever its width
+constexpr int ZEROS = 8;                      // pieces per lane
+template <class T> __device__ __forceinline__ void put_zeros(const Gradient &k, size_t block) {
+    constexpr int W = 16 / sizeof(T);
+    const size_t first = block * (256 * ZEROS * W), v0 = first / k.C, total = (size_t)k.V * k.C;
+    const unsigned start = (unsigned)(first - v0 * k.C);
+    T *out = static_cast<T *>(k.out);
+    auto empty = [&](size_t v) { return k.starts[v] == k.starts[v + 1]; };
+#pragma unroll
+    for (int z = 0; z < ZEROS; z++) {
+        const unsigned in = (z * 256 + threadIdx.x) * W, at = start + in, r = at / k.C, last = (at + W - 1) / k.C;
+        const size_t i = first + in;
+        if (i >= total) return;
+        const bool one = i + W <= total && empty(v0 + r);
+        if (one && (last == r || (last == r + 1 && empty(v0 + last)))) {
+            *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        if (i + W <= total && last == r) continue;          // (a row that has a sum)
+        for (int w = 0; w < W && i + w < total; w++)
+            if (empty(v0 + (at + w) / k.C)) out[i + w] = from_float<T>(0.f);
+    }
+}
+template <class T, int W> __global__ __launch_bounds__(256) void sums(const Gradient k) {
+    const long long work = (long long)k.chunks * k.slices;
+    if ((long long)blockIdx.x < work) sum_chunk<T, W>(k, blockIdx.x / k.slices, (int)((blockIdx.x % k.slices) * 256 + threadIdx.x) * W);
+    else put_zeros<T>(k, blockIdx.x - work);
+}
+// a token that goes on behind the chunk it begins in: its sums over the chunks, in their order
+template <class T, int W> __global__ __launch_bounds__(256) void join(const Gradient k) {
+    const int chunk = blockIdx.x, last = (chunk + 1) * CHUNK - 1, c = (blockIdx.y * 256 + threadIdx.x) * W;
+    const int key = k.keys[last];
+    if (key == k.V || k.keys[last + 1] != key || k.starts[key] < chunk * CHUNK || c >= k.C) return;
+    const int end = (k.starts[key + 1] - 1) / CHUNK;
+    float s[W];
+    load_vec(k.parts + ((size_t)chunk * 2 + 1) * k.C + c, s);
+    for (int j = chunk + 1; j <= end; j += AHEAD) {
+        float v[AHEAD][W];
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) load_vec(k.parts + (size_t)min(j + q, end) * 2 * k.C + c, v[q]);
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++)
+#pragma unroll
+            for (int w = 0; w < W; w++) s[w] += j + q <= end ? v[q][w] : 0.f;
+    }
+    put_row<T>(k, key, c, s);
 }
 
 // ---- launches
 static inline int tiles_of(int count) { return (count + TILE - 1) / TILE; }
-struct Regions { size_t keys[2], places[2], counts, starts, runs, all; };
+static inline int chunks_of(int count) { return (count + CHUNK - 1) / CHUNK; }
+struct Regions { size_t keys[2], places[2], counts, starts, parts, all; };
 static inline Regions regions(int count, int V, int C) {
     Regions r;
     size_t at = 0;
@@ -292,7 +330,7 @@ static inline Regions regions(int count, int V, int C) {
     }
     r.counts = take((size_t)tiles_of(count) * BINS * 4);
     r.starts = take(((size_t)V + 1) * 4);
-    r.runs = take((size_t)(count / RUN) * C * 4);
+    r.parts = take((size_t)chunks_of(count) * 2 * C * 4);
     r.all = at;
     return r;
 }
@@ -333,9 +371,12 @@ template <class I> static void sort(hipStream_t s, int count_, int V, const void
         at = p & 1;
     }
 }
-template <class T, int W> static void sums_w(hipStream_t s, const Gradient &k) {
-    if (k.count >= RUN) hipLaunchKernelGGL((sum_runs<T, W>), dim3(k.count / RUN, (k.C + 256 * W - 1) / (256 * W)), dim3(256), 0, s, k);
-    hipLaunchKernelGGL((sum_rows_of<T, W>), dim3((k.V + 3) / 4), dim3(256), 0, s, k);
+template <class T, int W> static void sums_w(hipStream_t s, Gradient k) {
+    k.chunks = chunks_of(k.count);
+    k.slices = (k.C + 256 * W - 1) / (256 * W);
+    const size_t zeros = ((size_t)k.V * k.C + 256 * ZEROS * (16 / sizeof(T)) - 1) / (256 * ZEROS * (16 / sizeof(T)));
+    hipLaunchKernelGGL((sums<T, W>), dim3((unsigned)((size_t)k.chunks * k.slices + zeros)), dim3(256), 0, s, k);
+    if (k.chunks > 1) hipLaunchKernelGGL((join<T, W>), dim3(k.chunks - 1, k.slices), dim3(256), 0, s, k);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, Gradient k, const void *tokens, bool wide, bool whole, void *workspace) {
     char *ws = static_cast<char *>(workspace);
@@ -347,9 +388,9 @@ template <class T> static hipError_t backward_t(hipStream_t s, Gradient k, const
     k.keys = reinterpret_cast<int *>(ws + r.keys[at]);
     k.places = reinterpret_cast<int *>(ws + r.places[at]);
     k.starts = starts;
-    k.runs = reinterpret_cast<float *>(ws + r.runs);
+    k.parts = reinterpret_cast<float *>(ws + r.parts);
     hipLaunchKernelGGL(find_starts, dim3(k.V / 256 + 1), dim3(256), 0, s, k.keys, k.count, k.V, starts);
-    if (whole) sums_w<T, 16 / sizeof(T)>(s, k);
+    if (whole) sums_w<T, 4>(s, k);
     else sums_w<T, 1>(s, k);
     return hipGetLastError();
 }
