@@ -7,8 +7,10 @@
 // half of the same up rows, so that a lane ends with g and u of the same places and the activation and product happen in registers: g and u
 // never reach memory, except that a backward's are kept in fp32: rounded to 16 bits they would add as much to the gradients' error as each of the two
 // roundings that cannot be left out, that of dg and du, which the matrix cores take in the streams' type, and that of the results (bf16, error of
-// the 2-norm: 3.1e-3 against 2.4e-3).  Backward, one pass makes dg and du, as rows and as columns; x and the weights are laid out with their
-// other index along memory, and then the three products are the same loop.
+// the 2-norm: 3.1e-3 against 2.4e-3).  Backward, one pass makes dg and du; the three products read
+// them, x and the weights as they lie, with the index that is summed along memory or across it (gx: along dg and du, across the weights; gWg and gWu: across both).
+#include <type_traits>
+
 #include "matrix_tiles.h"
 #include "vec.h"
 
@@ -67,7 +69,7 @@ struct Forward {
 
 template <class T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN) void forward(const Forward k, int rows, int columns) {
-    typedef tiles::Loop<T, BM, BN, WM, WN, 2> L;
+    typedef tiles::Loop<T, tiles::Along<T, BM, 64 * WM * WN>, tiles::Along<T, BN / 2, 64 * WM * WN>, BM, BN, WM, WN, 2> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
     tiles::tile_of(blockIdx.x, rows, columns, tm, tn);
@@ -103,11 +105,12 @@ __global__ __launch_bounds__(64 * WM * WN) void forward(const Forward k, int row
     }
 }
 
-// ---- a product of two operands with k along memory
+// ---- a product of two operands
 struct Product {
     int M, N, K;
-    const void *a, *b;
+    const void *a, *b, *b2;           // b2: B's rows of k from `turn` on, where k is across
     long long as, bs;
+    int turn, rows;                   // rows of k that are there, where k is across
     // out: rows below `split` (of which `live` are there) to out0, those from it on to out1; parts: fp32 sums over a share of k instead
     void *out0, *out1;
     long long os;
@@ -116,16 +119,23 @@ struct Product {
     int per;                          // of k to a share
 };
 
-template <class T, int BM, int BN, int WM, int WN>
+// ACROSS_A, ACROSS_B: k lies across memory in that operand
+template <class T, int BM, int BN, int WM, int WN, bool ACROSS_A, bool ACROSS_B>
 __global__ __launch_bounds__(64 * WM * WN) void product(const Product k, int rows, int columns) {
-    typedef tiles::Loop<T, BM, BN, WM, WN, 1> L;
+    typedef std::conditional_t<ACROSS_A, tiles::Across<T, BM, 64 * WM * WN>, tiles::Along<T, BM, 64 * WM * WN>> A;
+    typedef std::conditional_t<ACROSS_B, tiles::Across<T, BN, 64 * WM * WN>, tiles::Along<T, BN, 64 * WM * WN>> B;
+    typedef tiles::Loop<T, A, B, BM, BN, WM, WN, 1> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
     tiles::tile_of(blockIdx.x, rows, columns, tm, tn);
     const int m0 = tm * BM, n0 = tn * BN;
     L l;
-    l.a.place(static_cast<const T *>(k.a) + m0 * k.as, k.as, k.K, min(BM, k.M - m0));
-    l.b[0].place(static_cast<const T *>(k.b) + n0 * k.bs, k.bs, k.K, min(BN, k.N - n0));
+    const T *a = static_cast<const T *>(k.a), *b = static_cast<const T *>(k.b), *b2 = static_cast<const T *>(k.b2);
+    constexpr int E = tiles::piece<T>();          // (rows are whole pieces, what they hold may not be)
+    if constexpr (ACROSS_A) l.a.place(a, a, 0x7fffffff, k.as, m0, k.rows, (k.M + E - 1) / E * E);
+    else l.a.place(a + m0 * k.as, k.as, k.K, min(BM, k.M - m0));
+    if constexpr (ACROSS_B) l.b[0].place(b, b2, k.turn, k.bs, n0, k.rows, (k.N + E - 1) / E * E);
+    else l.b[0].place(b + n0 * k.bs, k.bs, k.K, min(BN, k.N - n0));
     const int k0 = blockIdx.y * k.per;
     l.run(k0, min(k0 + k.per, k.K), k.K, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
@@ -163,52 +173,32 @@ template <class T> __global__ __launch_bounds__(256) void widen(const T *in, lon
     const size_t r = i / Cs, c = i % Cs;
     if (r < (size_t)R) out[i] = (int)c < C ? in[r * stride + c] : from_float<T>(0.f);
 }
-// (R, C) -> (C, ld): out[c][r], zeros where r is past R; ld: R in whole tiles.  64 x 64 at a time through LDS
-template <class T> __global__ __launch_bounds__(256) void turn(const T *in, long long stride, int R, int C, T *out, long long ld) {
-    __shared__ T tile[64][66];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y
+template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, long long Fs) {
+    constexpr int V = 4;
+    const int f = (blockIdx.x * 256 + threadIdx.x) * V;
+    if (f >= Fs) return;
+    for (int r = blockIdx.y; r < R; r += gridDim.y) {
+        const float *row = kept + r * 2 * Fs;
+        float g[V], u[V], o[V], dg[V], du[V];
+        load4(row + f, g);
+        load4(row + Fs + f, u);
+        const T *from = gh + (long long)r * F;
+        if (WHOLE && f + V <= F) load4(from + f, o);
+        else
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int r = wave * 16 + i;
-        tile[r][lane] = r0 + r < R && c0 + lane < C ? in[(r0 + r) * stride + c0 + lane] : from_float<T>(0.f);
-    }
-    __syncthreads();
+            for (int e = 0; e < V; e++) o[e] = f + e < F ? to_float(from[f + e]) : 0.f;
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        const int c = wave * 16 + i;
-        if (c0 + c < C) out[(c0 + c) * ld + r0 + lane] = tile[lane][c];
-    }
-}
-// dg and du from g, u and gh: rows (R, 2 Fs) and columns (2 Fs, Rs), zeros outside
-template <class T> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, T *turned, long long Fs, long long Rs) {
-    __shared__ T tile[2][64][66];
-    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, f = c0 + lane;
-#pragma unroll 4
-    for (int i = 0; i < 16; i++) {
-        const int r = r0 + wave * 16 + i;
-        float dg = 0.f, du = 0.f;
-        if (r < R) {
-            if (f < F) {
-                const float g = kept[r * 2 * Fs + f], u = kept[r * 2 * Fs + Fs + f], o = to_float(gh[(long long)r * F + f]);
-                float value, slope;
-                activation(kind, g, value, slope);
-                dg = o * u * slope;
-                du = o * value;
-            }
-            d[r * 2 * Fs + f] = from_float<T>(dg);
-            d[r * 2 * Fs + Fs + f] = from_float<T>(du);
+        for (int e = 0; e < V; e++) {
+            float value, slope;
+            activation(kind, g[e], value, slope);
+            // (what is kept past F was never written)
+            dg[e] = f + e < F ? o[e] * u[e] * slope : 0.f;
+            du[e] = f + e < F ? o[e] * value : 0.f;
         }
-        tile[0][wave * 16 + i][lane] = from_float<T>(dg);
-        tile[1][wave * 16 + i][lane] = from_float<T>(du);
+        store4(d + r * 2 * Fs + f, dg);
+        store4(d + r * 2 * Fs + Fs + f, du);
     }
-    __syncthreads();
-#pragma unroll
-    for (int p = 0; p < 2; p++)
-#pragma unroll 4
-        for (int i = 0; i < 16; i++) {
-            const int c = wave * 16 + i;
-            turned[(p * Fs + c0 + c) * Rs + r0 + lane] = tile[p][lane][c];
-        }
 }
 
 // ---- few rows: a serving loop's single tokens.  What they cost is the weights, read once: a workgroup takes 16 gate rows and the same 16 up rows,
@@ -288,6 +278,11 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
 }
 
 // ---- launches
+template <class T> static const T *lay_out(hipStream_t s, const T *p, long long stride, int rows, int C, T *to) {
+    const int Cs = (int)rounded(C);
+    hipLaunchKernelGGL(widen<T>, dim3((unsigned)(((size_t)rows * Cs + 255) / 256)), dim3(256), 0, s, p, stride, rows, C, to, Cs);
+    return to;
+}
 static inline int tiles_of(long long n, int size) { return (int)((n + size - 1) / size); }
 template <class T> static size_t forward_scratch(int R, int C, int F) {
     if (C % tiles::piece<T>() == 0 || R <= FEW) return 0;
@@ -312,14 +307,9 @@ template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *s
     if (!whole) {
         const int Cs = (int)rounded(k.K);
         T *to = static_cast<T *>(scratch);
-        auto lay = [&](const void *&p, long long stride, int rows) {
-            hipLaunchKernelGGL(widen<T>, dim3((unsigned)(((size_t)rows * Cs + 255) / 256)), dim3(256), 0, s, static_cast<const T *>(p), stride, rows, k.K, to, Cs);
-            p = to;
-            to += (size_t)rows * Cs;
-        };
-        lay(k.x, k.xs, k.R);
-        lay(k.wg, k.ws, k.F);
-        lay(k.wu, k.ws, k.F);
+        k.x = lay_out(s, static_cast<const T *>(k.x), k.xs, k.R, k.K, to);
+        k.wg = lay_out(s, static_cast<const T *>(k.wg), k.ws, k.F, k.K, to + (size_t)k.R * Cs);
+        k.wu = lay_out(s, static_cast<const T *>(k.wu), k.ws, k.F, k.K, to + (size_t)(k.R + k.F) * Cs);
         k.xs = k.ws = k.K = Cs;
     }
     const int big = tiles_of(k.R, 256) * tiles_of(k.F, 128);
@@ -356,16 +346,16 @@ template <class T> static Plan plan_of(long long M, long long N, long long K) {
     p.per = (int)(each * tiles::depth<T>());
     return p;
 }
-struct Regions { size_t d, turned, x, w, parts, all; };
+struct Regions { size_t d, x, wg, wu, parts, all; };
 template <class T> static Regions regions(int R, int C, int F, bool want_x, bool want_w) {
-    const size_t Fs = rounded(F), Rs = rounded(R);
+    const size_t Fs = rounded(F), Rs = rounded(R), Cs = C % tiles::piece<T>() ? rounded(C) : 0;
     Regions r;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t was = at; at += (n + 255) / 256 * 256; return was; };
     r.d = take((size_t)R * 2 * Fs * sizeof(T));
-    r.turned = take(2 * Fs * Rs * sizeof(T));
-    r.x = take(want_w ? (size_t)C * Rs * sizeof(T) : 0);
-    r.w = take(want_x ? (size_t)C * 2 * Fs * sizeof(T) : 0);
+    r.x = take(want_w ? (size_t)R * Cs * sizeof(T) : 0);
+    r.wg = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
+    r.wu = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
     size_t parts = 0;
     if (want_x) {
         const Plan p = plan_of<T>(R, C, 2 * Fs);
@@ -379,34 +369,51 @@ template <class T> static Regions regions(int R, int C, int F, bool want_x, bool
     r.all = at;
     return r;
 }
-template <class T> static void product_launch(hipStream_t s, Product k, const Plan &p) {
+template <class T, bool ACROSS_A> static void product_launch(hipStream_t s, Product k, const Plan &p) {
     k.per = p.per;
     if (p.shares == 1) k.parts = nullptr;
     const dim3 grid(p.rows * p.columns, p.shares);
-    if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4>), grid, dim3(512), 0, s, k, p.rows, p.columns);
-    else hipLaunchKernelGGL((product<T, 128, 128, 2, 2>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4, ACROSS_A, true>), grid, dim3(512), 0, s, k, p.rows, p.columns);
+    else hipLaunchKernelGGL((product<T, 128, 128, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
     if (p.shares > 1) hipLaunchKernelGGL(join<T>, dim3((unsigned)(((size_t)k.M * k.os + 255) / 256)), dim3(256), 0, s, k, p.shares);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k, void *scratch) {
-    const long long Fs = rounded(k.F), Rs = rounded(k.R);
+    const int Fs = (int)rounded(k.F), Rs = (int)rounded(k.R);
     const bool want_x = k.gx, want_w = k.gwg;
     const Regions r = regions<T>(k.R, k.C, k.F, want_x, want_w);
     char *ws = static_cast<char *>(scratch);
-    T *d = reinterpret_cast<T *>(ws + r.d), *turned = reinterpret_cast<T *>(ws + r.turned), *xt = reinterpret_cast<T *>(ws + r.x), *wt = reinterpret_cast<T *>(ws + r.w);
+    T *d = reinterpret_cast<T *>(ws + r.d);
+    const T *x = static_cast<const T *>(k.x), *wg = static_cast<const T *>(k.wg), *wu = static_cast<const T *>(k.wu);
+    long long xs = k.xs, ld = k.ws;
+    if (k.C % tiles::piece<T>()) {
+        if (want_w) x = lay_out(s, x, xs, k.R, k.C, reinterpret_cast<T *>(ws + r.x));
+        if (want_x) {
+            wg = lay_out(s, wg, ld, k.F, k.C, reinterpret_cast<T *>(ws + r.wg));
+            wu = lay_out(s, wu, ld, k.F, k.C, reinterpret_cast<T *>(ws + r.wu));
+        }
+        xs = ld = rounded(k.C);
+    }
     float *parts = reinterpret_cast<float *>(ws + r.parts);
-    const dim3 wide(256);
-    hipLaunchKernelGGL(slopes<T>, dim3((unsigned)(Rs / 64), (unsigned)(Fs / 64)), wide, 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, turned, Fs, Rs);
+    const dim3 grid(tiles_of(Fs, 1024), std::min(k.R, 32768));
+    if (k.F % 4 == 0) hipLaunchKernelGGL((slopes<T, true>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs);
+    else hipLaunchKernelGGL((slopes<T, false>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs);
     if (want_x) {
-        const dim3 grid((unsigned)(Fs / 64), tiles_of(k.C, 64));
-        hipLaunchKernelGGL(turn<T>, grid, wide, 0, s, static_cast<const T *>(k.wg), k.ws, k.F, k.C, wt, 2 * Fs);
-        hipLaunchKernelGGL(turn<T>, grid, wide, 0, s, static_cast<const T *>(k.wu), k.ws, k.F, k.C, wt + Fs, 2 * Fs);
-        const Product p = {k.R, k.C, (int)(2 * Fs), d, wt, 2 * Fs, 2 * Fs, k.gx, k.gx, k.C, k.R, k.R, parts, 0};
-        product_launch<T>(s, p, plan_of<T>(k.R, k.C, 2 * Fs));
+        Product p = {};
+        p.M = k.R; p.N = k.C; p.K = 2 * Fs;
+        p.a = d; p.as = 2 * Fs;
+        p.b = wg; p.b2 = wu; p.bs = ld; p.turn = Fs; p.rows = k.F;
+        p.out0 = p.out1 = k.gx; p.os = k.C; p.split = p.live = k.R;
+        p.parts = parts;
+        product_launch<T, false>(s, p, plan_of<T>(p.M, p.N, p.K));
     }
     if (want_w) {
-        hipLaunchKernelGGL(turn<T>, dim3((unsigned)(Rs / 64), tiles_of(k.C, 64)), wide, 0, s, static_cast<const T *>(k.x), k.xs, k.R, k.C, xt, Rs);
-        const Product p = {(int)(2 * Fs), k.C, (int)Rs, turned, xt, Rs, Rs, k.gwg, k.gwu, k.C, (int)Fs, k.F, parts, 0};
-        product_launch<T>(s, p, plan_of<T>(2 * Fs, k.C, Rs));
+        Product p = {};
+        p.M = 2 * Fs; p.N = k.C; p.K = Rs;
+        p.a = d; p.as = 2 * Fs;
+        p.b = p.b2 = x; p.bs = xs; p.turn = 0x7fffffff; p.rows = k.R;
+        p.out0 = k.gwg; p.out1 = k.gwu; p.os = k.C; p.split = Fs; p.live = k.F;
+        p.parts = parts;
+        product_launch<T, true>(s, p, plan_of<T>(p.M, p.N, p.K));
     }
     return hipGetLastError();
 }

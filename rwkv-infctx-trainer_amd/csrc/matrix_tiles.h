@@ -1,4 +1,4 @@
-// Products  out[m][n] = sum over k of A[m][k] B[n][k]  of operands whose k is contiguous, tile by tile on the matrix cores: the loop that the
+// Products  out[m][n] = sum over k of A[m][k] B[n][k]  tile by tile on the matrix cores: the loop that the
 // gated feed-forward's products share.  A workgroup makes BM x BN outputs; 128 bytes of every row of A and B at a time (64 16-bit elements, 32 of
 // fp32) go from memory straight to LDS, the next 128 while these are multiplied.
 //
@@ -44,8 +44,8 @@ __device__ __forceinline__ i4 range_of(const void *p, long long bytes) {
 }
 constexpr unsigned NOWHERE = 0xfffffff0u;
 
-// One operand's share of a workgroup's tile: ROWS rows of K elements from `p` on, `ld` apart, of which `live` are there.
-template <class T, int ROWS, int THREADS> struct Side {
+// One operand's share of a workgroup's tile, ROWS rows with k along memory: `live` rows of K elements from `base` on, `ld` apart.
+template <class T, int ROWS, int THREADS> struct Along {
     static constexpr int ROUNDS = ROWS * 8 / THREADS;
     const char *p;
     long long bytes;                  // from p to the last live row's end
@@ -67,6 +67,77 @@ template <class T, int ROWS, int THREADS> struct Side {
 #pragma unroll
         for (int j = 0; j < ROUNDS; j++) to_lds(r, there ? at[j] : NOWHERE, lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
     }
+    // the operands of sixteen rows: `first` the lane's, the same for every sixteen; half: of the tile of k
+    struct Reader {
+        int first;
+        __device__ __forceinline__ Reader() {
+            const int lane = threadIdx.x & 63;
+            first = (lane & 15) * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+        }
+        __device__ __forceinline__ i4 read(const char *tile, int sixteen, int half) const {
+            return *reinterpret_cast<const i4 *>(tile + sixteen * (16 * 128) + (first ^ (half * 64)));
+        }
+    };
+};
+// The same of an operand with k across: ROWS columns of rows that are `ld` apart, a row per k; what lies between `end` and the end of the last row is not
+// there.  In LDS a row of k is ROWS elements; the pieces that one instruction takes of its rows are exchanged by the row, so that they lie over all banks.  16-bit
+// elements turn on their way to the registers (a transposing read gives a lane four of k of one column), fp32 ones are read one by one.
+template <class T, int ROWS, int THREADS> struct Across {
+    static constexpr int BYTES = ROWS * (int)sizeof(T), PIECES = BYTES / 16, PER = THREADS / PIECES, ROUNDS = depth<T>() / PER;
+    const char *p, *second;           // rows of k from `turn` on: second's, from its first
+    long long bytes, ld;              // from p to the end
+    int turn;
+    unsigned at[ROUNDS];
+    static __device__ __forceinline__ int exchange(int k) { return sizeof(T) == 2 ? ((k & 3) | (k >> 1 & 4)) << 1 : (k >> 2 & 3) << 2; }
+    // column n0 of rows that are there up to `rows`, `width` elements wide
+    __device__ __forceinline__ void place(const T *base, const T *base2, int turn_, long long ld_, int n0, int rows, int width) {
+        p = reinterpret_cast<const char *>(base + n0);
+        second = reinterpret_cast<const char *>(base2 + n0);
+        turn = turn_;
+        ld = ld_ * (long long)sizeof(T);
+        bytes = (long long)(rows - 1) * ld + (long long)(width - n0) * (long long)sizeof(T);
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++) {
+            const int k = threadIdx.x / PIECES + j * PER, c = (threadIdx.x % PIECES) ^ exchange(k);
+            at[j] = (unsigned)(k * ld) + c * 16;
+        }
+    }
+    __device__ __forceinline__ void fetch(int k, int, unsigned lds) const {
+        const bool behind = k >= turn;
+        const long long skip = (long long)(behind ? k - turn : k) * ld;
+        const i4 r = range_of((behind ? second : p) + skip, bytes - skip);
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++) to_lds(r, at[j], lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
+    }
+    struct Reader {
+        int first, mix;
+        __device__ __forceinline__ Reader() {
+            const int lane = threadIdx.x & 63, a = lane & 15, g = lane >> 4;
+            if constexpr (sizeof(T) == 2) {
+                first = (8 * g + (a >> 2)) * BYTES + 8 * (a & 3);
+                mix = ((a >> 2) | (g & 1) << 2) << 5;
+            } else {
+                first = 4 * g * BYTES + 4 * a;
+                mix = g << 6;
+            }
+        }
+        __device__ __forceinline__ i4 read(const char *tile, int sixteen, int half) const {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef s4 __attribute__((address_space(3))) lds_s4;
+            const char *at = tile + first + ((sixteen * (sizeof(T) == 2 ? 32 : 64)) ^ mix) + half * (depth<T>() / 2) * BYTES;
+            if constexpr (sizeof(T) == 2) {
+                s4 o[2];
+#pragma unroll
+                for (int q = 0; q < 2; q++) o[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4 *)(at + q * 4 * BYTES));
+                return __builtin_bit_cast(i4, o);
+            } else {
+                float o[4];
+#pragma unroll
+                for (int q = 0; q < 4; q++) o[q] = *reinterpret_cast<const float *>(at + q * BYTES);
+                return __builtin_bit_cast(i4, o);
+            }
+        }
+    };
 };
 
 // A launch's tiles in the order in which they are worked: the eight XCDs (a workgroup's number modulo 8) each take a run of
@@ -81,11 +152,10 @@ __device__ __forceinline__ void tile_of(int index, int rows, int columns, int &r
 
 // The loop over k of a workgroup of WM x WN wavefronts: acc[i][j] is the sum of 16 rows of A and 16 of B, a lane's element e the one of A's row
 // (lane & 15) and B's row 4 (lane >> 4) + e.  B's rows come in PARTS parts of BN / PARTS rows; a wavefront takes its share of each.
-template <class T, int BM, int BN, int WM, int WN, int PARTS> struct Loop {
-    static constexpr int THREADS = 64 * WM * WN, MT = BM / WM / 16, NT = BN / WN / 16, BYTES = (BM + BN) * 128;
-    static constexpr int LDS = 2 * BYTES;
-    Side<T, BM, THREADS> a;
-    Side<T, BN / PARTS, THREADS> b[PARTS];
+template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> struct Loop {
+    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16, BYTES = (BM + BN) * 128, LDS = 2 * BYTES;
+    A a;
+    B b[PARTS];
     f4 acc[MT][NT];
 
     __device__ __forceinline__ void fetch(int k, int K, unsigned lds) const {
@@ -95,32 +165,32 @@ template <class T, int BM, int BN, int WM, int WN, int PARTS> struct Loop {
     }
     // k from k0 (whole tiles) to k1
     __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
-        const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
         const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
 #pragma unroll
         for (int i = 0; i < MT; i++)
 #pragma unroll
             for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
-        const int row = lane & 15, first = row * 128 + (((lane >> 4) ^ (lane & 7)) << 4);
+        const typename A::Reader ra;
+        const typename B::Reader rb;
         fetch(k0, K, base);
         int which = 0;
         for (int k = k0; k < k1; k += depth<T>()) {
             // this tile is there, and every wavefront is done with the one before it
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (k + depth<T>() < k1) fetch(k + depth<T>(), K, base + (which ^ 1) * BYTES);
-            const char *A = lds + which * BYTES + wm * (MT * 16 * 128), *B = lds + which * BYTES + BM * 128;
+            const char *at = lds + which * BYTES;
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const int off = first ^ (s * 64);
                 i4 y[NT];
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
                     const int part = j / (NT / PARTS), jj = j % (NT / PARTS);
-                    y[j] = *reinterpret_cast<const i4 *>(B + (part * (BN / PARTS) + (wn * (NT / PARTS) + jj) * 16) * 128 + off);
+                    y[j] = rb.read(at + (BM + part * (BN / PARTS)) * 128, wn * (NT / PARTS) + jj, s);
                 }
 #pragma unroll
                 for (int i = 0; i < MT; i++) {
-                    const i4 x = *reinterpret_cast<const i4 *>(A + i * 16 * 128 + off);
+                    const i4 x = ra.read(at, wm * MT + i, s);
 #pragma unroll
                     for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(y[j], x, acc[i][j]);
                 }
