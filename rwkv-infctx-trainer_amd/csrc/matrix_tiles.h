@@ -163,8 +163,28 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
 #pragma unroll
         for (int p = 0; p < PARTS; p++) b[p].fetch(k, K, lds + (BM + p * (BN / PARTS)) * 128);
     }
-    // k from k0 (whole tiles) to k1
+    // a half tile's operands
+    struct Half { i4 x[MT], y[NT]; };
+    __device__ __forceinline__ void read(const typename A::Reader &ra, const typename B::Reader &rb, const char *at, int wm, int wn, int half, Half &h) const {
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int part = j / (NT / PARTS), jj = j % (NT / PARTS);
+            h.y[j] = rb.read(at + (BM + part * (BN / PARTS)) * 128, wn * (NT / PARTS) + jj, half);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i++) h.x[i] = ra.read(at, wm * MT + i, half);
+    }
+    __device__ __forceinline__ void multiply(const Half &h) {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(h.y[j], h.x[i], acc[i][j]);
+    }
+    // k from k0 (whole tiles) to k1.  Half a tile's operands are multiplied while the next half's are on their way from LDS; the one barrier of a tile stands
+    // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  The tile after
+    // that goes into the place of this one.
     __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
+        constexpr int D = depth<T>();
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
         const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
 #pragma unroll
@@ -173,30 +193,29 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
             for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
         const typename A::Reader ra;
         const typename B::Reader rb;
+        Half first, second;
         fetch(k0, K, base);
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        if (k0 + D < k1) fetch(k0 + D, K, base + BYTES);
+        read(ra, rb, lds, wm, wn, 0, first);
         int which = 0;
-        for (int k = k0; k < k1; k += depth<T>()) {
-            // this tile is there, and every wavefront is done with the one before it
+        // (the last tile apart: behind a branch the compiler waits for what either side may have asked for)
+        for (int k = k0; k + D < k1; k += D) {
+            read(ra, rb, lds + which * BYTES, wm, wn, 1, second);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(first);
+            __builtin_amdgcn_sched_barrier(0);
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (k + depth<T>() < k1) fetch(k + depth<T>(), K, base + (which ^ 1) * BYTES);
-            const char *at = lds + which * BYTES;
-#pragma unroll
-            for (int s = 0; s < 2; s++) {
-                i4 y[NT];
-#pragma unroll
-                for (int j = 0; j < NT; j++) {
-                    const int part = j / (NT / PARTS), jj = j % (NT / PARTS);
-                    y[j] = rb.read(at + (BM + part * (BN / PARTS)) * 128, wn * (NT / PARTS) + jj, s);
-                }
-#pragma unroll
-                for (int i = 0; i < MT; i++) {
-                    const i4 x = ra.read(at, wm * MT + i, s);
-#pragma unroll
-                    for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(y[j], x, acc[i][j]);
-                }
-            }
+            if (k + 2 * D < k1) fetch(k + 2 * D, K, base + which * BYTES);
             which ^= 1;
+            read(ra, rb, lds + which * BYTES, wm, wn, 0, first);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(second);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        read(ra, rb, lds + which * BYTES, wm, wn, 1, second);
+        multiply(first);
+        multiply(second);
     }
 };
 
