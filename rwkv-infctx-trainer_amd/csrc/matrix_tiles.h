@@ -59,13 +59,16 @@ template <class T, int ROWS, int THREADS> struct Along {
 #pragma unroll
         for (int j = 0; j < ROUNDS; j++) at[j] = (unsigned)((row + j * (THREADS / 8)) * ld * (long long)sizeof(T)) + c * 16;
     }
-    // the tile of k from `k` on into LDS at `lds`
-    __device__ __forceinline__ void fetch(int k, int K, unsigned lds) const {
+    // the tile of k from `k` on into LDS at `lds`, round by round
+    i4 range;
+    bool there;
+    __device__ __forceinline__ void ask(int k, int K) {
         const long long skip = (long long)k * sizeof(T);
-        const i4 r = range_of(p + skip, bytes - skip);
-        const bool there = k + column < K;                      // (K is whole pieces)
-#pragma unroll
-        for (int j = 0; j < ROUNDS; j++) to_lds(r, there ? at[j] : NOWHERE, lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
+        range = range_of(p + skip, bytes - skip);
+        there = k + column < K;                      // (K is whole pieces)
+    }
+    __device__ __forceinline__ void fetch(int j, unsigned lds) const {
+        to_lds(range, there ? at[j] : NOWHERE, lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
     }
     // the operands of sixteen rows: `first` the lane's, the same for every sixteen; half: of the tile of k
     struct Reader {
@@ -102,12 +105,14 @@ template <class T, int ROWS, int THREADS> struct Across {
             at[j] = (unsigned)(k * ld) + c * 16;
         }
     }
-    __device__ __forceinline__ void fetch(int k, int, unsigned lds) const {
+    i4 range;
+    __device__ __forceinline__ void ask(int k, int) {
         const bool behind = k >= turn;
         const long long skip = (long long)(behind ? k - turn : k) * ld;
-        const i4 r = range_of((behind ? second : p) + skip, bytes - skip);
-#pragma unroll
-        for (int j = 0; j < ROUNDS; j++) to_lds(r, at[j], lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
+        range = range_of((behind ? second : p) + skip, bytes - skip);
+    }
+    __device__ __forceinline__ void fetch(int j, unsigned lds) const {
+        to_lds(range, at[j], lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
     }
     struct Reader {
         int first, mix;
@@ -158,33 +163,46 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
     B b[PARTS];
     f4 acc[MT][NT];
 
-    __device__ __forceinline__ void fetch(int k, int K, unsigned lds) const {
-        a.fetch(k, K, lds);
+    static constexpr int LOADS = A::ROUNDS + PARTS * B::ROUNDS;
+    __device__ __forceinline__ void ask(int k, int K) {
+        a.ask(k, K);
 #pragma unroll
-        for (int p = 0; p < PARTS; p++) b[p].fetch(k, K, lds + (BM + p * (BN / PARTS)) * 128);
+        for (int p = 0; p < PARTS; p++) b[p].ask(k, K);
+    }
+    // share `g` of `of` of a tile's loads
+    __device__ __forceinline__ void fetch(int g, int of, unsigned lds) const {
+#pragma unroll
+        for (int q = 0; q < LOADS; q++) {
+            if (q < g * LOADS / of || q >= (g + 1) * LOADS / of) continue;
+            if (q < A::ROUNDS) a.fetch(q, lds);
+            else b[(q - A::ROUNDS) / B::ROUNDS].fetch((q - A::ROUNDS) % B::ROUNDS, lds + (BM + (q - A::ROUNDS) / B::ROUNDS * (BN / PARTS)) * 128);
+        }
     }
     // a half tile's operands
     struct Half { i4 x[MT], y[NT]; };
-    __device__ __forceinline__ void read(const typename A::Reader &ra, const typename B::Reader &rb, const char *at, int wm, int wn, int half, Half &h) const {
+    // share `g` of `of` of a half's reads: those that the multiplications begin with first
+    __device__ __forceinline__ void read(const typename A::Reader &ra, const typename B::Reader &rb, const char *at, int wm, int wn, int half, int g, int of, Half &h) const {
 #pragma unroll
-        for (int j = 0; j < NT; j++) {
-            const int part = j / (NT / PARTS), jj = j % (NT / PARTS);
-            h.y[j] = rb.read(at + (BM + part * (BN / PARTS)) * 128, wn * (NT / PARTS) + jj, half);
+        for (int q = 0; q < MT + NT; q++) {
+            if (q < g * (MT + NT) / of || q >= (g + 1) * (MT + NT) / of) continue;
+            if (q < NT) {
+                const int part = q / (NT / PARTS), jj = q % (NT / PARTS);
+                h.y[q] = rb.read(at + (BM + part * (BN / PARTS)) * 128, wn * (NT / PARTS) + jj, half);
+            } else {
+                h.x[q - NT] = ra.read(at, wm * MT + q - NT, half);
+            }
         }
-#pragma unroll
-        for (int i = 0; i < MT; i++) h.x[i] = ra.read(at, wm * MT + i, half);
     }
-    __device__ __forceinline__ void multiply(const Half &h) {
+    __device__ __forceinline__ void multiply(const Half &h, int i) {
 #pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(h.y[j], h.x[i], acc[i][j]);
+        for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(h.y[j], h.x[i], acc[i][j]);
     }
     // k from k0 (whole tiles) to k1.  Half a tile's operands are multiplied while the next half's are on their way from LDS; the one barrier of a tile stands
     // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  The tile after
-    // that goes into the place of this one.
+    // that goes into the place of this one.  Reads and loads are issued between the multiplications, a few at a time: issued together they would hold the
+    // matrix instructions behind them up (a tile's loads take the memory pipe half a tile's time).
     __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
-        constexpr int D = depth<T>();
+        constexpr int D = depth<T>(), EARLY = MT * 3 / 4;          // EARLY: shares of a half's reads, the rest of the multiplications cover the last ones
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
         const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
 #pragma unroll
@@ -194,28 +212,40 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
         const typename A::Reader ra;
         const typename B::Reader rb;
         Half first, second;
-        fetch(k0, K, base);
+        ask(k0, K);
+        fetch(0, 1, base);
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (k0 + D < k1) fetch(k0 + D, K, base + BYTES);
-        read(ra, rb, lds, wm, wn, 0, first);
+        ask(k0 + D, K);
+        if (k0 + D < k1) fetch(0, 1, base + BYTES);
+        read(ra, rb, lds, wm, wn, 0, 0, 1, first);
         int which = 0;
         // (the last tile apart: behind a branch the compiler waits for what either side may have asked for)
         for (int k = k0; k + D < k1; k += D) {
-            read(ra, rb, lds + which * BYTES, wm, wn, 1, second);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(first);
-            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                if (i < EARLY) read(ra, rb, lds + which * BYTES, wm, wn, 1, i, EARLY, second);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(first, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (k + 2 * D < k1) fetch(k + 2 * D, K, base + which * BYTES);
+            ask(k + 2 * D, K);          // (past K: zeros, which nobody reads)
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                if (i < EARLY) read(ra, rb, lds + (which ^ 1) * BYTES, wm, wn, 0, i, EARLY, first);
+                __builtin_amdgcn_sched_barrier(0);
+                multiply(second, i);
+                __builtin_amdgcn_sched_barrier(0);
+                fetch(i, MT, base + which * BYTES);
+            }
             which ^= 1;
-            read(ra, rb, lds + which * BYTES, wm, wn, 0, first);
-            __builtin_amdgcn_sched_barrier(0);
-            multiply(second);
-            __builtin_amdgcn_sched_barrier(0);
         }
-        read(ra, rb, lds + which * BYTES, wm, wn, 1, second);
-        multiply(first);
-        multiply(second);
+        read(ra, rb, lds + which * BYTES, wm, wn, 1, 0, 1, second);
+#pragma unroll
+        for (int i = 0; i < MT; i++) multiply(first, i);
+#pragma unroll
+        for (int i = 0; i < MT; i++) multiply(second, i);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // (nothing may come into LDS behind the workgroup's end)
     }
 };
 
