@@ -158,38 +158,37 @@ __device__ __forceinline__ void tile_of(int index, int rows, int columns, int &r
 // The loop over k of a workgroup of WM x WN wavefronts: acc[i][j] is the sum of 16 rows of A and 16 of B, a lane's element e the one of A's row
 // (lane & 15) and B's row 4 (lane >> 4) + e.  B's rows come in PARTS parts of BN / PARTS rows; a wavefront takes its share of each.
 template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> struct Loop {
-    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16, BYTES = (BM + BN) * 128, LDS = 2 * BYTES;
+    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16, ABYTES = BM * 128, BBYTES = BN * 128, LDS = 3 * ABYTES + 2 * BBYTES;
     A a;
     B b[PARTS];
     f4 acc[MT][NT];
 
-    static constexpr int LOADS = A::ROUNDS + PARTS * B::ROUNDS;
-    __device__ __forceinline__ void ask(int k, int K) {
-        a.ask(k, K);
+    __device__ __forceinline__ void ask_b(int k, int K) {
 #pragma unroll
         for (int p = 0; p < PARTS; p++) b[p].ask(k, K);
     }
     // share `g` of `of` of a tile's loads
-    __device__ __forceinline__ void fetch(int g, int of, unsigned lds) const {
+    __device__ __forceinline__ void fetch_a(int g, int of, unsigned lds) const {
 #pragma unroll
-        for (int q = 0; q < LOADS; q++) {
-            if (q < g * LOADS / of || q >= (g + 1) * LOADS / of) continue;
-            if (q < A::ROUNDS) a.fetch(q, lds);
-            else b[(q - A::ROUNDS) / B::ROUNDS].fetch((q - A::ROUNDS) % B::ROUNDS, lds + (BM + (q - A::ROUNDS) / B::ROUNDS * (BN / PARTS)) * 128);
-        }
+        for (int q = g * A::ROUNDS / of; q < (g + 1) * A::ROUNDS / of; q++) a.fetch(q, lds);
+    }
+    __device__ __forceinline__ void fetch_b(int g, int of, unsigned lds) const {
+        constexpr int ALL = PARTS * B::ROUNDS;
+#pragma unroll
+        for (int q = g * ALL / of; q < (g + 1) * ALL / of; q++) b[q / B::ROUNDS].fetch(q % B::ROUNDS, lds + q / B::ROUNDS * (BN / PARTS) * 128);
     }
     // a half tile's operands
     struct Half { i4 x[MT], y[NT]; };
     // share `g` of `of` of a half's reads: those that the multiplications begin with first
-    __device__ __forceinline__ void read(const typename A::Reader &ra, const typename B::Reader &rb, const char *at, int wm, int wn, int half, int g, int of, Half &h) const {
+    __device__ __forceinline__ void read(const typename A::Reader &ra, const typename B::Reader &rb, const char *at_a, const char *at_b, int wm, int wn, int half, int g, int of, Half &h) const {
 #pragma unroll
         for (int q = 0; q < MT + NT; q++) {
             if (q < g * (MT + NT) / of || q >= (g + 1) * (MT + NT) / of) continue;
             if (q < NT) {
                 const int part = q / (NT / PARTS), jj = q % (NT / PARTS);
-                h.y[q] = rb.read(at + (BM + part * (BN / PARTS)) * 128, wn * (NT / PARTS) + jj, half);
+                h.y[q] = rb.read(at_b + part * (BN / PARTS) * 128, wn * (NT / PARTS) + jj, half);
             } else {
-                h.x[q - NT] = ra.read(at, wm * MT + q - NT, half);
+                h.x[q - NT] = ra.read(at_a, wm * MT + q - NT, half);
             }
         }
     }
@@ -198,9 +197,10 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
         for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(h.y[j], h.x[i], acc[i][j]);
     }
     // k from k0 (whole tiles) to k1.  Half a tile's operands are multiplied while the next half's are on their way from LDS; the one barrier of a tile stands
-    // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  The tile after
-    // that goes into the place of this one.  Reads and loads are issued between the multiplications, a few at a time: issued together they would hold the
-    // matrix instructions behind them up (a tile's loads take the memory pipe half a tile's time).
+    // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  LDS holds
+    // three of A's tiles and two of B's, all that there is: A's tile after the next is asked for in a tile's first half, B's in the second, in the place of this
+    // one's.  Reads and loads are issued between the multiplications, a few at a time: issued together they hold the matrix instructions behind them up (a
+    // tile's loads take the memory pipe half a tile's time).
     __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
         constexpr int D = depth<T>(), EARLY = MT * 3 / 4;          // EARLY: shares of a half's reads, the rest of the multiplications cover the last ones
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -212,35 +212,43 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
         const typename A::Reader ra;
         const typename B::Reader rb;
         Half first, second;
-        ask(k0, K);
-        fetch(0, 1, base);
+        int a0 = 0, a1 = ABYTES, a2 = 2 * ABYTES, b0 = 3 * ABYTES, b1 = 3 * ABYTES + BBYTES;          // this tile's, the next one's, A's after that
+        a.ask(k0, K);
+        ask_b(k0, K);
+        fetch_a(0, 1, base + a0);
+        fetch_b(0, 1, base + b0);
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        ask(k0 + D, K);
-        if (k0 + D < k1) fetch(0, 1, base + BYTES);
-        read(ra, rb, lds, wm, wn, 0, 0, 1, first);
-        int which = 0;
+        a.ask(k0 + D, K);
+        ask_b(k0 + D, K);
+        fetch_a(0, 1, base + a1);
+        fetch_b(0, 1, base + b1);
+        read(ra, rb, lds + a0, lds + b0, wm, wn, 0, 0, 1, first);
         // (the last tile apart: behind a branch the compiler waits for what either side may have asked for)
         for (int k = k0; k + D < k1; k += D) {
+            a.ask(k + 2 * D, K);          // (past K: zeros, which nobody reads)
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                if (i < EARLY) read(ra, rb, lds + which * BYTES, wm, wn, 1, i, EARLY, second);
+                if (i < EARLY) read(ra, rb, lds + a0, lds + b0, wm, wn, 1, i, EARLY, second);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(first, i);
                 __builtin_amdgcn_sched_barrier(0);
+                fetch_a(i, MT, base + a2);
             }
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            ask(k + 2 * D, K);          // (past K: zeros, which nobody reads)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(A::ROUNDS) : "memory");
+            ask_b(k + 2 * D, K);
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                if (i < EARLY) read(ra, rb, lds + (which ^ 1) * BYTES, wm, wn, 0, i, EARLY, first);
+                if (i < EARLY) read(ra, rb, lds + a1, lds + b1, wm, wn, 0, i, EARLY, first);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(second, i);
                 __builtin_amdgcn_sched_barrier(0);
-                fetch(i, MT, base + which * BYTES);
+                fetch_b(i, MT, base + b0);
             }
-            which ^= 1;
+            const int a = a0, b = b0;
+            a0 = a1, a1 = a2, a2 = a;
+            b0 = b1, b1 = b;
         }
-        read(ra, rb, lds + which * BYTES, wm, wn, 1, 0, 1, second);
+        read(ra, rb, lds + a0, lds + b0, wm, wn, 1, 0, 1, second);
 #pragma unroll
         for (int i = 0; i < MT; i++) multiply(first, i);
 #pragma unroll
