@@ -202,7 +202,7 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
     // one's.  Reads and loads are issued between the multiplications, a few at a time: issued together they hold the matrix instructions behind them up (a
     // tile's loads take the memory pipe half a tile's time).
     __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
-        constexpr int D = depth<T>(), EARLY = MT * 3 / 4;          // EARLY: shares of a half's reads, the rest of the multiplications cover the last ones
+        constexpr int D = depth<T>();
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
         const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
 #pragma unroll
@@ -228,7 +228,7 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
             a.ask(k + 2 * D, K);          // (past K: zeros, which nobody reads)
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                if (i < EARLY) read(ra, rb, lds + a0, lds + b0, wm, wn, 1, i, EARLY, second);
+                read(ra, rb, lds + a0, lds + b0, wm, wn, 1, i, MT, second);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(first, i);
                 __builtin_amdgcn_sched_barrier(0);
@@ -238,7 +238,7 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
             ask_b(k + 2 * D, K);
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                if (i < EARLY) read(ra, rb, lds + a1, lds + b1, wm, wn, 0, i, EARLY, first);
+                read(ra, rb, lds + a1, lds + b1, wm, wn, 0, i, MT, first);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(second, i);
                 __builtin_amdgcn_sched_barrier(0);
