@@ -451,7 +451,7 @@ int wkv_embedding_backward(void *stream, long long count, int V, int C, int dtyp
  *   h = act(x w_gate') * (x w_up'),   act: 0 silu, 1 gelu (its tanh form), 2 relu
  * x (rows, C) with a row stride in elements, weights and h (rows, F) contiguous, all in `dtype`; sums in fp32, h rounded once.  Where C is whole pieces of
  * 16 bytes x, its stride and the weights are aligned to 16 bytes.  kept: NULL, or wkv_gated_product_kept_bytes (both products in fp32) for a backward call.
- * workspace: wkv_gated_product_forward_workspace bytes (none where C is whole pieces or rows are few).  rows up to 2^21, C and F below 2^20. */
+ * workspace: wkv_gated_product_forward_workspace bytes (none where C is whole pieces).  rows up to 2^21, C and F below 2^20. */
 size_t wkv_gated_product_kept_bytes(int rows, int C, int F, int dtype);
 size_t wkv_gated_product_forward_workspace(int rows, int C, int F, int dtype);
 int wkv_gated_product_forward(void *stream, int rows, int C, int F, int dtype, int activation, const void *x, long long x_stride, const void *w_gate,

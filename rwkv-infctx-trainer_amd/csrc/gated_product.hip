@@ -68,7 +68,7 @@ struct Forward {
 };
 
 template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN) void forward(const Forward k, int rows, int columns) {
+__global__ __launch_bounds__(64 * WM * WN, 256 / BM) void forward(const Forward k, int rows, int columns) {
     typedef tiles::Loop<T, tiles::Along<T, BM, 64 * WM * WN>, tiles::Along<T, BN / 2, 64 * WM * WN>, BM, BN, WM, WN, 2> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
@@ -121,7 +121,7 @@ struct Product {
 
 // ACROSS_A, ACROSS_B: k lies across memory in that operand
 template <class T, int BM, int BN, int WM, int WN, bool ACROSS_A, bool ACROSS_B>
-__global__ __launch_bounds__(64 * WM * WN) void product(const Product k, int rows, int columns) {
+__global__ __launch_bounds__(64 * WM * WN, 256 / BM) void product(const Product k, int rows, int columns) {
     typedef std::conditional_t<ACROSS_A, tiles::Across<T, BM, 64 * WM * WN>, tiles::Along<T, BM, 64 * WM * WN>> A;
     typedef std::conditional_t<ACROSS_B, tiles::Across<T, BN, 64 * WM * WN>, tiles::Along<T, BN, 64 * WM * WN>> B;
     typedef tiles::Loop<T, A, B, BM, BN, WM, WN, 1> L;
@@ -167,11 +167,27 @@ template <class T> __global__ __launch_bounds__(256) void join(const Product k, 
 }
 
 // ---- layouts
-// rows of C elements -> rows of Cs, zeros behind
-template <class T> __global__ __launch_bounds__(256) void widen(const T *in, long long stride, int R, int C, T *out, int Cs) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
-    const size_t r = i / Cs, c = i % Cs;
-    if (r < (size_t)R) out[i] = (int)c < C ? in[r * stride + c] : from_float<T>(0.f);
+// rows of C elements -> rows of Cs, zeros behind; up to three arrays in a launch
+struct Widen {
+    struct { const void *in; void *out; long long stride; size_t end; } array[3];          // end: of the elements written, over the arrays
+    int C, Cs;
+};
+template <class T> __global__ __launch_bounds__(256) void widen(const Widen k) {
+    constexpr int V = tiles::piece<T>();
+    size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V, first = 0;
+    int j = 0;
+    while (j < 2 && i >= k.array[j].end) first = k.array[j++].end;
+    if (i >= k.array[j].end) return;
+    i -= first;
+    const size_t r = i / k.Cs;
+    const int c = (int)(i - r * k.Cs);
+    const T *in = static_cast<const T *>(k.array[j].in) + r * k.array[j].stride;
+    T e[V];
+#pragma unroll
+    for (int q = 0; q < V; q++) e[q] = c + q < k.C ? in[c + q] : from_float<T>(0.f);
+    uint4 raw;
+    __builtin_memcpy(&raw, e, 16);
+    *reinterpret_cast<uint4 *>(static_cast<T *>(k.array[j].out) + i) = raw;
 }
 // dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y
 template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, long long Fs) {
@@ -202,7 +218,8 @@ template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int
 }
 
 // ---- few rows: a serving loop's single tokens.  What they cost is the weights, read once: a workgroup takes 16 gate rows and the same 16 up rows,
-// its four wavefronts every fourth tile of k; operands go straight from memory to registers.
+// its four wavefronts every fourth tile of k; operands go straight from memory to registers, so that nothing waits for a barrier or for LDS (1 row of 4096
+// into 14336 columns bf16, weights out of the cache: 46 us, 5.1 TB/s).
 constexpr int FEW = 64, FEW_WAVES = 4;
 template <class T, int GROUPS, bool WHOLE>                    // GROUPS of 16 rows of x; WHOLE: rows are whole pieces of 16 bytes
 __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
@@ -278,19 +295,66 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
 }
 
 // ---- launches
-template <class T> static const T *lay_out(hipStream_t s, const T *p, long long stride, int rows, int C, T *to) {
-    const int Cs = (int)rounded(C);
-    hipLaunchKernelGGL(widen<T>, dim3((unsigned)(((size_t)rows * Cs + 255) / 256)), dim3(256), 0, s, p, stride, rows, C, to, Cs);
-    return to;
-}
+struct Layout {
+    Widen k = {};
+    size_t all = 0;
+    int count = 0;
+    explicit Layout(int C) { k.C = C; k.Cs = (int)rounded(C); }
+    // from here on p is the copy at `to`
+    template <class T> void add(const T *&p, long long stride, int rows, void *to) {
+        all += (size_t)rows * k.Cs;
+        k.array[count++] = {p, to, stride, all};
+        p = static_cast<const T *>(to);
+    }
+    template <class T> void launch(hipStream_t s) {
+        for (int j = count; j < 3; j++) k.array[j].end = all;
+        if (all) hipLaunchKernelGGL(widen<T>, dim3((unsigned)((all / tiles::piece<T>() + 255) / 256)), dim3(256), 0, s, k);
+    }
+};
 static inline int tiles_of(long long n, int size) { return (int)((n + size - 1) / size); }
+// What `groups` workgroups of tiles of a size take, each `steps` tiles deep, in us: the longer of one workgroup's own time and, per compute unit, all of them's (a tile
+// of 256 has a compute unit to itself: whole rounds).  Fitted to 16 shapes in bf16, fp16 and fp32 from 16 to 4096 rows, where the choice by these
+// is the fastest or within 10 % of it: x (64, 2560) into 8960 columns bf16 49, 29, 23 by 256, 128, 64; (256, 4096) into 14336 84, 66, 91; (777, 2048) into
+// 7168 57, 65, 80; (301, 1001) into 2731 fp32 258, 86, 54.
+template <class T> static double cost_of(int size, long long groups, long long steps) {
+    const double cus = cu_count(), share = (double)groups / cus, n = (double)steps;
+    const bool narrow = sizeof(T) == 2;
+    if (size == 256) return (double)((groups + cu_count() - 1) / cu_count()) * ((narrow ? 1.35 : 7.6) * n + 10);
+    if (size == 128) return std::max((narrow ? 0.62 : 2.3) * n + 4, share * ((narrow ? 0.5 : 2.0) * n + 2));
+    return std::max((narrow ? 0.48 : 0.8) * n + 2, share * ((narrow ? 0.2 : 0.55) * n + 0.6));
+}
+// Up to 64 rows: whether to take their kernel.  It reads the weights at what memory gives, but x again for every 16 columns; the tiles are as good from some 16 rows on
+// where there is enough of the weights (bf16, weights out of the cache, in us by it and by tiles: (4096, 14336) 1 row 46 and 55, 17 rows 61 and 55, 64 rows 107 and 56;
+// (1024, 2816) 5 and 11, 6 and 11, 9 and 13; fp32 (1024, 4096) 13 and 31, 18 and 31, 24 and 31).
+// Rows that are not whole pieces are read element by element there, and copied for the tiles ((4095, 14335) bf16 1 row 153 and 200, 64 rows 377 and 202).
+template <class T> static bool few_pays(int R, int C, int F) {
+    const double mb = 2. * F * C * sizeof(T) / 1e6, groups = tiles_of(R, 16);
+    const bool whole = C % tiles::piece<T>() == 0;
+    const double few = whole ? 0.19 * mb * (1 + 0.32 * (groups - 1)) + 3 : 0.65 * mb * (1 + 0.45 * (groups - 1)) + 3;
+    const double tiled = std::max(0.22 * mb, cost_of<T>(64, tiles_of(F, 32), (C + tiles::depth<T>() - 1) / tiles::depth<T>())) + (whole ? 0 : 0.6 * mb + 8);
+    return few < tiled;
+}
+// How a product is shared out: the tiles' size, and k cut into shares where the tiles do not fill the compute units, their sums joined by another launch
+struct Plan { int size, rows, columns, shares, per; };
+template <class T> static Plan plan_of(long long M, long long N, long long K, bool cut) {
+    Plan best = {};
+    const long long steps = (K + tiles::depth<T>() - 1) / tiles::depth<T>();
+    double least = 1e30;
+    for (int size : {256, 128, 64})
+        for (long long shares = 1; shares <= (cut && size < 256 ? 16 : 1) && steps >= 4 * shares - 3; shares *= 2) {
+            const long long rows = tiles_of(M, size), columns = tiles_of(N, size), each = (steps + shares - 1) / shares, all = (steps + each - 1) / each;
+            const double cost = cost_of<T>(size, rows * columns * all, each) + (all > 1 ? 5 + (double)(all * M * N) * 8 / 4e6 : 0);
+            if (cost < least) least = cost, best = {size, (int)rows, (int)columns, (int)all, (int)(each * tiles::depth<T>())};
+        }
+    return best;
+}
 template <class T> static size_t forward_scratch(int R, int C, int F) {
-    if (C % tiles::piece<T>() == 0 || R <= FEW) return 0;
+    if (C % tiles::piece<T>() == 0) return 0;
     return ((size_t)R + 2 * (size_t)F) * rounded(C) * sizeof(T);
 }
 template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *scratch) {
     const bool whole = k.K % tiles::piece<T>() == 0;
-    if (k.R <= FEW) {
+    if (k.R <= FEW && few_pays<T>(k.R, k.K, k.F)) {
         const dim3 grid(tiles_of(k.F, 16));
         const int groups = tiles_of(k.R, 16);
 #define WKV_FEW(G)                                                                                             \
@@ -305,21 +369,24 @@ template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *s
         return hipGetLastError();
     }
     if (!whole) {
-        const int Cs = (int)rounded(k.K);
+        Layout l(k.K);
+        const int Cs = l.k.Cs;
         T *to = static_cast<T *>(scratch);
-        k.x = lay_out(s, static_cast<const T *>(k.x), k.xs, k.R, k.K, to);
-        k.wg = lay_out(s, static_cast<const T *>(k.wg), k.ws, k.F, k.K, to + (size_t)k.R * Cs);
-        k.wu = lay_out(s, static_cast<const T *>(k.wu), k.ws, k.F, k.K, to + (size_t)(k.R + k.F) * Cs);
+        const T *x = static_cast<const T *>(k.x), *wg = static_cast<const T *>(k.wg), *wu = static_cast<const T *>(k.wu);
+        l.add(x, k.xs, k.R, to);
+        l.add(wg, k.ws, k.F, to + (size_t)k.R * Cs);
+        l.add(wu, k.ws, k.F, to + (size_t)(k.R + k.F) * Cs);
+        l.launch<T>(s);
+        k.x = x; k.wg = wg; k.wu = wu;
         k.xs = k.ws = k.K = Cs;
     }
-    const int big = tiles_of(k.R, 256) * tiles_of(k.F, 128);
-    if (big >= cu_count()) {
-        const int rows = tiles_of(k.R, 256), columns = tiles_of(k.F, 128);
-        hipLaunchKernelGGL((forward<T, 256, 256, 2, 4>), dim3(rows * columns), dim3(512), 0, s, k, rows, columns);
-    } else {
-        const int rows = tiles_of(k.R, 128), columns = tiles_of(k.F, 64);
-        hipLaunchKernelGGL((forward<T, 128, 128, 2, 2>), dim3(rows * columns), dim3(256), 0, s, k, rows, columns);
-    }
+    // (a tile's columns are half gate, half up)
+    const Plan p = plan_of<T>(k.R, 2ll * k.F, k.K, false);
+    const int rows = p.rows, columns = tiles_of(k.F, p.size / 2);
+    const dim3 grid(rows * columns);
+    if (p.size == 256) hipLaunchKernelGGL((forward<T, 256, 256, 2, 4>), grid, dim3(512), 0, s, k, rows, columns);
+    else if (p.size == 128) hipLaunchKernelGGL((forward<T, 128, 128, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
+    else hipLaunchKernelGGL((forward<T, 64, 64, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
     return hipGetLastError();
 }
 
@@ -330,22 +397,6 @@ struct Backward {
     long long xs, ws;
     void *gx, *gwg, *gwu;             // gx, or gwg and gwu, may be NULL: not wanted
 };
-// How a product is shared out: tiles of 256 or 128, and k cut where the tiles do not fill the compute units
-struct Plan { int size, rows, columns, shares, per; };
-template <class T> static Plan plan_of(long long M, long long N, long long K) {
-    Plan p;
-    const int cus = cu_count();
-    p.size = (long long)tiles_of(M, 256) * tiles_of(N, 256) >= cus * 3 / 4 ? 256 : 128;
-    p.rows = tiles_of(M, p.size);
-    p.columns = tiles_of(N, p.size);
-    const long long steps = (K + tiles::depth<T>() - 1) / tiles::depth<T>();
-    long long shares = 1;
-    while (p.size == 128 && (long long)p.rows * p.columns * shares * 2 <= 2 * cus && steps >= 16 * shares) shares *= 2;
-    const long long each = (steps + shares - 1) / shares;
-    p.shares = (int)((steps + each - 1) / each);
-    p.per = (int)(each * tiles::depth<T>());
-    return p;
-}
 struct Regions { size_t d, x, wg, wu, parts, all; };
 template <class T> static Regions regions(int R, int C, int F, bool want_x, bool want_w) {
     const size_t Fs = rounded(F), Rs = rounded(R), Cs = C % tiles::piece<T>() ? rounded(C) : 0;
@@ -358,11 +409,11 @@ template <class T> static Regions regions(int R, int C, int F, bool want_x, bool
     r.wu = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
     size_t parts = 0;
     if (want_x) {
-        const Plan p = plan_of<T>(R, C, 2 * Fs);
+        const Plan p = plan_of<T>(R, C, 2 * Fs, true);
         if (p.shares > 1) parts = std::max(parts, (size_t)p.shares * R * C * 4);
     }
     if (want_w) {
-        const Plan p = plan_of<T>(2 * Fs, C, Rs);
+        const Plan p = plan_of<T>(2 * Fs, C, Rs, true);
         if (p.shares > 1) parts = std::max(parts, (size_t)p.shares * 2 * Fs * C * 4);
     }
     r.parts = take(parts);
@@ -374,7 +425,8 @@ template <class T, bool ACROSS_A> static void product_launch(hipStream_t s, Prod
     if (p.shares == 1) k.parts = nullptr;
     const dim3 grid(p.rows * p.columns, p.shares);
     if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4, ACROSS_A, true>), grid, dim3(512), 0, s, k, p.rows, p.columns);
-    else hipLaunchKernelGGL((product<T, 128, 128, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    else if (p.size == 128) hipLaunchKernelGGL((product<T, 128, 128, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    else hipLaunchKernelGGL((product<T, 64, 64, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
     if (p.shares > 1) hipLaunchKernelGGL(join<T>, dim3((unsigned)(((size_t)k.M * k.os + 255) / 256)), dim3(256), 0, s, k, p.shares);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k, void *scratch) {
@@ -386,11 +438,13 @@ template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k
     const T *x = static_cast<const T *>(k.x), *wg = static_cast<const T *>(k.wg), *wu = static_cast<const T *>(k.wu);
     long long xs = k.xs, ld = k.ws;
     if (k.C % tiles::piece<T>()) {
-        if (want_w) x = lay_out(s, x, xs, k.R, k.C, reinterpret_cast<T *>(ws + r.x));
+        Layout l(k.C);
+        if (want_w) l.add(x, xs, k.R, ws + r.x);
         if (want_x) {
-            wg = lay_out(s, wg, ld, k.F, k.C, reinterpret_cast<T *>(ws + r.wg));
-            wu = lay_out(s, wu, ld, k.F, k.C, reinterpret_cast<T *>(ws + r.wu));
+            l.add(wg, ld, k.F, ws + r.wg);
+            l.add(wu, ld, k.F, ws + r.wu);
         }
+        l.launch<T>(s);
         xs = ld = rounded(k.C);
     }
     float *parts = reinterpret_cast<float *>(ws + r.parts);
@@ -404,7 +458,7 @@ template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k
         p.b = wg; p.b2 = wu; p.bs = ld; p.turn = Fs; p.rows = k.F;
         p.out0 = p.out1 = k.gx; p.os = k.C; p.split = p.live = k.R;
         p.parts = parts;
-        product_launch<T, false>(s, p, plan_of<T>(p.M, p.N, p.K));
+        product_launch<T, false>(s, p, plan_of<T>(p.M, p.N, p.K, true));
     }
     if (want_w) {
         Product p = {};
@@ -413,7 +467,7 @@ template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k
         p.b = p.b2 = x; p.bs = xs; p.turn = 0x7fffffff; p.rows = k.R;
         p.out0 = k.gwg; p.out1 = k.gwu; p.os = k.C; p.split = Fs; p.live = k.F;
         p.parts = parts;
-        product_launch<T, true>(s, p, plan_of<T>(p.M, p.N, p.K));
+        product_launch<T, true>(s, p, plan_of<T>(p.M, p.N, p.K, true));
     }
     return hipGetLastError();
 }

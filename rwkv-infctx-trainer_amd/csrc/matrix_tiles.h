@@ -91,7 +91,11 @@ template <class T, int ROWS, int THREADS> struct Across {
     long long bytes, ld;              // from p to the end
     int turn;
     unsigned at[ROUNDS];
-    static __device__ __forceinline__ int exchange(int k) { return sizeof(T) == 2 ? ((k & 3) | (k >> 1 & 4)) << 1 : (k >> 2 & 3) << 2; }
+    // of the pieces' numbers in row k: an instruction takes two pieces (fp32: four) of each of rows 8 g .. 8 g + 3 (fp32: of rows 4 g)
+    static __device__ __forceinline__ int exchange(int k) {
+        if (sizeof(T) == 4) return (k >> 2 & 3) << 2;
+        return (PIECES >= 16 ? (k & 3) | (k >> 1 & 4) : (k >> 1 & 1) | (k >> 2 & 2)) << 1;
+    }
     // column n0 of rows that are there up to `rows`, `width` elements wide
     __device__ __forceinline__ void place(const T *base, const T *base2, int turn_, long long ld_, int n0, int rows, int width) {
         p = reinterpret_cast<const char *>(base + n0);
@@ -120,10 +124,10 @@ template <class T, int ROWS, int THREADS> struct Across {
             const int lane = threadIdx.x & 63, a = lane & 15, g = lane >> 4;
             if constexpr (sizeof(T) == 2) {
                 first = (8 * g + (a >> 2)) * BYTES + 8 * (a & 3);
-                mix = ((a >> 2) | (g & 1) << 2) << 5;
+                mix = exchange(8 * g + (a >> 2)) << 4;
             } else {
                 first = 4 * g * BYTES + 4 * a;
-                mix = g << 6;
+                mix = exchange(4 * g) << 4;
             }
         }
         __device__ __forceinline__ i4 read(const char *tile, int sixteen, int half) const {
