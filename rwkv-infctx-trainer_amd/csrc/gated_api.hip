@@ -57,8 +57,9 @@ bool recurrence_pairs(int D, int dtype, const wkv_rows *x, const wkv_rows *r, co
 
 // ---- embedding
 int check_embedding(long long count, int V, int C, int dtype, int index_bytes) {
-    if (count <= 0 || V <= 0 || C <= 0 || count > (1 << 28) || V > (1 << 24) || C > (1 << 24)) return WKV_ERR_DIMS;
-    if (count * C >= (1ll << 33) || (long long)V * C >= (1ll << 40)) return WKV_ERR_DIMS;
+    if (count <= 0 || V <= 0 || C <= 0 || count > (1 << 28) || V > (1 << 24) || C > (1 << 23)) return WKV_ERR_DIMS;
+    // (a grid has fewer than 2^32 threads)
+    if (count * C >= (1ll << 33) || (long long)V * C >= (1ll << 37)) return WKV_ERR_DIMS;
     if (index_bytes != 4 && index_bytes != 8) return WKV_ERR_DTYPE;
     return dtype_ok(dtype);
 }
@@ -67,13 +68,15 @@ int check_embedding(long long count, int V, int C, int dtype, int index_bytes) {
 constexpr int MAX_WIDTH = 1 << 20, MAX_ROWS = 1 << 21;
 int check_product(int rows, int C, int F, int dtype, int activation) {
     if (rows <= 0 || C <= 0 || F <= 0 || rows > MAX_ROWS || C > MAX_WIDTH || F > MAX_WIDTH - ffn::ROUND) return WKV_ERR_DIMS;
+    // (a grid of the smallest tiles has fewer than 2^32 threads)
+    if ((long long)rows * F >= (1ll << 35) || (long long)rows * C >= (1ll << 35) || (long long)F * C >= (1ll << 34)) return WKV_ERR_DIMS;
     if (activation < 0 || activation >= ffn::ACTIVATIONS) return WKV_ERR_ALGO;
     return dtype_ok(dtype);
 }
 // what is read in whole pieces is aligned to them
 int check_pieces(const void *p, long long stride, int C, int dtype) {
     if (!p) return WKV_ERR_NULL;
-    if (stride < C || stride > MAX_ROWS) return WKV_ERR_DIMS;
+    if (stride < C || stride > MAX_ROWS) return WKV_ERR_DIMS;          // (256 rows of a tile within 2^31 bytes)
     const bool whole = C % (16 / (int)element(dtype)) == 0;
     return aligned_to(p, whole ? 16 : element(dtype)) && (!whole || stride * element(dtype) % 16 == 0) ? WKV_OK : WKV_ERR_ALIGN;
 }

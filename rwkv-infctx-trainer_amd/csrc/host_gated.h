@@ -149,10 +149,12 @@ PyObject *py_embedding(PyObject *, PyObject *const *a, Py_ssize_t n) {
 Tensor whole_rows(const Tensor &t) {
     const Tensor r = as_rows(t);
     const int64_t size = r.element_size(), C = r.size(1);
-    if (r.stride(0) < C) return r.contiguous();          // (rows that share memory)
-    if (C * size % 16 != 0 || (r.stride(0) * size % 16 == 0 && (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0)) return r;
-    return plain(r);
+    if (r.size(0) > 1 && (r.stride(0) < C || r.stride(0) > (1 << 21))) return plain(r);          // (rows that share memory, or lie too far apart)
+    const bool there = (reinterpret_cast<uintptr_t>(r.data_ptr()) & 15) == 0 && (r.size(0) == 1 || r.stride(0) * size % 16 == 0);
+    return C * size % 16 != 0 || there ? r : plain(r);
 }
+// (that of a single row means nothing)
+int64_t whole_stride(const Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 class GatedProduct : public torch::autograd::Function<GatedProduct> {
 public:
     static variable_list forward(AutogradContext *ctx, const Tensor &x_, const Tensor &w_gate, const Tensor &w_up, int64_t activation) {
@@ -164,7 +166,7 @@ public:
         const Tensor h = fresh(shape, x.scalar_type()), kept = ctx ? fresh_bytes(abi.wkv_gated_product_kept_bytes(R, C, F, dt)) : Tensor();
         const size_t need = abi.wkv_gated_product_forward_workspace(R, C, F, dt);
         const Tensor ws = need ? fresh_bytes(need) : Tensor();
-        check(abi.wkv_gated_product_forward(dev.stream(), R, C, F, dt, (int)activation, ptr(x), x.stride(0), ptr(wg), ptr(wu), ptr(h), fptr(kept), ptr(ws), need),
+        check(abi.wkv_gated_product_forward(dev.stream(), R, C, F, dt, (int)activation, ptr(x), whole_stride(x), ptr(wg), ptr(wu), ptr(h), fptr(kept), ptr(ws), need),
               "wkv_gated_product_forward");
         if (ctx) {
             ctx->saved_data["call"] = std::vector<int64_t>{activation};
@@ -186,7 +188,7 @@ public:
         const Tensor gx = want_x ? fresh(shape, x.scalar_type()) : Tensor(), gg = want_w ? fresh({F, C}, x.scalar_type()) : Tensor();
         const Tensor gu = want_w ? fresh({F, C}, x.scalar_type()) : Tensor();
         const Tensor ws = fresh_bytes(abi.wkv_gated_product_backward_workspace(R, C, F, dt, want_x, want_w));
-        check(abi.wkv_gated_product_backward(dev.stream(), R, C, F, dt, activation, ptr(x), x.stride(0), ptr(wg), ptr(wu), fptr(kept), ptr(gh), ptr(gx), ptr(gg),
+        check(abi.wkv_gated_product_backward(dev.stream(), R, C, F, dt, activation, ptr(x), whole_stride(x), ptr(wg), ptr(wu), fptr(kept), ptr(gh), ptr(gx), ptr(gg),
                                              ptr(gu), ptr(ws), ws.numel()), "wkv_gated_product_backward");
         return {gx, gg, gu, Tensor()};
     }

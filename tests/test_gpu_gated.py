@@ -117,7 +117,7 @@ def check_feed_forward(x, wg, wu, gy, name, out, grads):
     """Per element.  With e the half step of the type (0 in fp32: it is in c) and c = (terms + 32) 2^-23 for fp32 sums of that many terms and a few operations
     after them, a sum is off by c times its terms' sizes G, U; the activations' slopes and the slopes' slopes are below 1.2.  A gradient's sum takes
     dg and du rounded (e) and off by what g and u were off; relu's slope is anything where g may be zero."""
-    d = lambda t: t.detach().cpu().double()
+    d = lambda t: t.detach().double()          # (on the GPU: the library's products in 64 bits)
     x, wg, wu, gy = d(x), d(wg), d(wu), d(gy)
     e = _step(out.dtype)
     leaf = [t.clone().requires_grad_(True) for t in (x, wg, wu)]
