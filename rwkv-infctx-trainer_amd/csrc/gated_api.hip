@@ -67,11 +67,12 @@ int check_embedding(long long count, int V, int C, int dtype, int index_bytes) {
 // ---- gated feed-forward.  256 rows of an operand lie within the 2^31 bytes of a buffer's range.
 constexpr int MAX_WIDTH = 1 << 20, MAX_ROWS = 1 << 21;
 int check_product(int rows, int C, int F, int dtype, int activation) {
+    if (int st = dtype_ok(dtype)) return st;
     if (rows <= 0 || C <= 0 || F <= 0 || rows > MAX_ROWS || C > MAX_WIDTH || F > MAX_WIDTH - ffn::ROUND) return WKV_ERR_DIMS;
-    // (a grid of the smallest tiles has fewer than 2^32 threads)
+    // (a grid of the smallest tiles has fewer than 2^32 threads, as has the one that lays rows out in whole pieces)
+    if (C % (16 / (int)element(dtype)) && (rows + 2ll * F) * ffn::rounded(C) >= (1ll << 34)) return WKV_ERR_DIMS;
     if ((long long)rows * F >= (1ll << 35) || (long long)rows * C >= (1ll << 35) || (long long)F * C >= (1ll << 34)) return WKV_ERR_DIMS;
-    if (activation < 0 || activation >= ffn::ACTIVATIONS) return WKV_ERR_ALGO;
-    return dtype_ok(dtype);
+    return activation < 0 || activation >= ffn::ACTIVATIONS ? WKV_ERR_ALGO : WKV_OK;
 }
 // what is read in whole pieces is aligned to them
 int check_pieces(const void *p, long long stride, int C, int dtype) {

@@ -57,6 +57,13 @@ template <class T> __device__ __forceinline__ void put4(T *row, int n, int N, bo
         if (n + e < N) row[n + e] = from_float<T>(v[e]);
 }
 
+// Tiles of k ahead, and the wavefronts to a SIMD that LDS then leaves room for.  Tiles of 256 and 128 fill it with two tiles ahead.  Those of 64 leave room for four
+// workgroups then, or for two with four tiles ahead, which is better where there are no more than two to a compute unit: nothing else hides what their loads wait for
+// ((24, 2560) into 8192 columns bf16, weights out of the cache, 31 -> 21 us; (150, 1024) into 2816 13.0 -> 10.4; but (600, 512) into 2000 fp32 31.5 -> 35.7).
+constexpr int DEEP = 4;
+constexpr int waves_per_simd(int size, int ahead) { return ahead == DEEP ? 2 : 256 / size; }
+static inline bool deep_pays(long long groups) { return groups <= 2ll * cu_count(); }
+
 // ---- forward
 struct Forward {
     int R, K, F, kind;
@@ -67,9 +74,9 @@ struct Forward {
     long long hs, Fs;
 };
 
-template <class T, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN, 256 / BM) void forward(const Forward k, int rows, int columns) {
-    typedef tiles::Loop<T, tiles::Along<T, BM, 64 * WM * WN>, tiles::Along<T, BN / 2, 64 * WM * WN>, BM, BN, WM, WN, 2> L;
+template <class T, int BM, int BN, int WM, int WN, int AHEAD>
+__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forward(const Forward k, int rows, int columns) {
+    typedef tiles::Loop<T, tiles::Along<T, BM, 64 * WM * WN>, tiles::Along<T, BN / 2, 64 * WM * WN>, BM, BN, WM, WN, 2, AHEAD> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
     tiles::tile_of(blockIdx.x, rows, columns, tm, tn);
@@ -120,11 +127,11 @@ struct Product {
 };
 
 // ACROSS_A, ACROSS_B: k lies across memory in that operand
-template <class T, int BM, int BN, int WM, int WN, bool ACROSS_A, bool ACROSS_B>
-__global__ __launch_bounds__(64 * WM * WN, 256 / BM) void product(const Product k, int rows, int columns) {
+template <class T, int BM, int BN, int WM, int WN, int AHEAD, bool ACROSS_A, bool ACROSS_B>
+__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void product(const Product k, int rows, int columns) {
     typedef std::conditional_t<ACROSS_A, tiles::Across<T, BM, 64 * WM * WN>, tiles::Along<T, BM, 64 * WM * WN>> A;
     typedef std::conditional_t<ACROSS_B, tiles::Across<T, BN, 64 * WM * WN>, tiles::Along<T, BN, 64 * WM * WN>> B;
-    typedef tiles::Loop<T, A, B, BM, BN, WM, WN, 1> L;
+    typedef tiles::Loop<T, A, B, BM, BN, WM, WN, 1, AHEAD> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
     tiles::tile_of(blockIdx.x, rows, columns, tm, tn);
@@ -384,9 +391,10 @@ template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *s
     const Plan p = plan_of<T>(k.R, 2ll * k.F, k.K, false);
     const int rows = p.rows, columns = tiles_of(k.F, p.size / 2);
     const dim3 grid(rows * columns);
-    if (p.size == 256) hipLaunchKernelGGL((forward<T, 256, 256, 2, 4>), grid, dim3(512), 0, s, k, rows, columns);
-    else if (p.size == 128) hipLaunchKernelGGL((forward<T, 128, 128, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
-    else hipLaunchKernelGGL((forward<T, 64, 64, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
+    if (p.size == 256) hipLaunchKernelGGL((forward<T, 256, 256, 2, 4, 2>), grid, dim3(512), 0, s, k, rows, columns);
+    else if (p.size == 128) hipLaunchKernelGGL((forward<T, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
+    else if (deep_pays(rows * columns)) hipLaunchKernelGGL((forward<T, 64, 64, 2, 2, DEEP>), grid, dim3(256), 0, s, k, rows, columns);
+    else hipLaunchKernelGGL((forward<T, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
     return hipGetLastError();
 }
 
@@ -424,9 +432,10 @@ template <class T, bool ACROSS_A> static void product_launch(hipStream_t s, Prod
     k.per = p.per;
     if (p.shares == 1) k.parts = nullptr;
     const dim3 grid(p.rows * p.columns, p.shares);
-    if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4, ACROSS_A, true>), grid, dim3(512), 0, s, k, p.rows, p.columns);
-    else if (p.size == 128) hipLaunchKernelGGL((product<T, 128, 128, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
-    else hipLaunchKernelGGL((product<T, 64, 64, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4, 2, ACROSS_A, true>), grid, dim3(512), 0, s, k, p.rows, p.columns);
+    else if (p.size == 128) hipLaunchKernelGGL((product<T, 128, 128, 2, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    else if (deep_pays((long long)p.rows * p.columns * p.shares)) hipLaunchKernelGGL((product<T, 64, 64, 2, 2, DEEP, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    else hipLaunchKernelGGL((product<T, 64, 64, 2, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
     if (p.shares > 1) hipLaunchKernelGGL(join<T>, dim3((unsigned)(((size_t)k.M * k.os + 255) / 256)), dim3(256), 0, s, k, p.shares);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k, void *scratch) {

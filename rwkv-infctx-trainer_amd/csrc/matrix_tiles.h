@@ -1,6 +1,6 @@
 // Products  out[m][n] = sum over k of A[m][k] B[n][k]  tile by tile on the matrix cores: the loop that the
 // gated feed-forward's products share.  A workgroup makes BM x BN outputs; 128 bytes of every row of A and B at a time (64 16-bit elements, 32 of
-// fp32) go from memory straight to LDS, the next 128 while these are multiplied.
+// fp32: a tile of k) go from memory straight to LDS, two to four tiles ahead of the one that is multiplied.
 //
 // In LDS a row's eight pieces of 16 bytes are exchanged by the row's low three bits, so that sixteen rows' equal pieces, which the
 // matrix instructions take, lie over all banks.  A piece is a matrix instruction's whole operand of one lane: eight 16-bit elements for
@@ -160,9 +160,11 @@ __device__ __forceinline__ void tile_of(int index, int rows, int columns, int &r
 }
 
 // The loop over k of a workgroup of WM x WN wavefronts: acc[i][j] is the sum of 16 rows of A and 16 of B, a lane's element e the one of A's row
-// (lane & 15) and B's row 4 (lane >> 4) + e.  B's rows come in PARTS parts of BN / PARTS rows; a wavefront takes its share of each.
-template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> struct Loop {
-    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16, ABYTES = BM * 128, BBYTES = BN * 128, LDS = 3 * ABYTES + 2 * BBYTES;
+// (lane & 15) and B's row 4 (lane >> 4) + e.  B's rows come in PARTS parts of BN / PARTS rows; a wavefront takes its share of each.  LDS holds AHEAD + 1
+// of A's tiles and AHEAD of B's.
+template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS, int AHEAD> struct Loop {
+    static constexpr int MT = BM / WM / 16, NT = BN / WN / 16, ABYTES = BM * 128, BBYTES = BN * 128, LDS = (AHEAD + 1) * ABYTES + AHEAD * BBYTES;
+    static constexpr int LOADS = A::ROUNDS + PARTS * B::ROUNDS;          // of a lane and tile
     A a;
     B b[PARTS];
     f4 acc[MT][NT];
@@ -201,10 +203,9 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
         for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(h.y[j], h.x[i], acc[i][j]);
     }
     // k from k0 (whole tiles) to k1.  Half a tile's operands are multiplied while the next half's are on their way from LDS; the one barrier of a tile stands
-    // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  LDS holds
-    // three of A's tiles and two of B's, all that there is: A's tile after the next is asked for in a tile's first half, B's in the second, in the place of this
-    // one's.  Reads and loads are issued between the multiplications, a few at a time: issued together they hold the matrix instructions behind them up (a
-    // tile's loads take the memory pipe half a tile's time).
+    // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  A's tile
+    // AHEAD from this one is asked for in a tile's first half, B's in the second, in the place of this one's.  Reads and loads are issued between the
+    // multiplications, a few at a time: issued together they hold the matrix instructions behind them up (a tile's loads take the memory pipe half a tile's time).
     __device__ __forceinline__ void run(int k0, int k1, int K, char *lds) {
         constexpr int D = depth<T>();
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
@@ -216,43 +217,50 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS> 
         const typename A::Reader ra;
         const typename B::Reader rb;
         Half first, second;
-        int a0 = 0, a1 = ABYTES, a2 = 2 * ABYTES, b0 = 3 * ABYTES, b1 = 3 * ABYTES + BBYTES;          // this tile's, the next one's, A's after that
-        a.ask(k0, K);
-        ask_b(k0, K);
-        fetch_a(0, 1, base + a0);
-        fetch_b(0, 1, base + b0);
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        a.ask(k0 + D, K);
-        ask_b(k0 + D, K);
-        fetch_a(0, 1, base + a1);
-        fetch_b(0, 1, base + b1);
-        read(ra, rb, lds + a0, lds + b0, wm, wn, 0, 0, 1, first);
+        int at_a[AHEAD + 1], at_b[AHEAD];          // this tile's, the next one's ...
+#pragma unroll
+        for (int q = 0; q <= AHEAD; q++) at_a[q] = q * ABYTES;
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) at_b[q] = (AHEAD + 1) * ABYTES + q * BBYTES;
+#pragma unroll
+        for (int q = 0; q < AHEAD; q++) {
+            a.ask(k0 + q * D, K);          // (past K: zeros, which nobody reads)
+            ask_b(k0 + q * D, K);
+            fetch_a(0, 1, base + at_a[q]);
+            fetch_b(0, 1, base + at_b[q]);
+        }
+        asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"((AHEAD - 1) * LOADS) : "memory");
+        read(ra, rb, lds + at_a[0], lds + at_b[0], wm, wn, 0, 0, 1, first);
         // (the last tile apart: behind a branch the compiler waits for what either side may have asked for)
         for (int k = k0; k + D < k1; k += D) {
-            a.ask(k + 2 * D, K);          // (past K: zeros, which nobody reads)
+            a.ask(k + AHEAD * D, K);
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                read(ra, rb, lds + a0, lds + b0, wm, wn, 1, i, MT, second);
+                read(ra, rb, lds + at_a[0], lds + at_b[0], wm, wn, 1, i, MT, second);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(first, i);
                 __builtin_amdgcn_sched_barrier(0);
-                fetch_a(i, MT, base + a2);
+                fetch_a(i, MT, base + at_a[AHEAD]);
             }
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(A::ROUNDS) : "memory");
-            ask_b(k + 2 * D, K);
+            // (all but what was asked for after the next tile's: A's and B's of the ones behind it, A's of the last)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((AHEAD - 2) * LOADS + A::ROUNDS) : "memory");
+            ask_b(k + AHEAD * D, K);
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                read(ra, rb, lds + a1, lds + b1, wm, wn, 0, i, MT, first);
+                read(ra, rb, lds + at_a[1], lds + at_b[1], wm, wn, 0, i, MT, first);
                 __builtin_amdgcn_sched_barrier(0);
                 multiply(second, i);
                 __builtin_amdgcn_sched_barrier(0);
-                fetch_b(i, MT, base + b0);
+                fetch_b(i, MT, base + at_b[0]);
             }
-            const int a = a0, b = b0;
-            a0 = a1, a1 = a2, a2 = a;
-            b0 = b1, b1 = b;
+            const int was_a = at_a[0], was_b = at_b[0];
+#pragma unroll
+            for (int q = 0; q < AHEAD; q++) at_a[q] = at_a[q + 1];
+#pragma unroll
+            for (int q = 0; q + 1 < AHEAD; q++) at_b[q] = at_b[q + 1];
+            at_a[AHEAD] = was_a, at_b[AHEAD - 1] = was_b;
         }
-        read(ra, rb, lds + a0, lds + b0, wm, wn, 1, 0, 1, second);
+        read(ra, rb, lds + at_a[0], lds + at_b[0], wm, wn, 1, 0, 1, second);
 #pragma unroll
         for (int i = 0; i < MT; i++) multiply(first, i);
 #pragma unroll
