@@ -4,7 +4,7 @@
 //
 // A token outside the table is a place without one: a row of zeros, no gradient.  Both directions are bound by memory.  The gradient is written
 // whole (V C, most of it zeros) from the places sorted by token: no atomics, fp32 sums in the places' order, the same bits every time.  Sorting: stable
-// passes over ten bits of the token at a most, counts per tile of places, then each tile's places to where the tiles and digits before leave off; up
+// passes over ten bits of the token at most, counts per tile of places, then each tile's places to where the tiles and digits before leave off; up
 // to one tile's worth in a single launch.  Sums: a workgroup takes 64 sorted places, whoever they belong to, so that it does not matter how often a token
 // comes; a token that lies within them is written as it ends, one that crosses their border leaves a part for a second launch.  The same launch
 // writes the zeros, which keeps memory busy beside the gathers' latency.
@@ -49,7 +49,7 @@ struct Sort {
     int count, V;                             // keys: tokens, V for none
     const void *tokens;                       // the first pass's keys; their places are 0, 1, ..
     const int *keys, *places;                 // the later passes'
-    int *to_keys, *to_places, *counts;        // counts (tiles, BINS)
+    int *to_keys, *to_places, *counts;        // counts (tiles + 1, BINS)
     int shift, bits;
 };
 template <class I> __device__ __forceinline__ int key_at(const Sort &k, int n) {
@@ -69,6 +69,33 @@ template <class I> __global__ __launch_bounds__(SORT_THREADS) void count(const S
     }
     __syncthreads();
     k.counts[(size_t)blockIdx.x * BINS + threadIdx.x] = bin[threadIdx.x];
+}
+
+// Many tiles' counts turned into those of the tiles before, with all tiles' behind the last: 64 digits per workgroup, its wavefronts a share of the tiles each.  Few
+// tiles' are added up by every tile for itself, which saves the launch (the whole gradient of 2^17, 2^18, 2^20, 2^24 places of 8 channels, so and with
+// this launch: 66 and 68 us, 78 and 77, 187 and 159, 6991 and 1872).
+constexpr int MANY = 48;
+static __global__ __launch_bounds__(SORT_THREADS) void sum_tiles(int *counts, int tiles) {
+    __shared__ int share[SORT_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per = (tiles + SORT_WAVES - 1) / SORT_WAVES, from = min(wave * per, tiles), to = min(from + per, tiles);
+    int *row = counts + blockIdx.x * 64 + lane, s = 0;
+#pragma unroll 8
+    for (int t = from; t < to; t++) s += row[(size_t)t * BINS];
+    share[wave][lane] = s;
+    __syncthreads();
+    int before = 0;
+    for (int w = 0; w < wave; w++) before += share[w][lane];
+    for (int t0 = from; t0 < to; t0 += 8) {
+        int n[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) n[j] = t0 + j < to ? row[(size_t)(t0 + j) * BINS] : 0;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (t0 + j < to) row[(size_t)(t0 + j) * BINS] = before;
+            before += n[j];
+        }
+    }
+    if (wave == SORT_WAVES - 1) row[(size_t)tiles * BINS] = before;
 }
 
 struct SortLds {
@@ -138,14 +165,19 @@ template <class I> __global__ __launch_bounds__(SORT_THREADS) void scatter(const
     }
     // of digit threadIdx.x: in the tiles before, and in all
     int before = 0, all = 0;
-    for (int t0 = 0; t0 < tiles; t0 += 8) {
-        int n[8];
+    if (tiles > MANY) {
+        before = k.counts[(size_t)blockIdx.x * BINS + threadIdx.x];
+        all = k.counts[(size_t)tiles * BINS + threadIdx.x];
+    } else {
+        for (int t0 = 0; t0 < tiles; t0 += 8) {
+            int n[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) n[j] = t0 + j < tiles ? k.counts[(size_t)(t0 + j) * BINS + threadIdx.x] : 0;
+            for (int j = 0; j < 8; j++) n[j] = t0 + j < tiles ? k.counts[(size_t)(t0 + j) * BINS + threadIdx.x] : 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            before += t0 + j < (int)blockIdx.x ? n[j] : 0;
-            all += n[j];
+            for (int j = 0; j < 8; j++) {
+                before += t0 + j < (int)blockIdx.x ? n[j] : 0;
+                all += n[j];
+            }
         }
     }
     m.base[threadIdx.x] = sum_before(m, all) + before;
@@ -328,7 +360,7 @@ static inline Regions regions(int count, int V, int C) {
         r.keys[i] = take((size_t)count * 4);
         r.places[i] = take((size_t)count * 4);
     }
-    r.counts = take((size_t)tiles_of(count) * BINS * 4);
+    r.counts = take(((size_t)tiles_of(count) + 1) * BINS * 4);
     r.starts = take(((size_t)V + 1) * 4);
     r.parts = take((size_t)chunks_of(count) * 2 * C * 4);
     r.all = at;
@@ -364,6 +396,7 @@ template <class I> static void sort(hipStream_t s, int count_, int V, const void
         k.to_keys = region(r.keys[p & 1]);
         k.to_places = region(r.places[p & 1]);
         hipLaunchKernelGGL(count<I>, dim3(tiles), dim3(SORT_THREADS), 0, s, k);
+        if (tiles > MANY) hipLaunchKernelGGL(sum_tiles, dim3(BINS / 64), dim3(SORT_THREADS), 0, s, k.counts, tiles);
         hipLaunchKernelGGL(scatter<I>, dim3(tiles), dim3(SORT_THREADS), 0, s, k, tiles);
         k.tokens = nullptr;
         k.keys = k.to_keys;

@@ -59,7 +59,7 @@ bool recurrence_pairs(int D, int dtype, const wkv_rows *x, const wkv_rows *r, co
 int check_embedding(long long count, int V, int C, int dtype, int index_bytes) {
     if (count <= 0 || V <= 0 || C <= 0 || count > (1 << 28) || V > (1 << 24) || C > (1 << 23)) return WKV_ERR_DIMS;
     // (a grid has fewer than 2^32 threads)
-    if (count * C >= (1ll << 33) || (long long)V * C >= (1ll << 37)) return WKV_ERR_DIMS;
+    if (count * C >= (1ll << 33) || (long long)V * C >= (1ll << 36)) return WKV_ERR_DIMS;
     if (index_bytes != 4 && index_bytes != 8) return WKV_ERR_DTYPE;
     return dtype_ok(dtype);
 }

@@ -492,6 +492,25 @@ def test_many_rows_and_sequences():
     w, gy = r(1000, 16).requires_grad_(True), r(700001, 16)
     (grad,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
     S.check_lookup(tokens, w, 1.0, gy, K.embedding(tokens, w), grad)
+    # more tiles than every tile adds up for itself, keys of two digits
+    tokens, gy = torch.randint(-3, 70000, (260000,), device="cuda", generator=g), r(260000, 4).float()
+    w = torch.zeros(70000, 4, device="cuda", requires_grad=True)
+    (grad,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
+    S.check_lookup(tokens, w, 1.0, gy, K.embedding(tokens, w), grad)
+
+
+def test_single_rows_and_places():
+    """x without a batch, a place without one."""
+    K = _kernels()
+    g = S._g(13)
+    x, a, b, w = torch.randn(24, generator=g).cuda(), *(torch.randn(10, 24, generator=g).cuda() for _ in range(2)), torch.randn(5, 24, generator=g).cuda()
+    leaf = [t.requires_grad_(True) for t in (x, a, b, w)]
+    one, whole = K.gated_feed_forward(x, a, b), K.gated_feed_forward(x[None], a, b)
+    assert one.shape == (10,) and torch.equal(one, whole[0])
+    row = K.embedding(torch.tensor(3, device="cuda"), w, 2.0)
+    assert row.shape == (24,) and torch.equal(row, 2 * w[3])
+    grads = torch.autograd.grad(one.sum() + row.sum(), leaf)
+    assert [t.shape for t in grads] == [t.shape for t in leaf] and torch.equal(grads[3], torch.zeros(5, 24, device="cuda").index_fill(0, torch.tensor([3], device="cuda"), 2.0))
 
 
 # ---- refusals
