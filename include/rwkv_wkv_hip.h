@@ -438,7 +438,8 @@ int wkv_gated_recurrence_backward(void *stream, int B, int T, int D, int dtype, 
                                   void *gx, void *gr, void *gi, float *gdecay, void *gz, float *gstate_in, void *workspace, size_t workspace_bytes);
 
 /* Rows of a table (V, C) by token:  out[n] = scale table[tokens[n]], n below count; tokens of 4 or 8 bytes (index_bytes).  A token below zero or from V on
- * is a place without one: a row of zeros.  out (count, C) and the table contiguous in `dtype`. */
+ * is a place without one: a row of zeros.  out (count, C) and the table contiguous in `dtype`.  count up to 2^28, V up to 2^24, C up to 2^23, count C below 2^33, V C
+ * below 2^36. */
 int wkv_embedding_forward(void *stream, long long count, int V, int C, int dtype, int index_bytes, float scale, const void *tokens, const void *table,
                           void *out);
 
@@ -451,7 +452,8 @@ int wkv_embedding_backward(void *stream, long long count, int V, int C, int dtyp
  *   h = act(x w_gate') * (x w_up'),   act: 0 silu, 1 gelu (its tanh form), 2 relu
  * x (rows, C) with a row stride in elements, weights and h (rows, F) contiguous, all in `dtype`; sums in fp32, h rounded once.  Where C is whole pieces of
  * 16 bytes x, its stride and the weights are aligned to 16 bytes.  kept: NULL, or wkv_gated_product_kept_bytes (both products in fp32) for a backward call.
- * workspace: wkv_gated_product_forward_workspace bytes (none where C is whole pieces).  rows up to 2^21, C and F below 2^20. */
+ * workspace: wkv_gated_product_forward_workspace bytes (none where C is whole pieces).  rows up to 2^21, C and F below
+ * 2^20, rows C and rows F below 2^35, F C below 2^34; where C is not whole pieces (rows + 2 F) C below 2^34.  x_stride up to 2^21. */
 size_t wkv_gated_product_kept_bytes(int rows, int C, int F, int dtype);
 size_t wkv_gated_product_forward_workspace(int rows, int C, int F, int dtype);
 int wkv_gated_product_forward(void *stream, int rows, int C, int F, int dtype, int activation, const void *x, long long x_stride, const void *w_gate,

@@ -74,18 +74,29 @@ struct Forward {
     long long hs, Fs;
 };
 
-template <class T, int BM, int BN, int WM, int WN, int AHEAD>
+// LIE: rows are read as they lie, whole tiles of k straight to LDS and what is left behind them, if anything, before, by way of registers
+template <class T, int BM, int BN, int WM, int WN, int AHEAD, bool LIE>
 __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forward(const Forward k, int rows, int columns) {
     typedef tiles::Loop<T, tiles::Along<T, BM, 64 * WM * WN>, tiles::Along<T, BN / 2, 64 * WM * WN>, BM, BN, WM, WN, 2, AHEAD> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
     tiles::tile_of(blockIdx.x, rows, columns, tm, tn);
     const int m0 = tm * BM, n0 = tn * (BN / 2);
+    const int K = LIE ? k.K / tiles::depth<T>() * tiles::depth<T>() : k.K, live = min(BM, k.R - m0), columns_live = min(BN / 2, k.F - n0);
+    const T *x = static_cast<const T *>(k.x) + m0 * k.xs, *wg = static_cast<const T *>(k.wg) + n0 * k.ws, *wu = static_cast<const T *>(k.wu) + n0 * k.ws;
     L l;
-    l.a.place(static_cast<const T *>(k.x) + m0 * k.xs, k.xs, k.K, min(BM, k.R - m0));
-    l.b[0].place(static_cast<const T *>(k.wg) + n0 * k.ws, k.ws, k.K, min(BN / 2, k.F - n0));
-    l.b[1].place(static_cast<const T *>(k.wu) + n0 * k.ws, k.ws, k.K, min(BN / 2, k.F - n0));
-    l.run(0, k.K, k.K, lds);
+    l.a.place(x, k.xs, K, live);
+    l.b[0].place(wg, k.ws, K, columns_live);
+    l.b[1].place(wu, k.ws, K, columns_live);
+    l.clear();
+    if (LIE && K < k.K) {
+        char *at_b = lds + (AHEAD + 1) * L::ABYTES;
+        l.a.carry(x, k.xs, live, K, k.K, lds);
+        l.b[0].carry(wg, k.ws, columns_live, K, k.K, at_b);
+        l.b[1].carry(wu, k.ws, columns_live, K, k.K, at_b + L::BBYTES / 2);
+        l.once(lds);
+    }
+    if (!LIE || K > 0) l.run(0, K, K, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
     const bool whole = k.hs % 4 == 0;
     T *h = static_cast<T *>(k.h);
@@ -144,6 +155,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void produ
     if constexpr (ACROSS_B) l.b[0].place(b, b2, k.turn, k.bs, n0, k.rows, (k.N + E - 1) / E * E);
     else l.b[0].place(b + n0 * k.bs, k.bs, k.K, min(BN, k.N - n0));
     const int k0 = blockIdx.y * k.per;
+    l.clear();
     l.run(k0, min(k0 + k.per, k.K), k.K, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
     const bool whole = k.os % 4 == 0;
@@ -189,11 +201,15 @@ template <class T> __global__ __launch_bounds__(256) void widen(const Widen k) {
     const size_t r = i / k.Cs;
     const int c = (int)(i - r * k.Cs);
     const T *in = static_cast<const T *>(k.array[j].in) + r * k.array[j].stride;
-    T e[V];
-#pragma unroll
-    for (int q = 0; q < V; q++) e[q] = c + q < k.C ? in[c + q] : from_float<T>(0.f);
     uint4 raw;
-    __builtin_memcpy(&raw, e, 16);
+    if (c + V <= k.C) {
+        __builtin_memcpy(&raw, in + c, 16);          // (one load, whatever the alignment)
+    } else {
+        T e[V];
+#pragma unroll
+        for (int q = 0; q < V; q++) e[q] = c + q < k.C ? in[c + q] : from_float<T>(0.f);
+        __builtin_memcpy(&raw, e, 16);
+    }
     *reinterpret_cast<uint4 *>(static_cast<T *>(k.array[j].out) + i) = raw;
 }
 // dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y
@@ -230,7 +246,7 @@ template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int
 constexpr int FEW = 64, FEW_WAVES = 4;
 template <class T, int GROUPS, bool WHOLE>                    // GROUPS of 16 rows of x; WHOLE: rows are whole pieces of 16 bytes
 __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
-    constexpr int E = tiles::piece<T>(), D = tiles::depth<T>(), AHEAD = !WHOLE ? 1 : GROUPS == 1 ? 4 : 2;
+    constexpr int E = tiles::piece<T>(), D = tiles::depth<T>(), STEP = FEW_WAVES * D, AHEAD = GROUPS == 1 ? 4 : 2;
     __shared__ f4 part[FEW_WAVES][GROUPS][2][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = blockIdx.x * 16, in = lane & 15;
     const int f = min(n0 + in, k.F - 1);
@@ -240,33 +256,38 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
     f4 g[GROUPS], u[GROUPS];
 #pragma unroll
     for (int i = 0; i < GROUPS; i++) g[i] = u[i] = f4{0.f, 0.f, 0.f, 0.f};
-    auto load = [&](const T *p, int at) -> i4 {
-        if constexpr (WHOLE) {
-            const i4 v = *reinterpret_cast<const i4 *>(p + (at < k.K ? at : 0));
-            return at < k.K ? v : i4{0, 0, 0, 0};
+    enum { PIECES, INSIDE, ELEMENTS };          // pieces that are there or not; all of them inside the rows, at any alignment; any end
+    auto load = [&](auto how, const T *p, int at) -> i4 {
+        i4 v = {0, 0, 0, 0};
+        if constexpr (decltype(how)::value == PIECES) {
+            const i4 there = *reinterpret_cast<const i4 *>(p + (at < k.K ? at : 0));
+            if (at < k.K) v = there;
+        } else if constexpr (decltype(how)::value == INSIDE) {
+            __builtin_memcpy(&v, p + at, 16);
         } else {
             T e[E];
 #pragma unroll
             for (int q = 0; q < E; q++) e[q] = at + q < k.K ? p[at + q] : from_float<T>(0.f);
-            i4 v;
             __builtin_memcpy(&v, e, 16);
-            return v;
         }
+        return v;
     };
-    for (int t = wave * D; t < k.K; t += FEW_WAVES * D * AHEAD) {
-        i4 a[AHEAD][2], b[AHEAD][2], y[AHEAD][2][GROUPS];
+    // `N` of the wavefront's tiles of k from t on
+    auto tiles_at = [&](auto how, auto many, int t) {
+        constexpr int N = decltype(many)::value;
+        i4 a[N][2], b[N][2], y[N][2][GROUPS];
 #pragma unroll
-        for (int q = 0; q < AHEAD; q++)
+        for (int q = 0; q < N; q++)
 #pragma unroll
             for (int s = 0; s < 2; s++) {
-                const int at = t + q * FEW_WAVES * D + ((lane >> 4) + 4 * s) * E;
-                a[q][s] = load(wg, at);
-                b[q][s] = load(wu, at);
+                const int at = t + q * STEP + ((lane >> 4) + 4 * s) * E;
+                a[q][s] = load(how, wg, at);
+                b[q][s] = load(how, wu, at);
 #pragma unroll
-                for (int i = 0; i < GROUPS; i++) y[q][s][i] = load(x[i], at);
+                for (int i = 0; i < GROUPS; i++) y[q][s][i] = load(how, x[i], at);
             }
 #pragma unroll
-        for (int q = 0; q < AHEAD; q++)
+        for (int q = 0; q < N; q++)
 #pragma unroll
             for (int s = 0; s < 2; s++)
 #pragma unroll
@@ -274,6 +295,16 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
                     g[i] = tiles::mma<T>(a[q][s], y[q][s][i], g[i]);
                     u[i] = tiles::mma<T>(b[q][s], y[q][s][i], u[i]);
                 }
+    };
+    typedef std::integral_constant<int, AHEAD> Many;
+    typedef std::integral_constant<int, 1> One;
+    int t = wave * D;
+    if (WHOLE) {
+        for (; t < k.K; t += STEP * AHEAD) tiles_at(std::integral_constant<int, PIECES>(), Many(), t);
+    } else {
+        for (; t + STEP * (AHEAD - 1) + D <= k.K; t += STEP * AHEAD) tiles_at(std::integral_constant<int, INSIDE>(), Many(), t);
+        for (; t + D <= k.K; t += STEP) tiles_at(std::integral_constant<int, INSIDE>(), One(), t);
+        if (t < k.K) tiles_at(std::integral_constant<int, ELEMENTS>(), One(), t);
     }
 #pragma unroll
     for (int i = 0; i < GROUPS; i++) {
@@ -330,19 +361,8 @@ template <class T> static double cost_of(int size, long long groups, long long s
     if (size == 128) return std::max((narrow ? 0.62 : 2.3) * n + 4, share * ((narrow ? 0.5 : 2.0) * n + 2));
     return std::max((narrow ? 0.48 : 0.8) * n + 2, share * ((narrow ? 0.2 : 0.55) * n + 0.6));
 }
-// Up to 64 rows: whether to take their kernel.  It reads the weights at what memory gives, but x again for every 16 columns; the tiles are as good from some 16 rows on
-// where there is enough of the weights (bf16, weights out of the cache, in us by it and by tiles: (4096, 14336) 1 row 46 and 55, 17 rows 61 and 55, 64 rows 107 and 56;
-// (1024, 2816) 5 and 11, 6 and 11, 9 and 13; fp32 (1024, 4096) 13 and 31, 18 and 31, 24 and 31).
-// Rows that are not whole pieces are read element by element there, and copied for the tiles ((4095, 14335) bf16 1 row 153 and 200, 64 rows 377 and 202).
-template <class T> static bool few_pays(int R, int C, int F) {
-    const double mb = 2. * F * C * sizeof(T) / 1e6, groups = tiles_of(R, 16);
-    const bool whole = C % tiles::piece<T>() == 0;
-    const double few = whole ? 0.19 * mb * (1 + 0.32 * (groups - 1)) + 3 : 0.65 * mb * (1 + 0.45 * (groups - 1)) + 3;
-    const double tiled = std::max(0.22 * mb, cost_of<T>(64, tiles_of(F, 32), (C + tiles::depth<T>() - 1) / tiles::depth<T>())) + (whole ? 0 : 0.6 * mb + 8);
-    return few < tiled;
-}
 // How a product is shared out: the tiles' size, and k cut into shares where the tiles do not fill the compute units, their sums joined by another launch
-struct Plan { int size, rows, columns, shares, per; };
+struct Plan { int size, rows, columns, shares, per; double cost; };
 template <class T> static Plan plan_of(long long M, long long N, long long K, bool cut) {
     Plan best = {};
     const long long steps = (K + tiles::depth<T>() - 1) / tiles::depth<T>();
@@ -351,17 +371,41 @@ template <class T> static Plan plan_of(long long M, long long N, long long K, bo
         for (long long shares = 1; shares <= (cut && size < 256 ? 16 : 1) && steps >= 4 * shares - 3; shares *= 2) {
             const long long rows = tiles_of(M, size), columns = tiles_of(N, size), each = (steps + shares - 1) / shares, all = (steps + each - 1) / each;
             const double cost = cost_of<T>(size, rows * columns * all, each) + (all > 1 ? 5 + (double)(all * M * N) * 8 / 4e6 : 0);
-            if (cost < least) least = cost, best = {size, (int)rows, (int)columns, (int)all, (int)(each * tiles::depth<T>())};
+            if (cost < least) least = cost, best = {size, (int)rows, (int)columns, (int)all, (int)(each * tiles::depth<T>()), cost};
         }
     return best;
 }
+// Up to 64 rows: whether to take their kernel.  It reads the weights at what memory gives and waits for nothing, but reads x again for every 16 columns (bf16, weights out of
+// the cache, in us by it and by tiles: (4096, 14336) 1 row 55 and 51, 16 rows 67 and 53, 64 rows 104 and 58; (1002, 2731) 6 and 9, 6 and 10, 9 and 11; fp32
+// (1001, 2731) 8 and 27, 9 and 27, 17 and 28; (4095, 14335) 122 and 174, 151 and 163, 258 and 174).  Rows that begin between 4 bytes cost it twice a row's loads: (4095, 14335) bf16
+// 105 and 54, 149 and 64, 293 and 83, rows that begin at 4 ((4094, 14335)) 64 and 60, 83 and 67, 147 and 84.
+template <class T> static bool few_pays(int R, int C, int F) {
+    if (R > FEW) return false;
+    const double mb = 2. * F * C * sizeof(T) / 1e6, groups = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+    const bool narrow = sizeof(T) == 2, whole = C % tiles::piece<T>() == 0;
+    const double few = 3 + mb * (!narrow ? 0.15 + 0.14 * groups : whole ? 0.22 + 0.0033 * R : C % 2 == 0 ? 0.26 + 0.0055 * R : 0.5 + 0.015 * R);
+    const double tiled = std::max((narrow ? 0.22 : 0.33) * mb, cost_of<T>(64, tiles_of(F, 32), (C + tiles::depth<T>() - 1) / tiles::depth<T>()));
+    return few < (narrow && !whole ? 1.2 : 1.) * tiled;
+}
+// Rows that are not whole pieces of 16 bytes: read as they lie (pieces that lie across lines take the memory pipe longer, by a third of the whole call's time with 16-bit elements,
+// next to nothing with fp32), or copied to rows that are, by another launch.  In us so and copied, bf16: (4095, 14335) 64 rows 83 and 158, 777 rows 267 and 317; (1001, 2731) 128 rows 11 and 18,
+// 777 rows 33 and 30, 4096 rows 92 and 70; (2050, 5001) 1500 rows 77 and 85, 4096 rows 217 and 205; fp32 (1001, 2731) 300 rows 48 and 57, 4096 rows 406 and 404.
+struct Choice { bool few, lie, copy; Plan plan; };
+template <class T> static Choice choose(int R, int C, int F) {
+    Choice c = {few_pays<T>(R, C, F), false, false, plan_of<T>(R, 2ll * F, C, false)};          // (a tile's columns are half gate, half up)
+    if (!c.few && C % tiles::piece<T>()) {
+        c.lie = (sizeof(T) == 2 ? 0.3 : 0.04) * c.plan.cost < 3 + ((double)R + 2. * F) * C * 2 * sizeof(T) / 5e6;
+        c.copy = !c.lie;
+    }
+    return c;
+}
 template <class T> static size_t forward_scratch(int R, int C, int F) {
-    if (C % tiles::piece<T>() == 0) return 0;
-    return ((size_t)R + 2 * (size_t)F) * rounded(C) * sizeof(T);
+    return choose<T>(R, C, F).copy ? ((size_t)R + 2 * (size_t)F) * rounded(C) * sizeof(T) : 0;
 }
 template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *scratch) {
-    const bool whole = k.K % tiles::piece<T>() == 0;
-    if (k.R <= FEW && few_pays<T>(k.R, k.K, k.F)) {
+    const Choice c = choose<T>(k.R, k.K, k.F);
+    if (c.few) {
+        const bool whole = k.K % tiles::piece<T>() == 0;
         const dim3 grid(tiles_of(k.F, 16));
         const int groups = tiles_of(k.R, 16);
 #define WKV_FEW(G)                                                                                             \
@@ -375,7 +419,7 @@ template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *s
 #undef WKV_FEW
         return hipGetLastError();
     }
-    if (!whole) {
+    if (c.copy) {
         Layout l(k.K);
         const int Cs = l.k.Cs;
         T *to = static_cast<T *>(scratch);
@@ -387,14 +431,19 @@ template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *s
         k.x = x; k.wg = wg; k.wu = wu;
         k.xs = k.ws = k.K = Cs;
     }
-    // (a tile's columns are half gate, half up)
-    const Plan p = plan_of<T>(k.R, 2ll * k.F, k.K, false);
+    const Plan &p = c.plan;
     const int rows = p.rows, columns = tiles_of(k.F, p.size / 2);
     const dim3 grid(rows * columns);
-    if (p.size == 256) hipLaunchKernelGGL((forward<T, 256, 256, 2, 4, 2>), grid, dim3(512), 0, s, k, rows, columns);
-    else if (p.size == 128) hipLaunchKernelGGL((forward<T, 128, 128, 2, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
-    else if (deep_pays(rows * columns)) hipLaunchKernelGGL((forward<T, 64, 64, 2, 2, DEEP>), grid, dim3(256), 0, s, k, rows, columns);
-    else hipLaunchKernelGGL((forward<T, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, k, rows, columns);
+#define WKV_FORWARD(SIZE, WN, AHEAD, WAVES)                                                                                                     \
+    do {                                                                                                                                        \
+        if (c.lie) hipLaunchKernelGGL((forward<T, SIZE, SIZE, 2, WN, AHEAD, true>), grid, dim3(64 * WAVES), 0, s, k, rows, columns);              \
+        else hipLaunchKernelGGL((forward<T, SIZE, SIZE, 2, WN, AHEAD, false>), grid, dim3(64 * WAVES), 0, s, k, rows, columns);                 \
+    } while (0)
+    if (p.size == 256) WKV_FORWARD(256, 4, 2, 8);
+    else if (p.size == 128) WKV_FORWARD(128, 2, 2, 4);
+    else if (deep_pays(rows * columns)) WKV_FORWARD(64, 2, DEEP, 4);
+    else WKV_FORWARD(64, 2, 2, 4);
+#undef WKV_FORWARD
     return hipGetLastError();
 }
 

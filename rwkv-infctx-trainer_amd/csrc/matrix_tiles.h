@@ -33,7 +33,8 @@ template <> __device__ __forceinline__ f4 mma<float>(i4 a, i4 b, f4 c) {
     return c;
 }
 
-// 16 bytes per lane from memory to LDS, the lanes' side by side from `lds` on; nothing waits for them here.  What lies outside the range comes as zeros.
+// 16 bytes per lane from memory to LDS, the lanes' side by side from `lds` on; nothing waits for them here.  What lies outside the range comes as zeros; the memory's
+// addresses may be of any alignment (of every even one checked on the hardware), LDS' are whole pieces.
 __device__ __forceinline__ void to_lds(i4 range, unsigned offset, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(range) : "memory");
 }
@@ -69,6 +70,18 @@ template <class T, int ROWS, int THREADS> struct Along {
     }
     __device__ __forceinline__ void fetch(int j, unsigned lds) const {
         to_lds(range, there ? at[j] : NOWHERE, lds + j * (THREADS * 16) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024);
+    }
+    // the same by way of registers, of a tile of k that ends at any element: zeros from `end` on
+    __device__ __forceinline__ void carry(const T *base, long long ld, int live, int k, int end, char *lds) const {
+#pragma unroll
+        for (int j = 0; j < ROUNDS; j++) {
+            const int row = (threadIdx.x >> 3) + j * (THREADS / 8);
+            const T *from = base + row * ld + k + column;
+            T e[piece<T>()];
+#pragma unroll
+            for (int q = 0; q < piece<T>(); q++) e[q] = row < live && k + column + q < end ? from[q] : from_float<T>(0.f);
+            __builtin_memcpy(lds + j * (THREADS * 16) + threadIdx.x * 16, e, 16);
+        }
     }
     // the operands of sixteen rows: `first` the lane's, the same for every sixteen; half: of the tile of k
     struct Reader {
@@ -159,7 +172,7 @@ __device__ __forceinline__ void tile_of(int index, int rows, int columns, int &r
     column = in / high;
 }
 
-// The loop over k of a workgroup of WM x WN wavefronts: acc[i][j] is the sum of 16 rows of A and 16 of B, a lane's element e the one of A's row
+// The loop over k of a workgroup of WM x WN wavefronts, on top of what acc holds: acc[i][j] is the sum of 16 rows of A and 16 of B, a lane's element e the one of A's row
 // (lane & 15) and B's row 4 (lane >> 4) + e.  B's rows come in PARTS parts of BN / PARTS rows; a wavefront takes its share of each.  LDS holds AHEAD + 1
 // of A's tiles and AHEAD of B's.
 template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS, int AHEAD> struct Loop {
@@ -202,6 +215,27 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS, 
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = mma<T>(h.y[j], h.x[i], acc[i][j]);
     }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < MT; i++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // a tile of k that lies in LDS, where the first of A's and of B's go
+    __device__ __forceinline__ void once(char *lds) {
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
+        const typename A::Reader ra;
+        const typename B::Reader rb;
+        __syncthreads();
+#pragma unroll
+        for (int half = 0; half < 2; half++) {
+            Half h;
+            read(ra, rb, lds, lds + (AHEAD + 1) * ABYTES, wm, wn, half, 0, 1, h);
+#pragma unroll
+            for (int i = 0; i < MT; i++) multiply(h, i);
+        }
+        __syncthreads();
+    }
     // k from k0 (whole tiles) to k1.  Half a tile's operands are multiplied while the next half's are on their way from LDS; the one barrier of a tile stands
     // between its halves, where every wavefront has read all of the tile and the next has come, so that there is work in registers on both sides of it.  A's tile
     // AHEAD from this one is asked for in a tile's first half, B's in the second, in the place of this one's.  Reads and loads are issued between the
@@ -210,10 +244,6 @@ template <class T, class A, class B, int BM, int BN, int WM, int WN, int PARTS, 
         constexpr int D = depth<T>();
         const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / WN, wn = wave % WN;
         const unsigned base = (unsigned)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char *)lds);
-#pragma unroll
-        for (int i = 0; i < MT; i++)
-#pragma unroll
-            for (int j = 0; j < NT; j++) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
         const typename A::Reader ra;
         const typename B::Reader rb;
         Half first, second;

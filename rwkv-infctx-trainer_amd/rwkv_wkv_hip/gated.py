@@ -41,8 +41,8 @@ def gated_feed_forward(x, w_gate, w_up, activation="silu"):
     """x (..., C), w_gate and w_up (F, C) as torch.nn.Linear keeps them -> act(x w_gate') * (x w_up') (..., F), act "silu", "gelu" (its tanh
     form) or "relu".  All of one type; sums in fp32, the result rounded once.  The second projection stays the caller's matrix product.
 
-    A recorded call keeps both projections' results in fp32 (2 F numbers per row) for its backward, which takes a workspace of 4 F + C elements per row and
-    2 F C for the weights laid out the other way."""
+    A recorded call keeps both projections' results in fp32 (2 F numbers per row) for its backward, whose workspace is their slopes, 2 F elements of x's type per row,
+    and the sums of a small product's shares.  Where C is not whole pieces of 16 bytes x and the weights are copied, in both directions."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
     return _call("gated_product", x, w_gate, w_up, ACTIVATIONS[activation])

@@ -50,8 +50,11 @@ def test_feed_forward(L):  # noqa: F811
     assert forward(h=ODD) == -4 and forward(x=at((1 << 40) + 2)) == -4 and forward(stride=66) == -4 and forward(w=ODD) == -4
     # rows that are not whole pieces of 16 bytes begin anywhere, but at an element
     assert forward(C=63, x=at((1 << 40) + 2), stride=65) == -6 and forward(C=63, x=at((1 << 40) + 1), stride=65) == -4
-    need = L.wkv_gated_product_forward_workspace(100, 63, 48, 1)
-    assert need > 0 and forward(C=63, size=need - 1) == -5 and forward(C=63, ws=NULL) == -2
+    # many rows that are not whole pieces are copied to such that are
+    big = dict(R=20000, C=1001, F=2731, stride=1001)
+    need = L.wkv_gated_product_forward_workspace(20000, 1001, 2731, 1)
+    assert need == (20000 + 2 * 2731) * 1024 * 2 and forward(**big, size=need - 1) == -5 and forward(**big, ws=NULL) == -2 and forward(**big) == -6
+    assert L.wkv_gated_product_forward_workspace(20000, 1000, 2731, 1) == 0 and L.wkv_gated_product_forward_workspace(100, 63, 48, 1) == 0
     assert L.wkv_gated_product_kept_bytes(3, 64, 50, 1) == 3 * 2 * 64 * 4 and L.wkv_gated_product_kept_bytes(3, 64, 0, 1) == 0
 
     size_of = L.wkv_gated_product_backward_workspace

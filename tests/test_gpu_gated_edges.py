@@ -162,7 +162,14 @@ def test_gradients_against_differences():
 
 # ---- the gated feed-forward
 @pytest.mark.parametrize("dtype,R,C,F", [(torch.bfloat16, 1500, 520, 4608), (torch.float16, 1100, 1024, 2816), (torch.bfloat16, 2048, 264, 8192), (torch.float32, 600, 520, 1500),
-                                         (torch.bfloat16, 40, 2048, 5000), (torch.bfloat16, 17, 2056, 4100), (torch.float32, 64, 512, 2000), (torch.bfloat16, 60, 1999, 700)])
+                                         (torch.bfloat16, 40, 2048, 5000), (torch.bfloat16, 17, 2056, 4100), (torch.float32, 64, 512, 2000), (torch.bfloat16, 60, 1999, 700),
+                                         # rows that are not whole pieces of 16 bytes, as they lie and copied, by tiles of 64, 128 and 256
+                                         (torch.bfloat16, 300, 1001, 2731), (torch.float16, 1024, 99, 2731), (torch.bfloat16, 400, 519, 14335), (torch.bfloat16, 100, 1999, 300),
+                                         (torch.float16, 6000, 99, 1500), (torch.bfloat16, 16000, 261, 1500), (torch.float32, 100, 99, 300), (torch.float32, 8192, 99, 300),
+                                         (torch.float32, 4096, 99, 8200), (torch.float32, 16000, 519, 1500), (torch.float16, 130, 1002, 700), (torch.bfloat16, 33, 4094, 3000),
+                                         # single rows and few, by every alignment of rows
+                                         (torch.bfloat16, 1, 4096, 5000), (torch.bfloat16, 3, 1002, 500), (torch.float16, 20, 1001, 500), (torch.bfloat16, 40, 1006, 300), (torch.float32, 9, 1001, 500),
+                                         (torch.float32, 30, 1002, 500), (torch.float32, 64, 1004, 500), (torch.float16, 1, 9, 1), (torch.float32, 2, 3, 5)])
 def test_feed_forward_by_every_size_of_tile(dtype, R, C, F):
     S.feed_forward(dtype, R, C, F, "silu")
 
@@ -182,6 +189,26 @@ def test_feed_forward_reads_rows_as_they_lie():
                 return [out, *torch.autograd.grad(out, leaf, gy[:len(out)])]
             for p, q in zip(run(x, a, b), run(x.contiguous(), a.contiguous(), b.contiguous())):
                 assert torch.equal(p, q)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("R,C,F", [(1, 99, 40), (12, 99, 40), (40, 90, 40), (200, 99, 40), (200, 35, 40), (5000, 99, 1500)])
+def test_feed_forward_reads_nothing_beside_its_rows(dtype, R, C, F):
+    """x's rows between NaNs, weights behind and before NaNs: what their copies give."""
+    K = _kernels()
+    g = S._g(R, C)
+    for shift in range(0, 9, 1 if R < 300 else 4):
+        wide = torch.full((R, C + 13), math.nan, dtype=dtype, device="cuda")
+        x = wide[:, shift:shift + C]
+        x.copy_(torch.randn(R, C, generator=g))
+        flat = torch.full((F * C + 2 * 8,), math.nan, dtype=dtype, device="cuda")
+        w = flat[8:8 + F * C].view(F, C)
+        w.copy_(torch.randn(F, C, generator=g) / 10)
+        leaf, copies = [x.detach().requires_grad_(True), w.detach().requires_grad_(True)], [t.clone().requires_grad_(True) for t in (x, w)]
+        a, b = K.gated_feed_forward(leaf[0], leaf[1], leaf[1]), K.gated_feed_forward(copies[0], copies[1], copies[1])
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+        for p, q in zip(torch.autograd.grad(a, leaf, torch.ones_like(a)), torch.autograd.grad(b, copies, torch.ones_like(b))):
+            assert torch.isfinite(p).all() and torch.equal(p, q)
 
 
 @pytest.mark.parametrize("dtype", TYPES)
