@@ -6,7 +6,7 @@
 // R C F 4 operations forward and 8 backward, on the matrix cores (matrix_tiles.h).  Forward, a workgroup's tile of B is half of gate rows and
 // half of the same up rows, so that a lane ends with g and u of the same places and the activation and product happen in registers: g and u
 // never reach memory, except that a backward's are kept in fp32: rounded to 16 bits they would add as much to the gradients' error as each of the two
-// roundings that cannot be left out, that of dg and du, which the matrix cores take in the streams' type, and that of the results (bf16, error of
+// roundings that are left, that of dg and du, which the matrix cores take in the streams' type, and that of the results (bf16, error of
 // the 2-norm: 3.1e-3 against 2.4e-3).  Backward, one pass makes dg and du; the three products read
 // them, x and the weights as they lie, with the index that is summed along memory or across it (gx: along dg and du, across the weights; gWg and gWu: across both).
 #include <type_traits>
@@ -128,13 +128,14 @@ struct Product {
     int M, N, K;
     const void *a, *b, *b2;           // b2: B's rows of k from `turn` on, where k is across
     long long as, bs;
-    int turn, rows;                   // rows of k that are there, where k is across
+    int turn, a_rows, b_rows;         // rows of k that are there, where k is across
     // out: rows below `split` (of which `live` are there) to out0, those from it on to out1; parts: fp32 sums over a share of k instead
     void *out0, *out1;
     long long os;
     int split, live;
     float *parts;
     int per;                          // of k to a share
+    bool pairs;                       // every two rows of A are one number in two parts: rows of the result where they lie along memory, of k where across
 };
 
 // ACROSS_A, ACROSS_B: k lies across memory in that operand
@@ -150,34 +151,39 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void produ
     L l;
     const T *a = static_cast<const T *>(k.a), *b = static_cast<const T *>(k.b), *b2 = static_cast<const T *>(k.b2);
     constexpr int E = tiles::piece<T>();          // (rows are whole pieces, what they hold may not be)
-    if constexpr (ACROSS_A) l.a.place(a, a, 0x7fffffff, k.as, m0, k.rows, (k.M + E - 1) / E * E);
+    if constexpr (ACROSS_A) l.a.place(a, a, 0x7fffffff, k.as, m0, k.a_rows, (k.M + E - 1) / E * E);
     else l.a.place(a + m0 * k.as, k.as, k.K, min(BM, k.M - m0));
-    if constexpr (ACROSS_B) l.b[0].place(b, b2, k.turn, k.bs, n0, k.rows, (k.N + E - 1) / E * E);
+    if constexpr (ACROSS_B) l.b[0].place(b, b2, k.turn, k.bs, n0, k.b_rows, (k.N + E - 1) / E * E, ACROSS_A && k.pairs);
     else l.b[0].place(b + n0 * k.bs, k.bs, k.K, min(BN, k.N - n0));
     const int k0 = blockIdx.y * k.per;
     l.clear();
     l.run(k0, min(k0 + k.per, k.K), k.K, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-    const bool whole = k.os % 4 == 0;
+    const bool whole = k.os % 4 == 0, pairs = !ACROSS_A && k.pairs;
+    const int M = pairs ? k.M / 2 : k.M;
 #pragma unroll
     for (int i = 0; i < L::MT; i++) {
-        const int m = m0 + (wm * L::MT + i) * 16 + (lane & 15);
-        const int r = m < k.split ? m : m - k.split;
-        if (m >= k.M || r >= k.live) continue;
+        const int in = m0 + (wm * L::MT + i) * 16 + (lane & 15), m = pairs ? in >> 1 : in, r = m < k.split ? m : m - k.split;
+        if (pairs)
+#pragma unroll
+            for (int j = 0; j < L::NT; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) l.acc[i][j][e] += __shfl_xor(l.acc[i][j][e], 1);
+        if (m >= M || r >= k.live || (pairs && in & 1)) continue;
 #pragma unroll
         for (int j = 0; j < L::NT; j++) {
             const int n = n0 + (wn * L::NT + j) * 16 + 4 * (lane >> 4);
             float o[4];
 #pragma unroll
             for (int e = 0; e < 4; e++) o[e] = l.acc[i][j][e];
-            if (k.parts) put4(k.parts + ((size_t)blockIdx.y * k.M + m) * k.os, n, k.N, whole, o);
+            if (k.parts) put4(k.parts + ((size_t)blockIdx.y * M + m) * k.os, n, k.N, whole, o);
             else put4(static_cast<T *>(m < k.split ? k.out0 : k.out1) + r * k.os, n, k.N, whole, o);
         }
     }
 }
 // the shares' sums, in their order
-template <class T> __global__ __launch_bounds__(256) void join(const Product k, int shares) {
-    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)k.M * k.os;
+template <class T> __global__ __launch_bounds__(256) void join(const Product k, int M, int shares) {
+    const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x, n = (size_t)M * k.os;
     if (i >= n) return;
     float s = k.parts[i];
     for (int p = 1; p < shares; p++) s += k.parts[p * n + i];
@@ -212,8 +218,8 @@ template <class T> __global__ __launch_bounds__(256) void widen(const Widen k) {
     }
     *reinterpret_cast<uint4 *>(static_cast<T *>(k.array[j].out) + i) = raw;
 }
-// dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y
-template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, long long Fs) {
+// dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y.  pairs: (2 R, 2 Fs), what a row's rounding leaves in the row behind it
+template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, long long Fs, bool pairs) {
     constexpr int V = 4;
     const int f = (blockIdx.x * 256 + threadIdx.x) * V;
     if (f >= Fs) return;
@@ -235,8 +241,17 @@ template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int
             dg[e] = f + e < F ? o[e] * u[e] * slope : 0.f;
             du[e] = f + e < F ? o[e] * value : 0.f;
         }
-        store4(d + r * 2 * Fs + f, dg);
-        store4(d + r * 2 * Fs + Fs + f, du);
+        T *to = d + (long long)r * (pairs ? 4 : 2) * Fs + f;
+        store4(to, dg);
+        store4(to + Fs, du);
+        if (!pairs) continue;
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            dg[e] -= to_float(from_float<T>(dg[e]));
+            du[e] -= to_float(from_float<T>(du[e]));
+        }
+        store4(to + 2 * Fs, dg);
+        store4(to + 3 * Fs, du);
     }
 }
 
@@ -454,23 +469,29 @@ struct Backward {
     long long xs, ws;
     void *gx, *gwg, *gwu;             // gx, or gwg and gwu, may be NULL: not wanted
 };
+// Whether the slopes go into the products in two parts, rounded and what that leaves.  With few rows nothing averages their rounding (2 or 3 rows in bf16: results up to half as far again
+// off the 64-bit ones as their own rounding makes them; in two parts that alone is left), and while the parts' rows fill no more than a tile the weights, which bound such calls, pay
+// for them ((16, 2560) into 8960 columns gx 31.5 -> 34.4 us, weights' gradients 36.2 -> 36.8; (64, 2560) would be 41 -> 50, 38 -> 42).
+constexpr int PAIRED = 32;
+template <class T> constexpr bool in_pairs(int R) { return sizeof(T) == 2 && R <= PAIRED; }
 struct Regions { size_t d, x, wg, wu, parts, all; };
 template <class T> static Regions regions(int R, int C, int F, bool want_x, bool want_w) {
-    const size_t Fs = rounded(F), Rs = rounded(R), Cs = C % tiles::piece<T>() ? rounded(C) : 0;
+    const size_t Fs = rounded(F), Cs = C % tiles::piece<T>() ? rounded(C) : 0;
     Regions r;
     size_t at = 0;
     auto take = [&](size_t n) { const size_t was = at; at += (n + 255) / 256 * 256; return was; };
-    r.d = take((size_t)R * 2 * Fs * sizeof(T));
+    const int pairs = in_pairs<T>(R) ? 2 : 1;
+    r.d = take((size_t)pairs * R * 2 * Fs * sizeof(T));
     r.x = take(want_w ? (size_t)R * Cs * sizeof(T) : 0);
     r.wg = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
     r.wu = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
     size_t parts = 0;
     if (want_x) {
-        const Plan p = plan_of<T>(R, C, 2 * Fs, true);
+        const Plan p = plan_of<T>(pairs * R, C, 2 * Fs, true);
         if (p.shares > 1) parts = std::max(parts, (size_t)p.shares * R * C * 4);
     }
     if (want_w) {
-        const Plan p = plan_of<T>(2 * Fs, C, Rs, true);
+        const Plan p = plan_of<T>(2 * Fs, C, rounded(pairs * R), true);
         if (p.shares > 1) parts = std::max(parts, (size_t)p.shares * 2 * Fs * C * 4);
     }
     r.parts = take(parts);
@@ -485,10 +506,12 @@ template <class T, bool ACROSS_A> static void product_launch(hipStream_t s, Prod
     else if (p.size == 128) hipLaunchKernelGGL((product<T, 128, 128, 2, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
     else if (deep_pays((long long)p.rows * p.columns * p.shares)) hipLaunchKernelGGL((product<T, 64, 64, 2, 2, DEEP, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
     else hipLaunchKernelGGL((product<T, 64, 64, 2, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
-    if (p.shares > 1) hipLaunchKernelGGL(join<T>, dim3((unsigned)(((size_t)k.M * k.os + 255) / 256)), dim3(256), 0, s, k, p.shares);
+    const int M = !ACROSS_A && k.pairs ? k.M / 2 : k.M;
+    if (p.shares > 1) hipLaunchKernelGGL(join<T>, dim3((unsigned)(((size_t)M * k.os + 255) / 256)), dim3(256), 0, s, k, M, p.shares);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k, void *scratch) {
-    const int Fs = (int)rounded(k.F), Rs = (int)rounded(k.R);
+    const int Fs = (int)rounded(k.F), R2 = in_pairs<T>(k.R) ? 2 * k.R : k.R;
+    const bool pairs = R2 != k.R;
     const bool want_x = k.gx, want_w = k.gwg;
     const Regions r = regions<T>(k.R, k.C, k.F, want_x, want_w);
     char *ws = static_cast<char *>(scratch);
@@ -507,22 +530,22 @@ template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k
     }
     float *parts = reinterpret_cast<float *>(ws + r.parts);
     const dim3 grid(tiles_of(Fs, 1024), std::min(k.R, 32768));
-    if (k.F % 4 == 0) hipLaunchKernelGGL((slopes<T, true>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs);
-    else hipLaunchKernelGGL((slopes<T, false>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs);
+    if (k.F % 4 == 0) hipLaunchKernelGGL((slopes<T, true>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs, pairs);
+    else hipLaunchKernelGGL((slopes<T, false>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs, pairs);
     if (want_x) {
         Product p = {};
-        p.M = k.R; p.N = k.C; p.K = 2 * Fs;
+        p.M = R2; p.N = k.C; p.K = 2 * Fs; p.pairs = pairs;
         p.a = d; p.as = 2 * Fs;
-        p.b = wg; p.b2 = wu; p.bs = ld; p.turn = Fs; p.rows = k.F;
+        p.b = wg; p.b2 = wu; p.bs = ld; p.turn = Fs; p.b_rows = k.F;
         p.out0 = p.out1 = k.gx; p.os = k.C; p.split = p.live = k.R;
         p.parts = parts;
         product_launch<T, false>(s, p, plan_of<T>(p.M, p.N, p.K, true));
     }
     if (want_w) {
         Product p = {};
-        p.M = 2 * Fs; p.N = k.C; p.K = Rs;
+        p.M = 2 * Fs; p.N = k.C; p.K = (int)rounded(R2); p.pairs = pairs;
         p.a = d; p.as = 2 * Fs;
-        p.b = p.b2 = x; p.bs = xs; p.turn = 0x7fffffff; p.rows = k.R;
+        p.b = p.b2 = x; p.bs = xs; p.turn = 0x7fffffff; p.a_rows = R2; p.b_rows = k.R;
         p.out0 = k.gwg; p.out1 = k.gwu; p.os = k.C; p.split = Fs; p.live = k.F;
         p.parts = parts;
         product_launch<T, true>(s, p, plan_of<T>(p.M, p.N, p.K, true));

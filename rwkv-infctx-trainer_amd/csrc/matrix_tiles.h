@@ -103,6 +103,7 @@ template <class T, int ROWS, int THREADS> struct Across {
     const char *p, *second;           // rows of k from `turn` on: second's, from its first
     long long bytes, ld;              // from p to the end
     int turn;
+    int shift;                        // 1: every row is taken for two of k
     unsigned at[ROUNDS];
     // of the pieces' numbers in row k: an instruction takes two pieces (fp32: four) of each of rows 8 g .. 8 g + 3 (fp32: of rows 4 g)
     static __device__ __forceinline__ int exchange(int k) {
@@ -110,20 +111,22 @@ template <class T, int ROWS, int THREADS> struct Across {
         return (PIECES >= 16 ? (k & 3) | (k >> 1 & 4) : (k >> 1 & 1) | (k >> 2 & 2)) << 1;
     }
     // column n0 of rows that are there up to `rows`, `width` elements wide
-    __device__ __forceinline__ void place(const T *base, const T *base2, int turn_, long long ld_, int n0, int rows, int width) {
+    __device__ __forceinline__ void place(const T *base, const T *base2, int turn_, long long ld_, int n0, int rows, int width, int shift_ = 0) {
         p = reinterpret_cast<const char *>(base + n0);
         second = reinterpret_cast<const char *>(base2 + n0);
         turn = turn_;
+        shift = shift_;
         ld = ld_ * (long long)sizeof(T);
         bytes = (long long)(rows - 1) * ld + (long long)(width - n0) * (long long)sizeof(T);
 #pragma unroll
         for (int j = 0; j < ROUNDS; j++) {
             const int k = threadIdx.x / PIECES + j * PER, c = (threadIdx.x % PIECES) ^ exchange(k);
-            at[j] = (unsigned)(k * ld) + c * 16;
+            at[j] = (unsigned)((k >> shift) * ld) + c * 16;
         }
     }
     i4 range;
     __device__ __forceinline__ void ask(int k, int) {
+        k >>= shift;
         const bool behind = k >= turn;
         const long long skip = (long long)(behind ? k - turn : k) * ld;
         range = range_of((behind ? second : p) + skip, bytes - skip);

@@ -248,6 +248,22 @@ def test_activations_far_out(name):
         assert torch.isfinite(a).all() and bool(((a.detach().cpu().double() - b).abs() <= tol * b.abs() + 1e-30).all()), (a.flatten(), b.flatten())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R,C,F", [(1, 64, 96), (3, 68, 205), (16, 520, 300), (17, 99, 130), (32, 256, 1024), (32, 1001, 333)])
+def test_feed_forward_gradients_of_few_rows_are_rounded_once(dtype, R, C, F):
+    """Up to 32 rows: within half a step of the 64-bit value, and of what fp32 sums of up to 2048 products leave (2048 2^-24 of the products' norms, taken as of the row's largest)."""
+    K = _kernels()
+    g = S._g(R, C, F)
+    t = [torch.randn(R, C, generator=g).to(dtype), *((torch.randn(F, C, generator=g) / C ** 0.5).to(dtype) for _ in range(2))]
+    gy = torch.randn(R, F, generator=g).to(dtype)
+    a, b = [v.cuda().requires_grad_(True) for v in t], [v.double().requires_grad_(True) for v in t]
+    got = torch.autograd.grad(K.gated_feed_forward(*a), a, gy.cuda())
+    want = torch.autograd.grad(O.gated_feed_forward(*b), b, gy.double())
+    for p, q in zip(got, want):
+        off, half = (p.cpu().double() - q).abs(), torch.finfo(dtype).eps / 2
+        assert bool((off <= half * 1.001 * q.abs() + 2048 * 2.0 ** -24 * q.abs().max() + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps).all())
+
+
 def test_feed_forward_gradients_that_are_wanted():
     """Only x's, only one weight's: what the whole call gives."""
     K = _kernels()
