@@ -61,7 +61,7 @@ template <class T> __device__ __forceinline__ void put4(T *row, int n, int N, bo
 // workgroups then, or for two with four tiles ahead, which is better where there are no more than two to a compute unit: nothing else hides what their loads wait for
 // ((24, 2560) into 8192 columns bf16, weights out of the cache, 31 -> 21 us; (150, 1024) into 2816 13.0 -> 10.4; but (600, 512) into 2000 fp32 31.5 -> 35.7).
 constexpr int DEEP = 4;
-constexpr int waves_per_simd(int size, int ahead) { return ahead == DEEP ? 2 : 256 / size; }
+constexpr int waves_per_simd(int size, int ahead) { return  ahead == DEEP ? 2 : 256 / size; }
 static inline bool deep_pays(long long groups) { return groups <= 2ll * cu_count(); }
 
 // ---- forward
@@ -76,13 +76,13 @@ struct Forward {
 
 // LIE: rows are read as they lie, whole tiles of k straight to LDS and what is left behind them, if anything, before, by way of registers
 template <class T, int BM, int BN, int WM, int WN, int AHEAD, bool LIE>
-__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forward(const Forward k, int rows, int columns) {
+__global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forward(const Forward k, int rows, int columns, int width) {
     typedef tiles::Loop<T, tiles::Along<T, BM, 64 * WM * WN>, tiles::Along<T, BN / 2, 64 * WM * WN>, BM, BN, WM, WN, 2, AHEAD> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
     tiles::tile_of(blockIdx.x, rows, columns, tm, tn);
-    const int m0 = tm * BM, n0 = tn * (BN / 2);
-    const int K = LIE ? k.K / tiles::depth<T>() * tiles::depth<T>() : k.K, live = min(BM, k.R - m0), columns_live = min(BN / 2, k.F - n0);
+    const int m0 = tm * BM, n0 = tn * width, end = min(n0 + width, k.F);
+    const int K = LIE ? k.K / tiles::depth<T>() * tiles::depth<T>() : k.K, live = min(BM, k.R - m0), columns_live = end - n0;
     const T *x = static_cast<const T *>(k.x) + m0 * k.xs, *wg = static_cast<const T *>(k.wg) + n0 * k.ws, *wu = static_cast<const T *>(k.wu) + n0 * k.ws;
     L l;
     l.a.place(x, k.xs, K, live);
@@ -114,10 +114,10 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forwa
                 u[e] = l.acc[i][j + L::NT / 2][e];
                 o[e] = activation(k.kind, g[e]) * u[e];
             }
-            put4(h + m * k.hs, n, k.F, whole, o);
+            put4(h + m * k.hs, n, end, whole, o);
             if (k.kept) {
-                put4(k.kept + m * (2 * k.Fs), n, k.F, true, g);
-                put4(k.kept + m * (2 * k.Fs) + k.Fs, n, k.F, true, u);
+                put4(k.kept + m * (2 * k.Fs), n, end, true, g);
+                put4(k.kept + m * (2 * k.Fs) + k.Fs, n, end, true, u);
             }
         }
     }
@@ -406,6 +406,14 @@ template <class T> static bool few_pays(int R, int C, int F) {
 // next to nothing with fp32), or copied to rows that are, by another launch.  In us so and copied, bf16: (4095, 14335) 64 rows 83 and 158, 777 rows 267 and 317; (1001, 2731) 128 rows 11 and 18,
 // 777 rows 33 and 30, 4096 rows 92 and 70; (2050, 5001) 1500 rows 77 and 85, 4096 rows 217 and 205; fp32 (1001, 2731) 300 rows 48 and 57, 4096 rows 406 and 404.
 struct Choice { bool few, lie, copy; Plan plan; };
+// Columns of a tile (gate and up rows each).  One row of tiles of 64 that is more than one to a compute unit and up to one and a half leaves some with twice the work, all of it loads:
+// there every compute unit takes its share of the columns as one tile of up to 48, as wide as that (x (64, 2560) into 8960 columns bf16 34.7 -> 24.6 us, 16 rows 27.0 -> 21.3,
+// (64, 4096) into 11008 46.3 -> 41.0; but 1 row of 4096 into 14336, seven quarters to a compute unit, 45 -> 49, and (64, 2048) into 7168, less than one, 16.7 -> 19.0; fp32 is bound by
+// the matrix cores, 45 and 45 us for (64, 1024) into 8960).
+template <class T> static int width_of(const Plan &p, int F) {
+    const int cus = cu_count(), small = tiles_of(F, 32);
+    return sizeof(T) == 2 && p.size == 64 && p.rows == 1 && small > cus && 2 * small <= 3 * cus ? (tiles_of(F, cus) + 3) / 4 * 4 : p.size / 2;
+}
 template <class T> static Choice choose(int R, int C, int F) {
     Choice c = {few_pays<T>(R, C, F), false, false, plan_of<T>(R, 2ll * F, C, false)};          // (a tile's columns are half gate, half up)
     if (!c.few && C % tiles::piece<T>()) {
@@ -447,17 +455,19 @@ template <class T> static hipError_t forward_t(hipStream_t s, Forward k, void *s
         k.xs = k.ws = k.K = Cs;
     }
     const Plan &p = c.plan;
-    const int rows = p.rows, columns = tiles_of(k.F, p.size / 2);
-    const dim3 grid(rows * columns);
-#define WKV_FORWARD(SIZE, WN, AHEAD, WAVES)                                                                                                     \
-    do {                                                                                                                                        \
-        if (c.lie) hipLaunchKernelGGL((forward<T, SIZE, SIZE, 2, WN, AHEAD, true>), grid, dim3(64 * WAVES), 0, s, k, rows, columns);              \
-        else hipLaunchKernelGGL((forward<T, SIZE, SIZE, 2, WN, AHEAD, false>), grid, dim3(64 * WAVES), 0, s, k, rows, columns);                 \
+    const int width = width_of<T>(p, k.F), columns = tiles_of(k.F, width);
+    const dim3 grid(p.rows * columns);
+#define WKV_FORWARD(BM, BN, WN, AHEAD, WAVES)                                                                                                    \
+    do {                                                                                                                                         \
+        if (c.lie) hipLaunchKernelGGL((forward<T, BM, BN, 2, WN, AHEAD, true>), grid, dim3(64 * WAVES), 0, s, k, p.rows, columns, width);         \
+        else hipLaunchKernelGGL((forward<T, BM, BN, 2, WN, AHEAD, false>), grid, dim3(64 * WAVES), 0, s, k, p.rows, columns, width);              \
     } while (0)
-    if (p.size == 256) WKV_FORWARD(256, 4, 2, 8);
-    else if (p.size == 128) WKV_FORWARD(128, 2, 2, 4);
-    else if (deep_pays(rows * columns)) WKV_FORWARD(64, 2, DEEP, 4);
-    else WKV_FORWARD(64, 2, 2, 4);
+    if (p.size == 256) WKV_FORWARD(256, 256, 4, 2, 8);
+    else if (p.size == 128) WKV_FORWARD(128, 128, 2, 2, 4);
+    else if (width > 32) {
+        if constexpr (sizeof(T) == 2) WKV_FORWARD(64, 128, 2, DEEP, 4);
+    } else if (deep_pays(p.rows * columns)) WKV_FORWARD(64, 64, 2, DEEP, 4);
+    else WKV_FORWARD(64, 64, 2, 2, 4);
 #undef WKV_FORWARD
     return hipGetLastError();
 }

@@ -167,6 +167,8 @@ def test_gradients_against_differences():
                                          (torch.bfloat16, 300, 1001, 2731), (torch.float16, 1024, 99, 2731), (torch.bfloat16, 400, 519, 14335), (torch.bfloat16, 100, 1999, 300),
                                          (torch.float16, 6000, 99, 1500), (torch.bfloat16, 16000, 261, 1500), (torch.float32, 100, 99, 300), (torch.float32, 8192, 99, 300),
                                          (torch.float32, 4096, 99, 8200), (torch.float32, 16000, 519, 1500), (torch.float16, 130, 1002, 700), (torch.bfloat16, 33, 4094, 3000),
+                                         # one row of tiles whose columns are shared out evenly
+                                         (torch.bfloat16, 50, 104, 9001), (torch.float16, 64, 99, 8960), (torch.bfloat16, 17, 128, 16384), (torch.bfloat16, 64, 72, 8193), (torch.float32, 64, 72, 8961),
                                          # single rows and few, by every alignment of rows
                                          (torch.bfloat16, 1, 4096, 5000), (torch.bfloat16, 3, 1002, 500), (torch.float16, 20, 1001, 500), (torch.bfloat16, 40, 1006, 300), (torch.float32, 9, 1001, 500),
                                          (torch.float32, 30, 1002, 500), (torch.float32, 64, 1004, 500), (torch.float16, 1, 9, 1), (torch.float32, 2, 3, 5)])
