@@ -6,8 +6,10 @@
 // whole (V C, most of it zeros) from the places sorted by token: no atomics, fp32 sums in the places' order, the same bits every time.  Sorting: stable
 // passes over ten bits of the token at most, counts per tile of places, then each tile's places to where the tiles and digits before leave off; up
 // to one tile's worth in a single launch.  Sums: a workgroup takes 64 sorted places, whoever they belong to, so that it does not matter how often a token
-// comes; a token that lies within them is written as it ends, one that crosses their border leaves a part for a second launch.  The same launch
-// writes the zeros, which keeps memory busy beside the gathers' latency.
+// comes; a token that lies within them is written as it ends, one that crosses their border leaves a part for a second launch.  The zeros are written beside what waits: of one tile,
+// the whole table beside the sorting (the few rows that have a sum are written again), else the tokens' that no place has beside the sums, whose gathers wait for memory.
+#include <type_traits>
+
 #include "common.h"
 #include "vec.h"
 
@@ -43,6 +45,35 @@ template <class T, class I, int W> __global__ __launch_bounds__(256) void lookup
     }
 }
 
+// ---- zeros: groups of 256 threads, each a run of the table as one row of elements, whatever its width, 16 bytes per lane.  E: an element's bits
+constexpr int ZEROS = 8;                      // pieces per lane
+struct Zeros {
+    void *out;
+    const int *starts;                        // by token, as find_starts leaves them; NULL: the whole table
+    int V, C;
+};
+static inline size_t groups_of_zeros(int V, int C, size_t size) { return ((size_t)V * C * size + 256 * ZEROS * 16 - 1) / (256 * ZEROS * 16); }
+template <class E> __device__ __forceinline__ void put_zeros(const Zeros &k, size_t group) {
+    constexpr int W = 16 / sizeof(E);
+    const size_t first = group * (256 * ZEROS * W), v0 = first / k.C, total = (size_t)k.V * k.C;
+    const unsigned start = (unsigned)(first - v0 * k.C);
+    E *out = static_cast<E *>(k.out);
+    auto empty = [&](size_t v) { return !k.starts || k.starts[v] == k.starts[v + 1]; };
+#pragma unroll
+    for (int z = 0; z < ZEROS; z++) {
+        const unsigned in = (z * 256 + (threadIdx.x & 255)) * W, at = start + in, r = at / k.C, last = (at + W - 1) / k.C;
+        const size_t i = first + in;
+        if (i >= total) return;
+        const bool one = i + W <= total && empty(v0 + r);
+        if (one && (last == r || (last == r + 1 && empty(v0 + last)))) {
+            *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
+            continue;
+        }
+        if (i + W <= total && last == r) continue;          // (a row that has a sum)
+        for (int w = 0; w < W && i + w < total; w++)
+            if (empty(v0 + (at + w) / k.C)) out[i + w] = 0;
+    }
+}
 // ---- sorting
 constexpr int TILE = 4096, SORT_THREADS = 1024, SORT_WAVES = 16, ROUNDS = TILE / SORT_THREADS, MAX_BITS = 10, BINS = 1 << MAX_BITS;
 struct Sort {
@@ -191,10 +222,14 @@ template <class I> __global__ __launch_bounds__(SORT_THREADS) void scatter(const
             k.to_places[to] = place[j];
         }
 }
-// up to one tile: every pass in one launch
-template <class I> __global__ __launch_bounds__(SORT_THREADS) void sort_few(const Sort k, int passes) {
+// up to one tile: every pass in one workgroup, and the zeros of the whole table in those behind it
+template <class I, class E> __global__ __launch_bounds__(SORT_THREADS) void sort_few(const Sort k, int passes, const Zeros zeros) {
     __shared__ SortLds m;
     __shared__ int keys[TILE], places[TILE];
+    if (blockIdx.x > 0) {
+        put_zeros<E>(zeros, (size_t)(blockIdx.x - 1) * (SORT_THREADS / 256) + (threadIdx.x >> 8));
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mask = (1 << k.bits) - 1;
     for (int p = 0; p < passes; p++) {
         int key[ROUNDS], place[ROUNDS], digit[ROUNDS], rank[ROUNDS], total;
@@ -249,7 +284,7 @@ struct Gradient {
     int count, V, C, slices, chunks;          // slices: of the channels, one per workgroup
     long long gs;                             // gout's row stride
     float scale;
-    const int *keys, *places, *starts;
+    const int *keys, *places;
     const void *gout;
     float *parts;                             // (chunks, 2, C): sums of a chunk's first token where it began before, and of its last where it goes on behind
     void *out;
@@ -300,40 +335,25 @@ template <class T, int W> __device__ __forceinline__ void sum_chunk(const Gradie
         }
     }
 }
-// the zeros of the tokens that no place has: 16 bytes per lane of the table as one row of elements, whatever its width
-constexpr int ZEROS = 8;                      // pieces per lane
-template <class T> __device__ __forceinline__ void put_zeros(const Gradient &k, size_t block) {
-    constexpr int W = 16 / sizeof(T);
-    const size_t first = block * (256 * ZEROS * W), v0 = first / k.C, total = (size_t)k.V * k.C;
-    const unsigned start = (unsigned)(first - v0 * k.C);
-    T *out = static_cast<T *>(k.out);
-    auto empty = [&](size_t v) { return k.starts[v] == k.starts[v + 1]; };
-#pragma unroll
-    for (int z = 0; z < ZEROS; z++) {
-        const unsigned in = (z * 256 + threadIdx.x) * W, at = start + in, r = at / k.C, last = (at + W - 1) / k.C;
-        const size_t i = first + in;
-        if (i >= total) return;
-        const bool one = i + W <= total && empty(v0 + r);
-        if (one && (last == r || (last == r + 1 && empty(v0 + last)))) {
-            *reinterpret_cast<uint4 *>(out + i) = make_uint4(0, 0, 0, 0);
-            continue;
-        }
-        if (i + W <= total && last == r) continue;          // (a row that has a sum)
-        for (int w = 0; w < W && i + w < total; w++)
-            if (empty(v0 + (at + w) / k.C)) out[i + w] = from_float<T>(0.f);
-    }
-}
-template <class T, int W> __global__ __launch_bounds__(256) void sums(const Gradient k) {
+template <class T, class E, int W> __global__ __launch_bounds__(256) void sums(const Gradient k, const Zeros zeros) {
     const long long work = (long long)k.chunks * k.slices;
     if ((long long)blockIdx.x < work) sum_chunk<T, W>(k, blockIdx.x / k.slices, (int)((blockIdx.x % k.slices) * 256 + threadIdx.x) * W);
-    else put_zeros<T>(k, blockIdx.x - work);
+    else put_zeros<E>(zeros, blockIdx.x - work);
 }
 // a token that goes on behind the chunk it begins in: its sums over the chunks, in their order
 template <class T, int W> __global__ __launch_bounds__(256) void join(const Gradient k) {
     const int chunk = blockIdx.x, last = (chunk + 1) * CHUNK - 1, c = (blockIdx.y * 256 + threadIdx.x) * W;
     const int key = k.keys[last];
-    if (key == k.V || k.keys[last + 1] != key || k.starts[key] < chunk * CHUNK || c >= k.C) return;
-    const int end = (k.starts[key + 1] - 1) / CHUNK;
+    if (key == k.V || k.keys[last + 1] != key || (chunk > 0 && k.keys[chunk * CHUNK - 1] == key) || c >= k.C) return;
+    // the last chunk that begins with it: strides that double until they leave it, then halve
+    int end = chunk + 1, stride = 1;
+    auto has = [&](int j) { return j < k.chunks && k.keys[j * CHUNK] == key; };
+    while (has(end + stride)) {
+        end += stride;
+        stride *= 2;
+    }
+    for (; stride > 0; stride /= 2)
+        if (has(end + stride)) end += stride;
     float s[W];
     load_vec(k.parts + ((size_t)chunk * 2 + 1) * k.C + c, s);
     for (int j = chunk + 1; j <= end; j += AHEAD) {
@@ -375,20 +395,22 @@ template <class T, class I> static hipError_t forward_t(hipStream_t s, const Loo
     else hipLaunchKernelGGL((lookup<T, I, 1>), grid, dim3(256), 0, s, k);
     return hipGetLastError();
 }
-template <class I> static void sort(hipStream_t s, int count_, int V, const void *tokens, char *ws, const Regions &r, int &at) {
+template <class I, class E> static void sort(hipStream_t s, const Gradient &g, const void *tokens, char *ws, const Regions &r, int &at) {
     int bits = 1;
-    while ((V >> bits) != 0) bits++;          // V itself is a key
-    const int passes = (bits + MAX_BITS - 1) / MAX_BITS, tiles = tiles_of(count_);
+    while ((g.V >> bits) != 0) bits++;          // V itself is a key
+    const int passes = (bits + MAX_BITS - 1) / MAX_BITS, tiles = tiles_of(g.count);
     Sort k = {};
-    k.count = count_; k.V = V; k.tokens = tokens;
+    k.count = g.count; k.V = g.V; k.tokens = tokens;
     k.bits = (bits + passes - 1) / passes;
     k.counts = reinterpret_cast<int *>(ws + r.counts);
     auto region = [&](size_t o) { return reinterpret_cast<int *>(ws + o); };
     at = 0;
     if (tiles == 1) {
+        constexpr int GROUPS = SORT_THREADS / 256;
+        const Zeros zeros = {g.out, nullptr, g.V, g.C};
         k.to_keys = region(r.keys[0]);
         k.to_places = region(r.places[0]);
-        hipLaunchKernelGGL(sort_few<I>, dim3(1), dim3(SORT_THREADS), 0, s, k, passes);
+        hipLaunchKernelGGL((sort_few<I, E>), dim3((unsigned)(1 + (groups_of_zeros(g.V, g.C, sizeof(E)) + GROUPS - 1) / GROUPS)), dim3(SORT_THREADS), 0, s, k, passes, zeros);
         return;
     }
     for (int p = 0; p < passes; p++) {
@@ -404,27 +426,31 @@ template <class I> static void sort(hipStream_t s, int count_, int V, const void
         at = p & 1;
     }
 }
-template <class T, int W> static void sums_w(hipStream_t s, Gradient k) {
-    k.chunks = chunks_of(k.count);
+template <class T, class E, int W> static void sums_w(hipStream_t s, Gradient k, const Zeros &zeros) {
     k.slices = (k.C + 256 * W - 1) / (256 * W);
-    const size_t zeros = ((size_t)k.V * k.C + 256 * ZEROS * (16 / sizeof(T)) - 1) / (256 * ZEROS * (16 / sizeof(T)));
-    hipLaunchKernelGGL((sums<T, W>), dim3((unsigned)((size_t)k.chunks * k.slices + zeros)), dim3(256), 0, s, k);
+    const size_t groups = zeros.starts ? groups_of_zeros(k.V, k.C, sizeof(E)) : 0;
+    hipLaunchKernelGGL((sums<T, E, W>), dim3((unsigned)((size_t)k.chunks * k.slices + groups)), dim3(256), 0, s, k, zeros);
     if (k.chunks > 1) hipLaunchKernelGGL((join<T, W>), dim3(k.chunks - 1, k.slices), dim3(256), 0, s, k);
 }
 template <class T> static hipError_t backward_t(hipStream_t s, Gradient k, const void *tokens, bool wide, bool whole, void *workspace) {
     char *ws = static_cast<char *>(workspace);
     const Regions r = regions(k.count, k.V, k.C);
     int at;
-    if (wide) sort<long long>(s, k.count, k.V, tokens, ws, r, at);
-    else sort<int>(s, k.count, k.V, tokens, ws, r, at);
-    int *starts = reinterpret_cast<int *>(ws + r.starts);
+    typedef std::conditional_t<sizeof(T) == 2, unsigned short, unsigned> E;
+    if (wide) sort<long long, E>(s, k, tokens, ws, r, at);
+    else sort<int, E>(s, k, tokens, ws, r, at);
     k.keys = reinterpret_cast<int *>(ws + r.keys[at]);
     k.places = reinterpret_cast<int *>(ws + r.places[at]);
-    k.starts = starts;
     k.parts = reinterpret_cast<float *>(ws + r.parts);
-    hipLaunchKernelGGL(find_starts, dim3(k.V / 256 + 1), dim3(256), 0, s, k.keys, k.count, k.V, starts);
-    if (whole) sums_w<T, 4>(s, k);
-    else sums_w<T, 1>(s, k);
+    k.chunks = chunks_of(k.count);
+    Zeros zeros = {k.out, nullptr, k.V, k.C};
+    if (tiles_of(k.count) > 1) {
+        int *starts = reinterpret_cast<int *>(ws + r.starts);
+        hipLaunchKernelGGL(find_starts, dim3(k.V / 256 + 1), dim3(256), 0, s, k.keys, k.count, k.V, starts);
+        zeros.starts = starts;
+    }
+    if (whole) sums_w<T, E, 4>(s, k, zeros);
+    else sums_w<T, E, 1>(s, k, zeros);
     return hipGetLastError();
 }
 
