@@ -5,7 +5,7 @@
 // A token outside the table is a place without one: a row of zeros, no gradient.  Both directions are bound by memory.  The gradient is written
 // whole (V C, most of it zeros) from the places sorted by token: no atomics, fp32 sums in the places' order, the same bits every time.  Sorting: stable
 // passes over ten bits of the token at most, counts per tile of places, then each tile's places to where the tiles and digits before leave off; up
-// to one tile's worth in a single launch.  Sums: a workgroup takes 64 sorted places, whoever they belong to, so that it does not matter how often a token
+// to one tile's worth in a single launch.  Sums: a workgroup takes a chunk of up to 64 sorted places, whoever they belong to, so that it does not matter how often a token
 // comes; a token that lies within them is written as it ends, one that crosses their border leaves a part for a second launch.  The zeros are written beside what waits: of one tile,
 // the whole table beside the sorting (the few rows that have a sum are written again), else the tokens' that no place has beside the sums, whose gathers wait for memory.
 #include <type_traits>
@@ -279,9 +279,15 @@ static __global__ __launch_bounds__(256) void find_starts(const int *keys, int c
 }
 
 // ---- sums
-constexpr int CHUNK = 64, AHEAD = 8;          // places of a chunk, and of those asked for together
+constexpr int CHUNK = 64, AHEAD = 8;          // the most places of a chunk, and those asked for together
+// A chunk is worked through one place after the other, so few places are cut finer, until there are enough to fill the machine; many are better off with fewer parts to join
+// (the whole gradient of 2^9 places of 512 channels by chunks of 8, 16, 32, 64: 22, 24, 28, 37 us, 2^14 53, 53, 53, 59, 2^17 95, 86, 81, 77).
+constexpr int chunk_of(long long count, int C) {
+    count *= (C + 1023) / 1024;
+    return count <= 1 << 12 ? 8 : count <= 1 << 14 ? 16 : count <= 1 << 16 ? 32 : CHUNK;
+}
 struct Gradient {
-    int count, V, C, slices, chunks;          // slices: of the channels, one per workgroup
+    int count, V, C, slices, chunk, chunks;   // slices: of the channels, one per workgroup
     long long gs;                             // gout's row stride
     float scale;
     const int *keys, *places;
@@ -297,8 +303,8 @@ template <class T, int W> __device__ __forceinline__ void put_row(const Gradient
 // a chunk's tokens, W channels per lane
 template <class T, int W> __device__ __forceinline__ void sum_chunk(const Gradient &k, int chunk, int c) {
     __shared__ int keys[CHUNK + 2], places[CHUNK];          // keys[0], keys[n + 1]: the neighbours'
-    const int p0 = chunk * CHUNK, n = min(CHUNK, k.count - p0);
-    if (threadIdx.x < CHUNK + 2) {
+    const int p0 = chunk * k.chunk, n = min(k.chunk, k.count - p0);
+    if ((int)threadIdx.x < k.chunk + 2) {
         const int p = p0 - 1 + (int)threadIdx.x;
         keys[threadIdx.x] = p >= 0 && p < k.count ? k.keys[p] : -1;
         if (threadIdx.x < n) places[threadIdx.x] = k.places[p0 + threadIdx.x];
@@ -342,12 +348,12 @@ template <class T, class E, int W> __global__ __launch_bounds__(256) void sums(c
 }
 // a token that goes on behind the chunk it begins in: its sums over the chunks, in their order
 template <class T, int W> __global__ __launch_bounds__(256) void join(const Gradient k) {
-    const int chunk = blockIdx.x, last = (chunk + 1) * CHUNK - 1, c = (blockIdx.y * 256 + threadIdx.x) * W;
+    const int chunk = blockIdx.x, last = (chunk + 1) * k.chunk - 1, c = (blockIdx.y * 256 + threadIdx.x) * W;
     const int key = k.keys[last];
-    if (key == k.V || k.keys[last + 1] != key || (chunk > 0 && k.keys[chunk * CHUNK - 1] == key) || c >= k.C) return;
+    if (key == k.V || k.keys[last + 1] != key || (chunk > 0 && k.keys[chunk * k.chunk - 1] == key) || c >= k.C) return;
     // the last chunk that begins with it: strides that double until they leave it, then halve
     int end = chunk + 1, stride = 1;
-    auto has = [&](int j) { return j < k.chunks && k.keys[j * CHUNK] == key; };
+    auto has = [&](int j) { return j < k.chunks && k.keys[j * k.chunk] == key; };
     while (has(end + stride)) {
         end += stride;
         stride *= 2;
@@ -370,7 +376,7 @@ template <class T, int W> __global__ __launch_bounds__(256) void join(const Grad
 
 // ---- launches
 static inline int tiles_of(int count) { return (count + TILE - 1) / TILE; }
-static inline int chunks_of(int count) { return (count + CHUNK - 1) / CHUNK; }
+static inline int chunks_of(int count, int C) { return (count + chunk_of(count, C) - 1) / chunk_of(count, C); }
 struct Regions { size_t keys[2], places[2], counts, starts, parts, all; };
 static inline Regions regions(int count, int V, int C) {
     Regions r;
@@ -382,7 +388,7 @@ static inline Regions regions(int count, int V, int C) {
     }
     r.counts = take(((size_t)tiles_of(count) + 1) * BINS * 4);
     r.starts = take(((size_t)V + 1) * 4);
-    r.parts = take((size_t)chunks_of(count) * 2 * C * 4);
+    r.parts = take((size_t)chunks_of(count, C) * 2 * C * 4);
     r.all = at;
     return r;
 }
@@ -442,7 +448,8 @@ template <class T> static hipError_t backward_t(hipStream_t s, Gradient k, const
     k.keys = reinterpret_cast<int *>(ws + r.keys[at]);
     k.places = reinterpret_cast<int *>(ws + r.places[at]);
     k.parts = reinterpret_cast<float *>(ws + r.parts);
-    k.chunks = chunks_of(k.count);
+    k.chunk = chunk_of(k.count, k.C);
+    k.chunks = chunks_of(k.count, k.C);
     Zeros zeros = {k.out, nullptr, k.V, k.C};
     if (tiles_of(k.count) > 1) {
         int *starts = reinterpret_cast<int *>(ws + r.starts);
