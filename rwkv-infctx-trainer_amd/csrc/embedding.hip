@@ -75,7 +75,7 @@ template <class E> __device__ __forceinline__ void put_zeros(const Zeros &k, siz
     }
 }
 // ---- sorting
-constexpr int TILE = 4096, SORT_THREADS = 1024, SORT_WAVES = 16, ROUNDS = TILE / SORT_THREADS, MAX_BITS = 10, BINS = 1 << MAX_BITS;
+constexpr int SORT_THREADS = 1024, SORT_WAVES = 16, MAX_BITS = 10, BINS = 1 << MAX_BITS, TILE = 4 * SORT_THREADS;          // TILE: places of a large tile
 struct Sort {
     int count, V;                             // keys: tokens, V for none
     const void *tokens;                       // the first pass's keys; their places are 0, 1, ..
@@ -88,14 +88,14 @@ template <class I> __device__ __forceinline__ int key_at(const Sort &k, int n) {
     const long long t = token_at<I>(k.tokens, n);
     return t >= 0 && t < k.V ? (int)t : k.V;
 }
-template <class I> __global__ __launch_bounds__(SORT_THREADS) void count(const Sort k) {
+template <class I, int ROUNDS> __global__ __launch_bounds__(SORT_THREADS) void count(const Sort k) {
     __shared__ int bin[BINS];
     bin[threadIdx.x] = 0;
     __syncthreads();
     const int mask = (1 << k.bits) - 1;
 #pragma unroll
     for (int j = 0; j < ROUNDS; j++) {
-        const long long n = (long long)blockIdx.x * TILE + j * SORT_THREADS + threadIdx.x;
+        const long long n = (long long)blockIdx.x * (ROUNDS * SORT_THREADS) + j * SORT_THREADS + threadIdx.x;
         if (n < k.count) atomicAdd(&bin[key_at<I>(k, (int)n) >> k.shift & mask], 1);          // (whole numbers: the order is nothing)
     }
     __syncthreads();
@@ -103,7 +103,7 @@ template <class I> __global__ __launch_bounds__(SORT_THREADS) void count(const S
 }
 
 // Many tiles' counts turned into those of the tiles before, with all tiles' behind the last: 64 digits per workgroup, its wavefronts a share of the tiles each.  Few
-// tiles' are added up by every tile for itself, which saves the launch (the whole gradient of 2^17, 2^18, 2^20, 2^24 places of 8 channels, so and with
+// tiles' are added up by every tile for itself, which saves the launch (the whole gradient of 2^17, 2^18, 2^20, 2^24 places of 8 channels by 32, 64, 256, 4096 tiles, so and with
 // this launch: 66 and 68 us, 78 and 77, 187 and 159, 6991 and 1872).
 constexpr int MANY = 48;
 static __global__ __launch_bounds__(SORT_THREADS) void sum_tiles(int *counts, int tiles) {
@@ -149,9 +149,9 @@ __device__ __forceinline__ int sum_before(SortLds &m, int v) {
     for (int w = 0; w < wave; w++) before += m.wave_sum[w];
     return before + s - v;
 }
-// One tile's stable ranks by digit: keys[j] is place wave * 256 + j * 64 + lane of it, `there` of them exist.  rank[j]: the places of the same digit before it
+// One tile's stable ranks by digit: keys[j] is place (wave * ROUNDS + j) * 64 + lane of it, `there` of them exist.  rank[j]: the places of the same digit before it
 // in its wavefront; seen: those in the wavefronts before.  total: of digit threadIdx.x in the tile.
-__device__ __forceinline__ void ranks(SortLds &m, const int (&digit)[ROUNDS], const bool (&there)[ROUNDS], int bits, int (&rank)[ROUNDS], int &total) {
+template <int ROUNDS> __device__ __forceinline__ void ranks(SortLds &m, const int (&digit)[ROUNDS], const bool (&there)[ROUNDS], int bits, int (&rank)[ROUNDS], int &total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int w = 0; w < SORT_WAVES; w++) m.seen[w][threadIdx.x] = 0;
@@ -180,14 +180,14 @@ __device__ __forceinline__ void ranks(SortLds &m, const int (&digit)[ROUNDS], co
         total += n;
     }
 }
-template <class I> __global__ __launch_bounds__(SORT_THREADS) void scatter(const Sort k, int tiles) {
+template <class I, int ROUNDS> __global__ __launch_bounds__(SORT_THREADS) void scatter(const Sort k, int tiles) {
     __shared__ SortLds m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mask = (1 << k.bits) - 1;
     int key[ROUNDS], place[ROUNDS], digit[ROUNDS], rank[ROUNDS], total;
     bool there[ROUNDS];
 #pragma unroll
     for (int j = 0; j < ROUNDS; j++) {
-        const long long n = (long long)blockIdx.x * TILE + wave * (64 * ROUNDS) + j * 64 + lane;
+        const long long n = (long long)blockIdx.x * (ROUNDS * SORT_THREADS) + wave * (64 * ROUNDS) + j * 64 + lane;
         there[j] = n < k.count;
         key[j] = there[j] ? key_at<I>(k, (int)n) : 0;
         place[j] = k.tokens || !there[j] ? (int)n : k.places[n];
@@ -225,6 +225,7 @@ template <class I> __global__ __launch_bounds__(SORT_THREADS) void scatter(const
 // up to one tile: every pass in one workgroup, and the zeros of the whole table in those behind it
 template <class I, class E> __global__ __launch_bounds__(SORT_THREADS) void sort_few(const Sort k, int passes, const Zeros zeros) {
     __shared__ SortLds m;
+    constexpr int ROUNDS = TILE / SORT_THREADS;
     __shared__ int keys[TILE], places[TILE];
     if (blockIdx.x > 0) {
         put_zeros<E>(zeros, (size_t)(blockIdx.x - 1) * (SORT_THREADS / 256) + (threadIdx.x >> 8));
@@ -375,7 +376,10 @@ template <class T, int W> __global__ __launch_bounds__(256) void join(const Grad
 }
 
 // ---- launches
-static inline int tiles_of(int count) { return (count + TILE - 1) / TILE; }
+// Rounds of 1024 places to a tile: one, which is sooner done, as long as the tiles' counts are few (the gradient of 2^13, 2^15, 2^18, 2^20 places of 8 channels by one and by
+// four: 31 and 41 us, 42 and 49, 70 and 77, 179 and 162).
+static inline int rounds_of(int count) { return count <= 1 << 18 ? 1 : TILE / SORT_THREADS; }
+static inline int tiles_of(int count) { return (count + rounds_of(count) * SORT_THREADS - 1) / (rounds_of(count) * SORT_THREADS); }
 static inline int chunks_of(int count, int C) { return (count + chunk_of(count, C) - 1) / chunk_of(count, C); }
 struct Regions { size_t keys[2], places[2], counts, starts, parts, all; };
 static inline Regions regions(int count, int V, int C) {
@@ -411,7 +415,7 @@ template <class I, class E> static void sort(hipStream_t s, const Gradient &g, c
     k.counts = reinterpret_cast<int *>(ws + r.counts);
     auto region = [&](size_t o) { return reinterpret_cast<int *>(ws + o); };
     at = 0;
-    if (tiles == 1) {
+    if (g.count <= TILE) {
         constexpr int GROUPS = SORT_THREADS / 256;
         const Zeros zeros = {g.out, nullptr, g.V, g.C};
         k.to_keys = region(r.keys[0]);
@@ -423,9 +427,11 @@ template <class I, class E> static void sort(hipStream_t s, const Gradient &g, c
         k.shift = p * k.bits;
         k.to_keys = region(r.keys[p & 1]);
         k.to_places = region(r.places[p & 1]);
-        hipLaunchKernelGGL(count<I>, dim3(tiles), dim3(SORT_THREADS), 0, s, k);
+        if (rounds_of(g.count) == 1) hipLaunchKernelGGL((count<I, 1>), dim3(tiles), dim3(SORT_THREADS), 0, s, k);
+        else hipLaunchKernelGGL((count<I, TILE / SORT_THREADS>), dim3(tiles), dim3(SORT_THREADS), 0, s, k);
         if (tiles > MANY) hipLaunchKernelGGL(sum_tiles, dim3(BINS / 64), dim3(SORT_THREADS), 0, s, k.counts, tiles);
-        hipLaunchKernelGGL(scatter<I>, dim3(tiles), dim3(SORT_THREADS), 0, s, k, tiles);
+        if (rounds_of(g.count) == 1) hipLaunchKernelGGL((scatter<I, 1>), dim3(tiles), dim3(SORT_THREADS), 0, s, k, tiles);
+        else hipLaunchKernelGGL((scatter<I, TILE / SORT_THREADS>), dim3(tiles), dim3(SORT_THREADS), 0, s, k, tiles);
         k.tokens = nullptr;
         k.keys = k.to_keys;
         k.places = k.to_places;
@@ -451,7 +457,7 @@ template <class T> static hipError_t backward_t(hipStream_t s, Gradient k, const
     k.chunk = chunk_of(k.count, k.C);
     k.chunks = chunks_of(k.count, k.C);
     Zeros zeros = {k.out, nullptr, k.V, k.C};
-    if (tiles_of(k.count) > 1) {
+    if (k.count > TILE) {
         int *starts = reinterpret_cast<int *>(ws + r.starts);
         hipLaunchKernelGGL(find_starts, dim3(k.V / 256 + 1), dim3(256), 0, s, k.keys, k.count, k.V, starts);
         zeros.starts = starts;

@@ -537,11 +537,12 @@ def test_many_rows_and_sequences():
     w, gy = r(1000, 16).requires_grad_(True), r(700001, 16)
     (grad,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
     S.check_lookup(tokens, w, 1.0, gy, K.embedding(tokens, w), grad)
-    # more tiles than every tile adds up for itself, keys of two digits
-    tokens, gy = torch.randint(-3, 70000, (260000,), device="cuda", generator=g), r(260000, 4).float()
+    # around what is sorted at once, in small and large tiles, and what every tile adds up for itself; keys of two digits
     w = torch.zeros(70000, 4, device="cuda", requires_grad=True)
-    (grad,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
-    S.check_lookup(tokens, w, 1.0, gy, K.embedding(tokens, w), grad)
+    for n in (1, 4095, 4096, 4097, 48 * 1024, 48 * 1024 + 1, 1 << 18, (1 << 18) + 1):
+        tokens, gy = torch.randint(-3, 70000, (n,), device="cuda", generator=g), r(n, 4).float()
+        (grad,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
+        S.check_lookup(tokens, w, 1.0, gy, K.embedding(tokens, w), grad)
 
 
 def test_single_rows_and_places():
