@@ -3,7 +3,8 @@
 //     g = x Wg',  u = x Wu',  h = act(g) u
 //     dg = gh u act'(g),  du = gh act(g),  gx = dg Wg + du Wu,  gWg = dg' x,  gWu = du' x
 //
-// R C F 4 operations forward and 8 backward, on the matrix cores (matrix_tiles.h).  Forward, a workgroup's tile of B is half of gate rows and
+// 4 R C F operations forward and 8 backward, on the matrix cores (matrix_tiles.h): bound by these with many rows (4096 rows of 4096 into 14336 columns bf16: forward
+// 830 us, 1160 TFLOP/s; gx 700 and weights' gradients 790, 1370 and 1220; the clock that power leaves decides), by the weights' bytes with few (1 row: 43 us, 5.4 TB/s).  Forward, a workgroup's tile of B is half of gate rows and
 // half of the same up rows, so that a lane ends with g and u of the same places and the activation and product happen in registers: g and u
 // never reach memory, except that a backward's are kept in fp32: rounded to 16 bits they would add as much to the gradients' error as each of the two
 // roundings that are left, that of dg and du, which the matrix cores take in the streams' type, and that of the results (bf16, error of
@@ -256,8 +257,8 @@ template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int
 }
 
 // ---- few rows: a serving loop's single tokens.  What they cost is the weights, read once: a workgroup takes 16 gate rows and the same 16 up rows,
-// its four wavefronts every fourth tile of k; operands go straight from memory to registers, so that nothing waits for a barrier or for LDS (1 row of 4096
-// into 14336 columns bf16, weights out of the cache: 46 us, 5.1 TB/s).
+// its four wavefronts every fourth tile of k; operands go straight from memory to registers, so that nothing waits for a barrier or for LDS (1 row of 1002
+// into 2731 columns bf16, weights out of the cache: 6.0 us with the launch).
 constexpr int FEW = 64, FEW_WAVES = 4;
 template <class T, int GROUPS, bool WHOLE>                    // GROUPS of 16 rows of x; WHOLE: rows are whole pieces of 16 bytes
 __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {

@@ -7,7 +7,7 @@
 //     g[t] = go[t] + a[t+1] g[t+1],   gx = g b sigmoid(i),   gi = g b x sigmoid'(i),   l = g (a h[t-1] - a^2 / b sigmoid(i) x),
 //     gr = l log a (1 - sigmoid(r)),   gdecay = -scale sigmoid(decay) sum of l sigmoid(r),   gz = gy h silu'(z)
 //
-// Bound by memory: every stream is read once and every result written once.  The recurrence is linear, so a run of tokens is the pair (product of a, its
+// Bound by memory: every stream is read once and every result written once (B8 T4096 D4096 bf16: forward 279 us, 4.8 TB/s, backward 495, 4.9).  The recurrence is linear, so a run of tokens is the pair (product of a, its
 // end from nothing), and pairs join.  A workgroup walks a sequence for 64 V channels, a step at a time: each of its wavefronts takes K tokens of the step for
 // all of the channels, makes its run's pair and leaves it in LDS; behind one barrier every wavefront joins the pairs before its own and finishes
 // its tokens from the state that gives, still in registers.  Where that makes too few workgroups the sequences are cut in time, and a pass over the decays
