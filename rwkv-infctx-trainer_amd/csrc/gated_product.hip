@@ -10,6 +10,7 @@
 // roundings that are left, that of dg and du, which the matrix cores take in the streams' type, and that of the results (bf16, error of
 // the 2-norm: 3.1e-3 against 2.4e-3).  Backward, one pass makes dg and du; the three products read
 // them, x and the weights as they lie, with the index that is summed along memory or across it (gx: along dg and du, across the weights; gWg and gWu: across both).
+#include <cmath>
 #include <type_traits>
 
 #include "matrix_tiles.h"
@@ -366,16 +367,22 @@ struct Layout {
     }
 };
 static inline int tiles_of(long long n, int size) { return (int)((n + size - 1) / size); }
-// What `groups` workgroups of tiles of a size take, each `steps` tiles deep, in us: the longer of one workgroup's own time and, per compute unit, all of them's (a tile
-// of 256 has a compute unit to itself: whole rounds).  Fitted to 16 shapes in bf16, fp16 and fp32 from 16 to 4096 rows, where the choice by these
-// is the fastest or within 10 % of it: x (64, 2560) into 8960 columns bf16 49, 29, 23 by 256, 128, 64; (256, 4096) into 14336 84, 66, 91; (777, 2048) into
-// 7168 57, 65, 80; (301, 1001) into 2731 fp32 258, 86, 54.
+// What `groups` workgroups of tiles of a size take, each `steps` tiles deep, in us: in rounds of one tile of 256, two of 128 or four of 64 to a compute unit, as many as LDS has room for (fp32
+// is bound by the matrix cores, and a unit's groups add up).  Fitted to shapes in bf16, fp16 and fp32 from 16 to 4096 rows, where the choice by these is the
+// fastest or within 10 % of it: by 256, 128, 64 x (200, 4096) into 14336 columns bf16 105, 79, 113, (300, 4096) 107, 128, 159, (400, 2560) into 8960 72, 81, 86,
+// (777, 2048) into 5632 53, 59, 69, (300, 1024) into 4096 28, 14, 12; (301, 1001) into 2731 fp32 258, 86, 54.
 template <class T> static double cost_of(int size, long long groups, long long steps) {
-    const double cus = cu_count(), share = (double)groups / cus, n = (double)steps;
-    const bool narrow = sizeof(T) == 2;
-    if (size == 256) return (double)((groups + cu_count() - 1) / cu_count()) * ((narrow ? 1.35 : 7.6) * n + 10);
-    if (size == 128) return std::max((narrow ? 0.62 : 2.3) * n + 4, share * ((narrow ? 0.5 : 2.0) * n + 2));
-    return std::max((narrow ? 0.48 : 0.8) * n + 2, share * ((narrow ? 0.2 : 0.55) * n + 0.6));
+    const long long cus = cu_count();
+    const double share = (double)groups / (double)cus, n = (double)steps;
+    if (sizeof(T) == 4) {
+        if (size == 256) return (double)((groups + cus - 1) / cus) * (7.6 * n + 10);
+        if (size == 128) return std::max(2.3 * n + 4, share * (2.0 * n + 2));
+        return std::max(0.8 * n + 2, share * (0.55 * n + 0.6));
+    }
+    if (size == 256) return (double)((groups + cus - 1) / cus) * (1.5 * n + 6);
+    if (size == 64) return std::max(0.48 * n + 2, std::ceil(share) * (0.235 * n + 0.6));
+    const long long rest = groups % (2 * cus);
+    return (double)(groups / (2 * cus)) * (1.08 * n + 2) + (rest == 0 ? 0 : rest <= cus ? 0.8 * n + 3 : 1.08 * n + 2);
 }
 // How a product is shared out: the tiles' size, and k cut into shares where the tiles do not fill the compute units, their sums joined by another launch
 struct Plan { int size, rows, columns, shares, per; double cost; };
