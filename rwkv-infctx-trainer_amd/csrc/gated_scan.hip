@@ -381,9 +381,9 @@ __global__ __launch_bounds__(64 * BACK_WAVES) void backward(const Call k) {
 #pragma unroll
             for (int v = 0; v < V; v++) {
                 const float zz = GATE ? zf[v] * zs[j][v] : 1.f, gt = fmaf(gf[v], zz, g[v]), gu = gt * u[j][v];
-                // u changes by log a as -u times a^2 / beta^2 = 1 / beta^2 - 1 (where a is one, as at a shut gate, u is zero and so is that: the largest
-                // number stands for infinity)
-                const float less = fminf(__builtin_amdgcn_rcpf(beta[j][v] * beta[j][v]), 3e38f) - 1.f;
+                // u changes by log a as -u times a^2 / beta^2: by a squared, for 1 / beta^2 - 1 has no digits left where a is small.  (Where a is one, as at a shut
+                // gate, u is zero and so is that: the largest number stands for infinity.)
+                const float less = a[j][v] * a[j][v] * fminf(__builtin_amdgcn_rcpf(beta[j][v] * beta[j][v]), 3e38f);
                 const float gl = gt * fmaf(-u[j][v], less, a[j][v] * hs[j][v]) * rs[j][v];
                 ox[v] = there ? gt * (beta[j][v] * is[j][v]) : 0.f;
                 oi[v] = there ? fmaf(-gu, is[j][v], gu) : 0.f;
