@@ -125,6 +125,13 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forwa
     }
 }
 
+// fp16 has 5 bits of exponent: slopes that fp32 holds would be infinite from 65504 on and lose digits below 2^-14, where a mean loss' gradients lie.  So fp16 slopes are
+// written times a power of two, the same for the whole call, that takes the largest finite one to 2^14 .. 2^15 (what is 2^-29 of it still has all its digits), and the
+// products divide their fp32 sums by it.  A pass of its own finds the largest, by 256 workgroups, and reads what the slopes' pass reads again (the whole
+// backward of 4096 rows of 4096 into 14336 columns 1656 -> 1775 us, of 777 of 2048 into 7168 139 -> 150, of 16 of 2560 into 8960 86 -> 87); bf16 and fp32 have no need of it.
+template <class T> constexpr bool scaled() { return std::is_same<T, f16>::value; }
+constexpr int LARGEST = 256;                  // workgroups, a number of each
+
 // ---- a product of two operands
 struct Product {
     int M, N, K;
@@ -138,6 +145,18 @@ struct Product {
     float *parts;
     int per;                          // of k to a share
     bool pairs;                       // every two rows of A are one number in two parts: rows of the result where they lie along memory, of k where across
+    const int *exponent;              // fp16: A is times 2 to it
+};
+// what undoes it: asked for before a product's loop, for behind a store it would be asked for again
+template <class T> struct Unscaled {
+    int down = 0;
+    __device__ __forceinline__ Unscaled(const Product &k) {
+        if constexpr (scaled<T>()) down = -*k.exponent;
+    }
+    __device__ __forceinline__ float operator()(float v) const {
+        if constexpr (scaled<T>()) return ldexpf(v, down);
+        return v;
+    }
 };
 
 // ACROSS_A, ACROSS_B: k lies across memory in that operand
@@ -158,6 +177,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void produ
     if constexpr (ACROSS_B) l.b[0].place(b, b2, k.turn, k.bs, n0, k.b_rows, (k.N + E - 1) / E * E, ACROSS_A && k.pairs);
     else l.b[0].place(b + n0 * k.bs, k.bs, k.K, min(BN, k.N - n0));
     const int k0 = blockIdx.y * k.per;
+    const Unscaled<T> unscaled(k);
     l.clear();
     l.run(k0, min(k0 + k.per, k.K), k.K, lds);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
@@ -177,7 +197,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void produ
             const int n = n0 + (wn * L::NT + j) * 16 + 4 * (lane >> 4);
             float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[e] = l.acc[i][j][e];
+            for (int e = 0; e < 4; e++) o[e] = k.parts ? l.acc[i][j][e] : unscaled(l.acc[i][j][e]);
             if (k.parts) put4(k.parts + ((size_t)blockIdx.y * M + m) * k.os, n, k.N, whole, o);
             else put4(static_cast<T *>(m < k.split ? k.out0 : k.out1) + r * k.os, n, k.N, whole, o);
         }
@@ -190,7 +210,7 @@ template <class T> __global__ __launch_bounds__(256) void join(const Product k, 
     float s = k.parts[i];
     for (int p = 1; p < shares; p++) s += k.parts[p * n + i];
     const int m = (int)(i / k.os), r = m < k.split ? m : m - k.split;
-    if (r < k.live) static_cast<T *>(m < k.split ? k.out0 : k.out1)[r * k.os + i % k.os] = from_float<T>(s);
+    if (r < k.live) static_cast<T *>(m < k.split ? k.out0 : k.out1)[r * k.os + i % k.os] = from_float<T>(Unscaled<T>(k)(s));
 }
 
 // ---- layouts
@@ -220,38 +240,86 @@ template <class T> __global__ __launch_bounds__(256) void widen(const Widen k) {
     }
     *reinterpret_cast<uint4 *>(static_cast<T *>(k.array[j].out) + i) = raw;
 }
-// dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y.  pairs: (2 R, 2 Fs), what a row's rounding leaves in the row behind it
-template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, long long Fs, bool pairs) {
-    constexpr int V = 4;
-    const int f = (blockIdx.x * 256 + threadIdx.x) * V;
+// dg and du of four places of a row from column f on, zeros past F
+template <class T, bool WHOLE> __device__ __forceinline__ void slopes_at(const float *row, const T *gh, int kind, int f, int F, long long Fs, float (&dg)[4], float (&du)[4]) {
+    float g[4], u[4], o[4];
+    load4(row + f, g);
+    load4(row + Fs + f, u);
+    if (WHOLE && f + 4 <= F) load4(gh + f, o);
+    else
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = f + e < F ? to_float(gh[f + e]) : 0.f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        float value, slope;
+        activation(kind, g[e], value, slope);
+        // (what is kept past F was never written)
+        dg[e] = f + e < F ? o[e] * u[e] * slope : 0.f;
+        du[e] = f + e < F ? o[e] * value : 0.f;
+    }
+}
+template <class T, bool WHOLE> __global__ __launch_bounds__(1024) void largest(int R, int F, int kind, const float *kept, const T *gh, long long Fs, float *most) {
+    __shared__ float wave_most[16];
+    const int pieces = (int)(Fs / 4), first = blockIdx.x * 1024 + threadIdx.x, rows = LARGEST * 1024 / pieces, rest = LARGEST * 1024 % pieces;
+    float m = 0.f;
+    for (int r = first / pieces, c = first % pieces; r < R;) {
+        float dg[4], du[4];
+        slopes_at<T, WHOLE>(kept + r * 2 * Fs, gh + (long long)r * F, kind, c * 4, F, Fs, dg, du);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float v = fmaxf(fabsf(dg[e]), 0.f), w = fmaxf(fabsf(du[e]), 0.f);          // (NaN: zero)
+            m = fmaxf(m, fmaxf(v < INFINITY ? v : 0.f, w < INFINITY ? w : 0.f));
+        }
+        r += rows;
+        c += rest;
+        if (c >= pieces) c -= pieces, r++;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int w = 1; w < 16; w++) m = fmaxf(m, wave_most[w]);
+    most[blockIdx.x] = m;
+}
+// the exponent of the call's power of two, for every lane of a wavefront
+__device__ __forceinline__ int exponent_of(const float *most) {
+    float v[4];
+    static_assert(LARGEST == 4 * 64, "four numbers to a lane");
+    load4(most + 4 * (threadIdx.x & 63), v);
+    float m = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d));
+    return m > 0.f ? 15 - __builtin_amdgcn_frexp_expf(m) : 0;
+}
+// dg and du (R, 2 Fs) from g, u and gh, zeros past F; a row per workgroup of y.  pairs: (2 R, 2 Fs), what a row's rounding leaves in the row behind it.  fp16: times 2 to the
+// exponent, which is left for the products
+template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int R, int F, int kind, const float *kept, const T *gh, T *d, long long Fs, bool pairs, const float *most, int *exponent) {
+    const int f = (blockIdx.x * 256 + threadIdx.x) * 4;
+    int up = 0;
+    if constexpr (scaled<T>()) {
+        up = exponent_of(most);
+        if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) *exponent = up;
+    }
     if (f >= Fs) return;
     for (int r = blockIdx.y; r < R; r += gridDim.y) {
-        const float *row = kept + r * 2 * Fs;
-        float g[V], u[V], o[V], dg[V], du[V];
-        load4(row + f, g);
-        load4(row + Fs + f, u);
-        const T *from = gh + (long long)r * F;
-        if (WHOLE && f + V <= F) load4(from + f, o);
-        else
+        float dg[4], du[4];
+        slopes_at<T, WHOLE>(kept + r * 2 * Fs, gh + (long long)r * F, kind, f, F, Fs, dg, du);
+        if constexpr (scaled<T>())
 #pragma unroll
-            for (int e = 0; e < V; e++) o[e] = f + e < F ? to_float(from[f + e]) : 0.f;
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-            float value, slope;
-            activation(kind, g[e], value, slope);
-            // (what is kept past F was never written)
-            dg[e] = f + e < F ? o[e] * u[e] * slope : 0.f;
-            du[e] = f + e < F ? o[e] * value : 0.f;
-        }
+            for (int e = 0; e < 4; e++) dg[e] = ldexpf(dg[e], up), du[e] = ldexpf(du[e], up);
         T *to = d + (long long)r * (pairs ? 4 : 2) * Fs + f;
         store4(to, dg);
         store4(to + Fs, du);
         if (!pairs) continue;
+        // (infinity is all in the first part)
+        auto left = [](float v) {
+            const float rounded = to_float(from_float<T>(v));
+            return fabsf(rounded) < INFINITY ? v - rounded : 0.f;
+        };
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            dg[e] -= to_float(from_float<T>(dg[e]));
-            du[e] -= to_float(from_float<T>(du[e]));
-        }
+        for (int e = 0; e < 4; e++) dg[e] = left(dg[e]), du[e] = left(du[e]);
         store4(to + 2 * Fs, dg);
         store4(to + 3 * Fs, du);
     }
@@ -492,7 +560,7 @@ struct Backward {
 // for them ((16, 2560) into 8960 columns gx 31.5 -> 34.4 us, weights' gradients 36.2 -> 36.8; (64, 2560) would be 41 -> 50, 38 -> 42).
 constexpr int PAIRED = 32;
 template <class T> constexpr bool in_pairs(int R) { return sizeof(T) == 2 && R <= PAIRED; }
-struct Regions { size_t d, x, wg, wu, parts, all; };
+struct Regions { size_t d, x, wg, wu, most, exponent, parts, all; };
 template <class T> static Regions regions(int R, int C, int F, bool want_x, bool want_w) {
     const size_t Fs = rounded(F), Cs = C % tiles::piece<T>() ? rounded(C) : 0;
     Regions r;
@@ -503,6 +571,8 @@ template <class T> static Regions regions(int R, int C, int F, bool want_x, bool
     r.x = take(want_w ? (size_t)R * Cs * sizeof(T) : 0);
     r.wg = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
     r.wu = take(want_x ? (size_t)F * Cs * sizeof(T) : 0);
+    r.most = take(scaled<T>() ? LARGEST * 4 : 0);
+    r.exponent = take(scaled<T>() ? 4 : 0);
     size_t parts = 0;
     if (want_x) {
         const Plan p = plan_of<T>(pairs * R, C, 2 * Fs, true);
@@ -548,11 +618,19 @@ template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k
     }
     float *parts = reinterpret_cast<float *>(ws + r.parts);
     const dim3 grid(tiles_of(Fs, 1024), std::min(k.R, 32768));
-    if (k.F % 4 == 0) hipLaunchKernelGGL((slopes<T, true>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs, pairs);
-    else hipLaunchKernelGGL((slopes<T, false>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, static_cast<const T *>(k.gh), d, Fs, pairs);
+    float *most = reinterpret_cast<float *>(ws + r.most);
+    int *exponent = reinterpret_cast<int *>(ws + r.exponent);
+    const T *gh = static_cast<const T *>(k.gh);
+    auto both = [&](auto whole) {
+        constexpr bool WHOLE = decltype(whole)::value;
+        if constexpr (scaled<T>()) hipLaunchKernelGGL((largest<T, WHOLE>), dim3(LARGEST), dim3(1024), 0, s, k.R, k.F, k.kind, k.kept, gh, Fs, most);
+        hipLaunchKernelGGL((slopes<T, WHOLE>), grid, dim3(256), 0, s, k.R, k.F, k.kind, k.kept, gh, d, Fs, pairs, most, exponent);
+    };
+    if (k.F % 4 == 0) both(std::true_type());
+    else both(std::false_type());
     if (want_x) {
         Product p = {};
-        p.M = R2; p.N = k.C; p.K = 2 * Fs; p.pairs = pairs;
+        p.M = R2; p.N = k.C; p.K = 2 * Fs; p.pairs = pairs; p.exponent = exponent;
         p.a = d; p.as = 2 * Fs;
         p.b = wg; p.b2 = wu; p.bs = ld; p.turn = Fs; p.b_rows = k.F;
         p.out0 = p.out1 = k.gx; p.os = k.C; p.split = p.live = k.R;
@@ -561,7 +639,7 @@ template <class T> static hipError_t backward_t(hipStream_t s, const Backward &k
     }
     if (want_w) {
         Product p = {};
-        p.M = 2 * Fs; p.N = k.C; p.K = (int)rounded(R2); p.pairs = pairs;
+        p.M = 2 * Fs; p.N = k.C; p.K = (int)rounded(R2); p.pairs = pairs; p.exponent = exponent;
         p.a = d; p.as = 2 * Fs;
         p.b = p.b2 = x; p.bs = xs; p.turn = 0x7fffffff; p.a_rows = R2; p.b_rows = k.R;
         p.out0 = k.gwg; p.out1 = k.gwu; p.os = k.C; p.split = Fs; p.live = k.F;

@@ -43,7 +43,8 @@ def gated_feed_forward(x, w_gate, w_up, activation="silu"):
 
     A recorded call keeps both projections' results in fp32 (2 F numbers per row) for its backward, whose workspace is their slopes, 2 F elements of x's type per row
     (twice that up to 32 rows), and the sums of a small product's shares.  Where C is not whole pieces of 16 bytes the backward copies x and the weights, the forward where
-    there are many rows.  The slopes are rounded to x's type, up to 32 rows to twice its digits."""
+    there are many rows.  The slopes are rounded to x's type, up to 32 rows to twice its digits; in fp16 they are scaled by a
+    power of two first, to the largest of the call, so that they have fp32's range: what is below 2^-29 of the largest loses digits."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation {activation!r} is none of {', '.join(ACTIVATIONS)}")
     return _call("gated_product", x, w_gate, w_up, ACTIVATIONS[activation])

@@ -54,3 +54,72 @@ def test_gradients_of_what_forgets_at_once(dtype, T, decay, gate):
             a = a[0, 0]
         worst = ((a - b).abs() / ((off + more) * b.abs() * (1 + off))).max().item()
         assert worst <= 1, f"gradient of {n}: {worst:.3g} of the bound"
+
+
+def _slopes(x, wg, wu, gy):
+    """In 64 bits, for silu: dg and du and what fp32 leaves of them: g and u are fp32 sums (c of their terms' sizes), slopes and slopes' slopes below 1.2."""
+    g, u = x @ wg.t(), x @ wu.t()
+    p = torch.sigmoid(g)
+    act, slope = g * p, p * (1 + g * (1 - p))
+    c = (x.shape[1] + 32) * 2.0 ** -23
+    G, U = x.abs() @ wg.abs().t(), x.abs() @ wu.abs().t()
+    off_g = gy.abs() * (1.2 * c * (U + G * u.abs() + c * G * U) + 2.0 ** -20 * u.abs())
+    return gy * u * slope, gy * act, off_g, gy.abs() * (1.2 * c * G + 2.0 ** -20 * act.abs())
+
+
+@pytest.mark.parametrize("R,C,F", [(1, 72, 200), (20, 99, 130), (32, 256, 515), (33, 256, 515), (300, 72, 1030), (700, 520, 1100)])
+@pytest.mark.parametrize("size", [1e-7, 1e-5, 1e-3, 3e4])
+@pytest.mark.parametrize("wide", [2.0 ** -5, 2.0 ** 5])
+def test_fp16_slopes_have_the_range_of_fp32(R, C, F, size, wide):
+    """Gradients coming in small as a mean loss' or as large as fp16 goes; the slopes between are no results, and neither overflow nor underflow shows.  ``wide`` scales the weights up
+    and x down, so that one of the two kinds of results has fp16's normal range where the slopes themselves have not.
+
+    An element: its rounding, 2^-11 or 2^-25; the slopes' rounding 2^-11, or of two parts 2^-22, and 2^-39 of the largest slope where that leaves fp16's normal
+    range (2^-25 of 2^14); fp32 sums.  What is past fp16's largest number is infinite, as any result."""
+    K = _kernels()
+    g = S._g(R, C, F)
+    n = lambda *s: torch.randn(*s, generator=g)
+    x = (n(R, C) / wide).half()
+    wg, wu = ((n(F, C) * (wide / C ** 0.5)).half() for _ in range(2))
+    gy = (n(R, F).clamp(-2, 2) * size).half()
+    leaf = [t.cuda().requires_grad_(True) for t in (x, wg, wu)]
+    got = torch.autograd.grad(K.gated_feed_forward(*leaf), leaf, gy.cuda())
+    x, wg, wu, gy = (t.double() for t in (x, wg, wu, gy))
+    dg, du, off_g, off_u = _slopes(x, wg, wu, gy)
+    e = 2.0 ** -22 if R <= 32 else 2.0 ** -11
+    tiny = 2.0 ** -39 * torch.stack([dg.abs().max(), du.abs().max()]).max()
+    bad_g, bad_u = (e * d.abs() + tiny + (1 + e) * o for d, o in ((dg, off_g), (du, off_u)))
+    sums = lambda terms: (terms + 32) * 2.0 ** -23 * (1 + e)
+    for name, a, ref, size_, off in (("x", got[0], dg @ wg + du @ wu, dg.abs() @ wg.abs() + du.abs() @ wu.abs(), bad_g @ wg.abs() + bad_u @ wu.abs()),
+                                     ("w_gate", got[1], dg.t() @ x, dg.t().abs() @ x.abs(), bad_g.t() @ x.abs()), ("w_up", got[2], du.t() @ x, du.t().abs() @ x.abs(), bad_u.t() @ x.abs())):
+        a, wrong = a.cpu().double(), off + sums(2 * F if name == "x" else R) * (size_ + off)
+        bound = 2.0 ** -11 * ref.abs() + (1 + 2.0 ** -11) * wrong + 2.0 ** -25
+        inside, outside = ref.abs() + wrong < 65504, ref.abs() - wrong > 65536
+        worst = ((a - ref).abs() / bound)[inside].max().item() if inside.any() else 0.0
+        assert worst <= 1, f"gradient of {name}: {worst:.3g} of the bound"          # (NaN is not)
+        assert bool((a == ref.sign() * float("inf"))[outside].all()), f"gradient of {name} past fp16"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("R", [1, 7, 32, 40])
+def test_an_infinite_gradient_is_infinite(dtype, R):
+    """One place's incoming gradient is infinite: what it reaches is infinite of the sign that the formula gives (NaN only where the formula adds both signs), the rest is
+    finite and off by no more than the test above allows: both roundings, the slopes' in two parts up to 32 rows, fp32 sums, and g and u from fp32 sums."""
+    K = _kernels()
+    C, F = 96, 70
+    g = S._g(R, 3)
+    x, wg, wu, gy = (torch.randn(*s, generator=g).to(dtype) for s in ((R, C), (F, C), (F, C), (R, F)))
+    gy[R // 2, 5] = float("inf")
+    leaf = [t.cuda().requires_grad_(True) for t in (x, wg, wu)]
+    got = torch.autograd.grad(K.gated_feed_forward(*leaf), leaf, gy.cuda())
+    x, wg, wu, gy = (t.double() for t in (x, wg, wu, gy))
+    dg, du, off_g, off_u = _slopes(x, wg, wu, gy)
+    e = torch.finfo(dtype).eps / 2
+    finite = lambda t: torch.where(torch.isfinite(t), t, 0.0).abs()
+    bad_g, bad_u = ((e * e if R <= 32 else e) * finite(d) + 2 * finite(o) for d, o in ((dg, off_g), (du, off_u)))
+    each = lambda p, q: (p @ wg.abs() + q @ wu.abs(), p.t() @ x.abs(), q.t() @ x.abs())
+    for a, ref, size, off in zip(got, (dg @ wg + du @ wu, dg.t() @ x, du.t() @ x), each(finite(dg), finite(du)), each(bad_g, bad_u)):
+        a = a.cpu().double()
+        assert torch.equal(a.isnan(), ref.isnan()) and torch.equal(a.isinf(), ref.isinf()) and bool((a == ref)[ref.isinf()].all())
+        bound = e * ref.abs() + (1 + e) * (off + (2 * F + 32) * 2.0 ** -23 * (size + off)) + 2.0 ** -24
+        assert bool(((a - ref).abs() <= bound)[torch.isfinite(ref)].all())
