@@ -438,7 +438,7 @@ template <class T> __global__ __launch_bounds__(256) void one(const Call k) {
         auto at = [&](const Rows &s) { return to_float(static_cast<const T *>(s.p)[b * s.batch + d]); };
         const float x = at(k.x), r = at(k.r), i = at(k.i), z = k.z.p ? at(k.z) : 0.f, lg = rate_of(k.decay[d], k.scale) * sigmoid(r), a = exp2_fast(lg);
         h = fmaf(a, before, __builtin_amdgcn_sqrtf(one_less_square(lg, a)) * sigmoid(i) * x);
-        o = k.z.p ? h * z * sigmoid(z) : h;
+        o = k.z.p ? h * (z * sigmoid(z)) : h;          // (silu first, as a prompt's: h z may be infinite where it is zero)
     }
     static_cast<T *>(k.y)[n] = from_float<T>(o);
     k.state_out[n] = h;

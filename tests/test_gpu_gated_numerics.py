@@ -56,6 +56,16 @@ def test_gradients_of_what_forgets_at_once(dtype, T, decay, gate):
         assert worst <= 1, f"gradient of {n}: {worst:.3g} of the bound"
 
 
+@pytest.mark.parametrize("T", [1, 2, 140])
+def test_a_gate_far_shut_leaves_zero(T):
+    """h silu(z) of a large state and a gate far below zero: silu(z) is zero there, whatever h z would be.  A single token gives what a prompt gives."""
+    D = 70
+    z = torch.full((1, T, D), -1e10, device="cuda")
+    zero = torch.zeros(1, T, D, device="cuda")
+    y, h = _kernels().gated_recurrence(zero, torch.full_like(zero, -200.0), zero, torch.zeros(D, device="cuda"), z=z, state=torch.full((1, D), 1e30, device="cuda"))
+    assert bool((y == 0).all()) and bool((h == 1e30).all())
+
+
 def _slopes(x, wg, wu, gy):
     """In 64 bits, for silu: dg and du and what fp32 leaves of them: g and u are fp32 sums (c of their terms' sizes), slopes and slopes' slopes below 1.2."""
     g, u = x @ wg.t(), x @ wu.t()
