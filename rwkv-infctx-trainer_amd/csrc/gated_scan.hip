@@ -389,7 +389,7 @@ __global__ __launch_bounds__(64 * BACK_WAVES) void backward(const Call k) {
                 oi[v] = there ? fmaf(-gu, is[j][v], gu) : 0.f;
                 orr[v] = there ? gl * (slope[v] * (1.f - rs[j][v])) : 0.f;
                 part[v] += there ? gl : 0.f;
-                if (GATE) oz[v] = there ? gf[v] * hs[j + 1][v] * fmaf(zs[j][v], 1.f - zz, zz) : 0.f;
+                if (GATE) oz[v] = there ? gf[v] * (hs[j + 1][v] * fmaf(zs[j][v], 1.f - zz, zz)) : 0.f;          // (gy h alone may be infinite)
                 g[v] = a[j][v] * gt;
             }
             l.store(gx, j, ox);

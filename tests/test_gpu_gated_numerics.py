@@ -66,6 +66,18 @@ def test_a_gate_far_shut_leaves_zero(T):
     assert bool((y == 0).all()) and bool((h == 1e30).all())
 
 
+@pytest.mark.parametrize("T", [1, 2, 140])
+def test_a_gate_far_shut_takes_no_gradient(T):
+    """The same backwards: silu's slope is zero there, and gy h, which fp32 does not hold, is never formed."""
+    D = 70
+    full = lambda v: torch.full((1, T, D), v, device="cuda")
+    leaf = [t.requires_grad_(True) for t in (full(1.0), full(-200.0), full(0.0), full(-1e10), torch.full((1, D), 1e30, device="cuda"))]
+    x, r, i, z, state = leaf
+    y, _ = _kernels().gated_recurrence(x, r, i, torch.zeros(D, device="cuda"), z=z, state=state)
+    for t in torch.autograd.grad(y, leaf, full(1e10)):
+        assert bool((t == 0).all())
+
+
 def _slopes(x, wg, wu, gy):
     """In 64 bits, for silu: dg and du and what fp32 leaves of them: g and u are fp32 sums (c of their terms' sizes), slopes and slopes' slopes below 1.2."""
     g, u = x @ wg.t(), x @ wu.t()
