@@ -253,8 +253,8 @@ template <class T, bool WHOLE> __device__ __forceinline__ void slopes_at(const f
     for (int e = 0; e < 4; e++) {
         float value, slope;
         activation(kind, g[e], value, slope);
-        // (what is kept past F was never written)
-        dg[e] = f + e < F ? o[e] * u[e] * slope : 0.f;
+        // (what is kept past F was never written; gh u alone may be infinite)
+        dg[e] = f + e < F ? o[e] * (u[e] * slope) : 0.f;
         du[e] = f + e < F ? o[e] * value : 0.f;
     }
 }

@@ -145,3 +145,18 @@ def test_an_infinite_gradient_is_infinite(dtype, R):
         assert torch.equal(a.isnan(), ref.isnan()) and torch.equal(a.isinf(), ref.isinf()) and bool((a == ref)[ref.isinf()].all())
         bound = e * ref.abs() + (1 + e) * (off + (2 * F + 32) * 2.0 ** -23 * (size + off)) + 2.0 ** -24
         assert bool(((a - ref).abs() <= bound)[torch.isfinite(ref)].all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("name", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("R", [3, 50])
+def test_a_shut_unit_takes_no_gradient(dtype, name, R):
+    """g far below zero: value and slope of the activation are zero, and gy u, which fp32 does not hold, is never formed."""
+    C, F = 16, 24
+    x, wg = torch.ones(R, C, dtype=dtype, device="cuda"), torch.full((F, C), -1e4, dtype=dtype, device="cuda")
+    wu = torch.full((F, C), 1e30, dtype=dtype, device="cuda")
+    leaf = [t.requires_grad_(True) for t in (x, wg, wu)]
+    y = _kernels().gated_feed_forward(*leaf, name)
+    assert bool((y == 0).all())
+    for t in torch.autograd.grad(y, leaf, torch.full_like(y, 1e10)):
+        assert bool((t == 0).all())
