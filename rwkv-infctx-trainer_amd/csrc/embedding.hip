@@ -27,21 +27,24 @@ template <class T, class I, int W> __global__ __launch_bounds__(256) void lookup
     const size_t first = (size_t)blockIdx.x * (256 * EACH), n0 = first / pieces, total = k.count * pieces;
     const unsigned start = (unsigned)(first - n0 * pieces);
     float v[EACH][W];
+    bool there[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         const unsigned at = start + e * 256 + threadIdx.x, r = at / pieces, c = at - r * pieces;
 #pragma unroll
         for (int w = 0; w < W; w++) v[e][w] = 0.f;
+        there[e] = false;
         if (first + e * 256 + threadIdx.x >= total) continue;
         const long long t = token_at<I>(k.tokens, n0 + r);
-        if (t >= 0 && t < k.V) load_vec(static_cast<const T *>(k.table) + t * k.ws + c * W, v[e]);
+        there[e] = t >= 0 && t < k.V;
+        if (there[e]) load_vec(static_cast<const T *>(k.table) + t * k.ws + c * W, v[e]);
     }
 #pragma unroll
     for (int e = 0; e < EACH; e++) {
         const size_t at = first + e * 256 + threadIdx.x;
         if (at >= total) continue;
 #pragma unroll
-        for (int w = 0; w < W; w++) v[e][w] *= k.scale;
+        for (int w = 0; w < W; w++) v[e][w] = there[e] ? v[e][w] * k.scale : 0.f;          // (zeros whatever the scale is)
         store_vec(static_cast<T *>(k.out) + at * W, v[e]);
     }
 }

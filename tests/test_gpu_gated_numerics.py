@@ -160,3 +160,16 @@ def test_a_shut_unit_takes_no_gradient(dtype, name, R):
     assert bool((y == 0).all())
     for t in torch.autograd.grad(y, leaf, torch.full_like(y, 1e10)):
         assert bool((t == 0).all())
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
+@pytest.mark.parametrize("scale", [float("inf"), float("nan"), -2.0])
+@pytest.mark.parametrize("C", [16, 7])
+def test_a_place_without_a_token_is_zero_whatever_the_scale(dtype, scale, C):
+    """The others are the scale times their rows; a zero without a sign where there is no token."""
+    tokens = torch.tensor([0, -1, 2, 3, -100, 1], device="cuda")
+    w = torch.arange(1, 3 * C + 1, device="cuda").view(3, C).to(dtype)
+    out = _kernels().embedding(tokens, w, scale)
+    none = (tokens < 0) | (tokens >= 3)
+    assert bool((out[none] == 0).all()) and not out[none].signbit().any()
+    assert torch.equal(out[~none], (w[tokens[~none]].float() * scale).to(dtype)) or (scale != scale and out[~none].isnan().all())
