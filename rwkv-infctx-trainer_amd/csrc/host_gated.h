@@ -194,17 +194,27 @@ public:
     }
 };
 
+// Operands of different types under autocast, as fp32 weights behind a projection's 16-bit output are: in autocast's type, as torch.nn.functional.linear takes them (a weight's
+// copy is kept for as long as autocast keeps it).  Operands of one type are taken as they come.
+void cast_by_autocast(std::initializer_list<Tensor *> operands) {
+    if (!at::autocast::is_autocast_enabled(at::kCUDA)) return;
+    const at::ScalarType first = (*operands.begin())->scalar_type();
+    if (std::all_of(operands.begin(), operands.end(), [&](const Tensor *t) { return t->scalar_type() == first; })) return;
+    for (Tensor *t : operands) *t = at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), *t, at::kCUDA);
+}
+
 // gated_product(x, w_gate, w_up, activation) -> h; None: traced
 PyObject *py_gated_product(PyObject *, PyObject *const *a, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     arity(n, 4);
     if (traced()) Py_RETURN_NONE;
-    const Tensor x = tensor(a[0]), wg = tensor(a[1]), wu = tensor(a[2]);
+    Tensor x = tensor(a[0]), wg = tensor(a[1]), wu = tensor(a[2]);
     const int activation = integer(a[3]);
     variable_list o;
     {
         NoLock no_lock;
         same_device(x, {&wg, &wu});
+        cast_by_autocast({&x, &wg, &wu});
         dtype_code(x);
         REQUIRE(x.dim() >= 1 && x.numel() > 0 && wg.dim() == 2 && wg.size(1) == x.size(-1) && wu.sizes().equals(wg.sizes()));
         REQUIRE(wg.scalar_type() == x.scalar_type() && wu.scalar_type() == x.scalar_type());

@@ -39,7 +39,8 @@ def gated_recurrence(x, r, i, decay, z=None, state=None, lengths=None, scale=8.0
 
 def gated_feed_forward(x, w_gate, w_up, activation="silu"):
     """x (..., C), w_gate and w_up (F, C) as torch.nn.Linear keeps them -> act(x w_gate') * (x w_up') (..., F), act "silu", "gelu" (its tanh
-    form) or "relu".  All of one type; sums in fp32, the result rounded once.  The second projection stays the caller's matrix product.
+    form) or "relu".  All of one type (under torch.autocast different ones are cast to
+    its type, as torch's own projections cast them); sums in fp32, the result rounded once.  The second projection stays the caller's matrix product.
 
     A recorded call keeps both projections' results in fp32 (2 F numbers per row) for its backward, whose workspace is their slopes, 2 F elements of x's type per row
     (twice that up to 32 rows), and the sums of a small product's shares.  Where C is not whole pieces of 16 bytes the backward copies x and the weights, the forward where
