@@ -443,7 +443,9 @@ int wkv_gated_recurrence_backward(void *stream, int B, int T, int D, int dtype, 
 int wkv_embedding_forward(void *stream, long long count, int V, int C, int dtype, int index_bytes, float scale, const void *tokens, const void *table,
                           void *out);
 
-/* The table's gradient, written whole: gtable[v] = scale times the sum, in fp32 and the places' order, of gout's rows (a row stride in elements) whose token is v. */
+/* The table's gradient, written whole: gtable[v] = scale times the sum in fp32 of gout's rows (a row stride in elements) whose token is v.  The places are sorted by token, each token's
+ * in their order, and summed in order by runs of up to 64 sorted places (8, 16, 32 or 64 by count and C); a token that lies in several runs has their sums added in order.  So how a row's
+ * sum is grouped, and with it its last bits, depends on the whole call; the same call gives the same bits. */
 size_t wkv_embedding_backward_workspace(long long count, int V, int C);
 int wkv_embedding_backward(void *stream, long long count, int V, int C, int dtype, int index_bytes, float scale, const void *tokens, const void *gout,
                            long long gout_stride, void *gtable, void *workspace, size_t workspace_bytes);

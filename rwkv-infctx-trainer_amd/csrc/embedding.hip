@@ -4,7 +4,7 @@
 //
 // A token outside the table is a place without one: a row of zeros, no gradient.  Both directions are bound by memory (32768 places of 2560 channels bf16, 65536 tokens: lookup 55 us,
 // 6 TB/s from the last-level cache's share; sums and zeros 101, 5 TB/s, behind 30 of sorting in small launches).  The gradient is written
-// whole (V C, most of it zeros) from the places sorted by token: no atomics on sums, fp32 ones in the places' order, the same bits every time.  Sorting: stable
+// whole (V C, most of it zeros) from the places sorted by token: no atomics on sums, fp32 ones in the places' order within a chunk and in the chunks' order over them, the same bits every time.  Sorting: stable
 // passes over ten bits of the token at most, counts per tile of places, then each tile's places to where the tiles and digits before leave off; up
 // to one tile's worth in a single launch.  Sums: a workgroup takes a chunk of up to 64 sorted places, whoever they belong to, so that it does not matter how often a token
 // comes; a token that lies within them is written as it ends, one that crosses their border leaves a part for a second launch.  The zeros are written beside what waits: of one tile,

@@ -55,7 +55,8 @@ def embedding(tokens, weight, scale=1.0):
     """tokens (...) int64 or int32, weight (V, C) -> scale * weight[tokens] (..., C) in weight's type, rounded once.
 
     A token below zero or from V on is a place without one, as padding has it: its row is zeros, and its gradient goes nowhere.  The gradient of ``weight`` is dense,
-    each row the sum in fp32, in the places' order, of its places' gradients."""
+    each row the fp32 sum of its places' gradients: by runs of up to 64 of the places sorted by token, each run in the places' order, then over the runs in order.  Where the
+    runs begin depends on the other places too, so a row's last bits do; the same call gives the same bits."""
     return _call("embedding", tokens, weight, float(scale))
 
 

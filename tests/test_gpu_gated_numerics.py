@@ -173,3 +173,41 @@ def test_a_place_without_a_token_is_zero_whatever_the_scale(dtype, scale, C):
     none = (tokens < 0) | (tokens >= 3)
     assert bool((out[none] == 0).all()) and not out[none].signbit().any()
     assert torch.equal(out[~none], (w[tokens[~none]].float() * scale).to(dtype)) or (scale != scale and out[~none].isnan().all())
+
+
+@pytest.mark.parametrize("first", [0, 1, 5, 8, 13])
+def test_embedding_sums_by_runs_of_the_sorted_places(first):
+    """Three tokens, of which the first's count moves the borders of the others' runs: up to 4096 places of up to 1024 channels, fp32 sums of 8 sorted places at a time, in order, added in
+    order.  Values whose sums depend on the grouping."""
+    n = torch.tensor([2.0 ** 30, 1.0, -2.0 ** 30, 3.0, 2.0 ** 29])
+    tokens = torch.cat([torch.zeros(first, dtype=torch.long), torch.tensor([1, 2, 1]).repeat(31), torch.tensor([-1, 3])])
+    gy = n.repeat(len(tokens))[:len(tokens)].repeat_interleave(8).view(-1, 8).contiguous()
+
+    def runs(tokens, gy):
+        order = torch.where((tokens >= 0) & (tokens < 3), tokens, 3).argsort(stable=True)
+        total = torch.zeros(3, 8)
+        for at in range(0, len(order), 8):
+            sums = {}
+            for p in order[at:at + 8].tolist():
+                t = int(tokens[p])
+                if 0 <= t < 3:
+                    sums[t] = sums[t] + gy[p] if t in sums else gy[p].clone()
+            for t, s in sums.items():
+                total[t] += s
+        return total
+
+    w = torch.zeros(3, 8, device="cuda", requires_grad=True)
+    (a,) = torch.autograd.grad(_kernels().embedding(tokens.cuda(), w), w, gy.cuda())
+    assert torch.equal(a.cpu(), runs(tokens, gy))
+
+
+def test_embedding_sums_are_grouped_by_the_whole_call():
+    """The grouping that the documentation states, by a case small enough to follow: 2^30, 1, -2^30, 1 and six zeros before them of another token.  Alone they lie in one run: 2^30 + 1 is 2^30 in fp32, so 1
+    is left.  Behind six others the run of 8 ends after the 1: 2^30 and then (-2^30 + 1 = -2^30): nothing is left."""
+    K = _kernels()
+    w = torch.zeros(2, 8, device="cuda", requires_grad=True)
+    gy = torch.tensor([0.0] * 6 + [2.0 ** 30, 1.0, -2.0 ** 30, 1.0]).repeat_interleave(8).view(-1, 8).cuda()
+    tokens = torch.tensor([0] * 6 + [1] * 4, device="cuda")
+    (alone,) = torch.autograd.grad(K.embedding(tokens[6:], w), w, gy[6:].contiguous())
+    (behind,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
+    assert bool((alone[1] == 1).all()) and bool((behind[1] == 0).all()) and not behind[0].any()
