@@ -135,7 +135,7 @@ constexpr int LARGEST = 256;                  // workgroups, a number of each
 // ---- a product of two operands
 struct Product {
     int M, N, K;
-    const void *a, *b, *b2;           // b2: B's rows of k from `turn` on, where k is across
+    const void *a, *b, *b2;           // b2: B's rows of k from `turn` on
     long long as, bs;
     int turn, a_rows, b_rows;         // rows of k that are there, where k is across
     // out: rows below `split` (of which `live` are there) to out0, those from it on to out1; parts: fp32 sums over a share of k instead
@@ -159,11 +159,11 @@ template <class T> struct Unscaled {
     }
 };
 
-// ACROSS_A, ACROSS_B: k lies across memory in that operand
-template <class T, int BM, int BN, int WM, int WN, int AHEAD, bool ACROSS_A, bool ACROSS_B>
+// ACROSS_A: k lies across memory in A, as it does in B
+template <class T, int BM, int BN, int WM, int WN, int AHEAD, bool ACROSS_A>
 __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void product(const Product k, int rows, int columns) {
     typedef std::conditional_t<ACROSS_A, tiles::Across<T, BM, 64 * WM * WN>, tiles::Along<T, BM, 64 * WM * WN>> A;
-    typedef std::conditional_t<ACROSS_B, tiles::Across<T, BN, 64 * WM * WN>, tiles::Along<T, BN, 64 * WM * WN>> B;
+    typedef tiles::Across<T, BN, 64 * WM * WN> B;
     typedef tiles::Loop<T, A, B, BM, BN, WM, WN, 1, AHEAD> L;
     __shared__ __align__(1024) char lds[L::LDS];
     int tm, tn;
@@ -174,8 +174,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void produ
     constexpr int E = tiles::piece<T>();          // (rows are whole pieces, what they hold may not be)
     if constexpr (ACROSS_A) l.a.place(a, a, 0x7fffffff, k.as, m0, k.a_rows, (k.M + E - 1) / E * E);
     else l.a.place(a + m0 * k.as, k.as, k.K, min(BM, k.M - m0));
-    if constexpr (ACROSS_B) l.b[0].place(b, b2, k.turn, k.bs, n0, k.b_rows, (k.N + E - 1) / E * E, ACROSS_A && k.pairs);
-    else l.b[0].place(b + n0 * k.bs, k.bs, k.K, min(BN, k.N - n0));
+    l.b[0].place(b, b2, k.turn, k.bs, n0, k.b_rows, (k.N + E - 1) / E * E, ACROSS_A && k.pairs);
     const int k0 = blockIdx.y * k.per;
     const Unscaled<T> unscaled(k);
     l.clear();
@@ -590,10 +589,10 @@ template <class T, bool ACROSS_A> static void product_launch(hipStream_t s, Prod
     k.per = p.per;
     if (p.shares == 1) k.parts = nullptr;
     const dim3 grid(p.rows * p.columns, p.shares);
-    if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4, 2, ACROSS_A, true>), grid, dim3(512), 0, s, k, p.rows, p.columns);
-    else if (p.size == 128) hipLaunchKernelGGL((product<T, 128, 128, 2, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
-    else if (deep_pays((long long)p.rows * p.columns * p.shares)) hipLaunchKernelGGL((product<T, 64, 64, 2, 2, DEEP, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
-    else hipLaunchKernelGGL((product<T, 64, 64, 2, 2, 2, ACROSS_A, true>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    if (p.size == 256) hipLaunchKernelGGL((product<T, 256, 256, 2, 4, 2, ACROSS_A>), grid, dim3(512), 0, s, k, p.rows, p.columns);
+    else if (p.size == 128) hipLaunchKernelGGL((product<T, 128, 128, 2, 2, 2, ACROSS_A>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    else if (deep_pays((long long)p.rows * p.columns * p.shares)) hipLaunchKernelGGL((product<T, 64, 64, 2, 2, DEEP, ACROSS_A>), grid, dim3(256), 0, s, k, p.rows, p.columns);
+    else hipLaunchKernelGGL((product<T, 64, 64, 2, 2, 2, ACROSS_A>), grid, dim3(256), 0, s, k, p.rows, p.columns);
     const int M = !ACROSS_A && k.pairs ? k.M / 2 : k.M;
     if (p.shares > 1) hipLaunchKernelGGL(join<T>, dim3((unsigned)(((size_t)M * k.os + 255) / 256)), dim3(256), 0, s, k, M, p.shares);
 }
