@@ -37,12 +37,13 @@ int check_operands(int T, int D, int dtype, const wkv_rows *x, const wkv_rows *r
     }
     return aligned16(decay) ? WKV_OK : WKV_ERR_ALIGN;
 }
-gated::Rows rows_of(const wkv_rows *o) { return o ? gated::Rows{o->p, o->batch, o->token} : gated::Rows{}; }
+// (of a single token the stride means nothing: that of rows side by side, so that what lies behind it is out of its range)
+gated::Rows rows_of(const wkv_rows *o, int T, int D) { return o ? gated::Rows{o->p, o->batch, T > 1 ? o->token : D} : gated::Rows{}; }
 gated::Call recurrence_call(int B, int T, int D, float scale, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i, const wkv_rows *z, const float *decay,
                             const int *lengths, const float *checkpoints, void *workspace) {
     gated::Call k = {};
     k.B = B; k.T = T; k.D = D; k.scale = scale;
-    k.x = rows_of(x); k.r = rows_of(r); k.i = rows_of(i); k.z = rows_of(z);
+    k.x = rows_of(x, T, D); k.r = rows_of(r, T, D); k.i = rows_of(i, T, D); k.z = rows_of(z, T, D);
     k.decay = decay; k.lengths = lengths;
     k.checkpoints = const_cast<float *>(checkpoints);
     k.pairs = static_cast<float *>(workspace);

@@ -211,3 +211,25 @@ def test_embedding_sums_are_grouped_by_the_whole_call():
     (alone,) = torch.autograd.grad(K.embedding(tokens[6:], w), w, gy[6:].contiguous())
     (behind,) = torch.autograd.grad(K.embedding(tokens, w), w, gy)
     assert bool((alone[1] == 1).all()) and bool((behind[1] == 0).all()) and not behind[0].any()
+
+
+@pytest.mark.parametrize("dtype", S.TYPES)
+def test_a_recorded_single_token_reads_itself_alone(dtype):
+    """A call of one token is a call of two that ends after the first, to the bit, whatever is not finite in it: an open gate of plus infinity makes infinite gradients, not NaN."""
+    B, D = 2, 66
+    g = S._g(B, D)
+    r = lambda *s: torch.randn(*s, generator=g).to(dtype).cuda()
+    x, a, i, z, gy = (r(B, 2, D) for _ in range(5))
+    state, decay, gs = torch.randn(B, D, generator=g).cuda(), torch.randn(D, generator=g).cuda(), torch.randn(B, D, generator=g).cuda()
+    z[0, 0, ::5] = float("inf")
+
+    def run(T, lengths):
+        leaf = [t.clone().requires_grad_(True) for t in (*(v[:, :T] for v in (x, a, i, z)), decay, state)]
+        y, new = _kernels().gated_recurrence(*leaf[:3], leaf[4], z=leaf[3], state=leaf[5], lengths=lengths)
+        grads = torch.autograd.grad([y, new], leaf, [gy[:, :T].contiguous(), gs])
+        return [y[:, :1], new, *(t[:, :1] for t in grads[:4]), *grads[4:]]
+
+    one, two = run(1, None), run(2, torch.ones(B, dtype=torch.int32, device="cuda"))
+    for p, q in zip(one, two):
+        assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.nan_to_num(7.0), q.nan_to_num(7.0))
+    assert one[2][0, 0, ::5].isinf().all() and torch.isfinite(one[2][1].float()).all()
