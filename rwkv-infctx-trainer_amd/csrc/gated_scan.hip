@@ -380,13 +380,13 @@ __global__ __launch_bounds__(64 * BACK_WAVES) void backward(const Call k) {
             if (GATE) R::floats(zk[j], zf);
 #pragma unroll
             for (int v = 0; v < V; v++) {
-                const float zz = GATE ? zf[v] * zs[j][v] : 1.f, gt = fmaf(gf[v], zz, g[v]), gu = gt * u[j][v];
+                const float zz = GATE ? zf[v] * zs[j][v] : 1.f, gt = fmaf(gf[v], zz, g[v]);          // (last of all factors: it times a state or input alone may be infinite)
                 // u changes by log a as -u times a^2 / beta^2: by a squared, for 1 / beta^2 - 1 has no digits left where a is small.  (Where a is one, as at a shut
                 // gate, u is zero and so is that: the largest number stands for infinity.)
                 const float less = a[j][v] * a[j][v] * fminf(__builtin_amdgcn_rcpf(beta[j][v] * beta[j][v]), 3e38f);
-                const float gl = gt * fmaf(-u[j][v], less, a[j][v] * hs[j][v]) * rs[j][v];
+                const float gl = gt * (fmaf(-u[j][v], less, a[j][v] * hs[j][v]) * rs[j][v]);
                 ox[v] = there ? gt * (beta[j][v] * is[j][v]) : 0.f;
-                oi[v] = there ? fmaf(-gu, is[j][v], gu) : 0.f;
+                oi[v] = there ? gt * fmaf(-u[j][v], is[j][v], u[j][v]) : 0.f;
                 orr[v] = there ? gl * (slope[v] * (1.f - rs[j][v])) : 0.f;
                 part[v] += there ? gl : 0.f;
                 if (GATE) oz[v] = there ? gf[v] * (hs[j + 1][v] * fmaf(zs[j][v], 1.f - zz, zz)) : 0.f;          // (gy h alone may be infinite)

@@ -78,6 +78,22 @@ def test_a_gate_far_shut_takes_no_gradient(T):
         assert bool((t == 0).all())
 
 
+@pytest.mark.parametrize("T", [1, 2, 140])
+@pytest.mark.parametrize("which", ["r", "i"])
+def test_a_gate_at_its_end_takes_no_gradient(T, which):
+    """A shut r keeps a large state, an open i lets a large input through: the sigmoid's slope is zero, and the incoming gradient times the state or the input, which fp32 does not
+    hold, is never formed."""
+    D = 70
+    full = lambda v: torch.full((1, T, D), v, device="cuda")
+    shut = which == "r"
+    x, r, i = (t.requires_grad_(True) for t in (full(0.0 if shut else 1e30), full(-200.0 if shut else 2.0), full(0.0 if shut else 200.0)))
+    decay = torch.full((D,), 3.0, device="cuda", requires_grad=True)
+    y, _ = _kernels().gated_recurrence(x, r, i, decay, state=torch.full((1, D), 1e30, device="cuda") if shut else None)
+    grads = torch.autograd.grad(y, (r, decay) if shut else (i,), full(1e10))
+    for t in grads:
+        assert bool((t == 0).all())
+
+
 def _slopes(x, wg, wu, gy):
     """In 64 bits, for silu: dg and du and what fp32 leaves of them: g and u are fp32 sums (c of their terms' sizes), slopes and slopes' slopes below 1.2."""
     g, u = x @ wg.t(), x @ wu.t()
