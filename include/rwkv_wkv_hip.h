@@ -424,7 +424,7 @@ int wkv_sample(void *stream, int rows, int V, int dtype, const void *logits, lon
  *   a[t] = exp(-scale softplus(decay) sigmoid(r[t])),  h[t] = a[t] h[t-1] + sqrt(1 - a[t]^2) sigmoid(i[t]) x[t],  y[t] = h[t] silu(z[t])
  * x, r, i, z (or NULL: y = h), y (B,T,D) in `dtype` (wkv_rows: any stride of batch, a token's from D up to 2^24); decay (D), state_in (NULL: zeros), state_out (B,D) fp32;
  * lengths as above.  checkpoints: NULL, or wkv_gated_recurrence_checkpoint_bytes (an fp32 state per 64 tokens) for a backward call.  state_out may be
- * state_in for a single token without checkpoints. */
+ * state_in for a single token without checkpoints.  B up to 65535, T up to 2^24, D below 2^24, B D below 2^30, B T D below 2^40; a single token's stride is not read. */
 size_t wkv_gated_recurrence_checkpoint_bytes(int B, int T, int D, int dtype);
 size_t wkv_gated_recurrence_forward_workspace(int B, int T, int D, int dtype);
 int wkv_gated_recurrence_forward(void *stream, int B, int T, int D, int dtype, float scale, const wkv_rows *x, const wkv_rows *r, const wkv_rows *i,

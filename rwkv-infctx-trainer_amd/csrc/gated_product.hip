@@ -4,7 +4,7 @@
 //     dg = gh u act'(g),  du = gh act(g),  gx = dg Wg + du Wu,  gWg = dg' x,  gWu = du' x
 //
 // 4 R C F operations forward and 8 backward, on the matrix cores (matrix_tiles.h): bound by these with many rows (4096 rows of 4096 into 14336 columns bf16: forward
-// 830 us, 1160 TFLOP/s; gx 700 and weights' gradients 790, 1370 and 1220; the clock that power leaves decides), by the weights' bytes with few (1 row: 43 us, 5.4 TB/s).  Forward, a workgroup's tile of B is half of gate rows and
+// 830 to 860 us, 1120 to 1160 TFLOP/s; gx 670 to 700 and weights' gradients 770 to 810, up to 1430 and 1250; the clock that power leaves decides), by the weights' bytes with few (1 row: 45 us, 5.2 TB/s).  Forward, a workgroup's tile of B is half of gate rows and
 // half of the same up rows, so that a lane ends with g and u of the same places and the activation and product happen in registers: g and u
 // never reach memory, except that a backward's are kept in fp32: rounded to 16 bits they would add as much to the gradients' error as each of the two
 // roundings that are left, that of dg and du, which the matrix cores take in the streams' type, and that of the results (bf16, error of
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64 * WM * WN, waves_per_simd(BM, AHEAD)) void forwa
 // fp16 has 5 bits of exponent: slopes that fp32 holds would be infinite from 65504 on and lose digits below 2^-14, where a mean loss' gradients lie.  So fp16 slopes are
 // written times a power of two, the same for the whole call, that takes the largest finite one to 2^14 .. 2^15 (what is 2^-29 of it still has all its digits), and the
 // products divide their fp32 sums by it.  A pass of its own finds the largest, by 256 workgroups, and reads what the slopes' pass reads again (the whole
-// backward of 4096 rows of 4096 into 14336 columns 1656 -> 1775 us, of 777 of 2048 into 7168 139 -> 150, of 16 of 2560 into 8960 86 -> 87); bf16 and fp32 have no need of it.
+// backward of 4096 rows of 4096 into 14336 columns 1656 -> 1775 us, of 777 of 2048 into 7168 140 -> 153, of 16 of 2560 into 8960 84 -> 88); bf16 and fp32 have no need of it.
 template <class T> constexpr bool scaled() { return std::is_same<T, f16>::value; }
 constexpr int LARGEST = 256;                  // workgroups, a number of each
 
@@ -326,7 +326,7 @@ template <class T, bool WHOLE> __global__ __launch_bounds__(256) void slopes(int
 
 // ---- few rows: a serving loop's single tokens.  What they cost is the weights, read once: a workgroup takes 16 gate rows and the same 16 up rows,
 // its four wavefronts every fourth tile of k; operands go straight from memory to registers, so that nothing waits for a barrier or for LDS (1 row of 1002
-// into 2731 columns bf16, weights out of the cache: 6.0 us with the launch).
+// into 2731 columns bf16, weights out of the cache: 7.2 us with the launch).
 constexpr int FEW = 64, FEW_WAVES = 4;
 template <class T, int GROUPS, bool WHOLE>                    // GROUPS of 16 rows of x; WHOLE: rows are whole pieces of 16 bytes
 __global__ __launch_bounds__(64 * FEW_WAVES) void few(const Forward k) {
@@ -465,10 +465,10 @@ template <class T> static Plan plan_of(long long M, long long N, long long K, bo
         }
     return best;
 }
-// Up to 64 rows: whether to take their kernel.  It reads the weights at what memory gives and waits for nothing, but reads x again for every 16 columns (bf16, weights out of
-// the cache, in us by it and by tiles: (4096, 14336) 1 row 55 and 51, 16 rows 67 and 53, 64 rows 104 and 58; (1002, 2731) 6 and 9, 6 and 10, 9 and 11; fp32
-// (1001, 2731) 8 and 27, 9 and 27, 17 and 28; (4095, 14335) 122 and 174, 151 and 163, 258 and 174).  Rows that begin between 4 bytes cost it twice a row's loads: (4095, 14335) bf16
-// 105 and 54, 149 and 64, 293 and 83, rows that begin at 4 ((4094, 14335)) 64 and 60, 83 and 67, 147 and 84.
+// Up to 64 rows: whether to take their kernel.  It reads the weights at what memory gives and waits for nothing, but reads x again for every 16 columns (weights out of
+// the cache, in us with the launch by it and by tiles: bf16 (4096, 14336) 1 row 50 and 46, 16 rows 62 and 47, 64 rows 102 and 52; (1002, 2731) 7.2 and 9.8, 7.4 and 10.1, 10.2 and 13.8; fp32
+// (1001, 2731) 9 and 27, 11 and 27, 18 and 28; (4095, 14335) 118 and 160, 147 and 156, 255 and 170; (1024, 8960) 26 and 42, 28 and 42, 62 and 43).  Rows that begin between 4 bytes cost it twice
+// a row's loads: bf16 (4095, 14335) 102 and 60, 148 and 59, 294 and 79, rows that begin at 4 ((4094, 14335)) 68 and 65, 82 and 62, 143 and 80.
 template <class T> static bool few_pays(int R, int C, int F) {
     if (R > FEW) return false;
     const double mb = 2. * F * C * sizeof(T) / 1e6, groups = R <= 16 ? 1 : R <= 32 ? 2 : 4;

@@ -7,11 +7,13 @@
 //     g[t] = go[t] + a[t+1] g[t+1],   gx = g b sigmoid(i),   gi = g b x sigmoid'(i),   l = g (a h[t-1] - a^2 / b sigmoid(i) x),
 //     gr = l log a (1 - sigmoid(r)),   gdecay = -scale sigmoid(decay) sum of l sigmoid(r),   gz = gy h silu'(z)
 //
-// Bound by memory: every stream is read once and every result written once (B8 T4096 D4096 bf16: forward 279 us, 4.8 TB/s, backward 495, 4.9).  The recurrence is linear, so a run of tokens is the pair (product of a, its
+// Bound by memory: every stream is read once and every result written once, where whole sequences make enough workgroups (B8 T4096 D4096 bf16, replayed: forward 277 us, 4.8 TB/s, backward
+// 500, 4.8; as single calls under a profiler 292 and 540).  The recurrence is linear, so a run of tokens is the pair (product of a, its
 // end from nothing), and pairs join.  A workgroup walks a sequence for 64 V channels, a step at a time: each of its wavefronts takes K tokens of the step for
 // all of the channels, makes its run's pair and leaves it in LDS; behind one barrier every wavefront joins the pairs before its own and finishes
 // its tokens from the state that gives, still in registers.  Where that makes too few workgroups the sequences are cut in time, and a pass over the decays
-// and inputs alone leaves every segment's pair first.  Backwards a step runs both ways at once: the states again, from one kept
+// and inputs alone leaves every segment's pair first: it reads x, r and i (backwards r, gy and z) once more, so that such calls stand at 1.5 to 3 times the streams' bytes
+// (B1 T4096 D4096 58 / 93 us, B1 T8192 D512 27 / 38).  Backwards a step runs both ways at once: the states again, from one kept
 // before every CHECK tokens, and their gradients.
 //
 // 1 - a^2 loses its digits where a is near one, the very channels that remember long: there it is formed from log a.
@@ -46,7 +48,7 @@ constexpr int OUTSIDE = (int)0x80000000u;                 // a lane's offset tha
 
 __device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(-LOG2E * v)); }
 
-// 1 - a^2 of a = 2^l: near one the polynomial of degree 4 in l nearest to (1 - 4^l) / l where 4^l is above exp(-1/2), right to 2^-22.5 of the value
+// 1 - a^2 of a = 2^l: near one the polynomial of degree 4 in l nearest to (1 - 4^l) / l where 4^l is above exp(-1/2), right to 2^-22.2 of the value
 __device__ __forceinline__ float one_less_square(float l, float a) {
     float p = fmaf(l, -0.03474162146449089f, -0.1514858603477478f);
     p = fmaf(p, l, -0.4437292814254761f);
@@ -453,11 +455,13 @@ struct ToDecay {
 };
 
 // ---- launches
-// How a call is shared out: channels per lane, and segments in time where whole sequences make too few workgroups.  A compute unit takes 5.7 us for a step of
-// two channels per lane and 3.6 us for one of one (forward, bf16; backward twice that), one workgroup after the other; a pass for the segments' pairs adds
-// two thirds, a launch and a walk over them.  Times of this rule's choice and the nearest other, forward / backward in us: B4 T777 D4096 one channel 31 / 54, two
-// in two segments 52 / 78; B1 T4096 D4096 two in eight 57 / 91, one in four 60 / 104; B5 T2048 D4096 two 113 / 213, one 145 / 256; B12 T2048
-// D4096 one 237 / 429, two 248 / 450; B1 T8192 D512 one in 32 27 / 37, two in 32 36 / 50.
+// How a call is shared out: channels per lane, and segments in time where whole sequences make too few workgroups.  The weights rank the choices and are no times: a step of a
+// workgroup counts 5.7 with two channels per lane and 3.6 with one, rounds of workgroups one after the other; a pass for the segments' pairs counts two thirds of the main one, and a
+// launch and a walk over the pairs.  They are fitted to bf16 (forward) and hold the order of the others': replayed forward / backward in us, this rule's choice first:
+// B4 T777 D4096 one channel 33 / 57, two 44 / 79, two in two segments 54 / 79; B1 T4096 D4096 two in eight 57 / 92, one in four 59 / 104; B5 T2048 D4096 two 112 / 213, one 141 / 256;
+// B12 T2048 D4096 one 239 / 434, two 253 / 463; B1 T8192 D512 one in 32 27 / 38, two in 32 35 / 50; B8 T4096 D4096 two 277 / 500, one 308 / 558; fp32 B2 T301 D1001 in three 15.2 / 21.5, whole 15.2 /
+// 22.5; B1 T4096 D4096 cut 98 / 167, in four 94 / 166, whole 155 / 283.  A step is 128 tokens (64 backwards) of a workgroup whatever T is, so many sequences of few tokens pay for
+// tokens that are not there: 16M elements as B64 T64 D4096 68 / 98, B256 T16 217 / 290, B2048 T2 1665 / 2184 for 33 / 60 of bytes.
 struct Plan { int v, span; };
 static inline Plan plan_of(int B, int T, int D, bool two) {
     const long long cus = cu_count(), steps = (T + STEP - 1) / STEP;

@@ -34,7 +34,7 @@ template <> __device__ __forceinline__ f4 mma<float>(i4 a, i4 b, f4 c) {
 }
 
 // 16 bytes per lane from memory to LDS, the lanes' side by side from `lds` on; nothing waits for them here.  What lies outside the range comes as zeros; the memory's
-// addresses may be of any alignment (of every even one checked on the hardware), LDS' are whole pieces.
+// addresses may be of any alignment (rows at every even one, by odd widths and sliced operands, are what the feed-forward's tests read), LDS' are whole pieces.
 __device__ __forceinline__ void to_lds(i4 range, unsigned offset, unsigned lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(__builtin_amdgcn_readfirstlane((int)lds)), "v"(offset), "s"(range) : "memory", "m0");
 }
