@@ -195,12 +195,17 @@ public:
 };
 
 // Operands of different types under autocast, as fp32 weights behind a projection's 16-bit output are: in autocast's type, as torch.nn.functional.linear takes them (a weight's
-// copy is kept for as long as autocast keeps it).  Operands of one type are taken as they come.
+// copy is kept for as long as autocast keeps it, but none made where no gradient is recorded: a recorded call after it would take that copy and lose the gradient).  Operands of
+// one type are taken as they come.
 void cast_by_autocast(std::initializer_list<Tensor *> operands) {
     if (!at::autocast::is_autocast_enabled(at::kCUDA)) return;
     const at::ScalarType first = (*operands.begin())->scalar_type();
     if (std::all_of(operands.begin(), operands.end(), [&](const Tensor *t) { return t->scalar_type() == first; })) return;
-    for (Tensor *t : operands) *t = at::autocast::cached_cast(at::autocast::get_autocast_dtype(at::kCUDA), *t, at::kCUDA);
+    const at::ScalarType type = at::autocast::get_autocast_dtype(at::kCUDA);
+    for (Tensor *t : operands) {
+        if (at::GradMode::is_enabled()) *t = at::autocast::cached_cast(type, *t, at::kCUDA);
+        else if (t->is_floating_point() && t->scalar_type() != at::kDouble) *t = as_type(*t, type);
+    }
 }
 
 // gated_product(x, w_gate, w_up, activation) -> h; None: traced

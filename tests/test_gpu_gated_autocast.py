@@ -73,3 +73,28 @@ def test_block_under_autocast(low, T, lengths):
         # (a parameter's two uses: autocast casts it once and adds both gradients in 16 bits, by hand it is cast twice and they are added in fp32: two half steps)
         assert a.dtype == p.dtype and torch.isfinite(a).all(), n
         assert bool(((a - b).abs() <= torch.finfo(low).eps * (b.abs() + b.abs().max())).all()), n
+
+
+def test_a_call_without_gradients_leaves_no_copy_behind():
+    """A recorded call after one without autograd, both under one autocast: the weights' gradients come."""
+    from rwkv_wkv_hip import gated as K
+    n = lambda *s: torch.randn(*s, device="cuda")
+    x, wg, wu = n(9, 40).bfloat16(), n(56, 40).requires_grad_(True), n(56, 40).requires_grad_(True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        with torch.no_grad():
+            first = K.gated_feed_forward(x, wg, wu)
+        out = K.gated_feed_forward(x, wg, wu)
+    assert out.requires_grad and torch.equal(first, out)
+    for t in torch.autograd.grad(out.float().sum(), (wg, wu)):
+        assert t.dtype == torch.float32 and t.any()
+
+
+def test_types_that_autocast_does_not_cast_are_refused():
+    from rwkv_wkv_hip import gated as K
+    n = lambda *s: torch.randn(*s, device="cuda")
+    for record in (True, False):
+        with torch.autocast("cuda", dtype=torch.bfloat16), torch.set_grad_enabled(record):
+            with pytest.raises((ValueError, AssertionError)):
+                K.gated_feed_forward(n(9, 40).double(), n(56, 40), n(56, 40))
+            with pytest.raises((ValueError, AssertionError)):
+                K.gated_feed_forward(n(9, 40).bfloat16(), n(56, 40).double(), n(56, 40))
