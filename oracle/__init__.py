@@ -2,7 +2,7 @@
 
 TEST INFRASTRUCTURE ONLY.  Nothing in the shipped package imports this
 directory; only the test-suite, the smoke check and the benchmark's
-``cpu_baseline`` leg do, and there only as the checker / the timed CPU
+``cpu_baseline`` leg do, and there only as the oracle / the timed CPU
 baseline.  The shipped operators fail loudly when the HIP library is missing
 instead of falling back to anything in here.
 

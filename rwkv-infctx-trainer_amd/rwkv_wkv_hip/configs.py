@@ -2,7 +2,7 @@
 
 Every tensor is drawn on the CPU in fp32 from one ``torch.Generator`` in a fixed
 order (r, k, v, raw decay, u, state, dy, dstate), then rounded to its storage
-dtype, so a CPU checker and the GPU operator see bit-identical inputs.  The
+dtype, so the CPU oracle and the GPU operator see bit-identical inputs.  The
 second parameter of N(.,.) is a standard deviation.
 
 cfg0  WKV5 forward only  B1 T512  C768  H12 fp32, zero state

@@ -249,3 +249,31 @@ def test_a_recorded_single_token_reads_itself_alone(dtype):
     for p, q in zip(one, two):
         assert torch.equal(p.isnan(), q.isnan()) and torch.equal(p.nan_to_num(7.0), q.nan_to_num(7.0))
     assert one[2][0, 0, ::5].isinf().all() and torch.isfinite(one[2][1].float()).all()
+
+
+@pytest.mark.parametrize("R", [5, 90])
+def test_fp16_slopes_scale_with_what_a_replay_holds(R):
+    """A captured training call finds its power of two on every replay: gradients that come in 2^-20 and 2^12 times as large give what the eager call gives, to the bit."""
+    K = _kernels()
+    g = S._g(R, 8)
+    n = lambda *s: torch.randn(*s, generator=g).half().cuda()
+    leaf = [t.requires_grad_(True) for t in (n(R, 64), n(48, 64) / 8, n(48, 64) / 8)]
+    leaf = [t.detach().requires_grad_(True) for t in leaf]
+    gy, base = n(R, 48), n(R, 48)
+    step = lambda: torch.autograd.grad(K.gated_feed_forward(*leaf), leaf, gy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for power in (0, -20, 12, -20):
+        gy.copy_((base.float() * 2.0 ** power).half())
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in captured]
+        for a, b in zip(got, step()):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) and b.any()
